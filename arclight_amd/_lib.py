@@ -80,6 +80,10 @@ SIGNATURES = {
                              + [ctypes.POINTER(abi.AlTensor)] * 2 + [_VP]),
     "al_attn_inputs_f32": (_I, [ctypes.POINTER(abi.AlAttnInputsArgs), _VP]),
     "al_fattn_f16_with_inputs": (_I, [ctypes.POINTER(abi.AlAttnInputsArgs), ctypes.POINTER(abi.AlFattnArgs)]),
+    # include/arclight_paged.h
+    "al_paged_append_f32": (_I, [ctypes.POINTER(abi.AlPagedAppendArgs)]),
+    "al_paged_fattn_f16": (_I, [ctypes.POINTER(abi.AlPagedFattnArgs)]),
+    "al_paged_fattn_workspace_bytes": (_U64, [ctypes.POINTER(abi.AlPagedFattnArgs)]),
     # include/arclight_matmul.h
     "al_mul_mat_q4_0_f32": (_I, [ctypes.POINTER(abi.AlTensor)] * 3 + [_VP]),
     "al_mul_mat_q4_0_check_inverse": (_I, [ctypes.POINTER(ctypes.c_ulonglong)]),

@@ -163,6 +163,33 @@ class AlAttnInputsArgs(ctypes.Structure):
     ]
 
 
+# include/arclight_paged.h
+class AlPagedAppendArgs(ctypes.Structure):
+    """al_paged_append_args."""
+    _fields_ = [
+        ("q", AlTensor), ("q_w", AlTensor), ("k", AlTensor), ("k_w", AlTensor), ("v", AlTensor),
+        ("pos", AlTensor), ("seq", AlTensor), ("q_out", AlTensor),
+        ("k_pool", AlTensor), ("v_pool", AlTensor), ("table", AlTensor),
+        ("eps", ctypes.c_float),
+        ("norm", ctypes.c_int32),
+        ("rope", ctypes.POINTER(AlRopeParams)),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class AlPagedFattnArgs(ctypes.Structure):
+    """al_paged_fattn_args."""
+    _fields_ = [
+        ("q", AlTensor), ("k_pool", AlTensor), ("v_pool", AlTensor), ("table", AlTensor),
+        ("lens", AlTensor), ("counts", AlTensor), ("sinks", AlTensor), ("dst", AlTensor),
+        ("scale", ctypes.c_float),
+        ("logit_softcap", ctypes.c_float),
+        ("stream", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 def qwen3_rope(n_ctx_orig=40960):
     """Qwen3's rope_ext parameters (models/qwen3.cpp:49-55)."""
     return AlRopeParams(128, AL_ROPE_NEOX, n_ctx_orig, 1000000.0, 1.0, 0.0, 1.0, 32.0, 1.0)

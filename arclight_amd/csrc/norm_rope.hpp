@@ -16,6 +16,11 @@ struct RopeConsts {
     float theta_scale, freq_scale, ext_factor, corr0, corr1, mscale;
 };
 
+// Fills them and the rotation mode (0 for rope == NULL, 1 normal, 2 NEOX) on
+// the host; what: the caller's name, for the message of a refusal.
+struct al_rope_params;
+int rope_consts(const char * what, const al_rope_params * rope, RopeConsts * out, int * mode);
+
 // Dims of pair i. MODE: 0 no rotation, 1 pairs (2i, 2i + 1), 2 NEOX pairs
 // (i, i + 64).
 template <int MODE> __device__ __forceinline__ int rope_d0(const int i) { return MODE == 1 ? 2 * i : i; }
@@ -116,6 +121,22 @@ __device__ __forceinline__ void norm_rope_group8(const float (&lo)[8], const flo
         if constexpr (MODE != 0) {
             y_lo[k] = n0 * rot[k].x - n1 * rot[k].y;
             y_hi[k] = n0 * rot[k].y + n1 * rot[k].x;
+        }
+    }
+}
+
+// The rotation alone, of rows held the same way.
+template <int MODE>
+__device__ __forceinline__ void rope_group8(const float (&lo)[8], const float (&hi)[8], const float2 (&rot)[8],
+                                            float (&y_lo)[8], float (&y_hi)[8]) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        y_lo[k] = lo[k];
+        y_hi[k] = hi[k];
+        if constexpr (MODE != 0) {
+            y_lo[k] = lo[k] * rot[k].x - hi[k] * rot[k].y;
+            y_hi[k] = lo[k] * rot[k].y + hi[k] * rot[k].x;
         }
     }
 }

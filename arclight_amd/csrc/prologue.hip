@@ -177,6 +177,34 @@ float yarn_corr_dim(int n_dims, int n_ctx_orig, float n_rot, float base) {
     return n_dims * logf(n_ctx_orig / (n_rot * 2 * (float) pi)) / (2 * logf(base));
 }
 
+}  // namespace
+
+int rope_consts(const char * what, const al_rope_params * rope, RopeConsts * out, int * mode) {
+    RopeConsts c;
+    memset(&c, 0, sizeof(c));
+    *mode = 0;
+    if (rope) {
+        if (rope->n_dims != 128) return al_fail(AL_ERR_UNSUPPORTED, "%s: n_dims %d (only the full head, 128)", what, rope->n_dims);
+        if (rope->mode == AL_ROPE_NEOX) *mode = 2;
+        else if (rope->mode == AL_ROPE_NORMAL) *mode = 1;
+        else return al_fail(AL_ERR_UNSUPPORTED, "%s: rope mode %d", what, rope->mode);
+        // host-side constants exactly as the reference's rope op computes them
+        c.theta_scale = powf(rope->freq_base, -2.0f / rope->n_dims);
+        const float start = floorf(yarn_corr_dim(rope->n_dims, rope->n_ctx_orig, rope->beta_fast, rope->freq_base));
+        const float end = ceilf(yarn_corr_dim(rope->n_dims, rope->n_ctx_orig, rope->beta_slow, rope->freq_base));
+        c.corr0 = fmaxf(0.0f, start);
+        c.corr1 = fminf((float) (rope->n_dims - 1), end);
+        c.freq_scale = rope->freq_scale;
+        c.ext_factor = rope->ext_factor;
+        c.mscale = rope->attn_factor;
+        if (rope->ext_factor != 0.0f) c.mscale *= 1.0f + 0.1f * logf(1.0f / rope->freq_scale);
+    }
+    *out = c;
+    return AL_OK;
+}
+
+namespace {
+
 // Checks the operands as al_rms_norm_rope_f32 documents them and fills p
 // and the rotation mode (0 none, 1 normal, 2 NEOX).
 int norm_rope_params(const al_tensor * x, const al_tensor * w, const al_tensor * pos, float eps,
@@ -195,22 +223,8 @@ int norm_rope_params(const al_tensor * x, const al_tensor * w, const al_tensor *
     int mode = 0;
     NormRopeParams p;
     memset(&p, 0, sizeof(p));
-    if (rope) {
-        if (rope->n_dims != 128) return al_fail(AL_ERR_UNSUPPORTED, "rms_norm_rope: n_dims %d (only the full head, 128)", rope->n_dims);
-        if (rope->mode == AL_ROPE_NEOX) mode = 2;
-        else if (rope->mode == AL_ROPE_NORMAL) mode = 1;
-        else return al_fail(AL_ERR_UNSUPPORTED, "rms_norm_rope: rope mode %d", rope->mode);
-        // host-side constants exactly as the reference's rope op computes them
-        p.rope.theta_scale = powf(rope->freq_base, -2.0f / rope->n_dims);
-        const float start = floorf(yarn_corr_dim(rope->n_dims, rope->n_ctx_orig, rope->beta_fast, rope->freq_base));
-        const float end = ceilf(yarn_corr_dim(rope->n_dims, rope->n_ctx_orig, rope->beta_slow, rope->freq_base));
-        p.rope.corr0 = fmaxf(0.0f, start);
-        p.rope.corr1 = fminf((float) (rope->n_dims - 1), end);
-        p.rope.freq_scale = rope->freq_scale;
-        p.rope.ext_factor = rope->ext_factor;
-        p.rope.mscale = rope->attn_factor;
-        if (rope->ext_factor != 0.0f) p.rope.mscale *= 1.0f + 0.1f * logf(1.0f / rope->freq_scale);
-    }
+    const int rc = rope_consts("rms_norm_rope", rope, &p.rope, &mode);
+    if (rc != AL_OK) return rc;
     p.x = (const char *) x->data; p.x_nb1 = (int64_t) x->nb[1]; p.x_nb2 = (int64_t) x->nb[2];
     p.w = w ? (const float *) w->data : nullptr;
     p.pos = (const int32_t *) pos->data;
@@ -227,8 +241,8 @@ int norm_rope_params(const al_tensor * x, const al_tensor * w, const al_tensor *
         p.rows64 = rows->type == AL_TYPE_I64;
         p.n_rows_dst = y->ne[1];
         p.y_nb1 = (int64_t) y->nb[1];
-        int rc = al_device_error_flag(&p.err);
-        if (rc != AL_OK) return rc;
+        const int rc_err = al_device_error_flag(&p.err);
+        if (rc_err != AL_OK) return rc_err;
     } else {
         if (y->type != AL_TYPE_F32 || y->ne[0] != 128 || y->ne[1] != H || y->ne[2] != T || y->nb[0] != 4)
             return al_fail(AL_ERR_INVALID, "rms_norm_rope: y must be f32 [128, H, T] with nb0 = 4");

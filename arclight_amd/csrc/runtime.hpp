@@ -11,4 +11,9 @@ void al_clear_error();
 // Per-device state, created on first use with the device current.
 int al_device_cu_count(int * n_cu);
 int al_device_lds_per_block(int * bytes);
-int al_device_error_flag(int ** flag);   // int[2]: {set, first bad index}
+int al_device_error_flag(int ** flag);   // [0, 1] set_rows, [2] a merge gave up waiting, [4..6] paged cache
+
+// Records of a call with no workspace of its own: `bytes` of the library's
+// workspace of (current device, stream), behind its counters. No initial
+// value; calls on one stream share it.
+int al_library_workspace(size_t bytes, void * stream, void ** ptr);
