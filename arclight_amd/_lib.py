@@ -84,6 +84,10 @@ SIGNATURES = {
     "al_paged_append_f32": (_I, [ctypes.POINTER(abi.AlPagedAppendArgs)]),
     "al_paged_fattn_f16": (_I, [ctypes.POINTER(abi.AlPagedFattnArgs)]),
     "al_paged_fattn_workspace_bytes": (_U64, [ctypes.POINTER(abi.AlPagedFattnArgs)]),
+    # include/arclight_lora.h
+    "al_lora_f32": (_I, [ctypes.POINTER(abi.AlLoraArgs)]),
+    "al_mul_mat_q4_0_lora_f32": (_I, [ctypes.POINTER(abi.AlLoraArgs)]),
+    "al_lora_workspace_bytes": (_U64, [ctypes.POINTER(abi.AlLoraArgs)]),
     # include/arclight_matmul.h
     "al_mul_mat_q4_0_f32": (_I, [ctypes.POINTER(abi.AlTensor)] * 3 + [_VP]),
     "al_mul_mat_q4_0_check_inverse": (_I, [ctypes.POINTER(ctypes.c_ulonglong)]),

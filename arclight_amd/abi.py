@@ -190,6 +190,18 @@ class AlPagedFattnArgs(ctypes.Structure):
     ]
 
 
+# include/arclight_lora.h
+class AlLoraArgs(ctypes.Structure):
+    """al_lora_args."""
+    _fields_ = [
+        ("a", AlTensor), ("b", AlTensor), ("ranks", AlTensor), ("scales", AlTensor), ("ids", AlTensor),
+        ("x", AlTensor), ("base", AlTensor), ("y", AlTensor), ("w", AlTensor),
+        ("stream", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 def qwen3_rope(n_ctx_orig=40960):
     """Qwen3's rope_ext parameters (models/qwen3.cpp:49-55)."""
     return AlRopeParams(128, AL_ROPE_NEOX, n_ctx_orig, 1000000.0, 1.0, 0.0, 1.0, 32.0, 1.0)

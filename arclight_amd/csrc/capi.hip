@@ -910,14 +910,15 @@ extern "C" int al_device_errors(void) {
     int * flag = nullptr;
     int rc = al_device_error_flag(&flag);
     if (rc != AL_OK) return rc;
-    int h[8] = {};
+    int h[12] = {};
     hipError_t e = hipMemcpy(h, flag, sizeof(h), hipMemcpyDeviceToHost);
     if (e != hipSuccess) return al_hip_fail(e, "hipMemcpy(error flag)");
-    if (h[0] || h[2] || h[4]) {
+    if (h[0] || h[2] || h[4] || h[8]) {
         e = hipMemset(flag, 0, sizeof(h));
         if (e != hipSuccess) return al_hip_fail(e, "hipMemset(error flag)");
         if (h[0]) return al_fail(AL_ERR_INVALID, "set_rows: row index %d out of range (ops.cpp:171)", h[1]);
         if (h[4]) return al_fail(AL_ERR_INVALID, "paged cache: %s", paged_error_text(h[5], h[6]).c_str());
+        if (h[8]) return al_fail(AL_ERR_INVALID, "lora: a row of adapter %d, which is not there or whose rank does not fit", h[9]);
         return al_fail(AL_ERR_HIP, "fattn: a merging workgroup gave up waiting for the other splits' records");
     }
     return AL_OK;

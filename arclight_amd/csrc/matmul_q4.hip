@@ -32,6 +32,7 @@
 
 #include "../../include/arclight_matmul.h"
 #include "kernel_args.hpp"
+#include "matmul_q4.hpp"
 #include "runtime.hpp"
 
 namespace {
@@ -602,7 +603,7 @@ extern "C" int al_mul_mat_q4_0_check_inverse(unsigned long long * mismatches) {
     return AL_OK;
 }
 
-extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, const al_tensor * y, void * stream) {
+int mul_mat_q4_0_check(const al_tensor * w, const al_tensor * x, const al_tensor * y, size_t * scratch_bytes) {
     if (!w || !x || !y || !w->data || !x->data || !y->data) return al_fail(AL_ERR_INVALID, "mul_mat_q4_0: w, x and y required");
     if (w->type != AL_TYPE_Q4_0 || x->type != AL_TYPE_F32 || y->type != AL_TYPE_F32)
         return al_fail(AL_ERR_UNSUPPORTED, "mul_mat_q4_0: types %d x %d -> %d (Q4_0 x f32 -> f32 only)", w->type, x->type, y->type);
@@ -617,7 +618,13 @@ extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, con
     if ((int64_t) w->nb[1] != nb * 18 || x->nb[0] != 4 || y->nb[0] != 4 || ((uintptr_t) w->data & 3) || ((uintptr_t) x->data & 15) ||
         (x->nb[1] & 15) || x->nb[1] < (uint64_t) K * 4 || y->nb[1] < (uint64_t) N * 4 || ((uintptr_t) y->data & 3))
         return al_fail(AL_ERR_INVALID, "mul_mat_q4_0: w rows must be contiguous blocks (nb1 = K/32*18, 4-byte aligned), x rows 16-byte aligned, rows not overlapping");
-    hipStream_t st = (hipStream_t) stream;
+    const int64_t padded = (T + kTile - 1) / kTile * kTile;
+    *scratch_bytes = T <= kFusedMaxT ? 0 : (size_t) (padded * K + padded * nb * 2);
+    return AL_OK;
+}
+
+int mul_mat_q4_0_run(const al_tensor * w, const al_tensor * x, const al_tensor * y, void * s, hipStream_t st) {
+    const int64_t K = w->ne[0], N = w->ne[1], T = x->ne[1], nb = K / 32;
     if (T <= kFusedMaxT) {
         switch (nb / 64) {
             case 2: return launch_fused_t<2>(w, x, y, (int) N, (int) K, (int) T, st);
@@ -628,10 +635,7 @@ extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, con
         }
     }
     const int tiles = (int) ((T + kTile - 1) / kTile);
-    const size_t qs_bytes = (size_t) tiles * kTile * (size_t) K, f_bytes = (size_t) tiles * kTile * (size_t) nb * 2;
-    void * s = nullptr;
-    int rc = scratch(qs_bytes + f_bytes, &s);
-    if (rc != AL_OK) return rc;
+    const size_t qs_bytes = (size_t) tiles * kTile * (size_t) K;
     uint4 * frag = (uint4 *) s;
     _Float16 * dx = (_Float16 *) ((char *) s + qs_bytes);
     const int items = tiles * (int) (nb / 2);
@@ -646,4 +650,13 @@ extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, con
         case 4: return launch_gemm<16>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, st);
         default: return al_fail(AL_ERR_UNSUPPORTED, "mul_mat_q4_0: K %lld", (long long) K);
     }
+}
+
+extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, const al_tensor * y, void * stream) {
+    size_t bytes = 0;
+    void * s = nullptr;
+    int rc = mul_mat_q4_0_check(w, x, y, &bytes);
+    if (rc == AL_OK && bytes) rc = scratch(bytes, &s);
+    if (rc != AL_OK) return rc;
+    return mul_mat_q4_0_run(w, x, y, s, (hipStream_t) stream);
 }

@@ -33,8 +33,18 @@ class Q4_0Matrix:
         self.buf.upload(blocks)
 
     def desc(self):
+        return Q4_0View(self.buf.ptr, self.K, self.N).desc()
+
+
+class Q4_0View:
+    """A Q4_0Matrix's blocks in device memory that something else owns."""
+
+    def __init__(self, ptr, K, N):
+        self.ptr, self.K, self.N = ptr, int(K), int(N)
+
+    def desc(self):
         row = self.K // abi.QK4_0 * abi.Q4_0_BLOCK_BYTES
-        return abi.make_tensor(self.buf.ptr, abi.AL_TYPE_Q4_0, [self.K, self.N, 1, 1],
+        return abi.make_tensor(self.ptr, abi.AL_TYPE_Q4_0, [self.K, self.N, 1, 1],
                                [abi.Q4_0_BLOCK_BYTES, row, row * self.N, row * self.N])
 
 
