@@ -2,11 +2,11 @@
 // (include/arclight_lora.h), for gfx950.
 //
 // Mathematics: v[t] = s_a A_a x[t], y[t] = base[t] + B_a v[t] for a = ids[t],
-// both in f32: the f16 weights are exact in f32, and the products run on the
-// f32 matrix instruction (16 x 16 x 4), so that activations of any size need
-// no scaling. Its rate is a sixteenth of f16's, and enough: at rank 16 the
-// products of 8000 tokens take 7 us of the matrix cores, the activations'
-// bytes 80.
+// to the accuracy of f32: the f16 weights are exact, and x and v are carried
+// as pairs of f16, hi + lo to 2^-22, after a power of two for each row (and
+// run of columns) that brings the largest to [2^11, 2^12), so that values of
+// any size keep their bits. Two f16 products of 16 x 16 x 32 take an eighth of
+// the matrix cores' time that f32 products (16 x 16 x 4) do.
 //
 // Rows are taken in tiles of 16. A tile's columns (its rows of x) are
 // independent in both products, so a tile of several adapters is computed
@@ -34,10 +34,9 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 16;                       // rows of x
 constexpr int kMaxR = 128;
-constexpr int kSlots = 4;                       // workgroups that share a tile's adapters
+constexpr int kParts = 8;                       // parts of K at most
 constexpr int kCols = 256;                      // outputs of a workgroup
 
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 
 struct LoraParams {
     const char * a;  int64_t a_nb1, a_nb2;      // rank row, adapter
@@ -50,13 +49,27 @@ struct LoraParams {
     char * y;           int64_t y_nb1;
     float * v;                                  // [ks][T][R]
     int32_t K, N, R, T, n_adapters;
-    int32_t ks, k_step;                         // parts of K, columns of one (a multiple of 128)
+    int32_t ks, k_step;                         // parts of K, columns of one (a multiple of 32)
+    int32_t chunks;                             // slices of kCols outputs of a workgroup
+    int32_t slots;                              // workgroups that share a tile's adapters
+    int32_t copy;                               // base is not y: rows without an adapter are copied
     int32_t y_vec;                              // y and base rows 16-byte aligned, N a multiple of 4
     int * err;
 };
 
-__device__ __forceinline__ floatx4 mfma_f32(const float a, const float b, const floatx4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+constexpr int min_c(int a, int b) { return a < b ? a : b; }
+
+// Power of two that brings a row's largest value to [2^11, 2^12), and its
+// inverse. top: the largest size of this lane's values, the row in the 4 lanes
+// {n, n + 16, n + 32, n + 48}.
+__device__ __forceinline__ void row_scale(float top, float & up, float & down) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_int(top), __float_as_int(top), false, false);
+    top = fmaxf(__int_as_float((int) a[0]), __int_as_float((int) a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_int(top), __float_as_int(top), false, false);
+    top = fmaxf(__int_as_float((int) b[0]), __int_as_float((int) b[1]));
+    const int ex = min(max((int) (__float_as_uint(top) >> 23), 12), 253) - 127;
+    up = __uint_as_float((uint32_t) (11 - ex + 127) << 23);
+    down = __uint_as_float((uint32_t) (ex - 11 + 127) << 23);
 }
 
 // Rank of adapter a, -1 for one that is not to be used.
@@ -82,157 +95,343 @@ __device__ __forceinline__ uint32_t leaders(const int id) {
     return out;
 }
 
-// Parts of v: columns k0 .. k0 + k_step - 1 of K, of a tile's rows. RT: tiles
-// of 16 ranks. Lane 16 g + n loads 8 columns of rank row n and of row n of x
-// (8 g .. 8 g + 7 of each 32); matrix step s takes column s of them.
-template <int RT>
-__global__ __launch_bounds__(64 * kWaves) void lora_shrink_kernel(const LoraParams p) {
-    __shared__ float part[kWaves][RT * 16][kTile + 1];
+// The adapter of a workgroup: the slot-th (and every p.slots-th after it) of
+// those that the tile's rows have, in the order of their first rows.
+struct Turn {
+    uint32_t todo;
+    __device__ __forceinline__ void skip(const int n) {
+        for (int i = 0; i < n && todo; ++i) todo &= todo - 1;
+    }
+};
+
+// The columns of a wave: rounds of 32 U from k0 to k1, beginning with another
+// round in every tile. Rows of x are often a power of two apart, and so the
+// same columns of all rows in the same few memory channels: waves that take
+// ranges apart from one another, and tiles that begin apart, use them all.
+struct Columns {
+    int k0, k1, rounds, at;
+    template <int U> __device__ __forceinline__ static Columns of(const LoraParams & p, const int part, const int tile, const int wave,
+                                                                  const int waves) {
+        const int a = part * p.k_step, b = min(a + p.k_step, p.K), own = (p.k_step / 32 + waves - 1) / waves * 32;
+        Columns c;
+        c.k0 = min(a + wave * own, b);
+        c.k1 = min(c.k0 + own, b);
+        c.rounds = (c.k1 - c.k0 + 32 * U - 1) / (32 * U);
+        c.at = c.rounds > 1 ? tile % c.rounds : 0;
+        return c;
+    }
+    template <int U> __device__ __forceinline__ int column() const { return k0 + at * 32 * U; }
+    __device__ __forceinline__ void next() { at = at + 1 == rounds ? 0 : at + 1; }
+};
+
+// This lane's columns of U runs of 32 from k on; column 0 for those
+// beyond k1, which shrink() zeroes.
+template <int U>
+__device__ __forceinline__ void load_x(const char * xr, const int k, const int k1, const int g, float4 (&x)[U][2]) {
+#pragma unroll
+    for (int b = 0; b < U; ++b) {
+        const int kl = k + 32 * b + 8 * g;                             // K is a multiple of 8
+        const float4 * at = (const float4 *) (xr + (int64_t) (kl < k1 ? kl : 0) * 4);
+        x[b][0] = at[0];
+        x[b][1] = at[1];
+    }
+}
+
+// Sum of A's rows with the tile's rows over a wave's columns, RT tiles of 16
+// ranks. Lane 16 g + n loads 8 columns of rank row n and of row n of x (8 g ..
+// 8 g + 7 of each 32). x holds the first round's activations. The next round's loads go out before this round's
+// products (the asm statements keep the compiler from sinking them to their
+// uses): without that all waves of a launch load and compute in step.
+template <int RT, int U>
+__device__ __forceinline__ void shrink(const LoraParams & p, const char * ar, const int rank, const char * xr, float4 (&x)[U][2],
+                                       Columns c, const int n, const int g, float (*part)[kTile + 1]) {
+    floatx4 acc[RT];
+#pragma unroll
+    for (int u = 0; u < RT; ++u) acc[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const char * rows[RT];
+#pragma unroll
+    for (int u = 0; u < RT; ++u) rows[u] = ar + (int64_t) min(16 * u + n, rank - 1) * p.a_nb1;
+    auto load_w = [&](const int k, half8 (&w)[U][RT]) {
+#pragma unroll
+        for (int b = 0; b < U; ++b) {
+            const int kl = k + 32 * b + 8 * g;
+#pragma unroll
+            for (int u = 0; u < RT; ++u) w[b][u] = *(const half8 *) (rows[u] + (int64_t) (kl < c.k1 ? kl : 0) * 2);
+        }
+        asm volatile("" ::: "memory");
+    };
+    auto multiply = [&](const int k, float4 (&y)[U][2], half8 (&w)[U][RT]) {
+        if (k + 32 * U > c.k1) {
+#pragma unroll
+            for (int b = 0; b < U; ++b)
+                if (k + 32 * b + 8 * g >= c.k1) {
+                    y[b][0] = y[b][1] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int u = 0; u < RT; ++u) w[b][u] = half8{};
+                }
+        }
+        float top = 0.0f, up, down;
+#pragma unroll
+        for (int b = 0; b < U; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                top = fmaxf(fmaxf(fmaxf(top, fabsf(y[b][h].x)), fmaxf(fabsf(y[b][h].y), fabsf(y[b][h].z))), fabsf(y[b][h].w));
+        row_scale(top, up, down);
+        floatx4 sum[RT];
+#pragma unroll
+        for (int u = 0; u < RT; ++u) sum[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < U; ++b) {
+            const float xs[8] = {y[b][0].x, y[b][0].y, y[b][0].z, y[b][0].w, y[b][1].x, y[b][1].y, y[b][1].z, y[b][1].w};
+            half8 hi, lo;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const float z = xs[s] * up;
+                hi[s] = (_Float16) z;
+                lo[s] = (_Float16) (z - (float) hi[s]);
+            }
+#pragma unroll
+            for (int u = 0; u < RT; ++u) sum[u] = mfma_16x16x32(w[b][u], hi, mfma_16x16x32(w[b][u], lo, sum[u]));
+        }
+#pragma unroll
+        for (int u = 0; u < RT; ++u) acc[u] += sum[u] * down;
+    };
+    if (c.rounds > 0) {
+        int k = c.column<U>();
+        half8 w[U][RT];
+        load_w(k, w);
+        for (int i = 1; i < c.rounds; ++i) {
+            c.next();
+            const int kn = c.column<U>();
+            float4 xn[U][2];
+            half8 wn[U][RT];
+            load_x<U>(xr, kn, c.k1, g, xn);
+            load_w(kn, wn);
+            multiply(k, x, w);
+            k = kn;
+#pragma unroll
+            for (int b = 0; b < U; ++b) {
+                x[b][0] = xn[b][0];
+                x[b][1] = xn[b][1];
+#pragma unroll
+                for (int u = 0; u < RT; ++u) w[b][u] = wn[b][u];
+            }
+        }
+        multiply(k, x, w);
+    }
+#pragma unroll
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[16 * u + 4 * g + i][n] = acc[u][i];
+}
+
+// Parts of v: the columns of one part of K, of a tile's rows with the
+// workgroup's adapters. RT: tiles of 16 ranks at most. The first round's
+// activations, which need no id, are loaded before the ids are known.
+template <int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, RT == 8 ? 2 : 4) void lora_shrink_kernel(const LoraParams p) {
+    constexpr int U = RT <= 2 ? 2 : 1;
+    __shared__ float part[WAVES][RT * 16][kTile + 1];
     prefetch_params(p);
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = blockIdx.x * kTile + n;
     const int id = t < p.T ? p.ids[t] : -1;
-    uint32_t todo = leaders(id);
-    for (int i = 0; i < (int) blockIdx.y && todo; ++i) todo &= todo - 1;
-    const int k0 = blockIdx.z * p.k_step, k1 = min(k0 + p.k_step, p.K);
+    const Columns c = Columns::of<U>(p, blockIdx.z, blockIdx.x, wave, WAVES);
     const char * xr = p.x + (int64_t) min(t, p.T - 1) * p.x_nb1;
-    while (todo) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
-        for (int i = 0; i < kSlots && todo; ++i) todo &= todo - 1;
-        const int rank = rank_of(p, a);
+    float4 x[U][2];
+    load_x<U>(xr, c.column<U>(), c.k1, g, x);
+    asm volatile("" ::: "memory");
+    const int row_rank = id >= 0 ? rank_of(p, id) : 0;                 // every row's at once, not adapter by adapter
+    const float row_scale = p.scales && row_rank > 0 ? p.scales[id] : 1.0f;
+    Turn turn{leaders(id)};
+    turn.skip(blockIdx.y);
+    for (bool again = false; turn.todo; turn.skip(p.slots), again = true) {
+        const int lead = __builtin_ctz(turn.todo);
+        const int a = __builtin_amdgcn_readlane(id, lead), rank = __builtin_amdgcn_readlane(row_rank, lead);
         if (rank < 0) {
             if (threadIdx.x == 0) lora_error(p, a);
             continue;
         }
         if (rank == 0) continue;
+        if (again && c.rounds != 1) load_x<U>(xr, c.column<U>(), c.k1, g, x);   // one round: x is still there
         const char * ar = p.a + (int64_t) a * p.a_nb2;
-        floatx4 acc[RT];
-#pragma unroll
-        for (int u = 0; u < RT; ++u) acc[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = k0 + 32 * wave; k < k1; k += 32 * kWaves) {
-            const int kl = k + 8 * g;
-            const bool in = kl < p.K;                                  // K is a multiple of 8
-            const int kc = in ? kl : 0;
-            float4 x0 = *(const float4 *) (xr + (int64_t) kc * 4), x1 = *(const float4 *) (xr + (int64_t) kc * 4 + 16);
-            if (!in) x0 = x1 = float4{0.0f, 0.0f, 0.0f, 0.0f};
-            const float xs[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-            for (int u = 0; u < RT; ++u) {
-                if (16 * u >= rank) break;
-                half8 w = *(const half8 *) (ar + (int64_t) min(16 * u + n, rank - 1) * p.a_nb1 + (int64_t) kc * 2);
-                if (!in) w = half8{};
-#pragma unroll
-                for (int s = 0; s < 8; ++s) acc[u] = mfma_f32((float) w[s], xs[s], acc[u]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < RT; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[wave][16 * u + 4 * g + i][n] = acc[u][i];
+        if (RT >= 8 && rank > 64)      shrink<min_c(RT, 8), U>(p, ar, rank, xr, x, c, n, g, part[wave]);
+        else if (RT >= 4 && rank > 32) shrink<min_c(RT, 4), U>(p, ar, rank, xr, x, c, n, g, part[wave]);
+        else if (RT >= 2 && rank > 16) shrink<min_c(RT, 2), U>(p, ar, rank, xr, x, c, n, g, part[wave]);
+        else                           shrink<1, U>(p, ar, rank, xr, x, c, n, g, part[wave]);
         __syncthreads();
-        const float scale = p.scales ? p.scales[a] : 1.0f;
-        for (int i = threadIdx.x; i < kTile * p.R; i += 64 * kWaves) {
-            const int tok = i / p.R, j = i - tok * p.R;
-            const int row = blockIdx.x * kTile + tok;
-            if (row >= p.T || p.ids[row] != a) continue;
+        const float scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(row_scale), lead));
+        const uint32_t rows = (uint32_t) __ballot(id == a) & 0xffffu;
+        for (int i = threadIdx.x; i < kTile * RT * 16; i += 64 * WAVES) {
+            const int tok = i / (RT * 16), j = i % (RT * 16);
+            if (j >= rank || !(rows >> tok & 1)) continue;
             float v = 0.0f;
-            if (j < rank) {
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) v += part[w][j][tok];
-                v *= scale;
-            }
-            p.v[((int64_t) blockIdx.z * p.T + row) * p.R + j] = v;
+            for (int w = 0; w < WAVES; ++w) v += part[w][j][tok];
+            p.v[((int64_t) blockIdx.z * p.T + blockIdx.x * kTile + tok) * p.R + j] = v * scale;
         }
         __syncthreads();
     }
 }
 
-// Outputs n0 .. n0 + 255 of a tile's rows. Lane 16 g + n holds outputs 4 g ..
-// 4 g + 3 of each 16, of row n.
-template <int RT>
+// p.chunks slices of 256 outputs of those of a tile's rows that have one of
+// the workgroup's adapters (slot 0: and of those that have none). Lane 16 g + n
+// holds outputs 4 g .. 4 g + 3 of each 16, of row n. The slices of a row come
+// next to one another in the grid, so that workgroups that run together use
+// all memory channels. VEC: rows of y and base in whole 16 bytes; SPLIT: v in
+// parts.
+template <int RT, bool VEC, bool SPLIT>
 __global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraParams p) {
     constexpr int kRow = RT * 16 + 4;
+    constexpr int kPiece = RT == 1 ? 16 : 32;                          // ranks of a lane's load of B: 4 or 8 in each quarter
+    constexpr int kSteps = kPiece / 4;
+    constexpr int kPieces = RT * 16 / kPiece;
+    typedef _Float16 piece __attribute__((ext_vector_type(kSteps)));
+    typedef short bits __attribute__((ext_vector_type(kSteps)));
     __shared__ __attribute__((aligned(16))) float v[kTile][kRow];
     prefetch_params(p);
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = blockIdx.x * kTile + n;
+    const int tile = blockIdx.y, slot = blockIdx.z;
+    const int row = tile * kTile + n;
     const int id = row < p.T ? p.ids[row] : -1;
-    const int n0 = blockIdx.y * kCols + 64 * wave;
-
-    floatx4 acc[4];
-    const char * br = p.base + (int64_t) min(row, p.T - 1) * p.base_nb1;
+    const int n0 = blockIdx.x * p.chunks * kCols + 64 * wave, n1 = min(n0 + p.chunks * kCols, p.N);
+    const char * br = p.base + (int64_t) min(row, p.T - 1) * p.base_nb1 + 16 * g;
+    char * yr = p.y + (int64_t) min(row, p.T - 1) * p.y_nb1 + 16 * g;
+    auto load = [&](const int c0, floatx4 (&x)[4]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int c = n0 + 16 * u + 4 * g;
-        if (p.y_vec) {
-            acc[u] = *(const floatx4 *) (br + (int64_t) min(c, p.N - 4) * 4);
-        } else {
+        for (int u = 0; u < 4; ++u) {
+            const int c = c0 + 16 * u + 4 * g;
+            if constexpr (VEC) {
+                if (c < p.N) x[u] = *(const floatx4 *) (br + (int64_t) (c0 + 16 * u) * 4);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[u][i] = *(const float *) (br + (int64_t) min(c + i, p.N - 1) * 4);
-        }
-    }
-    // v, its parts summed in order; zeros for rows without an adapter
-    for (int i = threadIdx.x; i < kTile * RT * 16; i += 64 * kWaves) {
-        const int tok = i / (RT * 16), j = i - tok * (RT * 16);
-        const int r = blockIdx.x * kTile + tok;
-        float s = 0.0f;
-        const int a = r < p.T ? p.ids[r] : -1;
-        const int rank = a >= 0 ? rank_of(p, a) : 0;
-        if (j < rank)
-            for (int k = 0; k < p.ks; ++k) s += p.v[((int64_t) k * p.T + r) * p.R + j];
-        v[tok][j] = s;
-    }
-    __syncthreads();
-
-    uint32_t todo = leaders(id);
-    while (todo) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
-        todo &= todo - 1;
-        const int rank = rank_of(p, a);
-        const bool mine = id == a;
-        if (rank < 0) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (mine) acc[u] = floatx4{1.0f, 1.0f, 1.0f, 1.0f} * __builtin_nanf("");
-            continue;
-        }
-        const char * b = p.b + (int64_t) a * p.b_nb2 + 8 * g;
-        floatx4 sum[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) sum[u] = acc[u];
-#pragma unroll
-        for (int q = 0; q < RT; ++q) {
-            if (16 * q >= rank) break;
-            const float4 x = *(const float4 *) &v[n][16 * q + 4 * g];
-            const float xs[4] = {x.x, x.y, x.z, x.w};
-            const int j0 = 16 * q + 4 * g;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int c = min(n0 + 16 * u + n, p.N - 1);
-                half4 w = j0 < p.R ? *(const half4 *) (b + (int64_t) c * p.b_nb1 + 32 * q) : half4{};
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    sum[u] = mfma_f32(j0 + s < rank ? (float) w[s] : 0.0f, xs[s], sum[u]);
+                for (int i = 0; i < 4; ++i)
+                    if (c + i < p.N) x[u][i] = *(const float *) (br + (int64_t) (c0 + 16 * u + i) * 4);
             }
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (mine) acc[u] = sum[u];
+    };
+    // the rows' ranks, and which of them are this workgroup's
+    const int rank = id >= 0 ? rank_of(p, id) : 0;
+    Turn turn{leaders(id)};
+    turn.skip(slot);
+    uint32_t mine = 0, turns = 0;
+    for (; turn.todo; turn.skip(p.slots)) {
+        const int l = __builtin_ctz(turn.todo);
+        turns |= 1u << l;
+        mine |= (uint32_t) __ballot(id == __builtin_amdgcn_readlane(id, l));
     }
-    if (row >= p.T) return;
-    char * yr = p.y + (int64_t) row * p.y_nb1;
+    if (slot == 0 && p.copy) mine |= (uint32_t) __ballot(id < 0 && row < p.T);
+    mine &= 0xffffu;
+    if (!mine) return;
+    const bool own = mine >> n & 1;
+    floatx4 acc[4], next[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int c = n0 + 16 * u + 4 * g;
-        if (p.y_vec) {
-            if (c < p.N) *(floatx4 *) (yr + (int64_t) c * 4) = acc[u];
-        } else {
+    for (int u = 0; u < 4; ++u) next[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (own) load(n0, next);
+    // v, its parts summed in order; zeros beyond the ranks
+    for (int i = threadIdx.x; i < kTile * RT * 4; i += 64 * kWaves) {
+        const int tok = i / (RT * 4), j = 4 * (i - tok * (RT * 4));
+        const int r = __shfl(rank, tok);
+        float4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (j < r && (mine >> tok & 1)) {
+            const float * src = p.v + ((int64_t) tile * kTile + tok) * p.R + j;
+            if constexpr (SPLIT) {
+                const int64_t part = (int64_t) p.T * p.R;
+                float4 x[kParts];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < p.N) *(float *) (yr + (int64_t) (c + i) * 4) = acc[u][i];
+                for (int k = 0; k < kParts; ++k) x[k] = *(const float4 *) (src + min(k, p.ks - 1) * part);
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int k = 0; k < kParts; ++k)
+                    if (k < p.ks) {
+                        s.x += x[k].x; s.y += x[k].y; s.z += x[k].z; s.w += x[k].w;
+                    }
+            } else {
+                s = *(const float4 *) src;
+            }
+            if (j + 1 >= r) s.y = 0.0f;
+            if (j + 2 >= r) s.z = 0.0f;
+            if (j + 3 >= r) s.w = 0.0f;
         }
+        *(float4 *) &v[tok][j] = s;
+    }
+    __syncthreads();
+    // this lane's ranks of row n, as the products' operands
+    piece hi[kPieces], lo[kPieces];
+    float up, down, top = 0.0f;
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) top = fmaxf(top, fabsf(v[n][q * kPiece + kSteps * g + s]));
+    row_scale(top, up, down);
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const float z = v[n][q * kPiece + kSteps * g + s] * up;
+            hi[q][s] = (_Float16) z;
+            lo[q][s] = (_Float16) (z - (float) hi[q][s]);
+        }
+
+    for (int c0 = n0; c0 < n1; c0 += kCols) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] = next[u];
+        if (own && c0 + kCols < n1) load(c0 + kCols, next);
+        for (uint32_t todo = turns; todo; todo &= todo - 1) {
+            const int l = __builtin_ctz(todo);
+            const int a = __builtin_amdgcn_readlane(id, l), r = __builtin_amdgcn_readlane(rank, l);
+            const char * b = p.b + (int64_t) a * p.b_nb2;
+            floatx4 sum[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q) {
+                if (q * kPiece >= r) break;
+                const int j0 = q * kPiece + kSteps * g;                // this lane's ranks
+                piece w[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    w[u] = *(const piece *) (b + (int64_t) min(c0 + 16 * u + n, p.N - 1) * p.b_nb1 + 2 * min(j0, p.R - kSteps));
+                if (q * kPiece + kPiece > r) {                         // what lies behind the rank may be NaN
+                    bits in;
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) in[s] = j0 + s < r ? -1 : 0;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) w[u] = __builtin_bit_cast(piece, __builtin_bit_cast(bits, w[u]) & in);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if constexpr (kSteps == 4) {
+                        sum[u] = __builtin_amdgcn_mfma_f32_16x16x16f16(w[u], lo[q], sum[u], 0, 0, 0);
+                        sum[u] = __builtin_amdgcn_mfma_f32_16x16x16f16(w[u], hi[q], sum[u], 0, 0, 0);
+                    } else {
+                        sum[u] = mfma_16x16x32(w[u], hi[q], mfma_16x16x32(w[u], lo[q], sum[u]));
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum[u] = acc[u] + sum[u] * down;
+            if (r < 0)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) sum[u] = floatx4{1.0f, 1.0f, 1.0f, 1.0f} * __builtin_nanf("");
+            if (id == a)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) acc[u] = sum[u];
+        }
+        if (own)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int c = c0 + 16 * u + 4 * g;
+                if constexpr (VEC) {
+                    if (c < p.N) *(floatx4 *) (yr + (int64_t) (c0 + 16 * u) * 4) = acc[u];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + i < p.N) *(float *) (yr + (int64_t) (c0 + 16 * u + i) * 4) = acc[u][i];
+                }
+            }
     }
 }
 
@@ -258,7 +457,7 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
                        (long long) K, (long long) x.ne[0], (long long) R, (long long) b.ne[0]);
     if (K < 8 || K % 8 || K > 65536 || R < 8 || R % 8 || R > kMaxR)
         return al_fail(AL_ERR_UNSUPPORTED, "lora: K %lld, R %lld (multiples of 8, at most 65536 and %d)", (long long) K, (long long) R, kMaxR);
-    if (A < 1 || A > (1 << 20) || N < 1 || N > (1 << 22) || T < 0 || T > (1 << 20))
+    if (A < 1 || A > (1 << 20) || N < 1 || N > (1 << 22) || T < 0 || T > (1 << 19))
         return al_fail(AL_ERR_UNSUPPORTED, "lora: sizes out of range");
     auto al = [](const al_tensor & t, uint64_t by) { return !(((uintptr_t) t.data | t.nb[1] | t.nb[2]) & (by - 1)); };
     if (a.nb[0] != 2 || b.nb[0] != 2 || !al(a, 16) || !al(b, 16))
@@ -296,8 +495,13 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     p.K = (int32_t) K; p.N = (int32_t) N; p.R = (int32_t) R; p.T = (int32_t) T; p.n_adapters = (int32_t) A;
     p.y_vec = N % 4 == 0 && !(((uintptr_t) y.data | y.nb[1] | (uintptr_t) base.data | base.nb[1]) & 15u);
     const int64_t tiles = (T + kTile - 1) / kTile;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({16, (K + 255) / 256, n_cu / std::max<int64_t>(1, tiles)}));
-    p.k_step = (int32_t) (((K + parts - 1) / parts + 127) / 128 * 128);
+    // few tiles: every adapter of a tile in a workgroup of its own, and K in
+    // parts of at least 512 columns
+    p.slots = tiles <= 4 ? kTile : tiles <= 64 ? 4 : 1;
+    p.copy = base.data != y.data;
+    p.chunks = 1;
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kParts, (K + 511) / 512, n_cu / std::max<int64_t>(1, 2 * tiles)}));
+    p.k_step = (int32_t) (((K + parts - 1) / parts + 31) / 32 * 32);
     p.ks = (int32_t) ((K + p.k_step - 1) / p.k_step);
     pl.v_bytes = ((size_t) p.ks * T * R * 4 + 255) / 256 * 256;
     if (project) {
@@ -310,11 +514,15 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
 
 template <int RT>
 hipError_t launch(const LoraParams & p, hipStream_t st) {
+    constexpr int kShrinkWaves = RT == 8 ? 4 : 8;                      // (LDS: the waves' parts)
     const unsigned tiles = (unsigned) ((p.T + kTile - 1) / kTile);
-    hipLaunchKernelGGL(lora_shrink_kernel<RT>, dim3(tiles, kSlots, (unsigned) p.ks), dim3(64 * kWaves), 0, st, p);
+    hipLaunchKernelGGL((lora_shrink_kernel<RT, kShrinkWaves>), dim3(tiles, (unsigned) p.slots, (unsigned) p.ks), dim3(64 * kShrinkWaves), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(lora_expand_kernel<RT>, dim3(tiles, (unsigned) ((p.N + kCols - 1) / kCols)), dim3(64 * kWaves), 0, st, p);
+    const dim3 grid((unsigned) ((p.N + kCols * p.chunks - 1) / (kCols * p.chunks)), tiles, (unsigned) p.slots);
+    if (p.y_vec && p.ks > 1) hipLaunchKernelGGL((lora_expand_kernel<RT, true, true>), grid, dim3(64 * kWaves), 0, st, p);
+    else if (p.y_vec)        hipLaunchKernelGGL((lora_expand_kernel<RT, true, false>), grid, dim3(64 * kWaves), 0, st, p);
+    else                     hipLaunchKernelGGL((lora_expand_kernel<RT, false, true>), grid, dim3(64 * kWaves), 0, st, p);
     return hipGetLastError();
 }
 
