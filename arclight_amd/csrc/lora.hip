@@ -26,62 +26,16 @@
 #include "../../include/arclight_lora.h"
 #include "device_common.hpp"
 #include "kernel_args.hpp"
+#include "lora.hpp"
 #include "matmul_q4.hpp"
 #include "runtime.hpp"
 
 namespace {
 
+using namespace lora;
+
 constexpr int kWaves = 4;
-constexpr int kTile = 16;                       // rows of x
-constexpr int kMaxR = 128;
-constexpr int kParts = 8;                       // parts of K at most
 constexpr int kCols = 256;                      // outputs of a workgroup
-
-
-struct LoraParams {
-    const char * a;  int64_t a_nb1, a_nb2;      // rank row, adapter
-    const char * b;  int64_t b_nb1, b_nb2;      // output, adapter
-    const int32_t * ranks;                      // or null
-    const float * scales;                       // or null
-    const int32_t * ids;
-    const char * x;     int64_t x_nb1;
-    const char * base;  int64_t base_nb1;
-    char * y;           int64_t y_nb1;
-    float * v;                                  // [ks][T][R]
-    int32_t K, N, R, T, n_adapters;
-    int32_t ks, k_step;                         // parts of K, columns of one (a multiple of 32)
-    int32_t chunks;                             // slices of kCols outputs of a workgroup
-    int32_t slots;                              // workgroups that share a tile's adapters
-    int32_t copy;                               // base is not y: rows without an adapter are copied
-    int32_t y_vec;                              // y and base rows 16-byte aligned, N a multiple of 4
-    int * err;
-};
-
-constexpr int min_c(int a, int b) { return a < b ? a : b; }
-
-// Power of two that brings a row's largest value to [2^11, 2^12), and its
-// inverse. top: the largest size of this lane's values, the row in the 4 lanes
-// {n, n + 16, n + 32, n + 48}.
-__device__ __forceinline__ void row_scale(float top, float & up, float & down) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_int(top), __float_as_int(top), false, false);
-    top = fmaxf(__int_as_float((int) a[0]), __int_as_float((int) a[1]));
-    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_int(top), __float_as_int(top), false, false);
-    top = fmaxf(__int_as_float((int) b[0]), __int_as_float((int) b[1]));
-    const int ex = min(max((int) (__float_as_uint(top) >> 23), 12), 253) - 127;
-    up = __uint_as_float((uint32_t) (11 - ex + 127) << 23);
-    down = __uint_as_float((uint32_t) (ex - 11 + 127) << 23);
-}
-
-// Rank of adapter a, -1 for one that is not to be used.
-__device__ __forceinline__ int rank_of(const LoraParams & p, const int a) {
-    if (a >= p.n_adapters) return -1;
-    const int r = p.ranks ? p.ranks[a] : p.R;
-    return r < 0 || r > p.R ? -1 : r;
-}
-
-__device__ __forceinline__ void lora_error(const LoraParams & p, const int a) {
-    if (atomicCAS(p.err + 8, 0, 1) == 0) p.err[9] = a;
-}
 
 // The rows of a tile whose adapter no earlier row of it has, of a wave whose
 // lanes hold row lane % 16's id (negative: none): one bit each.
@@ -104,132 +58,20 @@ struct Turn {
     }
 };
 
-// The columns of a wave: rounds of 32 U from k0 to k1, beginning with another
-// round in every tile. Rows of x are often a power of two apart, and so the
-// same columns of all rows in the same few memory channels: waves that take
-// ranges apart from one another, and tiles that begin apart, use them all.
-struct Columns {
-    int k0, k1, rounds, at;
-    template <int U> __device__ __forceinline__ static Columns of(const LoraParams & p, const int part, const int tile, const int wave,
-                                                                  const int waves) {
-        const int a = part * p.k_step, b = min(a + p.k_step, p.K), own = (p.k_step / 32 + waves - 1) / waves * 32;
-        Columns c;
-        c.k0 = min(a + wave * own, b);
-        c.k1 = min(c.k0 + own, b);
-        c.rounds = (c.k1 - c.k0 + 32 * U - 1) / (32 * U);
-        c.at = c.rounds > 1 ? tile % c.rounds : 0;
-        return c;
-    }
-    template <int U> __device__ __forceinline__ int column() const { return k0 + at * 32 * U; }
-    __device__ __forceinline__ void next() { at = at + 1 == rounds ? 0 : at + 1; }
-};
-
-// This lane's columns of U runs of 32 from k on; column 0 for those
-// beyond k1, which shrink() zeroes.
-template <int U>
-__device__ __forceinline__ void load_x(const char * xr, const int k, const int k1, const int g, float4 (&x)[U][2]) {
-#pragma unroll
-    for (int b = 0; b < U; ++b) {
-        const int kl = k + 32 * b + 8 * g;                             // K is a multiple of 8
-        const float4 * at = (const float4 *) (xr + (int64_t) (kl < k1 ? kl : 0) * 4);
-        x[b][0] = at[0];
-        x[b][1] = at[1];
-    }
+// Parts of v for at most 64 rows: (row, part of K) for each workgroup.
+template <int RT>
+__global__ __launch_bounds__(64 * shrink_waves<RT>(), RT == 8 ? 2 : 4) void lora_shrink_few_kernel(const LoraParams p) {
+    __shared__ float part[shrink_waves<RT>()][RT * 16][kTile + 1];
+    prefetch_params(p);
+    shrink_few<RT, shrink_waves<RT>()>(p, blockIdx.x, blockIdx.y, part);
 }
 
-// Sum of A's rows with the tile's rows over a wave's columns, RT tiles of 16
-// ranks. Lane 16 g + n loads 8 columns of rank row n and of row n of x (8 g ..
-// 8 g + 7 of each 32). x holds the first round's activations. The next round's loads go out before this round's
-// products (the asm statements keep the compiler from sinking them to their
-// uses): without that all waves of a launch load and compute in step.
-template <int RT, int U>
-__device__ __forceinline__ void shrink(const LoraParams & p, const char * ar, const int rank, const char * xr, float4 (&x)[U][2],
-                                       Columns c, const int n, const int g, float (*part)[kTile + 1]) {
-    floatx4 acc[RT];
-#pragma unroll
-    for (int u = 0; u < RT; ++u) acc[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    const char * rows[RT];
-#pragma unroll
-    for (int u = 0; u < RT; ++u) rows[u] = ar + (int64_t) min(16 * u + n, rank - 1) * p.a_nb1;
-    auto load_w = [&](const int k, half8 (&w)[U][RT]) {
-#pragma unroll
-        for (int b = 0; b < U; ++b) {
-            const int kl = k + 32 * b + 8 * g;
-#pragma unroll
-            for (int u = 0; u < RT; ++u) w[b][u] = *(const half8 *) (rows[u] + (int64_t) (kl < c.k1 ? kl : 0) * 2);
-        }
-        asm volatile("" ::: "memory");
-    };
-    auto multiply = [&](const int k, float4 (&y)[U][2], half8 (&w)[U][RT]) {
-        if (k + 32 * U > c.k1) {
-#pragma unroll
-            for (int b = 0; b < U; ++b)
-                if (k + 32 * b + 8 * g >= c.k1) {
-                    y[b][0] = y[b][1] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int u = 0; u < RT; ++u) w[b][u] = half8{};
-                }
-        }
-        float top = 0.0f, up, down;
-#pragma unroll
-        for (int b = 0; b < U; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                top = fmaxf(fmaxf(fmaxf(top, fabsf(y[b][h].x)), fmaxf(fabsf(y[b][h].y), fabsf(y[b][h].z))), fabsf(y[b][h].w));
-        row_scale(top, up, down);
-        floatx4 sum[RT];
-#pragma unroll
-        for (int u = 0; u < RT; ++u) sum[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int b = 0; b < U; ++b) {
-            const float xs[8] = {y[b][0].x, y[b][0].y, y[b][0].z, y[b][0].w, y[b][1].x, y[b][1].y, y[b][1].z, y[b][1].w};
-            half8 hi, lo;
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const float z = xs[s] * up;
-                hi[s] = (_Float16) z;
-                lo[s] = (_Float16) (z - (float) hi[s]);
-            }
-#pragma unroll
-            for (int u = 0; u < RT; ++u) sum[u] = mfma_16x16x32(w[b][u], hi, mfma_16x16x32(w[b][u], lo, sum[u]));
-        }
-#pragma unroll
-        for (int u = 0; u < RT; ++u) acc[u] += sum[u] * down;
-    };
-    if (c.rounds > 0) {
-        int k = c.column<U>();
-        half8 w[U][RT];
-        load_w(k, w);
-        for (int i = 1; i < c.rounds; ++i) {
-            c.next();
-            const int kn = c.column<U>();
-            float4 xn[U][2];
-            half8 wn[U][RT];
-            load_x<U>(xr, kn, c.k1, g, xn);
-            load_w(kn, wn);
-            multiply(k, x, w);
-            k = kn;
-#pragma unroll
-            for (int b = 0; b < U; ++b) {
-                x[b][0] = xn[b][0];
-                x[b][1] = xn[b][1];
-#pragma unroll
-                for (int u = 0; u < RT; ++u) w[b][u] = wn[b][u];
-            }
-        }
-        multiply(k, x, w);
-    }
-#pragma unroll
-    for (int u = 0; u < RT; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[16 * u + 4 * g + i][n] = acc[u][i];
-}
-
-// Parts of v: the columns of one part of K, of a tile's rows with the
+// Parts of v for more: the columns of one part of K, of a tile's rows with the
 // workgroup's adapters. RT: tiles of 16 ranks at most. The first round's
 // activations, which need no id, are loaded before the ids are known.
-template <int RT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, RT == 8 ? 2 : 4) void lora_shrink_kernel(const LoraParams p) {
+template <int RT>
+__global__ __launch_bounds__(64 * shrink_waves<RT>(), RT == 8 ? 2 : 4) void lora_shrink_kernel(const LoraParams p) {
+    constexpr int WAVES = shrink_waves<RT>();
     constexpr int U = RT <= 2 ? 2 : 1;
     __shared__ float part[WAVES][RT * 16][kTile + 1];
     prefetch_params(p);
@@ -275,13 +117,17 @@ __global__ __launch_bounds__(64 * WAVES, RT == 8 ? 2 : 4) void lora_shrink_kerne
     }
 }
 
-// p.chunks slices of 256 outputs of those of a tile's rows that have one of
-// the workgroup's adapters (slot 0: and of those that have none). Lane 16 g + n
-// holds outputs 4 g .. 4 g + 3 of each 16, of row n. The slices of a row come
-// next to one another in the grid, so that workgroups that run together use
-// all memory channels. VEC: rows of y and base in whole 16 bytes; SPLIT: v in
-// parts.
-template <int RT, bool VEC, bool SPLIT>
+// A slice of 256 outputs of rows that share a workgroup: with at most 64 rows
+// (FEW) those of row `blockIdx.y`'s adapter, if it is their first; with more
+// those of a tile that have one of the workgroup's adapters. Rows without an
+// adapter are copied where base is not y: by their own workgroup, or by the
+// tile's slot 0. Lane 16 g + n holds outputs 4 g .. 4 g + 3 of each 16, of row
+// n. The slices of a row come next to one another in the grid, so that
+// workgroups that run together use all memory channels. VEC: rows of y and
+// base in whole 16 bytes; SPLIT: v in parts.
+// Measured at 8000 rows of 4096 outputs, rank 16: 55 us, 4.8 TB/s, what a copy
+// reaches; with 1024 or more outputs to a workgroup 63 to 72.
+template <int RT, bool VEC, bool SPLIT, bool FEW>
 __global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraParams p) {
     constexpr int kRow = RT * 16 + 4;
     constexpr int kPiece = RT == 1 ? 16 : 32;                          // ranks of a lane's load of B: 4 or 8 in each quarter
@@ -293,92 +139,92 @@ __global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraPara
     prefetch_params(p);
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.y, slot = blockIdx.z;
-    const int row = tile * kTile + n;
-    const int id = row < p.T ? p.ids[row] : -1;
-    const int n0 = blockIdx.x * p.chunks * kCols + 64 * wave, n1 = min(n0 + p.chunks * kCols, p.N);
-    const char * br = p.base + (int64_t) min(row, p.T - 1) * p.base_nb1 + 16 * g;
-    char * yr = p.y + (int64_t) min(row, p.T - 1) * p.y_nb1 + 16 * g;
-    auto load = [&](const int c0, floatx4 (&x)[4]) {
+    const int c0 = blockIdx.x * kCols + 64 * wave;
+    // the columns' rows: which (row), whether they are this workgroup's
+    // (mine), their adapters and ranks, and the first column of each adapter
+    int row, id, rank;
+    uint32_t mine, turns;
+    uint64_t left = 0;
+    if constexpr (FEW) {
+        const int lead = blockIdx.y;
+        id = lane < p.T ? p.ids[lane] : -1;
+        const int a = __builtin_amdgcn_readlane(id, lead);
+        left = a >= 0 ? __ballot(id == a) : p.copy ? 1ull << lead : 0;
+        if (left == 0 || __builtin_ctzll(left) != lead) return;
+        id = a;
+        rank = a >= 0 ? rank_of(p, a) : 0;
+        turns = a >= 0 ? 1 : 0;
+    } else {
+        row = blockIdx.y * kTile + n;
+        id = row < p.T ? p.ids[row] : -1;
+        rank = id >= 0 ? rank_of(p, id) : 0;
+        Turn turn{leaders(id)};
+        turn.skip(blockIdx.z);
+        mine = turns = 0;
+        for (; turn.todo; turn.skip(p.slots)) {
+            const int l = __builtin_ctz(turn.todo);
+            turns |= 1u << l;
+            mine |= (uint32_t) __ballot(id == __builtin_amdgcn_readlane(id, l));
+        }
+        if (blockIdx.z == 0 && p.copy) mine |= (uint32_t) __ballot(id < 0 && row < p.T);
+        mine &= 0xffffu;
+        if (!mine) return;
+        row = min(row, p.T - 1);
+    }
+    do {
+        if constexpr (FEW) {
+            row = nth_row(left, n);
+            mine = (1u << min(__builtin_popcountll(left), kTile)) - 1;
+            left = without_16(left);
+        }
+        const bool own = mine >> n & 1;
+        const char * br = p.base + (int64_t) row * p.base_nb1 + 16 * g;
+        char * yr = p.y + (int64_t) row * p.y_nb1 + 16 * g;
+        floatx4 acc[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
+            acc[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             const int c = c0 + 16 * u + 4 * g;
             if constexpr (VEC) {
-                if (c < p.N) x[u] = *(const floatx4 *) (br + (int64_t) (c0 + 16 * u) * 4);
+                if (own && c < p.N) acc[u] = *(const floatx4 *) (br + (int64_t) (c0 + 16 * u) * 4);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (c + i < p.N) x[u][i] = *(const float *) (br + (int64_t) (c0 + 16 * u + i) * 4);
+                    if (own && c + i < p.N) acc[u][i] = *(const float *) (br + (int64_t) (c0 + 16 * u + i) * 4);
             }
         }
-    };
-    // the rows' ranks, and which of them are this workgroup's
-    const int rank = id >= 0 ? rank_of(p, id) : 0;
-    Turn turn{leaders(id)};
-    turn.skip(slot);
-    uint32_t mine = 0, turns = 0;
-    for (; turn.todo; turn.skip(p.slots)) {
-        const int l = __builtin_ctz(turn.todo);
-        turns |= 1u << l;
-        mine |= (uint32_t) __ballot(id == __builtin_amdgcn_readlane(id, l));
-    }
-    if (slot == 0 && p.copy) mine |= (uint32_t) __ballot(id < 0 && row < p.T);
-    mine &= 0xffffu;
-    if (!mine) return;
-    const bool own = mine >> n & 1;
-    floatx4 acc[4], next[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) next[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (own) load(n0, next);
-    // v, its parts summed in order; zeros beyond the ranks
-    for (int i = threadIdx.x; i < kTile * RT * 4; i += 64 * kWaves) {
-        const int tok = i / (RT * 4), j = 4 * (i - tok * (RT * 4));
-        const int r = __shfl(rank, tok);
-        float4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (j < r && (mine >> tok & 1)) {
-            const float * src = p.v + ((int64_t) tile * kTile + tok) * p.R + j;
-            if constexpr (SPLIT) {
-                const int64_t part = (int64_t) p.T * p.R;
-                float4 x[kParts];
-#pragma unroll
-                for (int k = 0; k < kParts; ++k) x[k] = *(const float4 *) (src + min(k, p.ks - 1) * part);
-                asm volatile("" ::: "memory");
-#pragma unroll
-                for (int k = 0; k < kParts; ++k)
-                    if (k < p.ks) {
-                        s.x += x[k].x; s.y += x[k].y; s.z += x[k].z; s.w += x[k].w;
-                    }
-            } else {
-                s = *(const float4 *) src;
+        // v, zeros beyond the ranks
+        for (int i = threadIdx.x; i < kTile * RT * 4; i += 64 * kWaves) {
+            const int tok = i / (RT * 4), j = 4 * (i - tok * (RT * 4));
+            const int r = __shfl(rank, tok), at = __shfl(row, tok);
+            float4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (j < r && (mine >> tok & 1)) {
+                if constexpr (SPLIT) s = sum_parts(p, at, j);
+                else s = *(const float4 *) (p.v + (int64_t) at * p.R + j);
+                if (j + 1 >= r) s.y = 0.0f;
+                if (j + 2 >= r) s.z = 0.0f;
+                if (j + 3 >= r) s.w = 0.0f;
             }
-            if (j + 1 >= r) s.y = 0.0f;
-            if (j + 2 >= r) s.z = 0.0f;
-            if (j + 3 >= r) s.w = 0.0f;
+            *(float4 *) &v[tok][j] = s;
         }
-        *(float4 *) &v[tok][j] = s;
-    }
-    __syncthreads();
-    // this lane's ranks of row n, as the products' operands
-    piece hi[kPieces], lo[kPieces];
-    float up, down, top = 0.0f;
+        __syncthreads();
+        // this lane's ranks of row n, as the products' operands
+        piece hi[kPieces], lo[kPieces];
+        float up, down, top = 0.0f;
 #pragma unroll
-    for (int q = 0; q < kPieces; ++q)
+        for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) top = fmaxf(top, fabsf(v[n][q * kPiece + kSteps * g + s]));
-    row_scale(top, up, down);
+            for (int s = 0; s < kSteps; ++s) top = fmaxf(top, fabsf(v[n][q * kPiece + kSteps * g + s]));
+        row_scale(top, up, down);
 #pragma unroll
-    for (int q = 0; q < kPieces; ++q)
+        for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const float z = v[n][q * kPiece + kSteps * g + s] * up;
-            hi[q][s] = (_Float16) z;
-            lo[q][s] = (_Float16) (z - (float) hi[q][s]);
-        }
+            for (int s = 0; s < kSteps; ++s) {
+                const float z = v[n][q * kPiece + kSteps * g + s] * up;
+                hi[q][s] = (_Float16) z;
+                lo[q][s] = (_Float16) (z - (float) hi[q][s]);
+            }
 
-    for (int c0 = n0; c0 < n1; c0 += kCols) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) acc[u] = next[u];
-        if (own && c0 + kCols < n1) load(c0 + kCols, next);
         for (uint32_t todo = turns; todo; todo &= todo - 1) {
             const int l = __builtin_ctz(todo);
             const int a = __builtin_amdgcn_readlane(id, l), r = __builtin_amdgcn_readlane(rank, l);
@@ -432,7 +278,8 @@ __global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraPara
                         if (c + i < p.N) *(float *) (yr + (int64_t) (c0 + 16 * u + i) * 4) = acc[u][i];
                 }
             }
-    }
+        if constexpr (FEW) __syncthreads();                                // v is read before the next rows' is written
+    } while (FEW && left);
 }
 
 struct Plan {
@@ -495,12 +342,14 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     p.K = (int32_t) K; p.N = (int32_t) N; p.R = (int32_t) R; p.T = (int32_t) T; p.n_adapters = (int32_t) A;
     p.y_vec = N % 4 == 0 && !(((uintptr_t) y.data | y.nb[1] | (uintptr_t) base.data | base.nb[1]) & 15u);
     const int64_t tiles = (T + kTile - 1) / kTile;
-    // few tiles: every adapter of a tile in a workgroup of its own, and K in
-    // parts of at least 512 columns
-    p.slots = tiles <= 4 ? kTile : tiles <= 64 ? 4 : 1;
+    // Up to 64 rows take a workgroup for each row, of which those of an
+    // adapter's first row work; more take tiles, whose adapters share 4
+    // workgroups up to 64 tiles, 1 beyond. K in parts of at least 512 columns
+    // while there are CUs for them.
+    p.slots = tiles <= 64 ? 4 : 1;
     p.copy = base.data != y.data;
-    p.chunks = 1;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kParts, (K + 511) / 512, n_cu / std::max<int64_t>(1, 2 * tiles)}));
+    const int64_t groups = T <= kFew ? 16 : 2 * tiles;
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kParts, (K + 511) / 512, n_cu / std::max<int64_t>(1, groups)}));
     p.k_step = (int32_t) (((K + parts - 1) / parts + 31) / 32 * 32);
     p.ks = (int32_t) ((K + p.k_step - 1) / p.k_step);
     pl.v_bytes = ((size_t) p.ks * T * R * 4 + 255) / 256 * 256;
@@ -512,18 +361,25 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     return AL_OK;
 }
 
+template <int RT, bool FEW>
+hipError_t launch_expand(const LoraParams & p, const dim3 grid, hipStream_t st) {
+    if (p.y_vec && p.ks > 1) hipLaunchKernelGGL((lora_expand_kernel<RT, true, true, FEW>), grid, dim3(64 * kWaves), 0, st, p);
+    else if (p.y_vec)        hipLaunchKernelGGL((lora_expand_kernel<RT, true, false, FEW>), grid, dim3(64 * kWaves), 0, st, p);
+    else                     hipLaunchKernelGGL((lora_expand_kernel<RT, false, true, FEW>), grid, dim3(64 * kWaves), 0, st, p);
+    return hipGetLastError();
+}
+
 template <int RT>
 hipError_t launch(const LoraParams & p, hipStream_t st) {
-    constexpr int kShrinkWaves = RT == 8 ? 4 : 8;                      // (LDS: the waves' parts)
-    const unsigned tiles = (unsigned) ((p.T + kTile - 1) / kTile);
-    hipLaunchKernelGGL((lora_shrink_kernel<RT, kShrinkWaves>), dim3(tiles, (unsigned) p.slots, (unsigned) p.ks), dim3(64 * kShrinkWaves), 0, st, p);
+    constexpr int kThreads = 64 * shrink_waves<RT>();
+    const unsigned tiles = (unsigned) ((p.T + kTile - 1) / kTile), slices = (unsigned) ((p.N + kCols - 1) / kCols);
+    const bool few = p.T <= kFew;
+    if (few) hipLaunchKernelGGL(lora_shrink_few_kernel<RT>, dim3((unsigned) p.T, (unsigned) p.ks), dim3(kThreads), 0, st, p);
+    else     hipLaunchKernelGGL(lora_shrink_kernel<RT>, dim3(tiles, (unsigned) p.slots, (unsigned) p.ks), dim3(kThreads), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned) ((p.N + kCols * p.chunks - 1) / (kCols * p.chunks)), tiles, (unsigned) p.slots);
-    if (p.y_vec && p.ks > 1) hipLaunchKernelGGL((lora_expand_kernel<RT, true, true>), grid, dim3(64 * kWaves), 0, st, p);
-    else if (p.y_vec)        hipLaunchKernelGGL((lora_expand_kernel<RT, true, false>), grid, dim3(64 * kWaves), 0, st, p);
-    else                     hipLaunchKernelGGL((lora_expand_kernel<RT, false, true>), grid, dim3(64 * kWaves), 0, st, p);
-    return hipGetLastError();
+    return few ? launch_expand<RT, true>(p, dim3(slices, (unsigned) p.T), st)
+               : launch_expand<RT, false>(p, dim3(slices, tiles, (unsigned) p.slots), st);
 }
 
 int run(const al_lora_args * g, bool project) {
