@@ -370,16 +370,19 @@ hipError_t launch_expand(const LoraParams & p, const dim3 grid, hipStream_t st) 
 }
 
 template <int RT>
-hipError_t launch(const LoraParams & p, hipStream_t st) {
+hipError_t launch_shrink(const LoraParams & p, hipStream_t st) {
     constexpr int kThreads = 64 * shrink_waves<RT>();
+    const unsigned tiles = (unsigned) ((p.T + kTile - 1) / kTile);
+    if (p.T <= kFew) hipLaunchKernelGGL(lora_shrink_few_kernel<RT>, dim3((unsigned) p.T, (unsigned) p.ks), dim3(kThreads), 0, st, p);
+    else             hipLaunchKernelGGL(lora_shrink_kernel<RT>, dim3(tiles, (unsigned) p.slots, (unsigned) p.ks), dim3(kThreads), 0, st, p);
+    return hipGetLastError();
+}
+
+template <int RT>
+hipError_t launch_expand(const LoraParams & p, hipStream_t st) {
     const unsigned tiles = (unsigned) ((p.T + kTile - 1) / kTile), slices = (unsigned) ((p.N + kCols - 1) / kCols);
-    const bool few = p.T <= kFew;
-    if (few) hipLaunchKernelGGL(lora_shrink_few_kernel<RT>, dim3((unsigned) p.T, (unsigned) p.ks), dim3(kThreads), 0, st, p);
-    else     hipLaunchKernelGGL(lora_shrink_kernel<RT>, dim3(tiles, (unsigned) p.slots, (unsigned) p.ks), dim3(kThreads), 0, st, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    return few ? launch_expand<RT, true>(p, dim3(slices, (unsigned) p.T), st)
-               : launch_expand<RT, false>(p, dim3(slices, tiles, (unsigned) p.slots), st);
+    return p.T <= kFew ? launch_expand<RT, true>(p, dim3(slices, (unsigned) p.T), st)
+                       : launch_expand<RT, false>(p, dim3(slices, tiles, (unsigned) p.slots), st);
 }
 
 int run(const al_lora_args * g, bool project) {
@@ -402,16 +405,18 @@ int run(const al_lora_args * g, bool project) {
         if (rc != AL_OK) return rc;
     }
     pl.p.v = (float *) ws;
-    if (project) {
-        rc = mul_mat_q4_0_run(&g->w, &g->x, &g->y, (char *) ws + pl.v_bytes, (hipStream_t) g->stream);
-        if (rc != AL_OK) return rc;
-    }
-    hipError_t e;
     const hipStream_t st = (hipStream_t) g->stream;
-    if (pl.p.R <= 16) e = launch<1>(pl.p, st);
-    else if (pl.p.R <= 32) e = launch<2>(pl.p, st);
-    else if (pl.p.R <= 64) e = launch<4>(pl.p, st);
-    else e = launch<8>(pl.p, st);
+    const LoraParams & p = pl.p;
+    const bool fused = project && mul_mat_q4_0_takes_lora(&g->w, p.T, p.R);
+    hipError_t e = hipSuccess;
+    if (!(fused && mul_mat_q4_0_shrinks(p.T)))
+        e = p.R <= 16 ? launch_shrink<1>(p, st) : p.R <= 32 ? launch_shrink<2>(p, st) : p.R <= 64 ? launch_shrink<4>(p, st) : launch_shrink<8>(p, st);
+    if (e != hipSuccess) return al_hip_fail(e, "lora: launch");
+    if (project) {
+        rc = mul_mat_q4_0_run(&g->w, &g->x, &g->y, fused ? &p : nullptr, (char *) ws + pl.v_bytes, st);
+        if (rc != AL_OK || fused) return rc;
+    }
+    e = p.R <= 16 ? launch_expand<1>(p, st) : p.R <= 32 ? launch_expand<2>(p, st) : p.R <= 64 ? launch_expand<4>(p, st) : launch_expand<8>(p, st);
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "lora: launch");
 }
 

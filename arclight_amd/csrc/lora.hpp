@@ -240,21 +240,28 @@ __device__ __forceinline__ void shrink_few(const LoraParams & p, const int lead,
 // Waves of a workgroup that computes parts of v (RT 8: its LDS).
 template <int RT> constexpr int shrink_waves() { return RT == 8 ? 4 : 8; }
 
-// v of ranks j .. j + 3 of a row: its parts summed in order. Ranks that the
-// row's adapter does not have were never written and are anything.
-__device__ __forceinline__ float4 sum_parts(const LoraParams & p, const int row, const int j) {
+// v of ranks j .. j + 3 of a row: its parts, and their sum in order. Ranks that
+// the row's adapter does not have were never written and are anything.
+__device__ __forceinline__ void load_parts(const LoraParams & p, const int row, const int j, float4 (&x)[kParts]) {
     const float * src = p.v + (int64_t) row * p.R + j;
     const int64_t part = (int64_t) p.T * p.R;
-    float4 x[kParts], s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < kParts; ++k) x[k] = *(const float4 *) (src + min(k, p.ks - 1) * part);
-    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ float4 sum_of(const LoraParams & p, const float4 (&x)[kParts]) {
+    float4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < kParts; ++k)
         if (k < p.ks) {
             s.x += x[k].x; s.y += x[k].y; s.z += x[k].z; s.w += x[k].w;
         }
     return s;
+}
+__device__ __forceinline__ float4 sum_parts(const LoraParams & p, const int row, const int j) {
+    float4 x[kParts];
+    load_parts(p, row, j, x);
+    asm volatile("" ::: "memory");
+    return sum_of(p, x);
 }
 
 // 8 ranks' share of an output: b . v over those below the rank.

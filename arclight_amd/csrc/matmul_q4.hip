@@ -32,6 +32,7 @@
 
 #include "../../include/arclight_matmul.h"
 #include "kernel_args.hpp"
+#include "lora.hpp"
 #include "matmul_q4.hpp"
 #include "runtime.hpp"
 
@@ -108,11 +109,9 @@ constexpr int kGemmWaves = 8;                    // waves of a workgroup, each w
 // lines; the block scales (f16, as the format stores them) as
 // [tile][block][token]. Tokens past T are zeros.
 // Latency-bound (one load round; reads are whole 128-byte lines per token).
-__global__ __launch_bounds__(256) void quantize_q8_kernel(const char * __restrict__ x, int64_t x_nb1, int nb, int T,
-                                                          int n_items, uint4 * __restrict__ frag, _Float16 * __restrict__ dx) {
+__device__ __forceinline__ void quantize_q8(const char * __restrict__ x, int64_t x_nb1, int nb, int T, const int item,
+                                            uint4 * __restrict__ frag, _Float16 * __restrict__ dx) {
     const int lane = threadIdx.x & 63;
-    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= n_items) return;
     const int tile = item / (nb / 2), pair = item - tile * (nb / 2);
     const int g = lane >> 4, tok = tile * kTile + (lane & 15);
     float4 f[2][2] = {};
@@ -149,6 +148,29 @@ __global__ __launch_bounds__(256) void quantize_q8_kernel(const char * __restric
     if (g < 2) dx[((int64_t) tile * nb + 2 * pair + g) * kTile + (lane & 15)] = (_Float16) (g ? d[1] : d[0]);
 }
 
+__global__ __launch_bounds__(256) void quantize_q8_kernel(const char * __restrict__ x, int64_t x_nb1, int nb, int T,
+                                                          int n_items, uint4 * __restrict__ frag, _Float16 * __restrict__ dx) {
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item < n_items) quantize_q8(x, x_nb1, nb, T, item, frag, dx);
+}
+
+// The same and the adapters' first product, which need nothing of each other,
+// in one launch: n_quantize workgroups of the one, then T x ks of the other.
+template <int RT>
+__global__ __launch_bounds__(64 * lora::shrink_waves<RT>(), RT == 8 ? 2 : 4) void quantize_shrink_kernel(
+    const char * __restrict__ x, int64_t x_nb1, int nb, int T, int n_items, uint4 * __restrict__ frag,
+    _Float16 * __restrict__ dx, int n_quantize, const lora::LoraParams p) {
+    constexpr int kWaves = lora::shrink_waves<RT>();
+    __shared__ float part[kWaves][RT * 16][lora::kTile + 1];
+    if ((int) blockIdx.x < n_quantize) {
+        const int item = blockIdx.x * kWaves + (threadIdx.x >> 6);
+        if (item < n_items) quantize_q8(x, x_nb1, nb, T, item, frag, dx);
+        return;
+    }
+    const int i = (int) blockIdx.x - n_quantize, k = i / T;
+    lora::shrink_few<RT, kWaves>(p, i - k * T, k, part);
+}
+
 // 9 to 64 tokens: a workgroup takes 16 weight rows and a tile of 16 tokens,
 // each of its 8 waves 1/8 of K. One MFMA 16x16x32 i8 is one block's integer
 // dot products of 16 tokens and 16 rows, exact, as the format needs them;
@@ -180,9 +202,12 @@ __global__ __launch_bounds__(256) void quantize_q8_kernel(const char * __restric
 // row, the tokens in series): K 8192, N 5120: 48 tokens 232 -> 21.9, 16
 // tokens 15.5; K 4096, N 2560: 37 tokens 39 -> 9.2, 16 tokens 22 -> 7.4; K
 // 4096, N 4096: 12 tokens 22 -> 7.5.
-template <int BL>
-__global__ __launch_bounds__(kGemmWaves * 64, 4) void gemm_q4_kernel(const char * w, int64_t w_nb1, int N, const uint4 * frag,
-                                                                  const uint4 * dx, int T, char * y, int64_t y_nb1) {
+// lora_p (LORA): the adapters' second product, added to the outputs: v of the
+// tile's rows is summed into LDS at the start; waves 4 to 7, which have no part
+// in the last sums, each take 4 of the tokens with their 16 rows of B.
+template <int BL, bool LORA>
+__device__ __forceinline__ void gemm_q4(const char * w, int64_t w_nb1, int N, const uint4 * frag, const uint4 * dx, int T, char * y,
+                                        int64_t y_nb1, const lora::LoraParams & lora_p) {
     constexpr int NB = 32 * BL;                                        // blocks of a row
     constexpr int kSteps = NB / (8 * kGemmWaves);
     constexpr int kDx = NB * kTile * 2, kRed = kGemmWaves * 4 * 256;
@@ -215,9 +240,27 @@ __global__ __launch_bounds__(kGemmWaves * 64, 4) void gemm_q4_kernel(const char 
         for (int d = 0; d < 4; ++d) a[s % kDepth][d] = frag[block(s, d) / 2 * 64 + lane];
         asm volatile("" ::: "memory");                                 // keeps the issue order
     };
+    // the parts of v go out before the weights, so that they are not waited
+    // for behind them: one item of 4 ranks a thread at most
+    __shared__ __align__(16) float v[LORA ? kTile : 1][LORA ? lora::kMaxR + 4 : 1];
+    __shared__ float low[LORA ? 4 : 1][64];
+    const int tok = tile * kTile + 4 * g + (wave & 3);                 // of the wave's last sums
+    int id = -1, rank = 0, at = kTile, j = 0;
+    float4 parts[LORA ? lora::kParts : 1];
+    if constexpr (LORA) {
+        static_assert(kTile * lora::kMaxR / 4 <= 64 * kGemmWaves, "one item a thread");
+        id = lora_p.ids[min(tok, T - 1)];
+        at = threadIdx.x / (lora_p.R / 4);
+        j = 4 * (threadIdx.x - at * (lora_p.R / 4));
+        if (at < kTile) lora::load_parts(lora_p, min(tile * kTile + at, T - 1), j, parts);
+        asm volatile("" ::: "memory");
+    }
 #pragma unroll
     for (int s = 0; s < kDepth; ++s) issue(s);
-
+    if constexpr (LORA) {
+        if (at < kTile) *(float4 *) &v[at][j] = lora::sum_of(lora_p, parts);
+        rank = id >= 0 ? rank_of(lora_p, id) : 0;
+    }
     typedef int int4v __attribute__((ext_vector_type(4)));
     typedef _Float16 half4 __attribute__((ext_vector_type(4)));
     constexpr int kSums = kSteps > 2 ? 8 : 4;                          // sums a lane keeps per output: per block of a step, or pair
@@ -257,24 +300,54 @@ __global__ __launch_bounds__(kGemmWaves * 64, 4) void gemm_q4_kernel(const char 
     float (*red)[4][64] = (float (*)[4][64]) lds;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float v[4];
+        float s[4];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) v[d] = kSums == 8 ? acc[0][d][i] + acc[kSums / 4 - 1][d][i] : acc[0][d][i];
-        red[wave][i][lane] = (v[0] + v[1]) + (v[2] + v[3]);
+        for (int d = 0; d < 4; ++d) s[d] = kSums == 8 ? acc[0][d][i] + acc[kSums / 4 - 1][d][i] : acc[0][d][i];
+        red[wave][i][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    if constexpr (LORA) {
+        if (wave >= 4) {
+            const char * br = lora_p.b + (int64_t) (rank > 0 ? id : 0) * lora_p.b_nb2 + (int64_t) min(n0 + r, N - 1) * lora_p.b_nb1;
+            float s = rank < 0 ? __builtin_nanf("") : 0.0f;
+            for (int j0 = 0; j0 < lora_p.R; j0 += 32) {
+                half8 b[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j0 + 8 * e < rank) b[e] = *(const half8 *) (br + 2 * (j0 + 8 * e));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j0 + 8 * e < rank) s += lora::dot8(b[e], &v[4 * g + (wave & 3)][j0 + 8 * e], rank - j0 - 8 * e);
+            }
+            low[wave - 4][lane] = s;
+        }
     }
     __syncthreads();
     // wave i < 4: token 4 (lane / 16) + i of the tile, row lane % 16
     if (wave < 4) {
-        float v[kGemmWaves];
+        float s[kGemmWaves];
 #pragma unroll
-        for (int u = 0; u < kGemmWaves; ++u) v[u] = red[u][wave][lane];
+        for (int u = 0; u < kGemmWaves; ++u) s[u] = red[u][wave][lane];
 #pragma unroll
         for (int h = kGemmWaves / 2; h >= 1; h /= 2)
 #pragma unroll
-            for (int u = 0; u < h; ++u) v[u] += v[u + h];
-        const int tok = tile * kTile + 4 * g + wave;
-        if (tok < T && n0 + r < N) *(float *) (y + (int64_t) tok * y_nb1 + (int64_t) (n0 + r) * 4) = v[0];
+            for (int u = 0; u < h; ++u) s[u] += s[u + h];
+        if constexpr (LORA)
+            if (id >= 0) s[0] += low[wave][lane];
+        if (tok < T && n0 + r < N) *(float *) (y + (int64_t) tok * y_nb1 + (int64_t) (n0 + r) * 4) = s[0];
     }
+}
+
+template <int BL>
+__global__ __launch_bounds__(kGemmWaves * 64, 4) void gemm_q4_kernel(const char * w, int64_t w_nb1, int N, const uint4 * frag,
+                                                                  const uint4 * dx, int T, char * y, int64_t y_nb1) {
+    gemm_q4<BL, false>(w, w_nb1, N, frag, dx, T, y, y_nb1, lora::LoraParams{});
+}
+
+template <int BL>
+__global__ __launch_bounds__(kGemmWaves * 64, 4) void gemm_q4_lora_kernel(const char * w, int64_t w_nb1, int N, const uint4 * frag,
+                                                                       const uint4 * dx, int T, char * y, int64_t y_nb1,
+                                                                       const lora::LoraParams p) {
+    gemm_q4<BL, true>(w, w_nb1, N, frag, dx, T, y, y_nb1, p);
 }
 
 // 1 / d as the IEEE division rounds it, for a Q8_0 block scale d >= 0 (0
@@ -384,12 +457,14 @@ __device__ __forceinline__ float wave_sum8_scatter(const float (&v)[8], const in
 // each thread issues the loads of all T tokens of its part of a block before
 // using any), then runs the dot products from LDS. One wavefront per row; with several tokens the rows' per-lane sums of all of
 // them meet in one scattering wave reduction.
-template <int BPL, int TMAX>
-__global__ __launch_bounds__(1024) void gemv_q4_fused_kernel(const char * w, int64_t w_nb1, int N, int K,
-                                                             const char * x, int64_t x_nb1, int T,
-                                                             char * __restrict__ y, int64_t y_nb1) {
+// lora_p (LORA): the adapters' second product, added to the outputs. The 8
+// lanes that hold a token's sum (all 64 for one token) take 8 ranks of the
+// row's B each, loaded with the weights; v is summed into LDS beside the
+// quantization.
+template <int BPL, int TMAX, bool LORA>
+__device__ __forceinline__ void gemv_q4_fused(const char * w, int64_t w_nb1, int N, int K, const char * x, int64_t x_nb1, int T,
+                                              char * __restrict__ y, int64_t y_nb1, const lora::LoraParams & lora_p) {
     extern __shared__ __align__(16) char lds[];
-    prefetch_params(w_nb1, y_nb1, blockDim.x);
     const int nb = K / 32;
     int8_t * qs = (int8_t *) lds;                                       // [T][K]
     float2 * sc = (float2 *) (lds + T * K);                             // [T][nb]: (block scale, value sum)
@@ -440,6 +515,33 @@ __global__ __launch_bounds__(1024) void gemv_q4_fused_kernel(const char * w, int
     asm volatile("" ::: "memory");                                     // keeps the issue order
     load_weights(c);
     asm volatile("" ::: "memory");
+    // the adapter of the lane's token, and its ranks 8 piece .. 8 piece + 7
+    // (and, above 64 ranks, 64 further on) of the row's B
+    const int tok = TMAX > 1 ? lane >> 3 : 0, piece = TMAX > 1 ? lane & 7 : lane;
+    float * v = (float *) (lds + T * K + 8 * T * nb);                   // LORA: [T][R]
+    constexpr int kPieces = TMAX > 1 ? 2 : 1;                           // (64 lanes hold every rank once)
+    half8 b[kPieces];
+    int id = -1, rank = 0;
+    if constexpr (LORA) {
+#pragma unroll
+        for (int t = 0; t < TMAX; ++t) {                                // (scalar loads: not behind the weights)
+            const int i = ld_uniform(lora_p.ids + min(t, T - 1));
+            if (tok == t && t < T) id = i;
+        }
+        if (id >= 0) {
+            rank = rank_of(lora_p, id);
+            if (rank >= 0) {
+                const char * br = lora_p.b + (int64_t) id * lora_p.b_nb2 + (int64_t) min(row, N - 1) * lora_p.b_nb1;
+#pragma unroll
+                for (int e = 0; e < kPieces; ++e)
+                    if (8 * piece + 64 * e < lora_p.R) b[e] = *(const half8 *) (br + 16 * piece + 128 * e);
+            }
+        }
+        for (int i = threadIdx.x; i < T * lora_p.R / 4; i += blockDim.x) {
+            const int at = i / (lora_p.R / 4);
+            ((float4 *) v)[i] = sum_parts(lora_p, at, 4 * (i - at * (lora_p.R / 4)));
+        }
+    }
 #pragma unroll
     for (int k = 0; k < PRE; ++k)
         if (k < rounds) quantize_item(threadIdx.x + k * blockDim.x, f[k]);
@@ -483,19 +585,53 @@ __global__ __launch_bounds__(1024) void gemv_q4_fused_kernel(const char * w, int
         }
         return part;
     };
+    float low = 0.0f;                                                   // the lane's ranks' share of its token's output
+    if constexpr (LORA) {
+        if (rank < 0) low = __builtin_nanf("");
+#pragma unroll
+        for (int e = 0; e < kPieces; ++e) {
+            const int j = 8 * piece + 64 * e;
+            if (j < rank) low += lora::dot8(b[e], v + tok * lora_p.R + j, rank - j);
+        }
+        if constexpr (TMAX > 1) {
+            low += dpp<kQuadXor1>(low);
+            low += dpp<kQuadXor2>(low);
+            low += dpp<kRowHalfMirror>(low);
+        } else {
+            low = wave_sum_to_last(low);
+        }
+    }
     if constexpr (TMAX > 1) {
         float part[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) part[t] = t < TMAX && t < T ? dot_t(t) : 0.0f;
-        const float tot = wave_sum8_scatter(part, lane);
+        float tot = wave_sum8_scatter(part, lane);
         const int t = lane >> 3;
+        if (LORA && id >= 0) tot += low;
         if ((lane & 7) == 0 && t < T) *(float *) (y + (int64_t) t * y_nb1 + (int64_t) row * 4) = tot;
     } else {
         for (int t = 0; t < T; ++t) {
-            const float part = wave_sum_to_last(dot_t(t));
+            float part = wave_sum_to_last(dot_t(t));
+            if (LORA && id >= 0) part += low;
             if (lane == 63) *(float *) (y + (int64_t) t * y_nb1 + (int64_t) row * 4) = part;
         }
     }
+}
+
+template <int BPL, int TMAX>
+__global__ __launch_bounds__(1024) void gemv_q4_fused_kernel(const char * w, int64_t w_nb1, int N, int K,
+                                                             const char * x, int64_t x_nb1, int T,
+                                                             char * __restrict__ y, int64_t y_nb1) {
+    prefetch_params(w_nb1, y_nb1, blockDim.x);
+    gemv_q4_fused<BPL, TMAX, false>(w, w_nb1, N, K, x, x_nb1, T, y, y_nb1, lora::LoraParams{});
+}
+
+template <int BPL, int TMAX>
+__global__ __launch_bounds__(1024) void gemv_q4_lora_kernel(const char * w, int64_t w_nb1, int N, int K, const char * x,
+                                                            int64_t x_nb1, int T, char * __restrict__ y, int64_t y_nb1,
+                                                            const lora::LoraParams p) {
+    prefetch_params(w_nb1, y_nb1, blockDim.x, p);
+    gemv_q4_fused<BPL, TMAX, true>(w, w_nb1, N, K, x, x_nb1, T, y, y_nb1, p);
 }
 
 // Most tokens of the one-launch kernel. Against the two launches for more
@@ -509,7 +645,8 @@ constexpr int kFusedMaxT = 8;
 size_t fused_lds_bytes(int64_t K, int64_t T) { return (size_t) (T * K + 8 * T * (K / 32)); }   // <= 160 KiB
 
 template <int BPL, int TMAX>
-int launch_fused(const al_tensor * w, const al_tensor * x, const al_tensor * y, int N, int K, int T, hipStream_t st) {
+int launch_fused(const al_tensor * w, const al_tensor * x, const al_tensor * y, int N, int K, int T, const lora::LoraParams * p,
+                 hipStream_t st) {
     int n_cu = 0;
     int rc = al_device_cu_count(&n_cu);
     if (rc != AL_OK) return rc;
@@ -517,35 +654,45 @@ int launch_fused(const al_tensor * w, const al_tensor * x, const al_tensor * y, 
     // per CU that keep a workgroup at 16 waves or fewer
     const int per_cu = (N + 16 * n_cu - 1) / (16 * n_cu);
     const int waves = std::max(1, (N + per_cu * n_cu - 1) / (per_cu * n_cu));
-    const size_t lds = fused_lds_bytes(K, T);
+    const size_t lds = fused_lds_bytes(K, T) + (p ? (size_t) T * p->R * 4 : 0);
     if (lds > 64 * 1024) {
-        hipError_t e = hipFuncSetAttribute((const void *) gemv_q4_fused_kernel<BPL, TMAX>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds);
+        const void * f = p ? (const void *) gemv_q4_lora_kernel<BPL, TMAX> : (const void *) gemv_q4_fused_kernel<BPL, TMAX>;
+        hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds);
         if (e != hipSuccess) return al_hip_fail(e, "mul_mat_q4_0: LDS attribute");
     }
-    hipLaunchKernelGGL((gemv_q4_fused_kernel<BPL, TMAX>), dim3((unsigned) ((N + waves - 1) / waves)), dim3(64 * waves), lds, st,
-                       (const char *) w->data, (int64_t) w->nb[1], N, K, (const char *) x->data, (int64_t) x->nb[1], T,
-                       (char *) y->data, (int64_t) y->nb[1]);
+    if (p)
+        hipLaunchKernelGGL((gemv_q4_lora_kernel<BPL, TMAX>), dim3((unsigned) ((N + waves - 1) / waves)), dim3(64 * waves), lds, st,
+                           (const char *) w->data, (int64_t) w->nb[1], N, K, (const char *) x->data, (int64_t) x->nb[1], T,
+                           (char *) y->data, (int64_t) y->nb[1], *p);
+    else
+        hipLaunchKernelGGL((gemv_q4_fused_kernel<BPL, TMAX>), dim3((unsigned) ((N + waves - 1) / waves)), dim3(64 * waves), lds, st,
+                           (const char *) w->data, (int64_t) w->nb[1], N, K, (const char *) x->data, (int64_t) x->nb[1], T,
+                           (char *) y->data, (int64_t) y->nb[1]);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "mul_mat_q4_0: fused launch");
 }
 
 template <int BPL>
-int launch_fused_t(const al_tensor * w, const al_tensor * x, const al_tensor * y, int N, int K, int T, hipStream_t st) {
+int launch_fused_t(const al_tensor * w, const al_tensor * x, const al_tensor * y, int N, int K, int T, const lora::LoraParams * p,
+                   hipStream_t st) {
     // Every wave loads and quantizes its share of TMAX rows, those past T for
     // nothing: at 2 to 4 tokens the kernel for 8 took, us per call, K 4096, N
     // 4096: 5.9 (4 tokens) and 5.2 (2) against 5.3 and 4.3; K 8192, N 5120: 15.9
     // (4) and 14.5 (3) against 12.7 and 11.5. Same bits.
-    if (T == 1) return launch_fused<BPL, 1>(w, x, y, N, K, T, st);
-    return T <= 4 ? launch_fused<BPL, 4>(w, x, y, N, K, T, st) : launch_fused<BPL, kFusedMaxT>(w, x, y, N, K, T, st);
+    if (T == 1) return launch_fused<BPL, 1>(w, x, y, N, K, T, p, st);
+    return T <= 4 ? launch_fused<BPL, 4>(w, x, y, N, K, T, p, st) : launch_fused<BPL, kFusedMaxT>(w, x, y, N, K, T, p, st);
 }
 
 template <int BL>
 int launch_gemm(const al_tensor * w, const al_tensor * y, int N, int tiles, int T, const uint4 * frag, const uint4 * dx,
-                hipStream_t st) {
+                const lora::LoraParams * p, hipStream_t st) {
     const dim3 grid((unsigned) ((N + 15) / 16), (unsigned) tiles);
-    hipLaunchKernelGGL(gemm_q4_kernel<BL>, grid, dim3(kGemmWaves * 64), 0, st, (const char *) w->data, (int64_t) w->nb[1], N,
-                       frag, dx, T, (char *) y->data, (int64_t) y->nb[1]);
+    if (p)
+        hipLaunchKernelGGL(gemm_q4_lora_kernel<BL>, grid, dim3(kGemmWaves * 64), 0, st, (const char *) w->data, (int64_t) w->nb[1], N,
+                           frag, dx, T, (char *) y->data, (int64_t) y->nb[1], *p);
+    else
+        hipLaunchKernelGGL(gemm_q4_kernel<BL>, grid, dim3(kGemmWaves * 64), 0, st, (const char *) w->data, (int64_t) w->nb[1], N,
+                           frag, dx, T, (char *) y->data, (int64_t) y->nb[1]);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "mul_mat_q4_0: launch");
 }
@@ -623,14 +770,15 @@ int mul_mat_q4_0_check(const al_tensor * w, const al_tensor * x, const al_tensor
     return AL_OK;
 }
 
-int mul_mat_q4_0_run(const al_tensor * w, const al_tensor * x, const al_tensor * y, void * s, hipStream_t st) {
+int mul_mat_q4_0_run(const al_tensor * w, const al_tensor * x, const al_tensor * y, const lora::LoraParams * p, void * s,
+                     hipStream_t st) {
     const int64_t K = w->ne[0], N = w->ne[1], T = x->ne[1], nb = K / 32;
     if (T <= kFusedMaxT) {
         switch (nb / 64) {
-            case 2: return launch_fused_t<2>(w, x, y, (int) N, (int) K, (int) T, st);
-            case 4: return launch_fused_t<4>(w, x, y, (int) N, (int) K, (int) T, st);
-            case 6: return launch_fused_t<6>(w, x, y, (int) N, (int) K, (int) T, st);
-            case 8: return launch_fused_t<8>(w, x, y, (int) N, (int) K, (int) T, st);
+            case 2: return launch_fused_t<2>(w, x, y, (int) N, (int) K, (int) T, p, st);
+            case 4: return launch_fused_t<4>(w, x, y, (int) N, (int) K, (int) T, p, st);
+            case 6: return launch_fused_t<6>(w, x, y, (int) N, (int) K, (int) T, p, st);
+            case 8: return launch_fused_t<8>(w, x, y, (int) N, (int) K, (int) T, p, st);
             default: return al_fail(AL_ERR_UNSUPPORTED, "mul_mat_q4_0: K %lld", (long long) K);
         }
     }
@@ -639,18 +787,41 @@ int mul_mat_q4_0_run(const al_tensor * w, const al_tensor * x, const al_tensor *
     uint4 * frag = (uint4 *) s;
     _Float16 * dx = (_Float16 *) ((char *) s + qs_bytes);
     const int items = tiles * (int) (nb / 2);
-    hipLaunchKernelGGL(quantize_q8_kernel, dim3((unsigned) ((items + 3) / 4)), dim3(256), 0, st,
-                       (const char *) x->data, (int64_t) x->nb[1], (int) nb, (int) T, items, frag, dx);
-    hipError_t e = hipGetLastError();
+    hipError_t e;
+    if (p) {
+        const int rt = p->R <= 16 ? 1 : p->R <= 32 ? 2 : p->R <= 64 ? 4 : 8, waves = rt == 8 ? 4 : 8;
+        const int n_quantize = (items + waves - 1) / waves;
+        const dim3 grid((unsigned) (n_quantize + T * p->ks));
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, (const char *) x->data, (int64_t) x->nb[1], (int) nb, (int) T,
+                               items, frag, dx, n_quantize, *p);
+        };
+        switch (rt) {
+            case 1: go(quantize_shrink_kernel<1>); break;
+            case 2: go(quantize_shrink_kernel<2>); break;
+            case 4: go(quantize_shrink_kernel<4>); break;
+            default: go(quantize_shrink_kernel<8>); break;
+        }
+    } else {
+        hipLaunchKernelGGL(quantize_q8_kernel, dim3((unsigned) ((items + 3) / 4)), dim3(256), 0, st,
+                           (const char *) x->data, (int64_t) x->nb[1], (int) nb, (int) T, items, frag, dx);
+    }
+    e = hipGetLastError();
     if (e != hipSuccess) return al_hip_fail(e, "mul_mat_q4_0: quantize launch");
     switch (nb / 128) {
-        case 1: return launch_gemm<4>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, st);
-        case 2: return launch_gemm<8>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, st);
-        case 3: return launch_gemm<12>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, st);
-        case 4: return launch_gemm<16>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, st);
+        case 1: return launch_gemm<4>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, p, st);
+        case 2: return launch_gemm<8>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, p, st);
+        case 3: return launch_gemm<12>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, p, st);
+        case 4: return launch_gemm<16>(w, y, (int) N, tiles, (int) T, frag, (const uint4 *) dx, p, st);
         default: return al_fail(AL_ERR_UNSUPPORTED, "mul_mat_q4_0: K %lld", (long long) K);
     }
 }
+
+bool mul_mat_q4_0_takes_lora(const al_tensor * w, int T, int R) {
+    return T > kFusedMaxT || fused_lds_bytes(w->ne[0], T) + (size_t) T * R * 4 <= (160u << 10);
+}
+
+bool mul_mat_q4_0_shrinks(int T) { return T > kFusedMaxT; }
 
 extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, const al_tensor * y, void * stream) {
     size_t bytes = 0;
@@ -658,5 +829,5 @@ extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, con
     int rc = mul_mat_q4_0_check(w, x, y, &bytes);
     if (rc == AL_OK && bytes) rc = scratch(bytes, &s);
     if (rc != AL_OK) return rc;
-    return mul_mat_q4_0_run(w, x, y, s, (hipStream_t) stream);
+    return mul_mat_q4_0_run(w, x, y, nullptr, s, (hipStream_t) stream);
 }

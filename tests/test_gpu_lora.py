@@ -177,7 +177,8 @@ def test_unknown_adapters_are_reported(gpu, T):
 
 
 PROJ = [(4096, 2560, 16, 8, 1), (4096, 4096, 32, 4, 3), (4096, 2560, 8, 12, 8), (8192, 5120, 64, 20, 9), (4096, 100, 24, 6, 16),
-        (8192, 1000, 16, 50, 48), (12288, 257, 128, 3, 64), (16384, 64, 8, 2, 2)]
+        (8192, 1000, 16, 50, 48), (12288, 257, 128, 3, 64), (16384, 64, 8, 2, 2), (16384, 48, 128, 3, 8), (4096, 300, 128, 5, 1), (8192, 31, 72, 9, 6),
+        (4096, 40, 40, 2, 60)]
 
 
 @pytest.mark.parametrize("i", range(len(PROJ)))
