@@ -27,11 +27,20 @@
 // it.
 //
 // Work. The cells that a batch's sequences hold differ and are known on the
-// device only. Every workgroup reads the lengths, cuts every sequence into
-// chunks of at most C tiles with C such that the chunks of a (KV head, row
-// group) are about as many as the workgroups that fit, and finds its own.
-// Sequences of one chunk are written at once, the parts of the others are
-// joined by a second launch.
+// device only. For each (KV head, row group) the tiles of all sequences are
+// thought of as one row, cut into equal parts for the workgroups that fit the
+// card; every workgroup reads the lengths and finds the sequences, or pieces
+// of them, of its own part. A sequence within one workgroup is written at
+// once; the pieces of the others go to records (at most two of a workgroup's
+// pieces are such), which a second launch joins. Chunks of one size for each
+// sequence, at most C tiles, left a batch of 24 sequences of 1400 to 4000
+// cells with a second, short round of workgroups (55.9 us).
+//
+// More than 16 query rows (T tokens of G heads) are taken by the workgroup's
+// waves side by side, 16 rows each, over the same cells: the second wave that
+// reads a line finds it in the L1. (Two row tiles in one wave need 500
+// registers, one wave for each SIMD: 54.9 us instead of XXX for 10 sequences of
+// up to 6 drafts over 2100 to 6000 cells.)
 
 #include <hip/hip_runtime.h>
 
@@ -58,449 +67,519 @@ struct PagedFattnParams {
     const int32_t * lens;
     const int32_t * counts;                             // or null
     const float * sinks;                                // or null
-    float * part;                                       // records: rows x 128 sums, then rows x {m, l}
-    int32_t T, G, Hkv, R, row_groups;
+    int2 * info;                                        // [unit][n_seq]: first workgroup of the sequence, pieces
+    float * part;                                       // records [unit][workgroup][2]: rows x 128 sums, rows x {m, l}
+    int32_t T, G, Hkv, R, row_groups, row_tiles;        // row tiles of 16 in a group
     uint32_t g_magic;                                   // ceil(2^32 / G) (0 for 1)
-    int32_t target;                                     // chunks aimed at for a (head, row group)
-    int32_t max_chunks;                                 // grid size: chunks there can be
+    int32_t target;                                     // workgroups of a unit (head, row group)
+    int32_t row_waves;                                  // join: waves of a row
     float scale, softcap;
 };
 
-__device__ __forceinline__ int wave_sum_int(int x) {
-#pragma unroll
-    for (int o = 32; o >= 1; o /= 2) x += __shfl_xor(x, o);
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_add(const int x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
+}
+// Sum of the lanes up to and with this one (DPP: within rows of 16, then the
+// rows' last lanes into those after them).
+__device__ __forceinline__ int wave_scan(int x) {
+    x = dpp_add<0x111, 0xf>(x);
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);
+    x = dpp_add<0x143, 0xc>(x);
     return x;
 }
 
-// What a row group of a sequence has to do.
+template <typename P>
+__device__ __forceinline__ int token_of(const P & p, const int r) {
+    return p.G == 1 ? r : (int) __umulhi((uint32_t) r, p.g_magic);
+}
+
+// What a row group has to do for a sequence, t0 and t1 its first and last token.
 struct SeqWork {
-    int len, count, limit;                      // cells (within the table), new tokens, cells its last row sees
+    int len, count;                             // cells (within the table), new tokens
     bool bad;
+    // cells that the group's last row sees, -1 if it has no row
+    __device__ __forceinline__ int limit(const int t0, const int t1) const {
+        return count > t0 ? min(max(len - count + 1 + min(t1, count - 1), 0), len) : -1;
+    }
 };
 
-__device__ __forceinline__ SeqWork seq_work(const PagedFattnParams & p, const int s, const int t0, const int t1) {
+__device__ __forceinline__ SeqWork seq_work(const PagedFattnParams & p, const int len, const int count) {
     SeqWork w;
-    const int cap = p.c.max_pages * p.c.page_size;
-    const int len = p.lens[s], count = p.counts ? p.counts[s] : p.T;
-    w.len = min(max(len, 0), cap);
+    w.len = min(max(len, 0), p.c.max_pages * p.c.page_size);
     w.count = min(max(count, 0), p.T);
     w.bad = len != w.len || count != w.count;
-    w.limit = w.count > t0 ? min(max(w.len - w.count + 1 + min(t1, w.count - 1), 0), w.len) : -1;
     return w;
 }
 
-__device__ __forceinline__ int tiles_of(const SeqWork & w) { return w.limit > 0 ? (w.limit + kTile - 1) / kTile : 0; }
-__device__ __forceinline__ int chunks_of(const SeqWork & w, const int C) {
-    return w.limit < 0 ? 0 : max(1, (tiles_of(w) + C - 1) / C);
+// Tiles of a sequence in the row of all tiles: one at least, so that rows that
+// see nothing are written too.
+__device__ __forceinline__ int tiles_of(const int limit) {
+    return limit < 0 ? 0 : max(1, (limit + kTile - 1) / kTile);
 }
 
-// Tiles of a chunk at most, the same in every wave of the launch's row group.
-__device__ __forceinline__ int chunk_tiles(const PagedFattnParams & p, const int lane, const int t0, const int t1) {
-    int sum = 0;
-    for (int s = lane; s < p.c.n_seq; s += 64) sum += tiles_of(seq_work(p, s, t0, t1));
-    sum = wave_sum_int(sum);
-    const int c = (sum + p.target - 1) / p.target;
-    return max(kMinTiles, (c + kWaves - 1) / kWaves * kWaves);
+// First tile of a workgroup's part, of S tiles cut into W parts; and the
+// workgroup whose part holds tile x.
+__device__ __forceinline__ int part_begin(const int w, const int S, const int W) { return (int) ((int64_t) w * S / W); }
+__device__ __forceinline__ int part_of(const int x, const int S, const int W) { return (int) (((int64_t) (x + 1) * W + S - 1) / S) - 1; }
+
+// Sequences 64 b .. 64 b + 63, one to a lane.
+struct Block {
+    int len, count, tiles, upto;                // as read; tiles, and those of all sequences up to this one
+    __device__ __forceinline__ void load(const PagedFattnParams & p, const int b, const int lane, const int t0, const int t1) {
+        const int s = 64 * b + lane;
+        const bool in = s < p.c.n_seq;
+        len = in ? p.lens[s] : 0;
+        count = !in ? 0 : p.counts ? p.counts[s] : p.T;
+        tiles = in ? tiles_of(seq_work(p, len, count).limit(t0, t1)) : 0;
+        upto = wave_scan(tiles);
+    }
+    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
+};
+
+template <typename P>
+__device__ __forceinline__ char * record(const P & p, const int unit, const int wg, const int slot) {
+    return (char *) p.part + (((int64_t) unit * p.target + wg) * 2 + slot) * (16 * p.row_tiles) * 130 * 4;
 }
 
-// The tokens of a row group.
-__device__ __forceinline__ void group_tokens(const PagedFattnParams & p, const int r0, const int rows, int & t0, int & t1) {
-    t0 = p.G == 1 ? r0 : (int) __umulhi((uint32_t) r0, p.g_magic);
-    const int last = min(r0 + rows, p.R) - 1;
-    t1 = p.G == 1 ? last : (int) __umulhi((uint32_t) last, p.g_magic);
+// e^(a - b) for running maxima a <= b, 1 where they are equal (both -inf too).
+__device__ __forceinline__ float grow(const float a, const float b) { return a == b ? 1.0f : exp_fast(a - b); }
+
+// Factor of a row's sums, with the sink as one more logit without a value: 0
+// for a row that saw nothing.
+template <typename P>
+__device__ __forceinline__ float row_factor(const P & p, const float M, float L, const int head) {
+    L *= 1.0f / kPScale;
+    float up = 1.0f / kPScale;
+    if (p.sinks) {
+        const float sink = p.sinks[head], top = fmaxf(M, sink);
+        const float e = grow(M, top);
+        up *= e;
+        L = L * e + grow(sink, top);
+    }
+    return L == 0.0f ? 0.0f : up / L;
 }
 
-__device__ __forceinline__ const char * record(const PagedFattnParams & p, const int unit, const int chunk, const int rows) {
-    return (const char *) p.part + ((int64_t) unit * p.max_chunks + chunk) * rows * 130 * 4;
+// The kernel's arguments as memory, to be loaded where they are used: held in
+// scalar registers from the start, those that only a piece's beginning and end
+// use displace what the loop over the cells needs.
+__device__ __forceinline__ const __attribute__((address_space(4))) PagedFattnParams & arguments() {
+    auto a = (const __attribute__((address_space(4))) PagedFattnParams *) __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return *a;
 }
 
-// NR: row tiles of 16 query rows. CAP: logits soft-capped.
-template <int NR, bool CAP>
-__global__ __launch_bounds__(64 * kWaves, NR == 1 ? 2 : 1) void paged_fattn_kernel(const PagedFattnParams p) {
+// ROWT: row tiles of 16 query rows that the waves take side by side (1, 2 or
+// 4); the tiles of cells go round the waves of a row tile. CAP: logits
+// soft-capped.
+template <int ROWT, bool CAP>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const PagedFattnParams p) {
+    constexpr int kCellWaves = kWaves / ROWT;
     __shared__ __attribute__((aligned(16))) float o_lds[kWaves][16][132];
-    __shared__ float ml_lds[NR][kWaves][16][2];
+    __shared__ float ml_lds[kWaves][16][2];
     prefetch_params(p);
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int unit = blockIdx.y, h = unit % p.Hkv, r0 = unit / p.Hkv * (16 * NR);
-    int t0, t1;
-    group_tokens(p, r0, 16 * NR, t0, t1);
+    const int rt = wave / kCellWaves, cw = wave % kCellWaves;
+    const int unit = blockIdx.y, h = unit % p.Hkv, group0 = unit / p.Hkv * (16 * ROWT);
+    // tokens of the group, and of the wave's row tile (empty past the last row)
+    const int t0 = token_of(p, group0), t1 = token_of(p, min(group0 + 16 * ROWT, p.R) - 1);
+    const int r0 = group0 + 16 * rt;
+    const int wt0 = token_of(p, min(r0, p.R - 1)), wt1 = token_of(p, min(r0 + 16, p.R) - 1);
 
-    // this workgroup's chunk
-    const int C = chunk_tiles(p, lane, t0, t1);
-    int seq = -1, chunk = 0, n_chunks = 0, before = 0;
-    for (int s0 = 0; s0 < p.c.n_seq && seq < 0; s0 += 64) {
-        const int s = s0 + lane;
-        const int mine = s < p.c.n_seq ? chunks_of(seq_work(p, s, t0, t1), C) : 0;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const int x = __shfl_up(upto, o);
-            if (lane >= o) upto += x;
-        }
-        const int x = (int) blockIdx.x - before;
-        const uint64_t hit = __ballot(x < upto);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            seq = s0 + l;
-            n_chunks = __builtin_amdgcn_readlane(mine, l);
-            chunk = x - (__builtin_amdgcn_readlane(upto, l) - n_chunks);
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
+    // this workgroup's part of all tiles
+    Block b;
+    b.load(p, 0, lane, t0, t1);
+    int S = b.total(), block = 0, before = 0;
+    for (int i = 1; 64 * i < p.c.n_seq; ++i) {
+        Block x;
+        x.load(p, i, lane, t0, t1);
+        S += x.total();
     }
-    if (seq < 0) return;
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    const SeqWork w = seq_work(p, seq, t0, t1);
-    bool bad = w.bad;
-    if (bad && threadIdx.x == 0)
-        paged_error(p.c, p.lens[seq] != w.len ? kPagedBadLength : kPagedBadCount, p.lens[seq] != w.len ? p.lens[seq] : p.counts[seq]);
-    const int tiles = tiles_of(w);
-    const int first = (int) ((int64_t) tiles * chunk / n_chunks), end = (int) ((int64_t) tiles * (chunk + 1) / n_chunks);
+    const int W = min(p.target, (S + kMinTiles - 1) / kMinTiles);
+    if ((int) blockIdx.x >= W) return;
+    const int stop = part_begin(blockIdx.x + 1, S, W);
 
-    // the query rows of this lane's columns: their limits, and their operands
-    // times a power of two that brings the largest value to [2^11, 2^12)
-    int limit[NR];
-    float fac[NR], m[NR], l[NR];
-    half8 q_hi[NR][4], q_lo[NR][4];
-    floatx4 acc[NR][8];
-#pragma unroll
-    for (int u = 0; u < NR; ++u) {
-        const int r = r0 + 16 * u + n;
-        const int t = p.G == 1 ? r : (int) __umulhi((uint32_t) r, p.g_magic);
+    for (int at = part_begin(blockIdx.x, S, W); at < stop;) {
+        // the sequence that holds tile `at`
+        while (at >= before + b.total()) {
+            before += b.total();
+            b.load(p, ++block, lane, t0, t1);
+        }
+        const int l64 = __builtin_ctzll(__ballot(at < before + b.upto));
+        const int seq = 64 * block + l64;
+        const int tiles = __builtin_amdgcn_readlane(b.tiles, l64);
+        const int base = before + __builtin_amdgcn_readlane(b.upto, l64) - tiles;
+        const int raw_len = __builtin_amdgcn_readlane(b.len, l64), raw_count = __builtin_amdgcn_readlane(b.count, l64);
+        const SeqWork w = seq_work(p, raw_len, raw_count);
+        const int first = at - base, end = min(tiles, stop - base);
+        at = base + end;
+        const bool whole = first == 0 && end == tiles;
+        const auto & ap = arguments();
+        if (threadIdx.x == 0) {
+            if (first == 0)
+                ap.info[(int64_t) unit * ap.c.n_seq + seq] =
+                    int2{(int) blockIdx.x, whole ? 1 : part_of(base + tiles - 1, S, W) - (int) blockIdx.x + 1};
+            if (w.bad) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
+        }
+        bool bad = w.bad;
+        const int seen = w.limit(wt0, wt1);                        // cells that the wave's last row sees
+        const int least = max(w.len - w.count + 1 + wt0, 0);       // cells that all its rows see
+
+        // The query row of this lane's column: its limit, and its operands
+        // times a power of two that brings the largest value to [2^11, 2^12)
+        const int r = r0 + n, t = token_of(p, min(r, p.R - 1));
         const bool valid = r < p.R && t < w.count;
-        limit[u] = valid ? w.len - w.count + 1 + t : w.limit;
-        float4 x[4][2];
-        const char * qr = p.q + (int64_t) seq * p.q_nb3 + (int64_t) (valid ? t : 0) * p.q_nb1 +
-                          (int64_t) (h * p.G + (valid ? r - t * p.G : 0)) * p.q_nb2 + 32 * g;
-        float top = 0.0f;
+        const int limit = valid ? w.len - w.count + 1 + t : seen;
+        half8 q_hi[4], q_lo[4];
+        float fac, m = -AL_INF, l = 0.0f;
+        floatx4 acc[8];
+        {
+            float4 x[4][2];
+            const char * qr = ap.q + (int64_t) seq * ap.q_nb3 + (int64_t) (valid ? t : 0) * ap.q_nb1 +
+                              (int64_t) (h * ap.G + (valid ? r - t * ap.G : 0)) * ap.q_nb2 + 32 * g;
+            float top = 0.0f;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+            for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                x[kk][e] = *(const float4 *) (qr + 128 * kk + 16 * e);
-                if (!valid) x[kk][e] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-                top = fmaxf(fmaxf(fmaxf(top, fabsf(x[kk][e].x)), fmaxf(fabsf(x[kk][e].y), fabsf(x[kk][e].z))), fabsf(x[kk][e].w));
+                for (int e = 0; e < 2; ++e) {
+                    x[kk][e] = *(const float4 *) (qr + 128 * kk + 16 * e);
+                    if (!valid) x[kk][e] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+                    top = fmaxf(fmaxf(fmaxf(top, fabsf(x[kk][e].x)), fmaxf(fabsf(x[kk][e].y), fabsf(x[kk][e].z))), fabsf(x[kk][e].w));
+                }
+            top = colmax4(top);
+            // 2^(11 - exponent of top), within the normal range
+            const int ex = min(max((int) (__float_as_uint(top) >> 23), 12), 253) - 127;
+            const float up = __uint_as_float((uint32_t) (11 - ex + 127) << 23), down = __uint_as_float((uint32_t) (ex - 11 + 127) << 23);
+            fac = p.scale * down;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                const float y[8] = {x[kk][0].x, x[kk][0].y, x[kk][0].z, x[kk][0].w, x[kk][1].x, x[kk][1].y, x[kk][1].z, x[kk][1].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float z = y[e] * up;
+                    const _Float16 hi = (_Float16) z;
+                    q_hi[kk][e] = hi;
+                    q_lo[kk][e] = (_Float16) (z - (float) hi);
+                }
             }
-        top = colmax4(top);
-        // 2^(11 - exponent of top), within the normal range
-        const int ex = min(max((int) (__float_as_uint(top) >> 23), 12), 253) - 127;
-        const float up = __uint_as_float((uint32_t) (11 - ex + 127) << 23), down = __uint_as_float((uint32_t) (ex - 11 + 127) << 23);
-        fac[u] = p.scale * down;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            const float y[8] = {x[kk][0].x, x[kk][0].y, x[kk][0].z, x[kk][0].w, x[kk][1].x, x[kk][1].y, x[kk][1].z, x[kk][1].w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float z = y[e] * up;
-                const _Float16 hi = (_Float16) z;
-                q_hi[u][kk][e] = hi;
-                q_lo[u][kk][e] = (_Float16) (z - (float) hi);
-            }
+            for (int j = 0; j < 8; ++j) acc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        m[u] = -AL_INF;
-        l[u] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[u][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const int least = max(w.len - w.count + 1 + t0, 0);         // cells that every row of the group sees
 
-    // Pages of a tile's cells: K by lanes n (group n / 4), V by lanes g. Cells
-    // past the last group that anyone sees are taken from that group.
-    struct Where {
-        int k_page, v_page;
-        int k_cell, v_cell;                                      // in the page
-    };
-    const int32_t * table = p.c.table + (int64_t) seq * p.c.t_nb1;
-    const uint32_t last_group = (uint32_t) max(w.limit - 1, 0) / 8;
-    auto look_up = [&](const int tile) {
-        Where a;
-        const uint32_t kg = min((uint32_t) tile * 4 + (n >> 2), last_group), vg = min((uint32_t) tile * 4 + g, last_group);
-        const uint32_t kp = page_of_group(p.c, kg), vp = page_of_group(p.c, vg);
-        a.k_page = table[kp];
-        a.v_page = table[vp];
-        a.k_cell = (int) (kg - kp * p.c.groups) * 8 + (n & 3);
-        a.v_cell = (int) (vg - vp * p.c.groups) * 8;
-        return a;
-    };
-    auto page = [&](const int x) {
-        const bool ok = (uint32_t) x < (uint32_t) p.c.n_pages;
-        bad |= !ok;
-        return ok ? x : 0;
-    };
-    const char * k_head = p.c.k + (int64_t) h * p.c.k_nb2 + 16 * g;
-    const char * v_head = p.c.v + (int64_t) h * p.c.v_nb2 + 16 * n;
-    half8 k[2][4];
-    u32x4 v[8];
-    auto load_k = [&](const Where & a) {
-        const char * b = k_head + page(a.k_page) * p.c.k_nb3 + a.k_cell * p.c.k_nb1;
+        // Pages of a tile's cells: K by lanes n (group n / 4), V by lanes g.
+        // Cells past the last group that the wave sees are taken from that one.
+        struct Where {
+            int k_page, v_page;
+            int k_cell, v_cell;                                      // in the page
+        };
+        const int32_t * table = p.c.table + (int64_t) seq * p.c.t_nb1;
+        const uint32_t last_group = (uint32_t) max(seen - 1, 0) / 8;
+        auto look_up = [&](const int tile) {
+            Where a;
+            const uint32_t kg = min((uint32_t) tile * 4 + (n >> 2), last_group), vg = min((uint32_t) tile * 4 + g, last_group);
+            const uint32_t kp = page_of_group(p.c, kg), vp = page_of_group(p.c, vg);
+            a.k_page = table[kp];
+            a.v_page = table[vp];
+            a.k_cell = (int) (kg - kp * p.c.groups) * 8 + (n & 3);
+            a.v_cell = (int) (vg - vp * p.c.groups) * 8;
+            return a;
+        };
+        auto page = [&](const int x) {
+            const bool ok = (uint32_t) x < (uint32_t) p.c.n_pages;
+            bad |= !ok;
+            return ok ? x : 0;
+        };
+        const char * k_head = p.c.k + (int64_t) h * p.c.k_nb2 + 16 * g;
+        const char * v_head = p.c.v + (int64_t) h * p.c.v_nb2 + 16 * n;
+        half8 k[2][4];
+        u32x4 v[8];
+        auto load_k = [&](const Where & a) {
+            const char * x = k_head + page(a.k_page) * p.c.k_nb3 + a.k_cell * p.c.k_nb1;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) k[e][kk] = *(const half8 *) (b + 4 * e * p.c.k_nb1 + 64 * kk);
-    };
-    auto load_v = [&](const Where & a) {
-        const char * b = v_head + page(a.v_page) * p.c.v_nb3 + a.v_cell * p.c.v_nb1;
+                for (int kk = 0; kk < 4; ++kk) k[e][kk] = *(const half8 *) (x + 4 * e * p.c.k_nb1 + 64 * kk);
+        };
+        auto load_v = [&](const Where & a) {
+            const char * x = v_head + page(a.v_page) * p.c.v_nb3 + a.v_cell * p.c.v_nb1;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = *(const u32x4 *) (b + i * p.c.v_nb1);
-    };
-    // V^T operand of dims 8 n + j: this lane's 8 cells of dim j
-    auto v_operand = [&](const int j) {
-        u32x4 a;
+            for (int i = 0; i < 8; ++i) v[i] = *(const u32x4 *) (x + i * p.c.v_nb1);
+        };
+        // V^T operand of dims 8 n + j: this lane's 8 cells of dim j
+        auto v_operand = [&](const int j) {
+            u32x4 a;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            a[i] = __builtin_amdgcn_perm(v[2 * i + 1][j / 2], v[2 * i][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-        return as_half8(a);
-    };
-
-    floatx4 s[NR][2];
-    auto scores = [&]() {
-#pragma unroll
-        for (int u = 0; u < NR; ++u)
+            for (int i = 0; i < 4; ++i)
+                a[i] = __builtin_amdgcn_perm(v[2 * i + 1][j / 2], v[2 * i][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+            return as_half8(a);
+        };
+        floatx4 s[2];
+        auto scores = [&]() {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                s[u][e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                s[e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) s[u][e] = mfma_16x16x32(k[e][kk], q_lo[u][kk], s[u][e]);
+                for (int kk = 0; kk < 4; ++kk) s[e] = mfma_16x16x32(k[e][kk], q_lo[kk], s[e]);
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) s[u][e] = mfma_16x16x32(k[e][kk], q_hi[u][kk], s[u][e]);
+                for (int kk = 0; kk < 4; ++kk) s[e] = mfma_16x16x32(k[e][kk], q_hi[kk], s[e]);
             }
-    };
-    half8 p_hi[NR], p_lo[NR];
-    // Probabilities of the tile against the rows' running maxima.
-    auto softmax = [&](const int tile) {
-        const int c0 = tile * kTile + 8 * g;
-        const bool masked = (tile + 1) * kTile > least;          // some row does not see all of it
-#pragma unroll
-        for (int u = 0; u < NR; ++u) {
+        };
+        half8 p_hi, p_lo;
+        // Probabilities of the tile against the rows' running maxima.
+        auto softmax = [&](const int tile) {
+            const int c0 = tile * kTile + 8 * g;
+            const bool masked = (tile + 1) * kTile > least;          // some row does not see all of it
             float x[8];
             float top = -AL_INF;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x[i] = s[u][i / 4][i % 4] * fac[u];
+                x[i] = s[i / 4][i % 4] * fac;
                 if constexpr (CAP) x[i] = p.softcap * tanhf(x[i] / p.softcap);
             }
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (c0 + i >= limit[u]) x[i] = -AL_INF;
+                    if (c0 + i >= limit) x[i] = -AL_INF;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
-            if (__any(top > m[u])) {
-                top = fmaxf(m[u], colmax4(top));
-                const float r = top > m[u] ? exp_fast(m[u] - top) : 1.0f;
-                m[u] = top;
-                l[u] *= r;
+            if (__any(top > m)) {
+                top = fmaxf(m, colmax4(top));
+                const float f = top > m ? exp_fast(m - top) : 1.0f;
+                m = top;
+                l *= f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[u][j] *= r;
+                for (int j = 0; j < 8; ++j) acc[j] *= f;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float e = exp_fast(x[i] - m[u]) * kPScale;
-                if (masked && c0 + i >= limit[u]) e = 0.0f;
-                l[u] += e;
+                float e = exp_fast(x[i] - m) * kPScale;
+                if (masked && c0 + i >= limit) e = 0.0f;
+                l += e;
                 const _Float16 hi = (_Float16) e;
-                p_hi[u][i] = hi;
-                p_lo[u][i] = (_Float16) (e - (float) hi);
+                p_hi[i] = hi;
+                p_lo[i] = (_Float16) (e - (float) hi);
             }
-        }
-    };
-    // o += P V of the tile. Cells past the sequence's last are stale memory:
-    // zeroed, as 0 times NaN is not 0. So are, row by row, the cells that only
-    // later tokens of the group see, where they hold no finite value.
-    auto product = [&](const int tile) {
-        if ((tile + 1) * kTile > least) {
-            const int c0 = tile * kTile + 8 * g;
-            bool odd = false;
+        };
+        // o += P V of the tile. Cells past the wave's last are stale memory:
+        // zeroed, as 0 times NaN is not 0. So are, one by one, the values that
+        // are not finite of cells that some row does not see; the rows that do
+        // see one get NaN in its dim, found by a product of ones.
+        auto product = [&](const int tile) {
+            if ((tile + 1) * kTile > least) {
+                const int c0 = tile * kTile + 8 * g;
+                uint32_t odd[2] = {0, 0};                            // bit 8 (i % 4) + j of word i / 4: cell i, dim j
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (c0 + i >= w.limit) v[i] = u32x4{0, 0, 0, 0};
+                for (int i = 0; i < 8; ++i) {
+                    if (c0 + i >= seen) v[i] = u32x4{0, 0, 0, 0};
+                    if (c0 + i >= least)
 #pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    odd |= c0 + i >= least && ((v[i][d] & 0x7c00u) == 0x7c00u || (v[i][d] & 0x7c000000u) == 0x7c000000u);
-            }
-            if (__any(odd)) {
-                for (int t = t0; t <= t1; ++t) {
-                    const int lim = w.len - w.count + 1 + t;
-                    u32x4 keep[8];
+                        for (int d = 0; d < 4; ++d) {
+                            if ((v[i][d] & 0x7c00u) == 0x7c00u) odd[i / 4] |= 1u << (8 * (i % 4) + 2 * d), v[i][d] &= 0xffff0000u;
+                            if ((v[i][d] & 0x7c000000u) == 0x7c000000u) odd[i / 4] |= 2u << (8 * (i % 4) + 2 * d), v[i][d] &= 0xffffu;
+                        }
+                }
+                if (__any((odd[0] | odd[1]) != 0)) {
+                    half8 sees;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        keep[i] = v[i];
-                        if (c0 + i >= lim) v[i] = u32x4{0, 0, 0, 0};
-                    }
+                    for (int i = 0; i < 8; ++i) sees[i] = c0 + i < limit ? (_Float16) 1.0f : (_Float16) 0.0f;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const half8 a = v_operand(j);
+                        half8 a;
 #pragma unroll
-                        for (int u = 0; u < NR; ++u) {
-                            const floatx4 x = mfma_16x16x32(a, p_hi[u], mfma_16x16x32(a, p_lo[u], acc[u][j]));
-                            if (limit[u] == lim) acc[u][j] = x;
-                        }
+                        for (int i = 0; i < 8; ++i) a[i] = odd[i / 4] >> (8 * (i % 4) + j) & 1 ? (_Float16) 1.0f : (_Float16) 0.0f;
+                        const floatx4 x = mfma_16x16x32(a, sees, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (x[e] > 0.0f) acc[j][e] = __builtin_nanf("");
                     }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = keep[i];
                 }
-                return;
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const half8 a = v_operand(j);
-#pragma unroll
-            for (int u = 0; u < NR; ++u) acc[u][j] = mfma_16x16x32(a, p_hi[u], mfma_16x16x32(a, p_lo[u], acc[u][j]));
-        }
-    };
+            for (int j = 0; j < 8; ++j) {
+                const half8 a = v_operand(j);
+                acc[j] = mfma_16x16x32(a, p_hi, mfma_16x16x32(a, p_lo, acc[j]));
+            }
+        };
 
-    // The wave's tiles, every kWaves-th of the chunk. The next tile's K is
-    // loaded once this one's scores are done, its V once this one's product
-    // is; pages are looked up a tile earlier. The last tile is a copy of its
-    // own, so that no branch around the loads makes the compiler wait for all
-    // of them.
-    if (first + wave < end) {
-        int tile = first + wave;
-        Where next = look_up(tile);
-        load_k(next);
-        load_v(next);
-        next = look_up(tile + kWaves);
-        for (; tile + kWaves < end; tile += kWaves) {
-            const Where after = look_up(tile + 2 * kWaves);
+        // The wave's tiles. The next tile's K is loaded once this one's scores
+        // are done, its V once this one's product is; pages are looked up a
+        // tile earlier (the first two before any K: a page that is waited for
+        // waits for all that was loaded before it). The last tile is a copy of
+        // its own, so that no branch around the loads makes the compiler wait
+        // for all of them.
+        const int wave_end = min(end, seen > 0 ? (seen + kTile - 1) / kTile : 0);
+        if (first + cw < wave_end) {
+            int tile = first + cw;
+            const Where here = look_up(tile);
+            Where next = look_up(tile + kCellWaves);
+            asm volatile("" ::: "memory");
+            load_k(here);
+            load_v(here);
+            for (; tile + kCellWaves < wave_end; tile += kCellWaves) {
+                const Where after = look_up(tile + 2 * kCellWaves);
+                scores();
+                load_k(next);
+                softmax(tile);
+                product(tile);
+                load_v(next);
+                next = after;
+            }
             scores();
-            load_k(next);
             softmax(tile);
             product(tile);
-            load_v(next);
-            next = after;
         }
-        scores();
-        softmax(tile);
-        product(tile);
-    }
 
-    // join the waves: maxima and sums, then the rescaled outputs through LDS
-    const bool any_bad = __any(bad);
-    if (any_bad && lane == 0 && !w.bad) paged_error(p.c, kPagedBadPage, seq);
-#pragma unroll
-    for (int u = 0; u < NR; ++u) {
-        l[u] = colsum4(l[u]);
-        if (any_bad) l[u] = __builtin_nanf("");
+        // join the row tile's waves: maxima and sums, then the rescaled outputs
+        // through LDS
+        const bool any_bad = __any(bad);
+        if (any_bad && lane == 0 && !w.bad) paged_error(p.c, kPagedBadPage, seq);
+        l = colsum4(l);
+        if (any_bad) l = __builtin_nanf("");
         if (g == 0) {
-            ml_lds[u][wave][n][0] = m[u];
-            ml_lds[u][wave][n][1] = l[u];
-        }
-    }
-    __syncthreads();
-    const int row = threadIdx.x >> 4, dim = (threadIdx.x & 15) * 8;
-    char * rec = const_cast<char *>(record(p, unit, blockIdx.x, 16 * NR));
-#pragma unroll
-    for (int u = 0; u < NR; ++u) {
-        float M = ml_lds[u][0][n][0];
-#pragma unroll
-        for (int i = 1; i < kWaves; ++i) M = fmaxf(M, ml_lds[u][i][n][0]);
-        const float f = m[u] == M ? 1.0f : exp_fast(m[u] - M);
-        if (u) __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float4 a = {acc[u][0][i] * f, acc[u][1][i] * f, acc[u][2][i] * f, acc[u][3][i] * f};
-            float4 b = {acc[u][4][i] * f, acc[u][5][i] * f, acc[u][6][i] * f, acc[u][7][i] * f};
-            *(float4 *) &o_lds[wave][n][8 * (4 * g + i)] = a;
-            *(float4 *) &o_lds[wave][n][8 * (4 * g + i) + 4] = b;
+            ml_lds[wave][n][0] = m;
+            ml_lds[wave][n][1] = l;
         }
         __syncthreads();
-        float Mr = ml_lds[u][0][row][0], L = 0.0f;
+        {
+            float M = m;
 #pragma unroll
-        for (int i = 1; i < kWaves; ++i) Mr = fmaxf(Mr, ml_lds[u][i][row][0]);
-        float o[8] = {};
+            for (int i = 0; i < kCellWaves; ++i) M = fmaxf(M, ml_lds[rt * kCellWaves + i][n][0]);
+            const float f = grow(m, M);
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            const float mi = ml_lds[u][i][row][0];
-            L += ml_lds[u][i][row][1] * (mi == Mr ? 1.0f : exp_fast(mi - Mr));
+            for (int i = 0; i < 4; ++i) {
+                *(float4 *) &o_lds[wave][n][8 * (4 * g + i)] = float4{acc[0][i] * f, acc[1][i] * f, acc[2][i] * f, acc[3][i] * f};
+                *(float4 *) &o_lds[wave][n][8 * (4 * g + i) + 4] = float4{acc[4][i] * f, acc[5][i] * f, acc[6][i] * f, acc[7][i] * f};
+            }
+        }
+        __syncthreads();
+        const auto & ep = arguments();
+        char * rec = record(ep, unit, blockIdx.x, first == 0 ? 1 : 0);
+        for (int item = threadIdx.x; item < 16 * ROWT * 16; item += 64 * kWaves) {
+            const int row = item >> 4, dim = (item & 15) * 8;        // of the group
+            const int w0 = row / 16 * kCellWaves, rr = row % 16;
+            const int gr = group0 + row, tok = token_of(ep, min(gr, ep.R - 1));
+            if (gr >= ep.R || tok >= w.count) continue;
+            float M = ml_lds[w0][rr][0], L = 0.0f, o[8] = {};
 #pragma unroll
-            for (int d = 0; d < 8; ++d) o[d] += o_lds[i][row][dim + d];
+            for (int i = 1; i < kCellWaves; ++i) M = fmaxf(M, ml_lds[w0 + i][rr][0]);
+#pragma unroll
+            for (int i = 0; i < kCellWaves; ++i) {
+                L += ml_lds[w0 + i][rr][1] * grow(ml_lds[w0 + i][rr][0], M);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) o[d] += o_lds[w0 + i][rr][dim + d];
+            }
+            float * d;
+            float f = 1.0f;
+            if (whole) {
+                const int head = h * ep.G + gr - tok * ep.G;
+                f = row_factor(ep, M, L, head);
+                d = (float *) (ep.dst + (int64_t) seq * ep.d_nb3 + (int64_t) tok * ep.d_nb2 + (int64_t) head * ep.d_nb1) + dim;
+            } else {
+                d = (float *) rec + row * 128 + dim;
+                if (dim == 0) *(float2 *) ((float *) rec + 16 * ROWT * 128 + row * 2) = float2{M, L};
+            }
+            *(float4 *) d = float4{o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+            *(float4 *) (d + 4) = float4{o[4] * f, o[5] * f, o[6] * f, o[7] * f};
         }
-        const int r = r0 + 16 * u + row;
-        const int t = p.G == 1 ? r : (int) __umulhi((uint32_t) r, p.g_magic);
-        if (r >= p.R || t >= w.count) continue;
-        if (n_chunks > 1) {
-            float * d = (float *) rec + (16 * u + row) * 128 + dim;
-            *(float4 *) d = float4{o[0], o[1], o[2], o[3]};
-            *(float4 *) (d + 4) = float4{o[4], o[5], o[6], o[7]};
-            if (dim == 0) *(float2 *) ((float *) rec + 16 * NR * 128 + (16 * u + row) * 2) = float2{Mr, L};
-            continue;
-        }
-        const int head = h * p.G + r - t * p.G;
-        // the sink as one more logit, without a value
-        L *= 1.0f / kPScale;
-        float up = 1.0f / kPScale;
-        if (p.sinks) {
-            const float sink = p.sinks[head], top = fmaxf(Mr, sink);
-            const float e = Mr == top ? 1.0f : exp_fast(Mr - top);
-            up *= e;
-            L = L * e + (sink == top ? 1.0f : exp_fast(sink - top));
-        }
-        const float inv = L == 0.0f ? 0.0f : up / L;
-        float * d = (float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) head * p.d_nb1) + dim;
-        *(float4 *) d = float4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        *(float4 *) (d + 4) = float4{o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv};
+        if (at < stop) __syncthreads();                              // the LDS is free for the next piece
     }
 }
 
-// Joins the chunks' parts: a workgroup per sequence and unit, a wave per row,
-// two dims to a lane.
-template <int NR>
+// Joins the pieces of the sequences that have several. p.row_waves waves (1 or
+// kWaves) take a row, the halves of a wave every second piece, 4 dims to a
+// lane; all loads of 8 of a half's pieces are in flight together.
 __global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(const PagedFattnParams p) {
+    __shared__ __attribute__((aligned(16))) float o_lds[kWaves][132];
     prefetch_params(p);
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, half = lane >> 5, d4 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int seq = blockIdx.x, unit = blockIdx.y, h = unit % p.Hkv, r0 = unit / p.Hkv * (16 * NR);
-    int t0, t1;
-    group_tokens(p, r0, 16 * NR, t0, t1);
-    const int C = chunk_tiles(p, lane, t0, t1);
-    const SeqWork w = seq_work(p, seq, t0, t1);
-    const int n_chunks = chunks_of(w, C);
-    if (n_chunks < 2) return;
-    int before = 0;
-    for (int s = lane; s < seq; s += 64) before += chunks_of(seq_work(p, s, t0, t1), C);
-    before = wave_sum_int(before);
-    for (int row = wave; row < 16 * NR; row += kWaves) {
-        const int r = r0 + row;
-        const int t = p.G == 1 ? r : (int) __umulhi((uint32_t) r, p.g_magic);
-        if (r >= p.R || t >= w.count) break;
-        const char * rec = record(p, unit, before, 16 * NR);
-        const int64_t step = 16 * NR * 130 * 4;
-        float M = -AL_INF;
-        for (int i = lane; i < n_chunks; i += 64) M = fmaxf(M, *(const float *) (rec + i * step + (16 * NR * 128 + row * 2) * 4));
+    const int rows = 16 * p.row_tiles, row_waves = p.row_waves;
+    const int seq = blockIdx.y, unit = blockIdx.z, h = unit % p.Hkv, group0 = unit / p.Hkv * rows;
+    const int row = row_waves == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
+    const int gr = group0 + row, t = token_of(p, min(gr, p.R - 1));
+    const int2 info = p.info[(int64_t) unit * p.c.n_seq + seq];
+    const int count = p.counts ? p.counts[seq] : p.T;
+    // (no row of the group: nothing was written to info)
+    const int t0 = token_of(p, group0);
+    if (min(count, p.T) <= t0 || info.y < 2) return;
+    const bool mine = gr < p.R && row < rows && t < min(count, p.T);
+    float M = -AL_INF, L = 0.0f;
+    float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine) {
+        for (int i0 = row_waves == 1 ? 0 : 16 * wave; i0 < info.y; i0 += 16 * row_waves) {
+            float2 ml[8];
+            float4 x[8];
 #pragma unroll
-        for (int o = 32; o >= 1; o /= 2) M = fmaxf(M, __shfl_xor(M, o));
-        float L = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < n_chunks; ++i) {
-            const float2 ml = *(const float2 *) (rec + i * step + (16 * NR * 128 + row * 2) * 4);
-            const float2 o = *(const float2 *) (rec + i * step + (row * 128 + 2 * lane) * 4);
-            const float e = ml.x == M ? 1.0f : exp_fast(ml.x - M);
-            L += ml.y * e;
-            x += o.x * e;
-            y += o.y * e;
+            for (int i = 0; i < 8; ++i) {
+                const int c = min(i0 + 2 * i + half, info.y - 1);
+                const char * rec = record(p, unit, info.x + c, c == 0 ? 1 : 0);
+                ml[i] = *(const float2 *) ((const float *) rec + rows * 128 + row * 2);
+                x[i] = *(const float4 *) ((const float *) rec + row * 128 + 4 * d4);
+            }
+            asm volatile("" ::: "memory");
+            float top = M;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i0 + 2 * i + half < info.y) top = fmaxf(top, ml[i].x);
+            const float f = grow(M, top);
+            L *= f; o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+            M = top;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i0 + 2 * i + half < info.y) {
+                    const float e = grow(ml[i].x, M);
+                    L += ml[i].y * e;
+                    o.x += x[i].x * e; o.y += x[i].y * e; o.z += x[i].z * e; o.w += x[i].w * e;
+                }
         }
-        const int head = h * p.G + r - t * p.G;
-        L *= 1.0f / kPScale;
-        float up = 1.0f / kPScale;
-        if (p.sinks) {
-            const float sink = p.sinks[head], top = fmaxf(M, sink);
-            const float e = M == top ? 1.0f : exp_fast(M - top);
-            up *= e;
-            L = L * e + (sink == top ? 1.0f : exp_fast(sink - top));
-        }
-        const float inv = L == 0.0f ? 0.0f : up / L;
-        *(float2 *) ((float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) head * p.d_nb1) + 2 * lane) =
-            float2{x * inv, y * inv};
     }
+    // the wave's halves, then the row's waves
+    {
+        const float M2 = __shfl_xor(M, 32), L2 = __shfl_xor(L, 32);
+        const float4 o2 = {__shfl_xor(o.x, 32), __shfl_xor(o.y, 32), __shfl_xor(o.z, 32), __shfl_xor(o.w, 32)};
+        const float top = fmaxf(M, M2), f = grow(M, top), f2 = grow(M2, top);
+        M = top;
+        L = half ? L2 * f2 + L * f : L * f + L2 * f2;
+        o = half ? float4{o2.x * f2 + o.x * f, o2.y * f2 + o.y * f, o2.z * f2 + o.z * f, o2.w * f2 + o.w * f}
+                 : float4{o.x * f + o2.x * f2, o.y * f + o2.y * f2, o.z * f + o2.z * f2, o.w * f + o2.w * f2};
+    }
+    if (row_waves > 1) {
+        if (half == 0) {
+            *(float4 *) &o_lds[wave][4 * d4] = o;
+            if (d4 == 0) o_lds[wave][128] = M, o_lds[wave][129] = L;
+        }
+        __syncthreads();
+        if (wave) return;
+        float top = M;
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, o_lds[i][128]);
+        L = 0.0f;
+        o = float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const float f = grow(o_lds[i][128], top);
+            const float4 x = *(const float4 *) &o_lds[i][4 * d4];
+            L += o_lds[i][129] * f;
+            o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+        }
+        M = top;
+    }
+    if (!mine || half) return;
+    const int head = h * p.G + gr - t * p.G;
+    const float f = row_factor(p, M, L, head);
+    *(float4 *) ((float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) head * p.d_nb1) + 4 * d4) =
+        float4{o.x * f, o.y * f, o.z * f, o.w * f};
 }
 
 struct Plan {
     PagedFattnParams p;
-    int nr = 1;
     bool empty = false;
-    size_t bytes = 0;                                   // records
+    size_t info_bytes = 0, bytes = 0;                   // of the info, of it and the records
 };
 
 bool aligned16(const al_tensor & t, int from) {
@@ -535,7 +614,7 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     if (a->sinks.data && (a->sinks.type != AL_TYPE_F32 || a->sinks.ne[0] != Hq || a->sinks.nb[0] != 4))
         return al_fail(AL_ERR_INVALID, "paged_fattn: sinks must be f32 [Hq]");
     if (!(a->logit_softcap >= 0.0f)) return al_fail(AL_ERR_INVALID, "paged_fattn: softcap %g", (double) a->logit_softcap);
-    if (T > (1 << 16) || Hq > (1 << 12) || T * Hq > (1 << 22) || n_seq > (1 << 16))
+    if (T > (1 << 16) || Hq > (1 << 12) || T * Hq > (1 << 22) || n_seq > 65535)
         return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
     pl.empty = T == 0 || n_seq == 0;
     p.q = (const char *) q.data; p.q_nb1 = q.nb[1]; p.q_nb2 = q.nb[2]; p.q_nb3 = q.nb[3];
@@ -546,29 +625,41 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     p.T = (int32_t) T; p.G = (int32_t) (Hq / Hkv); p.Hkv = (int32_t) Hkv;
     p.R = p.T * p.G;
     p.g_magic = p.G > 1 ? (uint32_t) (((1ull << 32) + (uint64_t) p.G - 1) / (uint64_t) p.G) : 0u;
-    pl.nr = p.R <= 16 ? 1 : 2;
-    const int rows = 16 * pl.nr;
+    p.row_tiles = p.R <= 16 ? 1 : p.R <= 32 ? 2 : 4;
+    const int rows = 16 * p.row_tiles;
     p.row_groups = (p.R + rows - 1) / rows;
     const int64_t units = (int64_t) p.row_groups * Hkv;
     if (units > 65535) return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
-    p.target = (int32_t) std::max<int64_t>(1, (pl.nr == 1 ? 2 : 1) * (int64_t) n_cu / std::max<int64_t>(1, units));
-    const int64_t most = ((int64_t) p.c.max_pages * p.c.page_size + kTile * kMinTiles - 1) / (kTile * kMinTiles);   // chunks of a sequence
-    p.max_chunks = (int32_t) std::min<int64_t>(p.target + n_seq, n_seq * std::max<int64_t>(1, most));
+    const int64_t most = n_seq * std::max<int64_t>(1, ((int64_t) p.c.max_pages * p.c.page_size + kTile - 1) / kTile);   // tiles there can be
+    p.target = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) n_cu / std::max<int64_t>(1, units), (most + kMinTiles - 1) / kMinTiles));
+    // few sequences have many pieces each
+    p.row_waves = p.target > 16 * n_seq ? kWaves : 1;
     p.scale = a->scale;
     p.softcap = a->logit_softcap;
-    pl.bytes = (size_t) units * p.max_chunks * rows * 130 * 4;
+    pl.info_bytes = ((size_t) units * n_seq * sizeof(int2) + 255) / 256 * 256;
+    pl.bytes = pl.info_bytes + (size_t) units * p.target * 2 * rows * 130 * 4;
     *out = pl;
     return AL_OK;
 }
 
-template <int NR>
+template <int ROWT>
+void launch(const PagedFattnParams & p, hipStream_t st) {
+    const dim3 grid((unsigned) p.target, (unsigned) (p.row_groups * p.Hkv));
+    if (p.softcap != 0.0f) hipLaunchKernelGGL((paged_fattn_kernel<ROWT, true>), grid, dim3(64 * kWaves), 0, st, p);
+    else                   hipLaunchKernelGGL((paged_fattn_kernel<ROWT, false>), grid, dim3(64 * kWaves), 0, st, p);
+}
+
 hipError_t launch(const PagedFattnParams & p, hipStream_t st) {
-    const dim3 grid((unsigned) p.max_chunks, (unsigned) (p.row_groups * p.Hkv));
-    if (p.softcap != 0.0f) hipLaunchKernelGGL((paged_fattn_kernel<NR, true>), grid, dim3(64 * kWaves), 0, st, p);
-    else                   hipLaunchKernelGGL((paged_fattn_kernel<NR, false>), grid, dim3(64 * kWaves), 0, st, p);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_join_kernel<NR>), dim3((unsigned) p.c.n_seq, (unsigned) (p.row_groups * p.Hkv)), dim3(64 * kWaves), 0, st, p);
+    switch (p.row_tiles) {
+        case 1: launch<1>(p, st); break;
+        case 2: launch<2>(p, st); break;
+        default: launch<4>(p, st); break;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.target == 1) return e;                    // one workgroup a unit: no pieces
+    const int rows = std::min(16 * p.row_tiles, p.R);
+    const dim3 grid((unsigned) (p.row_waves == 1 ? (rows + kWaves - 1) / kWaves : rows), (unsigned) p.c.n_seq, (unsigned) (p.row_groups * p.Hkv));
+    hipLaunchKernelGGL(paged_join_kernel, grid, dim3(64 * kWaves), 0, st, p);
     return hipGetLastError();
 }
 
@@ -625,11 +716,12 @@ extern "C" int al_paged_fattn_f16(const al_paged_fattn_args * a) {
         if (a->workspace_bytes < pl.bytes || ((uintptr_t) a->workspace & 15u))
             return al_fail(AL_ERR_WORKSPACE, "paged_fattn: workspace %llu bytes (16-byte aligned) < %zu needed",
                            (unsigned long long) a->workspace_bytes, pl.bytes);
-        pl.p.part = (float *) a->workspace;
+        pl.p.info = (int2 *) a->workspace;
     } else {
-        rc = al_library_workspace(pl.bytes, a->stream, (void **) &pl.p.part);
+        rc = al_library_workspace(pl.bytes, a->stream, (void **) &pl.p.info);
         if (rc != AL_OK) return rc;
     }
-    const hipError_t e = pl.nr == 1 ? launch<1>(pl.p, (hipStream_t) a->stream) : launch<2>(pl.p, (hipStream_t) a->stream);
+    pl.p.part = (float *) ((char *) pl.p.info + pl.info_bytes);
+    const hipError_t e = launch(pl.p, (hipStream_t) a->stream);
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "paged_fattn: launch");
 }
