@@ -121,10 +121,17 @@ __device__ __forceinline__ int tiles_of(const int limit) {
     return limit < 0 ? 0 : max(1, (limit + kTile - 1) / kTile);
 }
 
-// First tile of a workgroup's part, of S tiles cut into W parts; and the
-// workgroup whose part holds tile x.
-__device__ __forceinline__ int part_begin(const int w, const int S, const int W) { return (int) ((int64_t) w * S / W); }
-__device__ __forceinline__ int part_of(const int x, const int S, const int W) { return (int) (((int64_t) (x + 1) * W + S - 1) / S) - 1; }
+// S tiles cut into W parts, the first S % W of them one tile longer: the first
+// tile of a part, and the part that holds a tile.
+struct Parts {
+    int each, longer;
+    __device__ __forceinline__ Parts(const int S, const int W) : each(S / W), longer(S - S / W * W) {}
+    __device__ __forceinline__ int begin(const int w) const { return w * each + min(w, longer); }
+    __device__ __forceinline__ int of(const int x) const {
+        const int y = x - longer * (each + 1);
+        return y < 0 ? x / (each + 1) : longer + y / each;
+    }
+};
 
 // Sequences 64 b .. 64 b + 63, one to a lane.
 struct Block {
@@ -184,7 +191,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rt = wave / kCellWaves, cw = wave % kCellWaves;
-    const int unit = blockIdx.y, h = unit % p.Hkv, group0 = unit / p.Hkv * (16 * ROWT);
+    // the heads of the same cells next to one another in the grid
+    const int units = p.row_groups * p.Hkv, unit = blockIdx.x % units, wg = blockIdx.x / units;
+    const int h = unit % p.Hkv, group0 = unit / p.Hkv * (16 * ROWT);
     // tokens of the group, and of the wave's row tile (empty past the last row)
     const int t0 = token_of(p, group0), t1 = token_of(p, min(group0 + 16 * ROWT, p.R) - 1);
     const int r0 = group0 + 16 * rt;
@@ -200,10 +209,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         S += x.total();
     }
     const int W = min(p.target, (S + kMinTiles - 1) / kMinTiles);
-    if ((int) blockIdx.x >= W) return;
-    const int stop = part_begin(blockIdx.x + 1, S, W);
+    if (wg >= W) return;
+    const Parts parts(S, W);
+    const int stop = parts.begin(wg + 1);
 
-    for (int at = part_begin(blockIdx.x, S, W); at < stop;) {
+    for (int at = parts.begin(wg); at < stop;) {
         // the sequence that holds tile `at`
         while (at >= before + b.total()) {
             before += b.total();
@@ -222,13 +232,52 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         if (threadIdx.x == 0) {
             if (first == 0)
                 ap.info[(int64_t) unit * ap.c.n_seq + seq] =
-                    int2{(int) blockIdx.x, whole ? 1 : part_of(base + tiles - 1, S, W) - (int) blockIdx.x + 1};
+                    int2{wg, whole ? 1 : parts.of(base + tiles - 1) - wg + 1};
             if (w.bad) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         bool bad = w.bad;
         const int seen = w.limit(wt0, wt1);                        // cells that the wave's last row sees
         const int least = max(w.len - w.count + 1 + wt0, 0);       // cells that all its rows see
 
+        // Pages of a tile's cells: K by lanes n (group n / 4), V by lanes g.
+        // Cells past the last group that the wave sees are taken from that one.
+        struct Where {
+            int k_page, v_page;
+            int k_cell, v_cell;                                      // in the page
+        };
+        const int32_t * table = p.c.table + (int64_t) seq * p.c.t_nb1;
+        const uint32_t last_group = (uint32_t) max(seen - 1, 0) / 8;
+        auto look_up = [&](const int tile) {
+            Where a;
+            const uint32_t kg = min((uint32_t) tile * 4 + (n >> 2), last_group), vg = min((uint32_t) tile * 4 + g, last_group);
+            const uint32_t kp = page_of_group(p.c, kg), vp = page_of_group(p.c, vg);
+            a.k_page = table[kp];
+            a.v_page = table[vp];
+            a.k_cell = (int) (kg - kp * p.c.groups) * 8 + (n & 3);
+            a.v_cell = (int) (vg - vp * p.c.groups) * 8;
+            return a;
+        };
+        auto page = [&](const int x, const bool used) {
+            const bool ok = (uint32_t) x < (uint32_t) p.c.n_pages;
+            bad |= !ok && used;
+            return ok ? x : 0;
+        };
+        const char * k_head = p.c.k + (int64_t) h * p.c.k_nb2 + 16 * g;
+        const char * v_head = p.c.v + (int64_t) h * p.c.v_nb2 + 16 * n;
+        half8 k[2][4];
+        u32x4 v[8];
+        auto load_k = [&](const Where & a, const bool used) {
+            const char * x = k_head + page(a.k_page, used) * p.c.k_nb3 + a.k_cell * p.c.k_nb1;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) k[e][kk] = *(const half8 *) (x + 4 * e * p.c.k_nb1 + 64 * kk);
+        };
+        auto load_v = [&](const Where & a, const bool used) {
+            const char * x = v_head + page(a.v_page, used) * p.c.v_nb3 + a.v_cell * p.c.v_nb1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = *(const u32x4 *) (x + i * p.c.v_nb1);
+        };
         // The query row of this lane's column: its limit, and its operands
         // times a power of two that brings the largest value to [2^11, 2^12)
         const int r = r0 + n, t = token_of(p, min(r, p.R - 1));
@@ -237,16 +286,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         half8 q_hi[4], q_lo[4];
         float fac, m = -AL_INF, l = 0.0f;
         floatx4 acc[8];
+        // Everything that the first tile needs goes out before anything is
+        // computed: pages, query rows, then K and V (a wave without a tile
+        // loads another wave's and uses none of it).
+        const int wave_end = min(end, seen > 0 ? (seen + kTile - 1) / kTile : 0);
+        const bool has = first + cw < wave_end;
+        int tile = has ? first + cw : max(wave_end - 1, 0);
+        const Where here = look_up(tile);
+        Where next = look_up(tile + kCellWaves);
+        asm volatile("" ::: "memory");
+        float4 x[4][2];
         {
-            float4 x[4][2];
             const char * qr = ap.q + (int64_t) seq * ap.q_nb3 + (int64_t) (valid ? t : 0) * ap.q_nb1 +
                               (int64_t) (h * ap.G + (valid ? r - t * ap.G : 0)) * ap.q_nb2 + 32 * g;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[kk][e] = *(const float4 *) (qr + 128 * kk + 16 * e);
+        }
+        asm volatile("" ::: "memory");
+        load_k(here, has);
+        load_v(here, has);
+        asm volatile("" ::: "memory");
+        {
             float top = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    x[kk][e] = *(const float4 *) (qr + 128 * kk + 16 * e);
                     if (!valid) x[kk][e] = float4{0.0f, 0.0f, 0.0f, 0.0f};
                     top = fmaxf(fmaxf(fmaxf(top, fabsf(x[kk][e].x)), fmaxf(fabsf(x[kk][e].y), fabsf(x[kk][e].z))), fabsf(x[kk][e].w));
                 }
@@ -270,45 +337,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
             for (int j = 0; j < 8; ++j) acc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        // Pages of a tile's cells: K by lanes n (group n / 4), V by lanes g.
-        // Cells past the last group that the wave sees are taken from that one.
-        struct Where {
-            int k_page, v_page;
-            int k_cell, v_cell;                                      // in the page
-        };
-        const int32_t * table = p.c.table + (int64_t) seq * p.c.t_nb1;
-        const uint32_t last_group = (uint32_t) max(seen - 1, 0) / 8;
-        auto look_up = [&](const int tile) {
-            Where a;
-            const uint32_t kg = min((uint32_t) tile * 4 + (n >> 2), last_group), vg = min((uint32_t) tile * 4 + g, last_group);
-            const uint32_t kp = page_of_group(p.c, kg), vp = page_of_group(p.c, vg);
-            a.k_page = table[kp];
-            a.v_page = table[vp];
-            a.k_cell = (int) (kg - kp * p.c.groups) * 8 + (n & 3);
-            a.v_cell = (int) (vg - vp * p.c.groups) * 8;
-            return a;
-        };
-        auto page = [&](const int x) {
-            const bool ok = (uint32_t) x < (uint32_t) p.c.n_pages;
-            bad |= !ok;
-            return ok ? x : 0;
-        };
-        const char * k_head = p.c.k + (int64_t) h * p.c.k_nb2 + 16 * g;
-        const char * v_head = p.c.v + (int64_t) h * p.c.v_nb2 + 16 * n;
-        half8 k[2][4];
-        u32x4 v[8];
-        auto load_k = [&](const Where & a) {
-            const char * x = k_head + page(a.k_page) * p.c.k_nb3 + a.k_cell * p.c.k_nb1;
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) k[e][kk] = *(const half8 *) (x + 4 * e * p.c.k_nb1 + 64 * kk);
-        };
-        auto load_v = [&](const Where & a) {
-            const char * x = v_head + page(a.v_page) * p.c.v_nb3 + a.v_cell * p.c.v_nb1;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = *(const u32x4 *) (x + i * p.c.v_nb1);
-        };
         // V^T operand of dims 8 n + j: this lane's 8 cells of dim j
         auto v_operand = [&](const int j) {
             u32x4 a;
@@ -412,21 +440,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         // waits for all that was loaded before it). The last tile is a copy of
         // its own, so that no branch around the loads makes the compiler wait
         // for all of them.
-        const int wave_end = min(end, seen > 0 ? (seen + kTile - 1) / kTile : 0);
-        if (first + cw < wave_end) {
-            int tile = first + cw;
-            const Where here = look_up(tile);
-            Where next = look_up(tile + kCellWaves);
-            asm volatile("" ::: "memory");
-            load_k(here);
-            load_v(here);
+        if (has) {
             for (; tile + kCellWaves < wave_end; tile += kCellWaves) {
                 const Where after = look_up(tile + 2 * kCellWaves);
                 scores();
-                load_k(next);
+                load_k(next, true);
                 softmax(tile);
                 product(tile);
-                load_v(next);
+                load_v(next, true);
                 next = after;
             }
             scores();
@@ -458,7 +479,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         }
         __syncthreads();
         const auto & ep = arguments();
-        char * rec = record(ep, unit, blockIdx.x, first == 0 ? 1 : 0);
+        char * rec = record(ep, unit, wg, first == 0 ? 1 : 0);
         for (int item = threadIdx.x; item < 16 * ROWT * 16; item += 64 * kWaves) {
             const int row = item >> 4, dim = (item & 15) * 8;        // of the group
             const int w0 = row / 16 * kCellWaves, rr = row % 16;
@@ -644,7 +665,7 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
 
 template <int ROWT>
 void launch(const PagedFattnParams & p, hipStream_t st) {
-    const dim3 grid((unsigned) p.target, (unsigned) (p.row_groups * p.Hkv));
+    const dim3 grid((unsigned) (p.target * p.row_groups * p.Hkv));
     if (p.softcap != 0.0f) hipLaunchKernelGGL((paged_fattn_kernel<ROWT, true>), grid, dim3(64 * kWaves), 0, st, p);
     else                   hipLaunchKernelGGL((paged_fattn_kernel<ROWT, false>), grid, dim3(64 * kWaves), 0, st, p);
 }
