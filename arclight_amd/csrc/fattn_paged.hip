@@ -398,12 +398,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         // are not finite of cells that some row does not see; the rows that do
         // see one get NaN in its dim, found by a product of ones.
         auto product = [&](const int tile) {
-            if ((tile + 1) * kTile > least) {
-                const int c0 = tile * kTile + 8 * g;
+            const int c0 = tile * kTile + 8 * g;
+            if ((tile + 1) * kTile > seen) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c0 + i >= seen) v[i] = u32x4{0, 0, 0, 0};
+            }
+            if (least < seen && (tile + 1) * kTile > least) {        // (one token: never)
                 uint32_t odd[2] = {0, 0};                            // bit 8 (i % 4) + j of word i / 4: cell i, dim j
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (c0 + i >= seen) v[i] = u32x4{0, 0, 0, 0};
                     if (c0 + i >= least)
 #pragma unroll
                         for (int d = 0; d < 4; ++d) {
