@@ -8,15 +8,16 @@
 // any size keep their bits. Two f16 products of 16 x 16 x 32 take an eighth of
 // the matrix cores' time that f32 products (16 x 16 x 4) do.
 //
-// Rows are taken in tiles of 16. A tile's columns (its rows of x) are
-// independent in both products, so a tile of several adapters is computed
-// once for each of them and every column kept from its own adapter's: right
-// for any order of the ids, and done once where, as in a prompt, the rows of
-// a tile share one.
+// The products take 16 rows at a time, of one adapter: out of 64 rows at a time
+// those of each adapter are picked, in any order (rows that lie next to one
+// another, as a prompt's, come out as they are), so that A and B are read once
+// for 16 of them.
 //
-// Two launches: lora_shrink_kernel (v, K split over workgroups, partial sums
-// into the workspace) and lora_expand_kernel (sums the parts, then a slice of
-// the outputs).
+// Two launches: the first product into the workspace, K split over workgroups
+// where there are few rows, then the second, which sums the parts, for a slice
+// of the outputs. (Beside the Q4_0 projection: parts of its launches.) 300 rows
+// of 2048 -> 8192 in the order of their requests, ranks to 64: 13.6 us;
+// shuffled over 12 adapters 18.2, as every group of 16 rows then is of another.
 
 #include <hip/hip_runtime.h>
 
@@ -37,249 +38,171 @@ using namespace lora;
 constexpr int kWaves = 4;
 constexpr int kCols = 256;                      // outputs of a workgroup
 
-// The rows of a tile whose adapter no earlier row of it has, of a wave whose
-// lanes hold row lane % 16's id (negative: none): one bit each.
-__device__ __forceinline__ uint32_t leaders(const int id) {
-    uint32_t left = (uint32_t) __ballot(id >= 0) & 0xffffu, out = 0;
-    while (left) {
-        const int i = __builtin_ctz(left);
-        out |= 1u << i;
-        left &= ~(uint32_t) __ballot(id == __builtin_amdgcn_readlane(id, i));
-    }
-    return out;
-}
-
-// The adapter of a workgroup: the slot-th (and every p.slots-th after it) of
-// those that the tile's rows have, in the order of their first rows.
-struct Turn {
-    uint32_t todo;
-    __device__ __forceinline__ void skip(const int n) {
-        for (int i = 0; i < n && todo; ++i) todo &= todo - 1;
-    }
-};
-
-// Parts of v for at most 64 rows: (row, part of K) for each workgroup.
+// Parts of v for at most kFew rows: (row, part of K) for each workgroup.
 template <int RT>
 __global__ __launch_bounds__(64 * shrink_waves<RT>(), RT == 8 ? 2 : 4) void lora_shrink_few_kernel(const LoraParams p) {
-    __shared__ float part[shrink_waves<RT>()][RT * 16][kTile + 1];
+    __shared__ __attribute__((aligned(16))) float lds[shrink_waves<RT>() * shrink_lds<RT, shrink_unroll<RT>()>()];
     prefetch_params(p);
-    shrink_few<RT, shrink_waves<RT>()>(p, blockIdx.x, blockIdx.y, part);
+    shrink_few<RT, shrink_waves<RT>()>(p, blockIdx.x, blockIdx.y, lds);
 }
 
-// Parts of v for more: the columns of one part of K, of a tile's rows with the
-// workgroup's adapters. RT: tiles of 16 ranks at most. The first round's
-// activations, which need no id, are loaded before the ids are known.
+// Parts of v for more: every p.slots-th group of 64 rows for a workgroup.
+// Bound by x. Measured at 8000 rows of 4096, rank 16: 31 us, 4.3 TB/s.
 template <int RT>
 __global__ __launch_bounds__(64 * shrink_waves<RT>(), RT == 8 ? 2 : 4) void lora_shrink_kernel(const LoraParams p) {
     constexpr int WAVES = shrink_waves<RT>();
-    constexpr int U = RT <= 2 ? 2 : 1;
-    __shared__ float part[WAVES][RT * 16][kTile + 1];
+    __shared__ __attribute__((aligned(16))) float lds[WAVES * shrink_lds<RT, shrink_unroll<RT>()>()];
     prefetch_params(p);
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = blockIdx.x * kTile + n;
-    const int id = t < p.T ? p.ids[t] : -1;
-    const Columns c = Columns::of<U>(p, blockIdx.z, blockIdx.x, wave, WAVES);
-    const char * xr = p.x + (int64_t) min(t, p.T - 1) * p.x_nb1;
-    float4 x[U][2];
-    load_x<U>(xr, c.column<U>(), c.k1, g, x);
-    asm volatile("" ::: "memory");
-    const int row_rank = id >= 0 ? rank_of(p, id) : 0;                 // every row's at once, not adapter by adapter
-    const float row_scale = p.scales && row_rank > 0 ? p.scales[id] : 1.0f;
-    Turn turn{leaders(id)};
-    turn.skip(blockIdx.y);
-    for (bool again = false; turn.todo; turn.skip(p.slots), again = true) {
-        const int lead = __builtin_ctz(turn.todo);
-        const int a = __builtin_amdgcn_readlane(id, lead), rank = __builtin_amdgcn_readlane(row_rank, lead);
-        if (rank < 0) {
-            if (threadIdx.x == 0) lora_error(p, a);
-            continue;
-        }
-        if (rank == 0) continue;
-        if (again && c.rounds != 1) load_x<U>(xr, c.column<U>(), c.k1, g, x);   // one round: x is still there
-        const char * ar = p.a + (int64_t) a * p.a_nb2;
-        if (RT >= 8 && rank > 64)      shrink<min_c(RT, 8), U>(p, ar, rank, xr, x, c, n, g, part[wave]);
-        else if (RT >= 4 && rank > 32) shrink<min_c(RT, 4), U>(p, ar, rank, xr, x, c, n, g, part[wave]);
-        else if (RT >= 2 && rank > 16) shrink<min_c(RT, 2), U>(p, ar, rank, xr, x, c, n, g, part[wave]);
-        else                           shrink<1, U>(p, ar, rank, xr, x, c, n, g, part[wave]);
-        __syncthreads();
-        const float scale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(row_scale), lead));
-        const uint32_t rows = (uint32_t) __ballot(id == a) & 0xffffu;
-        for (int i = threadIdx.x; i < kTile * RT * 16; i += 64 * WAVES) {
-            const int tok = i / (RT * 16), j = i % (RT * 16);
-            if (j >= rank || !(rows >> tok & 1)) continue;
-            float v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) v += part[w][j][tok];
-            p.v[((int64_t) blockIdx.z * p.T + blockIdx.x * kTile + tok) * p.R + j] = v * scale;
-        }
-        __syncthreads();
+    const int lane = threadIdx.x & 63;
+    Group rows(p, blockIdx.y * 64, lane);
+    for (int k = blockIdx.x; rows.at(p, k, false, lane); k += p.slots) {
+        if (k != (int) blockIdx.x) __syncthreads();                    // the last group's sums are read
+        shrink_group<RT, WAVES>(p, rows, blockIdx.z, blockIdx.y * p.slots + blockIdx.x, lds);
     }
 }
 
-// A slice of 256 outputs of rows that share a workgroup: with at most 64 rows
-// (FEW) those of row `blockIdx.y`'s adapter, if it is their first; with more
-// those of a tile that have one of the workgroup's adapters. Rows without an
-// adapter are copied where base is not y: by their own workgroup, or by the
-// tile's slot 0. Lane 16 g + n holds outputs 4 g .. 4 g + 3 of each 16, of row
-// n. The slices of a row come next to one another in the grid, so that
-// workgroups that run together use all memory channels. VEC: rows of y and
-// base in whole 16 bytes; SPLIT: v in parts.
-// Measured at 8000 rows of 4096 outputs, rank 16: 55 us, 4.8 TB/s, what a copy
-// reaches; with 1024 or more outputs to a workgroup 63 to 72.
-template <int RT, bool VEC, bool SPLIT, bool FEW>
-__global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraParams p) {
-    constexpr int kRow = RT * 16 + 4;
+// A slice of 256 outputs of a group's rows (with base that is not y, rows
+// without an adapter are groups too, and copied). FEW: at most kFew rows, row
+// blockIdx.y's group; else every p.slots-th group of 64 rows for a workgroup.
+// The rows are the product's rows, the outputs its columns, output 4 n + u of a
+// wave's 64 in column n of product u: lane 16 g + n holds outputs 4 n .. 4 n + 3
+// of rows 4 g .. 4 g + 3, and a load or store covers 256 bytes of each of 4
+// rows. The slices of a row come next to one another in the grid, so that
+// workgroups that run together use all memory channels (the groups next to one
+// another: 70 us instead of 55 for 8000 rows of 4096 outputs; several slices to
+// a workgroup gained nothing). VEC: rows of y and base in whole 16 bytes;
+// SPLIT: v in parts.
+// Measured there, rank 16: 56 us, of 268 MB (4.8 TB/s, what a copy reaches).
+template <int RT, bool VEC, bool SPLIT>
+__device__ __forceinline__ void expand_group(const LoraParams & p, const Group & rows, float (*v)[RT * 16 + 4]) {
     constexpr int kPiece = RT == 1 ? 16 : 32;                          // ranks of a lane's load of B: 4 or 8 in each quarter
     constexpr int kSteps = kPiece / 4;
     constexpr int kPieces = RT * 16 / kPiece;
     typedef _Float16 piece __attribute__((ext_vector_type(kSteps)));
     typedef short bits __attribute__((ext_vector_type(kSteps)));
-    __shared__ __attribute__((aligned(16))) float v[kTile][kRow];
-    prefetch_params(p);
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c0 = blockIdx.x * kCols + 64 * wave;
-    // the columns' rows: which (row), whether they are this workgroup's
-    // (mine), their adapters and ranks, and the first column of each adapter
-    int row, id, rank;
-    uint32_t mine, turns;
-    uint64_t left = 0;
-    if constexpr (FEW) {
-        const int lead = blockIdx.y;
-        id = lane < p.T ? p.ids[lane] : -1;
-        const int a = __builtin_amdgcn_readlane(id, lead);
-        left = a >= 0 ? __ballot(id == a) : p.copy ? 1ull << lead : 0;
-        if (left == 0 || __builtin_ctzll(left) != lead) return;
-        id = a;
-        rank = a >= 0 ? rank_of(p, a) : 0;
-        turns = a >= 0 ? 1 : 0;
-    } else {
-        row = blockIdx.y * kTile + n;
-        id = row < p.T ? p.ids[row] : -1;
-        rank = id >= 0 ? rank_of(p, id) : 0;
-        Turn turn{leaders(id)};
-        turn.skip(blockIdx.z);
-        mine = turns = 0;
-        for (; turn.todo; turn.skip(p.slots)) {
-            const int l = __builtin_ctz(turn.todo);
-            turns |= 1u << l;
-            mine |= (uint32_t) __ballot(id == __builtin_amdgcn_readlane(id, l));
+    const int c0 = blockIdx.x * kCols + 64 * wave + 4 * n;            // the lane's outputs
+    const int rank = rows.a >= 0 ? __builtin_amdgcn_readfirstlane(rank_of(p, rows.a)) : 0;
+    // the lane's rows 4 g + i
+    int at[4];
+    float acc[4][4];                                               // [row][output]
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        at[i] = __shfl(rows.row, 4 * g + i);
+        const bool own = 4 * g + i < rows.count;
+        const float * br = (const float *) (p.base + (int64_t) at[i] * p.base_nb1) + c0;
+        if constexpr (VEC) {
+            float4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (own && c0 < p.N) x = *(const float4 *) br;
+            acc[i][0] = x.x; acc[i][1] = x.y; acc[i][2] = x.z; acc[i][3] = x.w;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[i][u] = own && c0 + u < p.N ? br[u] : 0.0f;
         }
-        if (blockIdx.z == 0 && p.copy) mine |= (uint32_t) __ballot(id < 0 && row < p.T);
-        mine &= 0xffffu;
-        if (!mine) return;
-        row = min(row, p.T - 1);
     }
-    do {
-        if constexpr (FEW) {
-            row = nth_row(left, n);
-            mine = (1u << min(__builtin_popcountll(left), kTile)) - 1;
-            left = without_16(left);
+    // v, zeros beyond the ranks
+    for (int i = threadIdx.x; i < kTile * RT * 4; i += 64 * kWaves) {
+        const int tok = i / (RT * 4), j = 4 * (i - tok * (RT * 4));
+        const int src = __shfl(rows.row, tok);
+        float4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (j < rank && tok < rows.count) {
+            if constexpr (SPLIT) s = sum_parts(p, src, j);
+            else s = *(const float4 *) (p.v + (int64_t) src * p.R + j);
+            if (j + 1 >= rank) s.y = 0.0f;
+            if (j + 2 >= rank) s.z = 0.0f;
+            if (j + 3 >= rank) s.w = 0.0f;
         }
-        const bool own = mine >> n & 1;
-        const char * br = p.base + (int64_t) row * p.base_nb1 + 16 * g;
-        char * yr = p.y + (int64_t) row * p.y_nb1 + 16 * g;
-        floatx4 acc[4];
+        *(float4 *) &v[tok][j] = s;
+    }
+    __syncthreads();
+    // this lane's ranks of row n, as the products' operands
+    piece hi[kPieces], lo[kPieces];
+    float up, down, top = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            acc[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-            const int c = c0 + 16 * u + 4 * g;
-            if constexpr (VEC) {
-                if (own && c < p.N) acc[u] = *(const floatx4 *) (br + (int64_t) (c0 + 16 * u) * 4);
-            } else {
+    for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (own && c + i < p.N) acc[u][i] = *(const float *) (br + (int64_t) (c0 + 16 * u + i) * 4);
-            }
+        for (int s = 0; s < kSteps; ++s) top = fmaxf(top, fabsf(v[n][q * kPiece + kSteps * g + s]));
+    row_scale(colmax4(top), up, down);
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const float z = v[n][q * kPiece + kSteps * g + s] * up;
+            hi[q][s] = (_Float16) z;
+            lo[q][s] = (_Float16) (z - (float) hi[q][s]);
         }
-        // v, zeros beyond the ranks
-        for (int i = threadIdx.x; i < kTile * RT * 4; i += 64 * kWaves) {
-            const int tok = i / (RT * 4), j = 4 * (i - tok * (RT * 4));
-            const int r = __shfl(rank, tok), at = __shfl(row, tok);
-            float4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (j < r && (mine >> tok & 1)) {
-                if constexpr (SPLIT) s = sum_parts(p, at, j);
-                else s = *(const float4 *) (p.v + (int64_t) at * p.R + j);
-                if (j + 1 >= r) s.y = 0.0f;
-                if (j + 2 >= r) s.z = 0.0f;
-                if (j + 3 >= r) s.w = 0.0f;
-            }
-            *(float4 *) &v[tok][j] = s;
-        }
-        __syncthreads();
-        // this lane's ranks of row n, as the products' operands
-        piece hi[kPieces], lo[kPieces];
-        float up, down, top = 0.0f;
+    float downs[4];
 #pragma unroll
-        for (int q = 0; q < kPieces; ++q)
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) top = fmaxf(top, fabsf(v[n][q * kPiece + kSteps * g + s]));
-        row_scale(top, up, down);
-#pragma unroll
-        for (int q = 0; q < kPieces; ++q)
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const float z = v[n][q * kPiece + kSteps * g + s] * up;
-                hi[q][s] = (_Float16) z;
-                lo[q][s] = (_Float16) (z - (float) hi[q][s]);
-            }
+    for (int i = 0; i < 4; ++i) downs[i] = __shfl(down, 4 * g + i);
 
-        for (uint32_t todo = turns; todo; todo &= todo - 1) {
-            const int l = __builtin_ctz(todo);
-            const int a = __builtin_amdgcn_readlane(id, l), r = __builtin_amdgcn_readlane(rank, l);
-            const char * b = p.b + (int64_t) a * p.b_nb2;
-            floatx4 sum[4];
+    if (rows.a >= 0) {
+        piece w[kPieces][4];
+        const char * b = p.b + (int64_t) rows.a * p.b_nb2;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) sum[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int q = 0; q < kPieces; ++q) {
+            if (q * kPiece >= rank) break;
+            const int j0 = q * kPiece + kSteps * g;            // this lane's ranks
 #pragma unroll
-            for (int q = 0; q < kPieces; ++q) {
-                if (q * kPiece >= r) break;
-                const int j0 = q * kPiece + kSteps * g;                // this lane's ranks
-                piece w[4];
+            for (int u = 0; u < 4; ++u)
+                w[q][u] = *(const piece *) (b + ((uint32_t) min(c0 + u, p.N - 1) * (uint32_t) p.b_nb1 + 2u * (uint32_t) min(j0, p.R - kSteps)));
+            if (q * kPiece + kPiece > rank) {                     // what lies behind the rank may be NaN
+                bits in;
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    w[u] = *(const piece *) (b + (int64_t) min(c0 + 16 * u + n, p.N - 1) * p.b_nb1 + 2 * min(j0, p.R - kSteps));
-                if (q * kPiece + kPiece > r) {                         // what lies behind the rank may be NaN
-                    bits in;
+                for (int s = 0; s < kSteps; ++s) in[s] = j0 + s < rank ? -1 : 0;
 #pragma unroll
-                    for (int s = 0; s < kSteps; ++s) in[s] = j0 + s < r ? -1 : 0;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) w[u] = __builtin_bit_cast(piece, __builtin_bit_cast(bits, w[u]) & in);
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if constexpr (kSteps == 4) {
-                        sum[u] = __builtin_amdgcn_mfma_f32_16x16x16f16(w[u], lo[q], sum[u], 0, 0, 0);
-                        sum[u] = __builtin_amdgcn_mfma_f32_16x16x16f16(w[u], hi[q], sum[u], 0, 0, 0);
-                    } else {
-                        sum[u] = mfma_16x16x32(w[u], hi[q], mfma_16x16x32(w[u], lo[q], sum[u]));
-                    }
-                }
+                for (int u = 0; u < 4; ++u) w[q][u] = __builtin_bit_cast(piece, __builtin_bit_cast(bits, w[q][u]) & in);
             }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) sum[u] = acc[u] + sum[u] * down;
-            if (r < 0)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) sum[u] = floatx4{1.0f, 1.0f, 1.0f, 1.0f} * __builtin_nanf("");
-            if (id == a)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) acc[u] = sum[u];
         }
-        if (own)
+        floatx4 sum[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q) {
+            if (q * kPiece >= rank) break;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int c = c0 + 16 * u + 4 * g;
-                if constexpr (VEC) {
-                    if (c < p.N) *(floatx4 *) (yr + (int64_t) (c0 + 16 * u) * 4) = acc[u];
+                if constexpr (kSteps == 4) {
+                    sum[u] = __builtin_amdgcn_mfma_f32_16x16x16f16(lo[q], w[q][u], sum[u], 0, 0, 0);
+                    sum[u] = __builtin_amdgcn_mfma_f32_16x16x16f16(hi[q], w[q][u], sum[u], 0, 0, 0);
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (c + i < p.N) *(float *) (yr + (int64_t) (c0 + 16 * u + i) * 4) = acc[u][i];
+                    sum[u] = mfma_16x16x32(hi[q], w[q][u], mfma_16x16x32(lo[q], w[q][u], sum[u]));
                 }
             }
-        if constexpr (FEW) __syncthreads();                                // v is read before the next rows' is written
-    } while (FEW && left);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[i][u] = rank < 0 ? __builtin_nanf("") : acc[i][u] + sum[u][i] * downs[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (4 * g + i >= rows.count) continue;
+        float * yr = (float *) (p.y + (int64_t) at[i] * p.y_nb1) + c0;
+        if constexpr (VEC) {
+            if (c0 < p.N) *(float4 *) yr = float4{acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (c0 + u < p.N) yr[u] = acc[i][u];
+        }
+    }
+}
+
+template <int RT, bool VEC, bool SPLIT, bool FEW>
+__global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraParams p) {
+    __shared__ __attribute__((aligned(16))) float v[kTile][RT * 16 + 4];
+    prefetch_params(p);
+    const int lane = threadIdx.x & 63;
+    Group rows(p, FEW ? 0 : blockIdx.z * 64, lane);
+    if constexpr (FEW) {
+        if (rows.from_row(blockIdx.y, lane) && (rows.a >= 0 || p.copy)) expand_group<RT, VEC, SPLIT>(p, rows, v);
+    } else {
+        for (int k = blockIdx.y; rows.at(p, k, p.copy, lane); k += p.slots) {
+            if (k != (int) blockIdx.y) __syncthreads();                // the last group's v is read
+            expand_group<RT, VEC, SPLIT>(p, rows, v);
+        }
+    }
 }
 
 struct Plan {
@@ -309,6 +232,8 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     auto al = [](const al_tensor & t, uint64_t by) { return !(((uintptr_t) t.data | t.nb[1] | t.nb[2]) & (by - 1)); };
     if (a.nb[0] != 2 || b.nb[0] != 2 || !al(a, 16) || !al(b, 16))
         return al_fail(AL_ERR_INVALID, "lora: rows of a and b must be contiguous and 16-byte aligned");
+    if ((uint64_t) R * a.nb[1] >= (1ull << 32) || (uint64_t) N * b.nb[1] >= (1ull << 32))
+        return al_fail(AL_ERR_UNSUPPORTED, "lora: an adapter spans more than 4 GB");
     if (x.nb[0] != 4 || ((uintptr_t) x.data & 15u) || x.nb[1] % 16 || y.nb[0] != 4 || ((uintptr_t) y.data & 3u) || y.nb[1] % 4 ||
         (T > 1 && y.nb[1] < (uint64_t) N * 4))
         return al_fail(AL_ERR_INVALID, "lora: rows of x must be 16-byte aligned, those of y contiguous and apart");
@@ -342,14 +267,17 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     p.K = (int32_t) K; p.N = (int32_t) N; p.R = (int32_t) R; p.T = (int32_t) T; p.n_adapters = (int32_t) A;
     p.y_vec = N % 4 == 0 && !(((uintptr_t) y.data | y.nb[1] | (uintptr_t) base.data | base.nb[1]) & 15u);
     const int64_t tiles = (T + kTile - 1) / kTile;
-    // Up to 64 rows take a workgroup for each row, of which those of an
-    // adapter's first row work; more take tiles, whose adapters share 4
-    // workgroups up to 64 tiles, 1 beyond. K in parts of at least 512 columns
-    // while there are CUs for them.
-    p.slots = tiles <= 64 ? 4 : 1;
+    // Up to kFew rows take a workgroup for each row, of which those of an
+    // adapter's first, 17th ... row work. Of more, each 64 have at least 4
+    // groups, which p.slots workgroups share: more of them where the launch
+    // would not fill the CUs, and an odd number, as workgroups go to the 8 XCDs
+    // in turn and the last slots have little to do (us with 5, 8, 9: 300 rows of
+    // shuffled adapters 23.2, 22.8, 18.2, 1000 of requests 22.4, 25.8, 23.3;
+    // with 4, 5, 8: 8000 rows 93, 86, 97).
+    p.slots = T <= 512 ? 9 : 5;
     p.copy = base.data != y.data;
-    const int64_t groups = T <= kFew ? 16 : 2 * tiles;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kParts, (K + 511) / 512, n_cu / std::max<int64_t>(1, groups)}));
+    // K in parts of at least 512 columns while the CUs are not full.
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kParts, (K + 511) / 512, T <= kFew ? n_cu / 16 : 2 * n_cu / tiles}));
     p.k_step = (int32_t) (((K + parts - 1) / parts + 31) / 32 * 32);
     p.ks = (int32_t) ((K + p.k_step - 1) / p.k_step);
     pl.v_bytes = ((size_t) p.ks * T * R * 4 + 255) / 256 * 256;
@@ -372,17 +300,17 @@ hipError_t launch_expand(const LoraParams & p, const dim3 grid, hipStream_t st) 
 template <int RT>
 hipError_t launch_shrink(const LoraParams & p, hipStream_t st) {
     constexpr int kThreads = 64 * shrink_waves<RT>();
-    const unsigned tiles = (unsigned) ((p.T + kTile - 1) / kTile);
+    const unsigned windows = (unsigned) ((p.T + 63) / 64);
     if (p.T <= kFew) hipLaunchKernelGGL(lora_shrink_few_kernel<RT>, dim3((unsigned) p.T, (unsigned) p.ks), dim3(kThreads), 0, st, p);
-    else             hipLaunchKernelGGL(lora_shrink_kernel<RT>, dim3(tiles, (unsigned) p.slots, (unsigned) p.ks), dim3(kThreads), 0, st, p);
+    else             hipLaunchKernelGGL(lora_shrink_kernel<RT>, dim3((unsigned) p.slots, windows, (unsigned) p.ks), dim3(kThreads), 0, st, p);
     return hipGetLastError();
 }
 
 template <int RT>
 hipError_t launch_expand(const LoraParams & p, hipStream_t st) {
-    const unsigned tiles = (unsigned) ((p.T + kTile - 1) / kTile), slices = (unsigned) ((p.N + kCols - 1) / kCols);
+    const unsigned windows = (unsigned) ((p.T + 63) / 64), slices = (unsigned) ((p.N + kCols - 1) / kCols);
     return p.T <= kFew ? launch_expand<RT, true>(p, dim3(slices, (unsigned) p.T), st)
-                       : launch_expand<RT, false>(p, dim3(slices, tiles, (unsigned) p.slots), st);
+                       : launch_expand<RT, false>(p, dim3(slices, (unsigned) p.slots, windows), st);
 }
 
 int run(const al_lora_args * g, bool project) {

@@ -161,14 +161,14 @@ __global__ __launch_bounds__(64 * lora::shrink_waves<RT>(), RT == 8 ? 2 : 4) voi
     const char * __restrict__ x, int64_t x_nb1, int nb, int T, int n_items, uint4 * __restrict__ frag,
     _Float16 * __restrict__ dx, int n_quantize, const lora::LoraParams p) {
     constexpr int kWaves = lora::shrink_waves<RT>();
-    __shared__ float part[kWaves][RT * 16][lora::kTile + 1];
+    __shared__ __align__(16) float lds[kWaves * lora::shrink_lds<RT, lora::shrink_unroll<RT>()>()];
     if ((int) blockIdx.x < n_quantize) {
         const int item = blockIdx.x * kWaves + (threadIdx.x >> 6);
         if (item < n_items) quantize_q8(x, x_nb1, nb, T, item, frag, dx);
         return;
     }
     const int i = (int) blockIdx.x - n_quantize, k = i / T;
-    lora::shrink_few<RT, kWaves>(p, i - k * T, k, part);
+    lora::shrink_few<RT, kWaves>(p, i - k * T, k, lds);
 }
 
 // 9 to 64 tokens: a workgroup takes 16 weight rows and a tile of 16 tokens,

@@ -40,7 +40,10 @@ extern "C" {
  *           (al_mul_mat_q4_0_lora_f32: not used)
  *   y       f32 ne = [N, T], nb0 = 4
  *   w       Q4_0 ne = [K, N] (al_mul_mat_q4_0_lora_f32 only)
- * K and R are multiples of 8, R at most 128, K at most 65536. An id of
+ * K and R are multiples of 8, R at most 128, K at most 65536, T at most 2^19,
+ * n_adapters at most 2^20; an adapter's A and its B span less than 4 GB each
+ * (AL_ERR_UNSUPPORTED otherwise). The rows of ids, x and y may name the
+ * adapters in any order. An id of
  * n_adapters or more, or a rank outside 0 to R, is not followed: the row is
  * NaN, and al_device_errors() returns AL_ERR_INVALID after the stream
  * completes.

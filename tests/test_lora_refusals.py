@@ -46,6 +46,8 @@ FAULTS = [
     (dict(ids=T(I32, [2])), abi.AL_ERR_INVALID),
     (dict(ranks=T(I32, [4])), abi.AL_ERR_INVALID),
     (dict(scales=T(F16, [5])), abi.AL_ERR_INVALID),
+    (dict(a=T(F16, [4096, 16, 5], nb=[2, 1 << 28, 1 << 32, 5 << 32])), abi.AL_ERR_UNSUPPORTED),    # an adapter's A of 4 GB
+    (dict(b=T(F16, [16, 2560, 5], nb=[2, 1 << 21, 2560 << 21, 12800 << 21])), abi.AL_ERR_UNSUPPORTED),
 ]
 
 
