@@ -8,16 +8,16 @@
 // any size keep their bits. Two f16 products of 16 x 16 x 32 take an eighth of
 // the matrix cores' time that f32 products (16 x 16 x 4) do.
 //
-// The products take 16 rows at a time, of one adapter: out of 64 rows at a time
-// those of each adapter are picked, in any order (rows that lie next to one
-// another, as a prompt's, come out as they are), so that A and B are read once
-// for 16 of them.
+// The products take 16 rows at a time, of one adapter: out of 64 or 256 rows at
+// a time those of each adapter are picked, in any order (rows that lie next to
+// one another, as a prompt's, come out as they are), so that A and B are read
+// once for 16 of them. The first launch leaves the groups for the second.
 //
 // Two launches: the first product into the workspace, K split over workgroups
 // where there are few rows, then the second, which sums the parts, for a slice
 // of the outputs. (Beside the Q4_0 projection: parts of its launches.) 300 rows
 // of 2048 -> 8192 in the order of their requests, ranks to 64: 13.6 us;
-// shuffled over 12 adapters 18.2, as every group of 16 rows then is of another.
+// shuffled over 12 adapters 17.4, as a group of rows then is of 5 on average.
 
 #include <hip/hip_runtime.h>
 
@@ -46,35 +46,45 @@ __global__ __launch_bounds__(64 * shrink_waves<RT>(), RT == 8 ? 2 : 4) void lora
     shrink_few<RT, shrink_waves<RT>()>(p, blockIdx.x, blockIdx.y, lds);
 }
 
-// Parts of v for more: every p.slots-th group of 64 rows for a workgroup.
-// Bound by x. Measured at 8000 rows of 4096, rank 16: 31 us, 4.3 TB/s.
-template <int RT>
+__device__ __forceinline__ int32_t * record(const LoraParams & p, const int window, const int k) {
+    return p.groups + (int64_t) (window * (p.window + p.slots) + k) * kRecord;
+}
+
+// Parts of v for more: every p.slots-th group of 64 W rows for a workgroup,
+// which leaves its groups, and the end of them, for the second launch.
+// Bound by x. Measured at 8000 rows of 4096, rank 16: 32 us, 4.1 TB/s.
+template <int RT, int W>
 __global__ __launch_bounds__(64 * shrink_waves<RT>(), RT == 8 ? 2 : 4) void lora_shrink_kernel(const LoraParams p) {
     constexpr int WAVES = shrink_waves<RT>();
     __shared__ __attribute__((aligned(16))) float lds[WAVES * shrink_lds<RT, shrink_unroll<RT>()>()];
     prefetch_params(p);
     const int lane = threadIdx.x & 63;
-    Group rows(p, blockIdx.y * 64, lane);
-    for (int k = blockIdx.x; rows.at(p, k, false, lane); k += p.slots) {
-        if (k != (int) blockIdx.x) __syncthreads();                    // the last group's sums are read
+    for (int k = blockIdx.x;; k += p.slots) {
+        Group<W> rows(p, blockIdx.y * 64 * W, lane);                   // anew, to leave the registers to the products
+        const bool more = rows.at(p, k, p.copy, lane);
+        if (!more) rows.count = 0;
+        if (blockIdx.z == 0 && threadIdx.x < 64) put_rows(record(p, blockIdx.y, k), rows, lane);
+        if (!more) break;
+        if (rows.a < 0) continue;
         shrink_group<RT, WAVES>(p, rows, blockIdx.z, blockIdx.y * p.slots + blockIdx.x, lds);
+        __syncthreads();                                               // the sums are read before the next group's
     }
 }
 
 // A slice of 256 outputs of a group's rows (with base that is not y, rows
 // without an adapter are groups too, and copied). FEW: at most kFew rows, row
-// blockIdx.y's group; else every p.slots-th group of 64 rows for a workgroup.
+// blockIdx.y's group; else every p.slots-th group of p.window rows for a workgroup.
 // The rows are the product's rows, the outputs its columns, output 4 n + u of a
 // wave's 64 in column n of product u: lane 16 g + n holds outputs 4 n .. 4 n + 3
 // of rows 4 g .. 4 g + 3, and a load or store covers 256 bytes of each of 4
 // rows. The slices of a row come next to one another in the grid, so that
 // workgroups that run together use all memory channels (the groups next to one
-// another: 70 us instead of 55 for 8000 rows of 4096 outputs; several slices to
+// another: 70 us instead of 55, then, for 8000 rows of 4096 outputs; several slices to
 // a workgroup gained nothing). VEC: rows of y and base in whole 16 bytes;
 // SPLIT: v in parts.
-// Measured there, rank 16: 56 us, of 268 MB (4.8 TB/s, what a copy reaches).
+// Measured there, rank 16: 51.7 us, 5.1 TB/s, what a copy reaches.
 template <int RT, bool VEC, bool SPLIT>
-__device__ __forceinline__ void expand_group(const LoraParams & p, const Group & rows, float (*v)[RT * 16 + 4]) {
+__device__ __forceinline__ void expand_group(const LoraParams & p, const Rows & rows, float (*v)[RT * 16 + 4]) {
     constexpr int kPiece = RT == 1 ? 16 : 32;                          // ranks of a lane's load of B: 4 or 8 in each quarter
     constexpr int kSteps = kPiece / 4;
     constexpr int kPieces = RT * 16 / kPiece;
@@ -194,11 +204,13 @@ __global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraPara
     __shared__ __attribute__((aligned(16))) float v[kTile][RT * 16 + 4];
     prefetch_params(p);
     const int lane = threadIdx.x & 63;
-    Group rows(p, FEW ? 0 : blockIdx.z * 64, lane);
     if constexpr (FEW) {
+        Group<1> rows(p, 0, lane);
         if (rows.from_row(blockIdx.y, lane) && (rows.a >= 0 || p.copy)) expand_group<RT, VEC, SPLIT>(p, rows, v);
     } else {
-        for (int k = blockIdx.y; rows.at(p, k, p.copy, lane); k += p.slots) {
+        for (int k = blockIdx.y;; k += p.slots) {
+            const Rows rows = get_rows(record(p, blockIdx.z, k), lane);
+            if (rows.count == 0) break;
             if (k != (int) blockIdx.y) __syncthreads();                // the last group's v is read
             expand_group<RT, VEC, SPLIT>(p, rows, v);
         }
@@ -208,7 +220,7 @@ __global__ __launch_bounds__(64 * kWaves) void lora_expand_kernel(const LoraPara
 struct Plan {
     LoraParams p;
     bool empty = false;
-    size_t v_bytes = 0, q_bytes = 0;            // v, then the projection's scratch
+    size_t v_bytes = 0, g_bytes = 0, q_bytes = 0;       // v, then the groups or the projection's scratch
 };
 
 int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
@@ -268,19 +280,23 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     p.y_vec = N % 4 == 0 && !(((uintptr_t) y.data | y.nb[1] | (uintptr_t) base.data | base.nb[1]) & 15u);
     const int64_t tiles = (T + kTile - 1) / kTile;
     // Up to kFew rows take a workgroup for each row, of which those of an
-    // adapter's first, 17th ... row work. Of more, each 64 have at least 4
-    // groups, which p.slots workgroups share: more of them where the launch
-    // would not fill the CUs, and an odd number, as workgroups go to the 8 XCDs
-    // in turn and the last slots have little to do (us with 5, 8, 9: 300 rows of
-    // shuffled adapters 23.2, 22.8, 18.2, 1000 of requests 22.4, 25.8, 23.3;
-    // with 4, 5, 8: 8000 rows 93, 86, 97).
-    p.slots = T <= 512 ? 9 : 5;
+    // adapter's first, 17th ... row work. Of more, groups are picked out of 64
+    // rows at a time or of 256, which costs more for a small batch in the order
+    // of its requests and saves half the groups of a shuffled one (us, ordered
+    // and shuffled over 12 adapters: 300 rows 13.5, 17.4 with 64, 15.6, 16.1
+    // with 256; 500 18.0, 21.7 and 16.6, 17.8; 2000 35.2, 61.4 and 35.4, 43.2).
+    // They have at least 4 or 16 groups, which p.slots workgroups share, an odd
+    // number, as workgroups go to the 8 XCDs in turn and the last slots have
+    // little to do (8000 rows with 4, 5, 8 for 64 rows: 93, 86, 97).
+    p.window = T <= 384 ? 64 : 256;
+    p.slots = p.window == 64 ? 9 : 21;
     p.copy = base.data != y.data;
     // K in parts of at least 512 columns while the CUs are not full.
     const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kParts, (K + 511) / 512, T <= kFew ? n_cu / 16 : 2 * n_cu / tiles}));
     p.k_step = (int32_t) (((K + parts - 1) / parts + 31) / 32 * 32);
     p.ks = (int32_t) ((K + p.k_step - 1) / p.k_step);
     pl.v_bytes = ((size_t) p.ks * T * R * 4 + 255) / 256 * 256;
+    if (!project && T > kFew) pl.g_bytes = (size_t) ((T + p.window - 1) / p.window) * (p.window + p.slots) * kRecord * 4;
     if (project) {
         const int rc = mul_mat_q4_0_check(&g->w, &x, &y, &pl.q_bytes);
         if (rc != AL_OK) return rc;
@@ -300,15 +316,16 @@ hipError_t launch_expand(const LoraParams & p, const dim3 grid, hipStream_t st) 
 template <int RT>
 hipError_t launch_shrink(const LoraParams & p, hipStream_t st) {
     constexpr int kThreads = 64 * shrink_waves<RT>();
-    const unsigned windows = (unsigned) ((p.T + 63) / 64);
+    const unsigned windows = (unsigned) ((p.T + p.window - 1) / p.window);
     if (p.T <= kFew) hipLaunchKernelGGL(lora_shrink_few_kernel<RT>, dim3((unsigned) p.T, (unsigned) p.ks), dim3(kThreads), 0, st, p);
-    else             hipLaunchKernelGGL(lora_shrink_kernel<RT>, dim3((unsigned) p.slots, windows, (unsigned) p.ks), dim3(kThreads), 0, st, p);
+    else if (p.window == 64) hipLaunchKernelGGL((lora_shrink_kernel<RT, 1>), dim3((unsigned) p.slots, windows, (unsigned) p.ks), dim3(kThreads), 0, st, p);
+    else hipLaunchKernelGGL((lora_shrink_kernel<RT, 4>), dim3((unsigned) p.slots, windows, (unsigned) p.ks), dim3(kThreads), 0, st, p);
     return hipGetLastError();
 }
 
 template <int RT>
 hipError_t launch_expand(const LoraParams & p, hipStream_t st) {
-    const unsigned windows = (unsigned) ((p.T + 63) / 64), slices = (unsigned) ((p.N + kCols - 1) / kCols);
+    const unsigned windows = (unsigned) ((p.T + p.window - 1) / p.window), slices = (unsigned) ((p.N + kCols - 1) / kCols);
     return p.T <= kFew ? launch_expand<RT, true>(p, dim3(slices, (unsigned) p.T), st)
                        : launch_expand<RT, false>(p, dim3(slices, (unsigned) p.slots, windows), st);
 }
@@ -322,7 +339,7 @@ int run(const al_lora_args * g, bool project) {
     if (rc == AL_OK) rc = make_plan(g, project, n_cu, &pl);
     if (rc == AL_OK) rc = al_device_error_flag(&pl.p.err);
     if (rc != AL_OK) return rc;
-    const size_t need = pl.v_bytes + pl.q_bytes;
+    const size_t need = pl.v_bytes + pl.g_bytes + pl.q_bytes;
     void * ws = g->workspace;
     if (ws) {
         if (g->workspace_bytes < need || ((uintptr_t) ws & 15u))
@@ -333,6 +350,7 @@ int run(const al_lora_args * g, bool project) {
         if (rc != AL_OK) return rc;
     }
     pl.p.v = (float *) ws;
+    pl.p.groups = (int32_t *) ((char *) ws + pl.v_bytes);
     const hipStream_t st = (hipStream_t) g->stream;
     const LoraParams & p = pl.p;
     const bool fused = project && mul_mat_q4_0_takes_lora(&g->w, p.T, p.R);
@@ -358,5 +376,5 @@ extern "C" uint64_t al_lora_workspace_bytes(const al_lora_args * args) {
     int n_cu = 0;
     Plan pl;
     if (al_device_cu_count(&n_cu) != AL_OK || make_plan(args, args && args->w.data != nullptr, n_cu, &pl) != AL_OK) return 0;
-    return pl.empty ? 0 : pl.v_bytes + pl.q_bytes;
+    return pl.empty ? 0 : pl.v_bytes + pl.g_bytes + pl.q_bytes;
 }

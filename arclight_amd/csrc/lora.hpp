@@ -13,7 +13,7 @@ namespace lora {
 constexpr int kTile = 16;                       // rows of x of a matrix product
 constexpr int kMaxR = 128;
 constexpr int kParts = 8;                       // parts of K at most
-constexpr int kFew = 64;                        // rows whose ids a wave's lanes hold
+constexpr int kFew = 64;                        // rows whose ids a wave's lanes hold, one each
 
 struct LoraParams {
     const char * a;  int64_t a_nb1, a_nb2;      // rank row, adapter
@@ -25,9 +25,10 @@ struct LoraParams {
     const char * base;  int64_t base_nb1;
     char * y;           int64_t y_nb1;
     float * v;                                  // [ks][T][R]
+    int32_t * groups;                           // [T / window][window + slots] records (more than kFew rows)
     int32_t K, N, R, T, n_adapters;
     int32_t ks, k_step;                         // parts of K, columns of one (a multiple of 32)
-    int32_t slots;                              // workgroups that share the groups of 64 rows (more than kFew rows)
+    int32_t window, slots;                      // rows that groups are picked from, workgroups that share those (more than kFew rows)
     int32_t copy;                               // base is not y: rows without an adapter are copied
     int32_t y_vec;                              // y and base rows 16-byte aligned, N a multiple of 4
     int * err;
@@ -59,53 +60,98 @@ __device__ __forceinline__ void lora_error(const LoraParams & p, const int a) {
     if (atomicCAS(p.err + 8, 0, 1) == 0) p.err[9] = a;
 }
 
-// Up to 16 rows that share an adapter (a < 0: have none), of the 64 from row
-// `first` on, whose ids the lanes of a wave hold. Lane n < 16 has the n-th in
-// `row` (the first one beyond the last).
-struct Group {
-    int id, first;                              // this lane's row's id; the 64 rows
+// Up to 16 rows that share an adapter (a < 0: have none). Lane n < 16 has the
+// n-th in `row` (the first one beyond the last).
+struct Rows {
     int a, count, row;
+};
+// As the first launch leaves them for the second.
+constexpr int kRecord = 20;                     // rows, a, count
+__device__ __forceinline__ void put_rows(int32_t * at, const Rows r, const int lane) {
+    if (lane < 18) at[lane] = lane == 17 ? +r.count : lane == 16 ? +r.a : +r.row;
+}
+__device__ __forceinline__ Rows get_rows(const int32_t * at, const int lane) {
+    const int x = at[min(lane, 17)];
+    return {__builtin_amdgcn_readlane(x, 16), __builtin_amdgcn_readlane(x, 17), x};
+}
+
+// Picks them out of the 64 W rows from `first` on, whose ids the lanes of a
+// wave hold.
+template <int W>
+struct Group : Rows {
+    int id[W], first;                           // the ids of rows first + 64 w + lane
     __device__ __forceinline__ Group(const LoraParams & p, const int first, const int lane) : first(first) {
-        id = first + lane < p.T ? p.ids[first + lane] : -1;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int r = first + 64 * w + lane;
+            id[w] = r < p.T ? p.ids[r] : -1;
+        }
     }
-    // The rows of `same` from its 16 chunk-th on: each sends its number to the
-    // lane of its place (the others' go to lane 63, which nothing reads).
-    __device__ __forceinline__ void take(const uint64_t same, const int chunk, const int lane) {
-        const int place = __builtin_amdgcn_mbcnt_hi((uint32_t) (same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) same, 0)) - chunk * kTile;
-        const bool mine = (same >> lane & 1) && place >= 0 && place < kTile;
-        row = __builtin_amdgcn_ds_permute(4 * (mine ? place : 63), first + lane);
-        count = min(__builtin_popcountll(same) - chunk * kTile, kTile);
+    // The `all` rows of `same` from its 16 chunk-th on: each sends its number to
+    // the lane of its place (the others' go to lane 63, which nothing reads;
+    // lanes that nothing is sent to get 0).
+    __device__ __forceinline__ void take(const uint64_t (&same)[W], const int all, const int chunk, const int lane) {
+        int before = -chunk * kTile;
+        row = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int place = __builtin_amdgcn_mbcnt_hi((uint32_t) (same[w] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) same[w], before));
+            const bool mine = (same[w] >> lane & 1) && place >= 0 && place < kTile;
+            row |= __builtin_amdgcn_ds_permute(4 * (mine ? place : 63), 64 * w + lane);
+            before += __builtin_popcountll(same[w]);
+        }
+        row += first;
+        count = min(all - chunk * kTile, kTile);
         if (lane >= count) row = __builtin_amdgcn_readfirstlane(row);
     }
     // Those of row `lead` on that share its adapter, if it is the first of
-    // them, or the 17th, the 33rd ...; false if another row is.
+    // them, or the 17th, the 33rd ...; false if another row is. (W = 1)
     __device__ __forceinline__ bool from_row(const int lead, const int lane) {
-        a = __builtin_amdgcn_readlane(id, lead);
-        const uint64_t same = a < 0 ? 1ull << lead : __ballot(id == a);
-        const int before = __builtin_popcountll(same & ((1ull << lead) - 1));
+        a = __builtin_amdgcn_readlane(id[0], lead);
+        const uint64_t same[1] = {a < 0 ? 1ull << lead : __ballot(id[0] == a)};
+        const int before = __builtin_popcountll(same[0] & ((1ull << lead) - 1));
         if (before % kTile) return false;
-        take(same, before / kTile, lane);
+        take(same, __builtin_popcountll(same[0]), before / kTile, lane);
         return true;
     }
     // The k-th group, adapters in the order of their first rows, then, if
     // `none` is set, the rows without one; false beyond the last.
     __device__ __forceinline__ bool at(const LoraParams & p, int k, const bool none, const int lane) {
-        uint64_t left = __ballot(id >= 0), same = 0;
-        while (left) {
-            a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-            same = __ballot(id == a);
-            left &= ~same;
-            const int chunks = (__builtin_popcountll(same) + kTile - 1) / kTile;
-            if (k < chunks) {
-                take(same, k, lane);
-                return true;
+        uint64_t left[W], same[W];
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            left[w] = __ballot(id[w] >= 0);
+            same[w] = 0;
+        }
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            while (left[v]) {
+                a = __builtin_amdgcn_readlane(id[v], __builtin_ctzll(left[v]));
+                all = 0;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    same[w] = w < v ? 0 : __ballot(id[w] == a);
+                    left[w] &= ~same[w];
+                    all += __builtin_popcountll(same[w]);
+                }
+                const int chunks = (all + kTile - 1) / kTile;
+                if (k < chunks) {
+                    take(same, all, k, lane);
+                    return true;
+                }
+                k -= chunks;
             }
-            k -= chunks;
         }
         a = -1;
-        same = none ? __ballot(id < 0 && first + lane < p.T) : 0;
-        if (k * kTile >= __builtin_popcountll(same)) return false;
-        take(same, k, lane);
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            same[w] = none ? __ballot(id[w] < 0 && first + 64 * w + lane < p.T) : 0;
+            all += __builtin_popcountll(same[w]);
+        }
+        if (k * kTile >= all) return false;
+        take(same, all, k, lane);
         return true;
     }
 };
@@ -275,7 +321,7 @@ __device__ __forceinline__ void shrink(const LoraParams & p, const char * ar, co
 // that A is read once for 16 rows of an adapter. lds: shrink_lds floats for
 // each wave. turn: what tells workgroups that run side by side apart.
 template <int RT, int WAVES>
-__device__ __forceinline__ void shrink_group(const LoraParams & p, const Group & rows, const int part_k, const int turn, float * lds) {
+__device__ __forceinline__ void shrink_group(const LoraParams & p, const Rows rows, const int part_k, const int turn, float * lds) {
     constexpr int U = shrink_unroll<RT>(), kLds = shrink_lds<RT, U>();
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -308,7 +354,7 @@ __device__ __forceinline__ void shrink_group(const LoraParams & p, const Group &
 // The same with at most kFew rows: row `lead`'s group, if it is its first.
 template <int RT, int WAVES>
 __device__ __forceinline__ void shrink_few(const LoraParams & p, const int lead, const int part_k, float * lds) {
-    Group rows(p, 0, threadIdx.x & 63);
+    Group<1> rows(p, 0, threadIdx.x & 63);
     if (rows.from_row(lead, threadIdx.x & 63) && rows.a >= 0) shrink_group<RT, WAVES>(p, rows, part_k, 0, lds);
 }
 

@@ -1,6 +1,8 @@
 """Low-rank adapters of many requests on the GPU against the definition in 64
 bits: alone and beside the Q4_0 projection, for one row to many, any order of
 adapters, ranks below the slot's, odd sizes and strides."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
@@ -281,3 +283,34 @@ def test_workspace_of_the_caller(gpu):
     with pytest.raises(_lib.ArclightError) as e:
         lora.ProjectCall(ad, w, _put(x), _put(ids), y, workspace=device.DeviceBuffer(need - 256)).run()
     assert e.value.status == abi.AL_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("T", [65, 256, 384, 385, 513, 900])
+@pytest.mark.parametrize("how", ["each its own", "in turn", "none", "two kinds of none"])
+def test_groups_of_rows(gpu, T, how):
+    """Every row of another adapter, 33 in turn, no row with one, with the
+    last row's alone: base is copied, in a workspace of the size that is asked
+    for and no more, that held other values."""
+    from arclight_amd import device, fattn, lora
+    _case(f"lora groups: T={T}, {how}")
+    rng = np.random.default_rng(280 + T)
+    K, N, R = 64, 20, 8
+    n = T if how == "each its own" else 33
+    a, b = _adapters(rng, n, R, K, N, [R] * n)
+    ids = {"each its own": rng.permutation(n), "in turn": np.arange(T) % 33, "none": np.full(T, -1),
+           "two kinds of none": np.where(np.arange(T) == T - 1, 5, -1 - np.arange(T) % 2 * 1000)}[how].astype(np.int32)
+    x, base = rng.standard_normal((T, K)).astype(np.float32), rng.standard_normal((T, N)).astype(np.float32)
+    ad = lora.Adapters(_put(a.view(np.uint16)), _put(b.view(np.uint16)))
+    xd, idd, bd, y = _put(x), _put(ids), _put(base), _put(np.full((T, N), 7.0, np.float32))
+    need = lora.ApplyCall(ad, xd, idd, bd, y).workspace_bytes()
+    ws = device.DeviceBuffer(need + 4096)
+    ws.upload(np.full(need + 4096, 0xa5, np.uint8))
+    fit = SimpleNamespace(ptr=ws.ptr, nbytes=need)
+    for _ in range(2):
+        lora.ApplyCall(ad, xd, idd, bd, y, workspace=fit).run()
+    device.synchronize()
+    fattn.device_errors()
+    tail = np.zeros(need + 4096, np.uint8)
+    ws.download(tail)
+    assert np.all(tail[need:] == 0xa5)
+    _check(y.numpy(np.float32), _ref(x, a, b, np.ones(n), [R] * n, ids, base), how)
