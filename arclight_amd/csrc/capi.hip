@@ -53,6 +53,7 @@ namespace {
 struct Workspace {
     void * ptr = nullptr;
     size_t bytes = 0;
+    std::vector<void *> old;                    // smaller ones before it
 };
 
 struct DeviceState {
@@ -134,24 +135,24 @@ static int library_workspace(size_t bytes, void * stream, void ** ptr) {
     std::lock_guard<std::mutex> lk(g_mu);
     Workspace & w = st->ws[stream];
     if (w.bytes < bytes) {
-        if (w.ptr) {
-            hipError_t e = hipDeviceSynchronize();   // also graphs replayed from a capture on this stream
-            if (e != hipSuccess) return al_hip_fail(e, "hipDeviceSynchronize");
-            e = hipFree(w.ptr);
-            if (e != hipSuccess) return al_hip_fail(e, "hipFree(workspace)");
-            w.ptr = nullptr;
-            w.bytes = 0;
-        }
         // room for any prefill call (at most one 128-row record a CU, 17 MB)
         // and any one-stream decode call, so that those never grow it (a
         // growth waits for the device and fails inside a capture)
-        const size_t sz = std::max(bytes, (size_t) 20 << 20);
-        hipError_t e = hipMalloc(&w.ptr, sz);
+        // A graph captured on the stream goes on using the smaller one, which
+        // is kept; a new one is at least twice its size, so that those kept
+        // are less than the one in use.
+        const size_t sz = std::max({bytes, 2 * w.bytes, (size_t) 20 << 20});
+        void * next = nullptr;
+        hipError_t e = hipMalloc(&next, sz);
         if (e != hipSuccess) return al_fail(AL_ERR_HIP, "hipMalloc(workspace %zu bytes): %s", sz, hipGetErrorString(e));
-        e = hipMemset(w.ptr, 0, sz);
-        if (e != hipSuccess) return al_hip_fail(e, "hipMemset(workspace)");
-        e = hipDeviceSynchronize();               // zeroed before the stream's kernels use it
-        if (e != hipSuccess) return al_hip_fail(e, "hipDeviceSynchronize");
+        e = hipMemset(next, 0, sz);
+        if (e == hipSuccess) e = hipDeviceSynchronize();       // zeroed before the stream's kernels use it
+        if (e != hipSuccess) {
+            (void) hipFree(next);
+            return al_hip_fail(e, "hipMemset(workspace)");
+        }
+        if (w.ptr) w.old.push_back(w.ptr);
+        w.ptr = next;
         w.bytes = sz;
     }
     *ptr = w.ptr;
@@ -177,7 +178,9 @@ extern "C" int al_fattn_release_stream(void * stream) {
         // the stream's kernels (and graphs replayed on it) may still use it
         hipError_t e = hipDeviceSynchronize();
         if (e != hipSuccess) return al_hip_fail(e, "hipDeviceSynchronize");
-        e = hipFree(it->second.ptr);
+        std::vector<void *> & old = it->second.old;
+        for (; !old.empty() && e == hipSuccess; old.pop_back()) e = hipFree(old.back());
+        if (e == hipSuccess) e = hipFree(it->second.ptr);
         if (e != hipSuccess) return al_hip_fail(e, "hipFree(workspace)");
     }
     st->ws.erase(it);

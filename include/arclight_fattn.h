@@ -93,7 +93,8 @@ typedef struct al_tensor {
  *
  * workspace: device scratch for split-KV partials. NULL lets the library use
  * its own buffer for the current device and args->stream (allocated on first
- * use, grown when needed, kept until al_fattn_release_stream; a graph
+ * use; a larger one when needed, beside which those before it are kept for the
+ * graphs that use them; freed by al_fattn_release_stream; a graph
  * captured on a stream uses that stream's, so the stream needs one eager call
  * of the same shapes before the capture: allocating inside a capture fails;
  * callers that cannot make one use al_fattn_f16_noalloc).

@@ -314,3 +314,51 @@ def test_groups_of_rows(gpu, T, how):
     ws.download(tail)
     assert np.all(tail[need:] == 0xa5)
     _check(y.numpy(np.float32), _ref(x, a, b, np.ones(n), [R] * n, ids, base), how)
+
+
+def test_a_growing_workspace_leaves_the_graphs_theirs(gpu):
+    """A captured call replayed after calls on its stream that need a larger
+    workspace of the library's, and buffers that would take a freed one's
+    place."""
+    from arclight_amd import _lib, device, fattn, lora
+    _case("lora: a workspace that grows")
+    rng = np.random.default_rng(290)
+    K, N, R, n, T = 512, 64, 16, 4, 50
+    a, b = _adapters(rng, n, R, K, N, [R] * n)
+    ad = lora.Adapters(_put(a.view(np.uint16)), _put(b.view(np.uint16)))
+    x, ids, base = rng.standard_normal((T, K)).astype(np.float32), _ids(rng, T, n, "any"), rng.standard_normal((T, N)).astype(np.float32)
+    ref = _ref(x, a, b, np.ones(n), [R] * n, ids, base)
+    y = _put(np.zeros((T, N), np.float32))
+    st = device.Stream()
+    small = lora.ApplyCall(ad, _put(x), _put(ids), _put(base), y, st)
+    small.run()
+    st.synchronize()
+    g = device.Graph(st, small.run)
+    kept = []
+    for i, rows in enumerate((50000, 120000)):                         # v of 26 and 61 MB
+        a1, b1 = _adapters(rng, 2, 128, 8, 4, [128] * 2)
+        x1, i1, base1 = rng.standard_normal((rows, 8)).astype(np.float32), _ids(rng, rows, 2, "any"), np.zeros((rows, 4), np.float32)
+        y1 = _put(base1)
+        big = lora.ApplyCall(lora.Adapters(_put(a1.view(np.uint16)), _put(b1.view(np.uint16))), _put(x1), _put(i1), _put(base1), y1, st)
+        assert big.workspace_bytes() > (20 << 20) * (i + 1)
+        big.run()
+        st.synchronize()
+        some = rng.choice(rows, 500, replace=False)
+        some[0] = rows - 1
+        _check(y1.numpy(np.float32)[some], _ref(x1[some], a1, b1, np.ones(2), [128] * 2, i1[some], base1[some]), f"{rows} rows")
+        kept += [_put(np.full(5 << 20, 1e30, np.float32)) for _ in range(2)]
+        for _ in range(2):
+            y.buf.zero()
+            device.synchronize()
+            g.launch(st)
+            st.synchronize()
+            _check(y.numpy(np.float32), ref, "replay")
+    assert all(np.all(k.numpy(np.float32) == np.float32(1e30)) for k in kept)
+    fattn.device_errors()
+    g.destroy()
+    assert _lib.load().al_fattn_release_stream(st.handle) == 0
+    small.run()
+    st.synchronize()
+    _check(y.numpy(np.float32), ref, "after the release")
+    assert _lib.load().al_fattn_release_stream(st.handle) == 0
+    st.destroy()
