@@ -646,7 +646,8 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     if (a->sinks.data && (a->sinks.type != AL_TYPE_F32 || a->sinks.ne[0] != Hq || a->sinks.nb[0] != 4))
         return al_fail(AL_ERR_INVALID, "paged_fattn: sinks must be f32 [Hq]");
     if (!(a->logit_softcap >= 0.0f)) return al_fail(AL_ERR_INVALID, "paged_fattn: softcap %g", (double) a->logit_softcap);
-    if (T > (1 << 16) || Hq > (1 << 12) || T * Hq > (1 << 22) || n_seq > 65535)
+    // (a row's token is found exactly while rows times heads of a group stay below 2^32)
+    if (T > (1 << 16) || Hq > (1 << 12) || T * Hq > (1 << 22) || n_seq > 65535 || T * (Hq / Hkv) * (Hq / Hkv) >= (1ll << 32))
         return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
     pl.empty = T == 0 || n_seq == 0;
     p.q = (const char *) q.data; p.q_nb1 = q.nb[1]; p.q_nb2 = q.nb[2]; p.q_nb3 = q.nb[3];

@@ -14,7 +14,8 @@
  *
  * The pools (one of K and one of V for each layer):
  *   f16 ne = [128, P, Hkv, n_pages], nb0 = 2, the other strides free
- *   multiples of 16 bytes, data 16-byte aligned. P is a multiple of 8.
+ *   multiples of 16 bytes, data 16-byte aligned. P is a multiple of 8, at most
+ *   2^20, max_pages P at most 2^30 and max_pages P^2 below 2^38.
  *   A pool of [page][cell][head][128] is the layout of the ring: a sequence
  *   whose pages follow one another is a ring view for al_fattn_f16.
  * The table: i32 ne = [max_pages, n_seq], device, nb0 = 4. Entries behind a
@@ -55,7 +56,9 @@ extern "C" {
  *          before the rotation; zero: rotated as they are (q_w and k_w have
  *          to be NULL)
  *   rope   NULL for no rotation
- * nb0 = 4 everywhere; rows of q, k, v and q_out at multiples of 4 bytes.
+ * nb0 = 4 everywhere; rows of q, k, v and q_out at multiples of 4 bytes. T is
+ * at most 2^24, Hq 4096. q_out may be q; it may not overlap it otherwise, nor
+ * k or v.
  * q_out rows and cached keys have the bits that al_attn_inputs_f32 gives.
  * Two rows of one call that name the same cell leave one of the two there,
  * or parts of both.
@@ -97,7 +100,9 @@ int al_paged_append_f32(const al_paged_append_args * args);
  * logit_softcap * tanh(scale * q . k / logit_softcap) when logit_softcap is
  * not 0. What cells that a row does not see hold, NaN and infinities too,
  * does not reach it.
- * Hq is a multiple of Hkv. Queries and probabilities are carried as pairs of
+ * Hq is a multiple of Hkv, G = Hq / Hkv. T is at most 2^16, Hq 4096, T Hq
+ * 2^22, n_seq 65535, T G / 64 Hkv 65535, T G^2 below 2^32
+ * (AL_ERR_UNSUPPORTED otherwise). dst may not overlap q. Queries and probabilities are carried as pairs of
  * f16, so that results are those of f32 arithmetic (relative error about
  * 1e-6), unlike al_fattn_f16's. A sequence with an error that the kernel
  * records has NaN rows.
