@@ -262,7 +262,10 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     if (T > 0 && (base.data != y.data || base.nb[1] != y.nb[1])) {
         const uintptr_t b0 = (uintptr_t) base.data, b1 = b0 + (uint64_t) (T - 1) * base.nb[1] + (uint64_t) N * 4;
         const uintptr_t y0 = (uintptr_t) y.data, y1 = y0 + (uint64_t) (T - 1) * y.nb[1] + (uint64_t) N * 4;
-        if (b0 < y1 && y0 < b1) return al_fail(AL_ERR_INVALID, "lora: base overlaps y and is not y");
+        // rows side by side, as columns of one wider matrix, are apart too
+        const uint64_t s = y.nb[1], d = s ? (b0 - y0 + (b0 < y0 ? (y0 - b0 + s - 1) / s * s : 0)) % s : 0, row = (uint64_t) N * 4;
+        const bool apart = base.nb[1] == s && d >= row && s - d >= row;
+        if (b0 < y1 && y0 < b1 && !apart) return al_fail(AL_ERR_INVALID, "lora: base overlaps y and is not y");
     }
     Plan pl;
     LoraParams & p = pl.p;

@@ -36,9 +36,10 @@ extern "C" {
  *   ids     i32 [T], device: the adapter of each row, negative: none
  *   x       f32 ne = [K, T], nb0 = 4, rows 16-byte aligned
  *   base    f32 ne = [N, T], nb0 = 4, or data NULL: y's own content (y +=).
- *           May be y itself, and may not overlap it otherwise.
+ *           May be y itself, or columns beside y's of a wider matrix, and may
+ *           not overlap it otherwise.
  *           (al_mul_mat_q4_0_lora_f32: not used)
- *   y       f32 ne = [N, T], nb0 = 4
+ *   y       f32 ne = [N, T], nb0 = 4. May not overlap x.
  *   w       Q4_0 ne = [K, N] (al_mul_mat_q4_0_lora_f32 only)
  * K and R are multiples of 8, R at most 128, K at most 65536, T at most 2^19,
  * n_adapters at most 2^20; an adapter's A and its B span less than 4 GB each

@@ -91,3 +91,18 @@ def test_struct_layout_matches_c(tmp_path):
     subprocess.run(["gcc", "-std=c11", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [ctypes.sizeof(abi.AlLoraArgs)] + [getattr(abi.AlLoraArgs, f).offset for f in fields]
+
+
+def test_base_beside_y_in_one_matrix_is_not_refused():
+    """Columns of one wider matrix, in either order, are apart; those that
+    share a column are not. (T = 3 rows; the workspace's size tells, or, where
+    there is no device, the refusal's absence.)"""
+    lib = _lib.load()
+    N, row = 2560, 2 * 2560 * 4
+    wide = lambda off: T(F32, [N, 3], SOME + off, [4, row, 0, 0])  # noqa: E731
+    small = T(F32, [N, 3], SOME, [4, row, 0, 0])
+    for base, y, refused in ((wide(N * 4), small, False), (small, wide(N * 4), False), (wide(N * 4 - 4), small, True),
+                             (small, wide(N * 4 - 4), True), (wide(N * 4 + 4), small, True), (wide(row), small, True)):
+        a = args(base=base, y=y, ids=T(I32, [3]), workspace=SOME, workspace_bytes=1)
+        status = lib.al_lora_f32(ctypes.byref(a))                      # too small a workspace: nothing runs
+        assert (status == abi.AL_ERR_INVALID) == refused and status != abi.AL_OK, (status, lib.al_last_error())
