@@ -362,3 +362,33 @@ def test_a_growing_workspace_leaves_the_graphs_theirs(gpu):
     _check(y.numpy(np.float32), ref, "after the release")
     assert _lib.load().al_fattn_release_stream(st.handle) == 0
     st.destroy()
+
+
+def test_two_streams_and_columns_of_one_matrix(gpu):
+    """Calls on two streams, each with the library's workspace of its stream;
+    base and y are columns of one matrix, either first."""
+    from arclight_amd import device, fattn, lora
+    _case("lora on two streams")
+    rng = np.random.default_rng(300)
+    K, N, R, n, T = 2048, 512, 32, 5, 130
+    sides = []
+    for i in range(2):
+        a, b = _adapters(rng, n, R, K, N, [R] * n)
+        x, ids = rng.standard_normal((T, K)).astype(np.float32), _ids(rng, T, n, "any")
+        wide = rng.standard_normal((T, 2 * N)).astype(np.float32)
+        d = _put(wide)
+        cols = [device.DeviceTensor(d.buf, abi.AL_TYPE_F32, (T, N), (2 * N * 4, 4), off) for off in (0, N * 4)]
+        st = device.Stream()
+        ad = lora.Adapters(_put(a.view(np.uint16)), _put(b.view(np.uint16)))
+        base, y = cols[i], cols[1 - i]
+        sides.append((st, lora.ApplyCall(ad, _put(x), _put(ids), base, y, st), d, wide, i, _ref(x, a, b, np.ones(n), [R] * n, ids, wide[:, i * N:(i + 1) * N])))
+    for _ in range(20):
+        for s in sides:
+            s[1].run()
+    device.synchronize()
+    fattn.device_errors()
+    for st, _, d, wide, i, ref in sides:
+        got = d.numpy(np.float32)
+        assert np.array_equal(got[:, i * N:(i + 1) * N], wide[:, i * N:(i + 1) * N])
+        _check(got[:, (1 - i) * N:(2 - i) * N], ref, f"stream {i}")
+        st.destroy()
