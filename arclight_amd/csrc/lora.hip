@@ -358,7 +358,7 @@ int run(const al_lora_args * g, bool project) {
     const LoraParams & p = pl.p;
     const bool fused = project && mul_mat_q4_0_takes_lora(&g->w, p.T, p.R);
     hipError_t e = hipSuccess;
-    if (!(fused && mul_mat_q4_0_shrinks(p.T)))
+    if (!(fused && mul_mat_q4_0_shrinks(&g->w, p.T, p.R)))
         e = p.R <= 16 ? launch_shrink<1>(p, st) : p.R <= 32 ? launch_shrink<2>(p, st) : p.R <= 64 ? launch_shrink<4>(p, st) : launch_shrink<8>(p, st);
     if (e != hipSuccess) return al_hip_fail(e, "lora: launch");
     if (project) {

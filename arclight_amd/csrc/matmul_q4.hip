@@ -455,13 +455,19 @@ __device__ __forceinline__ float wave_sum8_scatter(const float (&v)[8], const in
 // rows' weight loads, quantizes all T activation rows into LDS meanwhile
 // (they are small and L2-resident after the first workgroup touches them;
 // each thread issues the loads of all T tokens of its part of a block before
-// using any), then runs the dot products from LDS. One wavefront per row; with several tokens the rows' per-lane sums of all of
-// them meet in one scattering wave reduction.
+// using any), then runs the dot products from LDS. One wavefront per row; with
+// several tokens the rows' per-lane sums of all of them meet in one scattering
+// wave reduction.
 // lora_p (LORA): the adapters' second product, added to the outputs. The 8
 // lanes that hold a token's sum (all 64 for one token) take 8 ranks of the
 // row's B each, loaded with the weights; v is summed into LDS beside the
 // quantization.
-template <int BPL, int TMAX, bool LORA>
+// kMake (one token): no launch comes before, and every workgroup computes the
+// token's v from all of A, 8 rows of A for 512 columns to a wave at a time,
+// while the weights arrive. 4096 -> 4096, 16 ranks: 6.3 us instead of 8.0.
+enum class Lora { kNone, kAdd, kMake };       // adapters: none; their first product is there; it is made here
+
+template <int BPL, int TMAX, Lora LORA>
 __device__ __forceinline__ void gemv_q4_fused(const char * w, int64_t w_nb1, int N, int K, const char * x, int64_t x_nb1, int T,
                                               char * __restrict__ y, int64_t y_nb1, const lora::LoraParams & lora_p) {
     extern __shared__ __align__(16) char lds[];
@@ -508,6 +514,8 @@ __device__ __forceinline__ void gemv_q4_fused(const char * w, int64_t w_nb1, int
                 if (t < T) quantize_part(g[t][0], g[t][1], part, qs + t * K + 32 * sl + 8 * part, sc + t * nb + sl);
         }
     };
+    int own_id = -1;
+    if constexpr (LORA == Lora::kMake) own_id = ld_uniform(lora_p.ids);
     // the first rounds' activations (L2) before the weights (HBM): the
     // quantization then waits only for the former
 #pragma unroll
@@ -522,7 +530,7 @@ __device__ __forceinline__ void gemv_q4_fused(const char * w, int64_t w_nb1, int
     constexpr int kPieces = TMAX > 1 ? 2 : 1;                           // (64 lanes hold every rank once)
     half8 b[kPieces];
     int id = -1, rank = 0;
-    if constexpr (LORA) {
+    if constexpr (LORA == Lora::kAdd) {
 #pragma unroll
         for (int t = 0; t < TMAX; ++t) {                                // (scalar loads: not behind the weights)
             const int i = ld_uniform(lora_p.ids + min(t, T - 1));
@@ -542,12 +550,68 @@ __device__ __forceinline__ void gemv_q4_fused(const char * w, int64_t w_nb1, int
             ((float4 *) v)[i] = sum_parts(lora_p, at, 4 * (i - at * (lora_p.R / 4)));
         }
     }
+    // kMake: the workgroup's own v, in units of 512 columns and 8 ranks for a
+    // wave; lane j holds rank j of the row's B (at most 64)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int n_k = K / 512;
+    int units = 0;
+    float bj = 0.0f, scale = 1.0f;
+    float4 xa[2];
+    half8 aw[8];
+    auto load_unit = [&](const int u) {
+        const int rb = u / n_k, k = 512 * (u - rb * n_k) + 8 * lane;
+        const float4 * xb = (const float4 *) ((const float *) x + k);
+        xa[0] = xb[0];
+        xa[1] = xb[1];
+        const char * ar = lora_p.a + (int64_t) id * lora_p.a_nb2 + 2 * k;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) aw[j] = *(const half8 *) (ar + (int64_t) (8 * rb + j) * lora_p.a_nb1);
+    };
+    if constexpr (LORA == Lora::kMake) {
+        id = own_id;
+        if (id >= 0 && id < lora_p.n_adapters) {                       // (the slot's ranks beyond its own are not used)
+            if (wave < n_k * (lora_p.R / 8)) load_unit(wave);
+            if (lane < lora_p.R)
+                bj = (float) ((const _Float16 *) (lora_p.b + (int64_t) id * lora_p.b_nb2 + (int64_t) min(row, N - 1) * lora_p.b_nb1))[lane];
+        }
+        if (id >= 0) {
+            rank = __builtin_amdgcn_readfirstlane(rank_of(lora_p, id));
+            if (rank < 0 && blockIdx.x == 0 && threadIdx.x == 0) lora::lora_error(lora_p, id);
+            if (lora_p.scales && rank > 0) scale = lora_p.scales[id];
+            units = rank > 0 ? n_k * ((rank + 7) / 8) : 0;
+        }
+    }
 #pragma unroll
     for (int k = 0; k < PRE; ++k)
         if (k < rounds) quantize_item(threadIdx.x + k * blockDim.x, f[k]);
     for (int k = PRE; k < rounds; ++k) {
         load_item(threadIdx.x + k * blockDim.x, f[0]);
         quantize_item(threadIdx.x + k * blockDim.x, f[0]);
+    }
+    if constexpr (LORA == Lora::kMake) {
+        for (int u = wave; u < units; u += waves) {
+            if (u != wave) load_unit(u);
+            float sum[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float s = (float) aw[j][0] * xa[0].x;
+                s = fmaf((float) aw[j][1], xa[0].y, s);
+                s = fmaf((float) aw[j][2], xa[0].z, s);
+                s = fmaf((float) aw[j][3], xa[0].w, s);
+                s = fmaf((float) aw[j][4], xa[1].x, s);
+                s = fmaf((float) aw[j][5], xa[1].y, s);
+                s = fmaf((float) aw[j][6], xa[1].z, s);
+                sum[j] = fmaf((float) aw[j][7], xa[1].w, s);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] = wave_sum_to_last(sum[j]);
+            if (lane == 63) {
+                const int rb = u / n_k;
+                float4 * to = (float4 *) (v + (u - rb * n_k) * lora_p.R + 8 * rb);
+                to[0] = float4{sum[0], sum[1], sum[2], sum[3]};
+                to[1] = float4{sum[4], sum[5], sum[6], sum[7]};
+            }
+        }
     }
     __syncthreads();
     if (row >= N) return;
@@ -586,7 +650,19 @@ __device__ __forceinline__ void gemv_q4_fused(const char * w, int64_t w_nb1, int
         return part;
     };
     float low = 0.0f;                                                   // the lane's ranks' share of its token's output
-    if constexpr (LORA) {
+    if constexpr (LORA == Lora::kMake) {
+        if (lane < rank) {
+            for (int k = 0; k < n_k; k += 8) {                           // (K is a multiple of 4096)
+                float part[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) part[i] = v[(k + i) * lora_p.R + lane];
+                low += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+            }
+            low *= scale * bj;
+        }
+        if (rank < 0) low = __builtin_nanf("");                          // (summed over the lanes with the row's dot product)
+    }
+    if constexpr (LORA == Lora::kAdd) {
         if (rank < 0) low = __builtin_nanf("");
 #pragma unroll
         for (int e = 0; e < kPieces; ++e) {
@@ -607,12 +683,14 @@ __device__ __forceinline__ void gemv_q4_fused(const char * w, int64_t w_nb1, int
         for (int t = 0; t < 8; ++t) part[t] = t < TMAX && t < T ? dot_t(t) : 0.0f;
         float tot = wave_sum8_scatter(part, lane);
         const int t = lane >> 3;
-        if (LORA && id >= 0) tot += low;
+        if (LORA == Lora::kAdd && id >= 0) tot += low;
         if ((lane & 7) == 0 && t < T) *(float *) (y + (int64_t) t * y_nb1 + (int64_t) row * 4) = tot;
     } else {
         for (int t = 0; t < T; ++t) {
-            float part = wave_sum_to_last(dot_t(t));
-            if (LORA && id >= 0) part += low;
+            float part = dot_t(t);
+            if (LORA == Lora::kMake && id >= 0) part += low;
+            part = wave_sum_to_last(part);
+            if (LORA == Lora::kAdd && id >= 0) part += low;
             if (lane == 63) *(float *) (y + (int64_t) t * y_nb1 + (int64_t) row * 4) = part;
         }
     }
@@ -623,15 +701,15 @@ __global__ __launch_bounds__(1024) void gemv_q4_fused_kernel(const char * w, int
                                                              const char * x, int64_t x_nb1, int T,
                                                              char * __restrict__ y, int64_t y_nb1) {
     prefetch_params(w_nb1, y_nb1, blockDim.x);
-    gemv_q4_fused<BPL, TMAX, false>(w, w_nb1, N, K, x, x_nb1, T, y, y_nb1, lora::LoraParams{});
+    gemv_q4_fused<BPL, TMAX, Lora::kNone>(w, w_nb1, N, K, x, x_nb1, T, y, y_nb1, lora::LoraParams{});
 }
 
-template <int BPL, int TMAX>
+template <int BPL, int TMAX, Lora LORA>
 __global__ __launch_bounds__(1024) void gemv_q4_lora_kernel(const char * w, int64_t w_nb1, int N, int K, const char * x,
                                                             int64_t x_nb1, int T, char * __restrict__ y, int64_t y_nb1,
                                                             const lora::LoraParams p) {
     prefetch_params(w_nb1, y_nb1, blockDim.x, p);
-    gemv_q4_fused<BPL, TMAX, true>(w, w_nb1, N, K, x, x_nb1, T, y, y_nb1, p);
+    gemv_q4_fused<BPL, TMAX, LORA>(w, w_nb1, N, K, x, x_nb1, T, y, y_nb1, p);
 }
 
 // Most tokens of the one-launch kernel. Against the two launches for more
@@ -641,6 +719,7 @@ __global__ __launch_bounds__(1024) void gemv_q4_lora_kernel(const char * w, int6
 // steps make them, stay here because this kernel needs no scratch, so that
 // they can be captured into a graph whatever ran before.
 constexpr int kFusedMaxT = 8;
+constexpr int kCus = 256;
 
 size_t fused_lds_bytes(int64_t K, int64_t T) { return (size_t) (T * K + 8 * T * (K / 32)); }   // <= 160 KiB
 
@@ -654,14 +733,17 @@ int launch_fused(const al_tensor * w, const al_tensor * x, const al_tensor * y, 
     // per CU that keep a workgroup at 16 waves or fewer
     const int per_cu = (N + 16 * n_cu - 1) / (16 * n_cu);
     const int waves = std::max(1, (N + per_cu * n_cu - 1) / (per_cu * n_cu));
-    const size_t lds = fused_lds_bytes(K, T) + (p ? (size_t) T * p->R * 4 : 0);
+    const bool make = TMAX == 1 && p && mul_mat_q4_0_shrinks(w, T, p->R);
+    const size_t lds = fused_lds_bytes(K, T) + (p ? (size_t) (make ? K / 512 : T) * p->R * 4 : 0);
+    constexpr Lora kOne = TMAX == 1 ? Lora::kMake : Lora::kAdd;
+    auto adapted = make ? gemv_q4_lora_kernel<BPL, TMAX, kOne> : gemv_q4_lora_kernel<BPL, TMAX, Lora::kAdd>;
     if (lds > 64 * 1024) {
-        const void * f = p ? (const void *) gemv_q4_lora_kernel<BPL, TMAX> : (const void *) gemv_q4_fused_kernel<BPL, TMAX>;
+        const void * f = p ? (const void *) adapted : (const void *) gemv_q4_fused_kernel<BPL, TMAX>;
         hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds);
         if (e != hipSuccess) return al_hip_fail(e, "mul_mat_q4_0: LDS attribute");
     }
     if (p)
-        hipLaunchKernelGGL((gemv_q4_lora_kernel<BPL, TMAX>), dim3((unsigned) ((N + waves - 1) / waves)), dim3(64 * waves), lds, st,
+        hipLaunchKernelGGL(adapted, dim3((unsigned) ((N + waves - 1) / waves)), dim3(64 * waves), lds, st,
                            (const char *) w->data, (int64_t) w->nb[1], N, K, (const char *) x->data, (int64_t) x->nb[1], T,
                            (char *) y->data, (int64_t) y->nb[1], *p);
     else
@@ -821,7 +903,16 @@ bool mul_mat_q4_0_takes_lora(const al_tensor * w, int T, int R) {
     return T > kFusedMaxT || fused_lds_bytes(w->ne[0], T) + (size_t) T * R * 4 <= (160u << 10);
 }
 
-bool mul_mat_q4_0_shrinks(int T) { return T > kFusedMaxT; }
+bool mul_mat_q4_0_shrinks(const al_tensor * w, int T, int R) {
+    if (T > kFusedMaxT) return true;
+    // Of one token every workgroup can make v itself and save a launch, but
+    // reads all of A: worth it while a CU's workgroups read up to 400 KB (us,
+    // with the launch before and with its own: K 4096, N 4096, 8 ranks 9.8 / 6.3,
+    // 16 9.5 / 6.8, 32 10.0 / 8.1, 64 10.6 / 11.5; K 8192, N 5120, two a CU, 8
+    // ranks 14.5 / 13.7, 16 14.7 / 17.5; K 12288, N 4096, 16 ranks 14.3 / 13.2).
+    const int64_t per_cu = (w->ne[1] + 16 * kCus - 1) / (16 * kCus);
+    return T == 1 && R <= 64 && per_cu * w->ne[0] * R <= 3 << 16;
+}
 
 extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, const al_tensor * y, void * stream) {
     size_t bytes = 0;

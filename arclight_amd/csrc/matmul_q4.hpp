@@ -12,9 +12,9 @@ int mul_mat_q4_0_check(const al_tensor * w, const al_tensor * x, const al_tensor
 
 // The call, with scratch of that size (checked arguments). p: the adapters'
 // products added (NULL: none), where mul_mat_q4_0_takes_lora; their first one
-// is part of it for the token counts that mul_mat_q4_0_shrinks says, and has
+// is part of it for the sizes that mul_mat_q4_0_shrinks says, and has
 // to be there before it otherwise.
 int mul_mat_q4_0_run(const al_tensor * w, const al_tensor * x, const al_tensor * y, const lora::LoraParams * p, void * scratch,
                      hipStream_t stream);
 bool mul_mat_q4_0_takes_lora(const al_tensor * w, int T, int R);
-bool mul_mat_q4_0_shrinks(int T);
+bool mul_mat_q4_0_shrinks(const al_tensor * w, int T, int R);

@@ -392,3 +392,37 @@ def test_two_streams_and_columns_of_one_matrix(gpu):
         assert np.array_equal(got[:, i * N:(i + 1) * N], wide[:, i * N:(i + 1) * N])
         _check(got[:, (1 - i) * N:(2 - i) * N], ref, f"stream {i}")
         st.destroy()
+
+
+@pytest.mark.parametrize("K, N, R", [(4096, 2560, 16), (4096, 4099, 32), (8192, 33, 24), (12288, 20, 16), (4096, 70, 48), (8192, 4100, 8),
+                                     (16384, 5, 16), (4096, 4097, 40), (4096, 96, 64)])
+def test_one_token_through_the_projection(gpu, K, N, R):
+    """Sizes on both sides of where one token's launches become one; each rank
+    from none to the slot's, scales, no adapter, and adapters that are not to
+    be used."""
+    from arclight_amd import _lib, device, fattn, lora, matmul
+    _case(f"project one token {K} {N} {R}")
+    rng = np.random.default_rng(310)
+    ranks = np.array([0, 1, 7, 8, R - 1, R, R + 1, -2])
+    n = len(ranks)
+    a, b = _adapters(rng, n, R, K, N, np.clip(ranks, 0, R))
+    scales = (rng.random(n) * 2).astype(np.float32)
+    wo = O.random_q4_0(rng, N, K)
+    w = matmul.Q4_0Matrix(wo.view(np.uint8), K, N)
+    ad = lora.Adapters(_put(a.view(np.uint16)), _put(b.view(np.uint16)), _put(scales), _put(ranks.astype(np.int32)))
+    x = (rng.standard_normal((1, K)) * 3).astype(np.float32)
+    xd, base = _put(x), O.mul_mat_q4_0(wo, x)
+    more = (K // 32 + 16) * 2 * EPS32 * abs_bound(dequant_q4_0(wo), dequant_q8_0(O.quantize_q8_0(x)))
+    for i in (-1, *range(n), n, 1 << 30):
+        y = _put(np.full((1, N), 5.0, np.float32))
+        lora.project(ad, w, xd, _put(np.array([i], np.int32)), y)
+        device.synchronize()
+        if i >= 6:
+            with pytest.raises(_lib.ArclightError) as e:
+                fattn.device_errors()
+            assert e.value.status == abi.AL_ERR_INVALID and np.all(np.isnan(y.numpy(np.float32))), i
+            continue
+        fattn.device_errors()
+        ref, bound = _ref(x, a, b, scales, ranks, [i], base)
+        err = np.abs(y.numpy(np.float32).astype(np.float64) - ref)
+        assert np.all(err <= bound + more), (i, float((err / (bound + more)).max()))
