@@ -664,6 +664,7 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     const int64_t units = (int64_t) p.row_groups * Hkv;
     if (units > 65535) return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
     const int64_t most = n_seq * std::max<int64_t>(1, ((int64_t) p.c.max_pages * p.c.page_size + kTile - 1) / kTile);   // tiles there can be
+    if (most > INT32_MAX) return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
     // One workgroup a CU, 48 to 64 KB of its waves' loads in flight: more only
     // lengthen the queues (us with one / two / four: 24 sequences to 4000 cells
     // 51.3 / 52.6 / 54.6, 100000 cells of 64 heads 79.4 / 81.7 / 85.7, 8000 cells
@@ -676,7 +677,7 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     p.scale = a->scale;
     p.softcap = a->logit_softcap;
     pl.info_bytes = ((size_t) units * n_seq * sizeof(int2) + 255) / 256 * 256;
-    pl.bytes = pl.info_bytes + (size_t) units * p.target * 2 * rows * 130 * 4;
+    pl.bytes = pl.info_bytes + (p.target > 1 ? (size_t) units * p.target * 2 * rows * 130 * 4 : 0);     // one workgroup a unit: no pieces
     *out = pl;
     return AL_OK;
 }

@@ -76,8 +76,8 @@ int al_lora_f32(const al_lora_args * args);
  * blocks that the projection rounds them to). */
 int al_mul_mat_q4_0_lora_f32(const al_lora_args * args);
 
-/* Bytes of a caller's workspace that either call needs for these arguments; 0
- * for refused ones. */
+/* Bytes of a caller's workspace that al_mul_mat_q4_0_lora_f32 needs for these
+ * arguments, or without w al_lora_f32; 0 for refused ones. */
 uint64_t al_lora_workspace_bytes(const al_lora_args * args);
 
 #ifdef __cplusplus

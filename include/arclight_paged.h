@@ -101,11 +101,11 @@ int al_paged_append_f32(const al_paged_append_args * args);
  * not 0. What cells that a row does not see hold, NaN and infinities too,
  * does not reach it.
  * Hq is a multiple of Hkv, G = Hq / Hkv. T is at most 2^16, Hq 4096, T Hq
- * 2^22, n_seq 65535, T G / 64 Hkv 65535, T G^2 below 2^32
- * (AL_ERR_UNSUPPORTED otherwise). dst may not overlap q. Queries and probabilities are carried as pairs of
- * f16, so that results are those of f32 arithmetic (relative error about
- * 1e-6), unlike al_fattn_f16's. A sequence with an error that the kernel
- * records has NaN rows.
+ * 2^22, n_seq 65535, T G / 64 Hkv 65535; T G^2 is below 2^32, n_seq max_pages
+ * P / 32 below 2^31 (AL_ERR_UNSUPPORTED otherwise). dst may not overlap q.
+ * Queries and probabilities are carried as pairs of f16, so that results are
+ * those of f32 arithmetic (relative error about 1e-6), unlike al_fattn_f16's.
+ * A sequence with an error that the kernel records has NaN rows.
  * workspace: device scratch (al_paged_fattn_workspace_bytes), NULL: the
  * library's own for (current device, stream), as al_fattn_f16: then one
  * eager call of the same shapes has to come before a capture. Calls and

@@ -58,6 +58,8 @@ POOL_FAULTS = [
 @pytest.mark.parametrize("change, status", POOL_FAULTS + [
     (dict(q=T(F32, [128, 1024, 4095, 3]), dst=T(F32, [128, 4095, 1024, 3]), k_pool=T(F16, [128, 16, 1, 10]),
           v_pool=T(F16, [128, 16, 1, 10])), abi.AL_ERR_UNSUPPORTED),    # rows x heads past 32 bits: the division is not exact
+    (dict(q=T(F32, [128, 1, 32, 65]), dst=T(F32, [128, 32, 1, 65]), table=T(I32, [1 << 26, 65]), lens=T(I32, [65])),
+     abi.AL_ERR_UNSUPPORTED),                                          # tiles of all sequences past 31 bits
     (dict(q=T(F32, [128, 1, 32, 3], data=None)), abi.AL_ERR_INVALID),
     (dict(lens=T(I32, [3], data=None)), abi.AL_ERR_INVALID),
     (dict(q=T(F16, [128, 1, 32, 3])), abi.AL_ERR_UNSUPPORTED),
