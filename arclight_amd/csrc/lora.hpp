@@ -385,8 +385,15 @@ __device__ __forceinline__ float4 sum_parts(const LoraParams & p, const int row,
 // 8 ranks' share of an output: b . v over those below the rank.
 __device__ __forceinline__ float dot8(const half8 b, const float * v, const int ranks) {
     float s = 0.0f;
+    if (ranks >= 8) {
+        const float4 x = ((const float4 *) v)[0], y = ((const float4 *) v)[1];
+        const float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = __builtin_fmaf(e < ranks ? (float) b[e] : 0.0f, e < ranks ? v[e] : 0.0f, s);
+        for (int e = 0; e < 8; ++e) s = __builtin_fmaf((float) b[e], z[e], s);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = __builtin_fmaf(e < ranks ? (float) b[e] : 0.0f, e < ranks ? v[e] : 0.0f, s);
+    }
     return s;
 }
 

@@ -162,6 +162,7 @@ __global__ __launch_bounds__(64 * lora::shrink_waves<RT>(), RT == 8 ? 2 : 4) voi
     _Float16 * __restrict__ dx, int n_quantize, const lora::LoraParams p) {
     constexpr int kWaves = lora::shrink_waves<RT>();
     __shared__ __align__(16) float lds[kWaves * lora::shrink_lds<RT, lora::shrink_unroll<RT>()>()];
+    prefetch_params(x_nb1, n_quantize, p);
     if ((int) blockIdx.x < n_quantize) {
         const int item = blockIdx.x * kWaves + (threadIdx.x >> 6);
         if (item < n_items) quantize_q8(x, x_nb1, nb, T, item, frag, dx);
@@ -347,6 +348,7 @@ template <int BL>
 __global__ __launch_bounds__(kGemmWaves * 64, 4) void gemm_q4_lora_kernel(const char * w, int64_t w_nb1, int N, const uint4 * frag,
                                                                        const uint4 * dx, int T, char * y, int64_t y_nb1,
                                                                        const lora::LoraParams p) {
+    prefetch_params(w_nb1, y_nb1, p);
     gemm_q4<BL, true>(w, w_nb1, N, frag, dx, T, y, y_nb1, p);
 }
 
