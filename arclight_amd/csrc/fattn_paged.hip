@@ -29,9 +29,9 @@
 // Work. The cells that a batch's sequences hold differ and are known on the
 // device only. For each (KV head, row group) the tiles of all sequences are
 // thought of as one row, cut into equal parts for the workgroups that fit the
-// card; every workgroup reads the lengths and finds the sequences, or pieces
-// of them, of its own part. A sequence within one workgroup is written at
-// once; the pieces of the others go to records (at most two of a workgroup's
+// card (between sequences, where all are short); every workgroup reads the
+// lengths and finds the sequences, or pieces of them, of its own part. A
+// sequence within one workgroup is written at once; the pieces of the others go to records (at most two of a workgroup's
 // pieces are such), which a second launch joins. (Joined by the workgroup that
 // ends last instead: 100000 cells 88 us instead of 83, as the records then have
 // to pass through memory that all XCDs see.)
@@ -62,7 +62,8 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kTile = 32;                       // cells of a wave's step
-constexpr int kMinTiles = 4;                    // least tiles of a chunk: one for each wave
+constexpr int kMinTiles = 4;                    // least tiles of a part: one for each wave
+constexpr int kWhole = 16;                      // sequences of up to so many tiles are not cut
 constexpr float kPScale = 16384.0f;             // probabilities: 2^14 p stays normal in f16 down to p = 2^-28
 
 struct PagedFattnParams {
@@ -76,7 +77,7 @@ struct PagedFattnParams {
     float * part;                                       // records [unit][workgroup][2]: rows x 128 sums, rows x {m, l}
     int32_t T, G, Hkv, R, row_groups, row_tiles;        // row tiles of 16 in a group
     uint32_t g_magic;                                   // ceil(2^32 / G) (0 for 1)
-    int32_t target;                                     // workgroups of a unit (head, row group)
+    int32_t target, long_target;                        // workgroups of a unit (head, row group), those that long sequences use
     int32_t row_waves;                                  // join: waves of a row
     float scale, softcap;
 };
@@ -84,6 +85,10 @@ struct PagedFattnParams {
 template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ int dpp_add(const int x) {
     return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
+}
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_max(const int x) {                 // (of values that are not negative)
+    return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false));
 }
 // Sum of the lanes up to and with this one (DPP: within rows of 16, then the
 // rows' last lanes into those after them).
@@ -150,6 +155,17 @@ struct Block {
         upto = wave_scan(tiles);
     }
     __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
+    __device__ __forceinline__ int active() const { return __builtin_popcountll(__ballot(tiles > 0)); }
+    __device__ __forceinline__ int longest() const {
+        int x = tiles;
+        x = dpp_max<0x111, 0xf>(x);
+        x = dpp_max<0x112, 0xf>(x);
+        x = dpp_max<0x114, 0xf>(x);
+        x = dpp_max<0x118, 0xf>(x);
+        x = dpp_max<0x142, 0xa>(x);
+        x = dpp_max<0x143, 0xc>(x);
+        return __builtin_amdgcn_readlane(x, 63);
+    }
 };
 
 template <typename P>
@@ -205,20 +221,52 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
     const int wt0 = token_of(p, min(r0, p.R - 1)), wt1 = token_of(p, min(r0 + 16, p.R) - 1);
 
     // this workgroup's part of all tiles
+    const int n_blocks = (p.c.n_seq + 63) / 64;
     Block b;
     b.load(p, 0, lane, t0, t1);
-    int S = b.total(), block = 0, before = 0;
-    for (int i = 1; 64 * i < p.c.n_seq; ++i) {
+    int S = b.total(), active = b.active(), longest = b.longest(), block = 0, before = 0;
+    for (int i = 1; i < n_blocks; ++i) {
         Block x;
         x.load(p, i, lane, t0, t1);
         S += x.total();
+        active += x.active();
+        longest = max(longest, x.longest());
     }
-    const int W = min(p.target, (S + kMinTiles - 1) / kMinTiles);
+    // Several sequences of up to kWhole tiles each are left whole, one or some to
+    // a workgroup: equal parts cut them at places of their own, and a second
+    // piece costs a workgroup more than the rounds that the cut saves (us, cut
+    // and whole: 4 sequences of up to 200 cells 13.4, 10.1, 64 of 100 16.4, 11.5,
+    // 10 of 500 14.1, 12.3; whole up to 32 tiles: 128 of 700 56.4, 60.2). Else
+    // kMinTiles a workgroup at least, or a sequence; p.target workgroups for
+    // sequences of up to 16 tiles on average, p.long_target for longer ones.
+    const bool cut = longest > kWhole || active == 1;
+    const int W = cut ? min(S > 16 * active ? p.long_target : p.target, max((S + kMinTiles - 1) / kMinTiles, active)) : min(p.target, active);
     if (wg >= W) return;
     const Parts parts(S, W);
-    const int stop = parts.begin(wg + 1);
+    int at = parts.begin(wg), stop = parts.begin(wg + 1);
+    if (!cut) {
+        const Parts seqs(active, W);
+        auto tile_of = [&](int i) {                                    // first tile of the i-th sequence that has any
+            Block x = b;
+            for (int k = 0, tiles = 0;;) {
+                const uint64_t mask = __ballot(x.tiles > 0);
+                const int have = __builtin_popcountll(mask);
+                if (i < have) {
+                    const int nth = __builtin_amdgcn_mbcnt_hi((uint32_t) (mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) mask, 0));
+                    const int l = __builtin_ctzll(__ballot(x.tiles > 0 && nth == i));
+                    return tiles + __builtin_amdgcn_readlane(x.upto, l) - __builtin_amdgcn_readlane(x.tiles, l);
+                }
+                i -= have;
+                tiles += x.total();
+                if (++k == n_blocks) return tiles;
+                x.load(p, k, lane, t0, t1);
+            }
+        };
+        at = tile_of(seqs.begin(wg));
+        stop = tile_of(seqs.begin(wg + 1));
+    }
 
-    for (int at = parts.begin(wg); at < stop;) {
+    while (at < stop) {
         // the sequence that holds tile `at`
         while (at >= before + b.total()) {
             before += b.total();
@@ -669,11 +717,14 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     // lengthen the queues (us with one / two / four: 24 sequences to 4000 cells
     // 51.3 / 52.6 / 54.6, 100000 cells of 64 heads 79.4 / 81.7 / 85.7, 8000 cells
     // 13.2 / 14.2 / 13.9). Two where row tiles share the loads (verify of 10
-    // sequences 48.5 / 47.1 / 50.0).
-    const int64_t wgs = (p.row_tiles == 1 ? 1 : 2) * (int64_t) n_cu;
-    p.target = (int32_t) std::max<int64_t>(1, std::min<int64_t>(wgs / std::max<int64_t>(1, units), (most + kMinTiles - 1) / kMinTiles));
+    // sequences 48.5 / 47.1 / 50.0), and for many short sequences, whose ends
+    // are not hidden (96 to 300 cells 30.8 / 24.9, 128 to 700 57.2 / 57.2).
+    const int64_t per_cu = n_cu / std::max<int64_t>(1, units);
+    const int64_t useful = std::max(n_seq, (most + kMinTiles - 1) / kMinTiles);
+    p.target = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * n_cu / std::max<int64_t>(1, units), useful));
+    p.long_target = p.row_tiles == 1 ? (int32_t) std::max<int64_t>(1, std::min<int64_t>(per_cu, p.target)) : p.target;
     // few sequences have many pieces each
-    p.row_waves = p.target > 16 * n_seq ? kWaves : 1;
+    p.row_waves = p.long_target > 16 * n_seq ? kWaves : 1;
     p.scale = a->scale;
     p.softcap = a->logit_softcap;
     pl.info_bytes = ((size_t) units * n_seq * sizeof(int2) + 255) / 256 * 256;

@@ -487,3 +487,29 @@ def test_decode_steps_of_a_batch(gpu, replayed):
     if graph is not None:
         graph.destroy()
     stream.destroy()
+
+
+@pytest.mark.parametrize("n, longest, T, Hq, Hkv", [(2, 40, 1, 8, 8), (70, 500, 1, 32, 8), (64, 512, 1, 4, 4), (65, 513, 1, 4, 4),
+                                                    (300, 60, 1, 8, 2), (130, 200, 7, 8, 8), (40, 300, 20, 8, 2), (200, 33, 3, 64, 8)])
+def test_sequences_left_whole_or_cut(gpu, n, longest, T, Hq, Hkv):
+    """Short sequences, some to a workgroup, over one block of 64 lanes and
+    more; the longest at, below and above where they are cut; empty slots at
+    both ends and between; counts from none to all."""
+    _case(f"paged attention, {n} sequences of up to {longest}")
+    rng = np.random.default_rng(17)
+    lens = [int(x) for x in rng.integers(0, longest + 1, n)]
+    lens[n // 2] = longest
+    counts = [int(min(x, c)) for x, c in zip(lens, rng.integers(0, T + 1, n))]
+    counts[n // 2] = T
+    counts[0] = 0
+    if n > 2:
+        counts[-1] = counts[n // 3] = 0
+    pool = P.Pool(rng, lens, Hkv, 16)
+    q = (rng.standard_normal((n, T, Hq, D)) * 2).astype(np.float32)
+    ref = P.attention(pool, q, lens, counts, 1 / math.sqrt(D))
+    _check(_attend(pool, q, lens, counts), ref, f"{n} sequences")
+    if T == 1:                                                         # every one of the batch with a token
+        _check(_attend(pool, q, lens), P.attention(pool, q, lens, [1] * n, 1 / math.sqrt(D)), f"{n} sequences, all")
+    only = [0] * n                                                     # one alone
+    only[n // 2] = T
+    _check(_attend(pool, q, lens, only), P.attention(pool, q, lens, only, 1 / math.sqrt(D)), "one of them")
