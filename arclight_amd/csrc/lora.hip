@@ -290,9 +290,11 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     // with 256; 500 18.0, 21.7 and 16.6, 17.8; 2000 35.2, 61.4 and 35.4, 43.2).
     // They have at least 4 or 16 groups, which p.slots workgroups share, an odd
     // number, as workgroups go to the 8 XCDs in turn and the last slots have
-    // little to do (8000 rows with 4, 5, 8 for 64 rows: 93, 86, 97).
+    // little to do (8000 rows with 4, 5, 8 for 64 rows: 93, 86, 97). Many
+    // adapters make many groups (us with 9 and 17: 122 rows shuffled over 29
+    // adapters 36.2, 28.0, 300 rows over 9 13.7, 17.0).
     p.window = T <= 384 ? 64 : 256;
-    p.slots = p.window == 64 ? 9 : 21;
+    p.slots = p.window == 256 ? 21 : A < 16 ? 9 : 17;
     p.copy = base.data != y.data;
     // K in parts of at least 512 columns while the CUs are not full.
     const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kParts, (K + 511) / 512, T <= kFew ? n_cu / 16 : 2 * n_cu / tiles}));
