@@ -426,3 +426,31 @@ def test_one_token_through_the_projection(gpu, K, N, R):
         ref, bound = _ref(x, a, b, scales, ranks, [i], base)
         err = np.abs(y.numpy(np.float32).astype(np.float64) - ref)
         assert np.all(err <= bound + more), (i, float((err / (bound + more)).max()))
+
+
+@pytest.mark.parametrize("T", [40, 70])
+def test_rows_past_32_bits(gpu, T):
+    """Rows of x, base and y 2^27 bytes apart, adapters 3 GB apart."""
+    from arclight_amd import device, fattn, lora
+    _case(f"lora: offsets past 4 GB, T={T}")
+    rng = np.random.default_rng(320)
+    K, N, R, n, apart, slot = 256, 64, 8, 3, 1 << 27, 3 << 30
+    a, b = _adapters(rng, n, R, K, N, [R] * n)
+    ids = _ids(rng, T, n, "any")
+    x, base = rng.standard_normal((T, K)).astype(np.float32), rng.standard_normal((T, N)).astype(np.float32)
+    rows = device.DeviceBuffer(apart * (T - 1) + 4096)                 # x at 0, base at 1024, y at 2048 of each row
+    for t in range(T):
+        rows.upload(x[t], apart * t)
+        rows.upload(base[t], apart * t + 1024)
+    slots = device.DeviceBuffer(slot * (n - 1) + 8192)                 # A at 0, B at 4096 of each slot
+    for i in range(n):
+        slots.upload(a[i].view(np.uint16), slot * i)
+        slots.upload(b[i].view(np.uint16), slot * i + 4096)
+    view = lambda cols, off: device.DeviceTensor(rows, abi.AL_TYPE_F32, (T, cols), (apart, 4), off)  # noqa: E731
+    ad = lora.Adapters(device.DeviceTensor(slots, abi.AL_TYPE_F16, (n, R, K), (slot, K * 2, 2)),
+                       device.DeviceTensor(slots, abi.AL_TYPE_F16, (n, N, R), (slot, R * 2, 2), 4096))
+    lora.ApplyCall(ad, view(K, 0), _put(ids), view(N, 1024), view(N, 2048)).run()
+    device.synchronize()
+    fattn.device_errors()
+    got = np.stack([rows.download(np.empty(N, np.float32), apart * t + 2048) for t in range(T)])
+    _check(got, _ref(x, a, b, np.ones(n), [R] * n, ids, base), "offsets")

@@ -513,3 +513,31 @@ def test_sequences_left_whole_or_cut(gpu, n, longest, T, Hq, Hkv):
     only = [0] * n                                                     # one alone
     only[n // 2] = T
     _check(_attend(pool, q, lens, only), P.attention(pool, q, lens, only, 1 / math.sqrt(D)), "one of them")
+
+
+def test_append_past_32_bits(gpu):
+    """Pages 2.5 GB apart: the cells of the last ones lie beyond 4 GB."""
+    from arclight_amd import device, fattn, paged
+    _case("paged append, pages past 4 GB")
+    rng = np.random.default_rng(24)
+    Hkv, page, n_pages = 2, 8, 3
+    apart = 5 * 2 ** 29
+    pools = []
+    for _ in range(2):
+        buf = device.DeviceBuffer(apart * (n_pages - 1) + page * Hkv * D * 2)
+        for i in range(n_pages):
+            buf.upload(np.full((page, Hkv, D), 0x3c00, np.uint16), apart * i)
+        pools.append(device.DeviceTensor(buf, abi.AL_TYPE_F16, (n_pages, page, Hkv, D), (apart, Hkv * D * 2, D * 2, 2)))
+    cache = paged.PagedCache(*pools, _put(np.array([[1, 2, 0]], np.int32)))
+    pos = np.array([17, 0, 15, 8], np.int32)                        # pages 0, 1, 2, 2
+    k, v = (rng.standard_normal((4, Hkv, D)).astype(np.float32) for _ in range(2))
+    paged.append(cache, None, _put(k), _put(v), _put(pos), _put(np.zeros(4, np.int32)), norm=False)
+    device.synchronize()
+    fattn.device_errors()
+    for t, x in zip(pools, (k, v)):
+        for at in range(n_pages):
+            want = np.full((page, Hkv, D), 0x3c00, np.uint16)
+            for i, p_ in enumerate(pos):
+                if [1, 2, 0][p_ // page] == at:
+                    want[p_ % page] = x[i].astype(np.float16).view(np.uint16)
+            assert np.array_equal(t.buf.download(np.empty((page, Hkv, D), np.uint16), apart * at), want), at
