@@ -271,7 +271,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         // the sequence that holds tile `at`
         while (at >= before + b.total()) {
             before += b.total();
-            b.load(p, ++block, lane, t0, t1);
+            if (++block >= n_blocks) return;                         // (lengths that change meanwhile: not without an end)
+            b.load(p, block, lane, t0, t1);
         }
         const int l64 = __builtin_ctzll(__ballot(at < before + b.upto));
         const int seq = 64 * block + l64;
