@@ -54,6 +54,7 @@ struct Workspace {
     void * ptr = nullptr;
     size_t bytes = 0;
     std::vector<void *> old;                    // smaller ones before it
+    void * operands = nullptr;                  // al_library_operands
 };
 
 struct DeviceState {
@@ -166,6 +167,33 @@ int al_library_workspace(size_t bytes, void * stream, void ** ptr) {
     return rc;
 }
 
+// One for each stream, as above. Of one size, so that none grows, and without
+// an initial value, so that it can be made inside a capture: in the relaxed
+// mode a thread that captures may allocate.
+int al_library_operands(size_t bytes, void * stream, void ** ptr) {
+    int dev;
+    DeviceState * st;
+    const int rc = device_state(&dev, &st);
+    if (rc != AL_OK) return rc;
+    if (bytes > kOperandBytes) return al_fail(AL_ERR_WORKSPACE, "operands of %zu bytes > %zu", bytes, kOperandBytes);
+    std::lock_guard<std::mutex> lk(g_mu);
+    void *& own = st->ws[stream].operands;
+    if (!own) {
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
+        if (e != hipSuccess) return al_hip_fail(e, "hipThreadExchangeStreamCaptureMode");
+        e = hipMalloc(&own, kOperandBytes);
+        const hipError_t back = hipThreadExchangeStreamCaptureMode(&mode);
+        if (e != hipSuccess) {
+            own = nullptr;
+            return al_hip_fail(e, "hipMalloc(operands)");
+        }
+        if (back != hipSuccess) return al_hip_fail(back, "hipThreadExchangeStreamCaptureMode");
+    }
+    *ptr = own;
+    return AL_OK;
+}
+
 extern "C" int al_fattn_release_stream(void * stream) {
     int dev;
     DeviceState * st;
@@ -174,13 +202,18 @@ extern "C" int al_fattn_release_stream(void * stream) {
     std::lock_guard<std::mutex> lk(g_mu);
     auto it = st->ws.find(stream);
     if (it == st->ws.end()) return AL_OK;
-    if (it->second.ptr) {
+    Workspace & w = it->second;
+    if (w.ptr || w.operands) {
         // the stream's kernels (and graphs replayed on it) may still use it
         hipError_t e = hipDeviceSynchronize();
         if (e != hipSuccess) return al_hip_fail(e, "hipDeviceSynchronize");
-        std::vector<void *> & old = it->second.old;
-        for (; !old.empty() && e == hipSuccess; old.pop_back()) e = hipFree(old.back());
-        if (e == hipSuccess) e = hipFree(it->second.ptr);
+        for (; !w.old.empty() && e == hipSuccess; w.old.pop_back()) e = hipFree(w.old.back());
+        if (e == hipSuccess) e = hipFree(w.ptr);
+        if (e == hipSuccess) {
+            w.ptr = nullptr;
+            w.bytes = 0;
+            e = hipFree(w.operands);
+        }
         if (e != hipSuccess) return al_hip_fail(e, "hipFree(workspace)");
     }
     st->ws.erase(it);

@@ -19,7 +19,7 @@
 // nibbles, the weights' offset of 8 folded into one multiply by the block's
 // value sum; lane sums meet in a DPP wave reduction.
 // Longer inputs (up to 64 tokens) take two launches: quantize_q8_kernel
-// (into library scratch, laid out as MFMA operands) and gemm_q4_kernel, whose
+// (into the stream's own memory, laid out as MFMA operands) and gemm_q4_kernel, whose
 // integer dot products run on the matrix cores. The 4-bit weights, 18 bytes
 // per 32, are read from memory once; with more than 16 tokens every tile of
 // 16 reads them again from the caches.
@@ -28,7 +28,6 @@
 
 #include <algorithm>
 #include <cstring>
-#include <mutex>
 
 #include "../../include/arclight_matmul.h"
 #include "kernel_args.hpp"
@@ -718,8 +717,8 @@ __global__ __launch_bounds__(1024) void gemv_q4_lora_kernel(const char * w, int6
 // tokens (us per call): K 4096, N 4096: 7.0 / 8.2 at 5 tokens, 8.3 / 8.2 at 8;
 // K 8192, N 5120: 13.2 / 15.8 at 4, 17.9 / 15.6 at 5, 21.7 / 15.7 at 8. At K
 // 8192 the line for time alone would be 4; calls of 5 to 8 tokens, as verify
-// steps make them, stay here because this kernel needs no scratch, so that
-// they can be captured into a graph whatever ran before.
+// steps make them, stay here because this kernel needs no memory beside its
+// operands.
 constexpr int kFusedMaxT = 8;
 constexpr int kCus = 256;
 
@@ -779,40 +778,6 @@ int launch_gemm(const al_tensor * w, const al_tensor * y, int N, int tiles, int 
                            frag, dx, T, (char *) y->data, (int64_t) y->nb[1]);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "mul_mat_q4_0: launch");
-}
-
-// Per-device scratch for the quantized activations; the first allocation
-// has room for every call (64 tokens of K = 16384: 1.1 MB), so that none
-// grows it, which would fail inside a capture.
-struct Scratch {
-    void * p = nullptr;
-    size_t bytes = 0;
-};
-std::mutex g_mu;
-Scratch g_scratch[64];
-
-int scratch(size_t bytes, void ** out) {
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return al_hip_fail(e, "hipGetDevice");
-    if (dev < 0 || dev >= 64) return al_fail(AL_ERR_INVALID, "mul_mat_q4_0: device %d", dev);
-    std::lock_guard<std::mutex> lk(g_mu);
-    Scratch & s = g_scratch[dev];
-    if (s.bytes < bytes) {
-        if (s.p) {
-            e = hipDeviceSynchronize();
-            if (e == hipSuccess) e = hipFree(s.p);
-            if (e != hipSuccess) return al_hip_fail(e, "mul_mat_q4_0: scratch free");
-            s.p = nullptr;
-            s.bytes = 0;
-        }
-        const size_t sz = std::max(bytes, (size_t) 2 << 20);
-        e = hipMalloc(&s.p, sz);
-        if (e != hipSuccess) return al_hip_fail(e, "mul_mat_q4_0: scratch");
-        s.bytes = sz;
-    }
-    *out = s.p;
-    return AL_OK;
 }
 
 }  // namespace
@@ -920,7 +885,7 @@ extern "C" int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, con
     size_t bytes = 0;
     void * s = nullptr;
     int rc = mul_mat_q4_0_check(w, x, y, &bytes);
-    if (rc == AL_OK && bytes) rc = scratch(bytes, &s);
+    if (rc == AL_OK && bytes) rc = al_library_operands(bytes, stream, &s);
     if (rc != AL_OK) return rc;
     return mul_mat_q4_0_run(w, x, y, nullptr, s, (hipStream_t) stream);
 }

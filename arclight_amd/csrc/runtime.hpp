@@ -17,3 +17,9 @@ int al_device_error_flag(int ** flag);   // [0, 1] set_rows, [2] a merge gave up
 // workspace of (current device, stream), behind its counters. No initial
 // value; calls on one stream share it.
 int al_library_workspace(size_t bytes, void * stream, void ** ptr);
+
+// The quantized activations of the Q4_0 projection: memory of (current device,
+// stream) apart from its workspace, kOperandBytes whatever `bytes` (64 tokens
+// of K = 16384 take 1.1 MB). Allocated on first use, inside a capture too.
+constexpr size_t kOperandBytes = (size_t) 2 << 20;
+int al_library_operands(size_t bytes, void * stream, void ** ptr);

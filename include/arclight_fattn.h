@@ -180,7 +180,7 @@ int al_fattn_apply_node_hints(al_fattn_args * args, const int32_t * op_params);
 
 /*
  * Frees the library workspace of (current device, stream) that calls with
- * workspace == NULL made, after waiting for the device (its kernels and any
+ * workspace == NULL made, and what al_mul_mat_q4_0_f32 keeps there, after waiting for the device (its kernels and any
  * graph replayed on the stream may still use it). No counterpart in the
  * reference (its op uses per-thread scratch of the graph's work buffer,
  * nnml/src/ops/arm/arm.cpp:2299-2302). A later call allocates again. AL_OK

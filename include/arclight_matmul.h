@@ -34,8 +34,12 @@ extern "C" {
  *   x  f32 ne = [K, T], nb0 = 4
  *   y  f32 ne = [N, T], nb0 = 4
  * K must be 4096, 8192, 12288 or 16384 (the Qwen3 output projections: 4096
- * for 4B, 8192 for 32B) and T at most 64; x rows 16-byte aligned. Uses library-owned device scratch for the quantized
- * activations. Enqueues on `stream`.
+ * for 4B, 8192 for 32B) and T at most 64; x rows 16-byte aligned. Enqueues on
+ * `stream`. More than 8 tokens are quantized into 2 MB of device memory that
+ * the library keeps for each (current device, stream): allocated by the first
+ * such call, inside a capture too, freed by al_fattn_release_stream. Calls on
+ * different streams do not share it. A graph uses that of the stream it was
+ * captured on, and its replays have to be ordered with that stream's calls.
  */
 int al_mul_mat_q4_0_f32(const al_tensor * w, const al_tensor * x, const al_tensor * y, void * stream);
 
