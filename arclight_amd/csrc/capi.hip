@@ -16,9 +16,9 @@
 
 #include "../../include/arclight_fattn.h"
 #include "../../include/arclight_prologue.h"
+#include "device_errors.hpp"
 #include "fattn_kernels.hpp"
 #include "kv_write.hpp"
-#include "paged.hpp"
 #include "runtime.hpp"
 
 namespace {
@@ -931,31 +931,19 @@ extern "C" const char * al_last_error(void) { return g_last_error.c_str(); }
 
 extern "C" const char * al_version(void) { return "arclight_amd fattn 0.1 (gfx950)"; }
 
-static std::string paged_error_text(int what, int value) {
-    const std::string v = std::to_string(value);
-    switch (what) {
-        case kPagedBadPage:   return "sequence " + v + " has a page outside the pool";
-        case kPagedBadLength: return "a length of " + v + " cells is not within the table";
-        case kPagedBadCount:  return "a sequence with " + v + " new tokens";
-        case kPagedBadSeq:    return "a token of sequence " + v + ", which the table does not have";
-        default:              return "a token at position " + v + ", which is not within the table";
-    }
-}
-
 extern "C" int al_device_errors(void) {
     int * flag = nullptr;
     int rc = al_device_error_flag(&flag);
     if (rc != AL_OK) return rc;
-    int h[12] = {};
+    int h[kErrWords] = {};
     hipError_t e = hipMemcpy(h, flag, sizeof(h), hipMemcpyDeviceToHost);
     if (e != hipSuccess) return al_hip_fail(e, "hipMemcpy(error flag)");
-    if (h[0] || h[2] || h[4] || h[8]) {
+    std::string text;
+    const int status = device_error_status(h, text);
+    if (status != AL_OK) {
         e = hipMemset(flag, 0, sizeof(h));
         if (e != hipSuccess) return al_hip_fail(e, "hipMemset(error flag)");
-        if (h[0]) return al_fail(AL_ERR_INVALID, "set_rows: row index %d out of range (ops.cpp:171)", h[1]);
-        if (h[4]) return al_fail(AL_ERR_INVALID, "paged cache: %s", paged_error_text(h[5], h[6]).c_str());
-        if (h[8]) return al_fail(AL_ERR_INVALID, "lora: a row of adapter %d, which is not there or whose rank does not fit", h[9]);
-        return al_fail(AL_ERR_HIP, "fattn: a merging workgroup gave up waiting for the other splits' records");
+        return al_fail(status, "%s", text.c_str());
     }
     return AL_OK;
 }

@@ -7,6 +7,7 @@
 
 #include "../../include/arclight_lora.h"
 #include "device_common.hpp"
+#include "device_errors.hpp"
 
 namespace lora {
 
@@ -57,7 +58,7 @@ __device__ __forceinline__ int rank_of(const LoraParams & p, const int a) {
 }
 
 __device__ __forceinline__ void lora_error(const LoraParams & p, const int a) {
-    if (atomicCAS(p.err + 8, 0, 1) == 0) p.err[9] = a;
+    if (atomicCAS(p.err + kErrLora, 0, 1) == 0) p.err[kErrLora + 1] = a;
 }
 
 // Up to 16 rows that share an adapter (a < 0: have none). Lane n < 16 has the

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "../../include/arclight_paged.h"
+#include "device_errors.hpp"
 
 // Pools of f16 [128, P, Hkv, n_pages] and the sequences' page tables. Strides
 // in bytes, the table's in entries.
@@ -16,15 +17,13 @@ struct PagedPools {
     int32_t n_seq, n_pages, max_pages, page_size;
     int32_t groups;                            // page_size / 8: pages in groups of 8 cells
     uint32_t magic;                            // ceil(2^32 / groups) (0 for 1)
-    int * err;                                 // device error flags: [4] set, [5] a PagedError, [6] its value
+    int * err;                                 // device error words (device_errors.hpp)
 };
 
-enum PagedError { kPagedBadPage = 1, kPagedBadLength = 2, kPagedBadCount = 3, kPagedBadSeq = 4, kPagedBadPos = 5 };
-
 __device__ __forceinline__ void paged_error(const PagedPools & p, const int what, const int value) {
-    if (atomicCAS(p.err + 4, 0, 1) == 0) {
-        p.err[5] = what;
-        p.err[6] = value;
+    if (atomicCAS(p.err + kErrPaged, 0, 1) == 0) {
+        p.err[kErrPaged + 1] = what;
+        p.err[kErrPaged + 2] = value;
     }
 }
 

@@ -11,7 +11,7 @@ void al_clear_error();
 // Per-device state, created on first use with the device current.
 int al_device_cu_count(int * n_cu);
 int al_device_lds_per_block(int * bytes);
-int al_device_error_flag(int ** flag);   // [0, 1] set_rows, [2] a merge gave up waiting, [4..6] paged cache, [8, 9] lora
+int al_device_error_flag(int ** flag);   // its words: device_errors.hpp
 
 // Records of a call with no workspace of its own: `bytes` of the library's
 // workspace of (current device, stream), behind its counters. No initial

@@ -235,11 +235,14 @@ int al_set_rows_f32_f16(const al_tensor * dst, const al_tensor * src,
 
 /*
  * Reports and clears errors that kernels recorded on the current device
- * (out-of-range set_rows indices: AL_ERR_INVALID; a decode merge that gave
- * up waiting for the other splits of its launch, about a second, which a
- * correct run never does: AL_ERR_HIP, and that call's merged rows hold
- * NaN). Call after synchronizing the stream. Returns AL_OK or the error
- * with al_last_error() set.
+ * (out-of-range set_rows indices, what the paged cache or the adapters found
+ * wrong: AL_ERR_INVALID; a decode merge that gave up waiting for the other
+ * splits of its launch, about a second, which a correct run never does:
+ * AL_ERR_HIP, and that call's merged rows hold NaN). Call after
+ * synchronizing the stream. Returns AL_OK or the error with al_last_error()
+ * set. Of each kind the first is reported. Several kinds are reported
+ * together, al_last_error() names them all; the status is then AL_ERR_HIP for
+ * a merge that gave up, unless there was a set_rows index too.
  */
 int al_device_errors(void);
 
