@@ -155,6 +155,10 @@ struct Block {
         tiles = in ? tiles_of(seq_work(p, len, count).limit(t0, t1)) : 0;
         upto = wave_scan(tiles);
     }
+    // A negative count makes an empty slot, which no workgroup comes to.
+    __device__ __forceinline__ void report(const PagedFattnParams & p) const {
+        if (count < 0) paged_error(p.c, kPagedBadCount, count);
+    }
     __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
     __device__ __forceinline__ int active() const { return __builtin_popcountll(__ballot(tiles > 0)); }
     __device__ __forceinline__ int longest() const {
@@ -225,10 +229,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
     const int n_blocks = (p.c.n_seq + 63) / 64;
     Block b;
     b.load(p, 0, lane, t0, t1);
+    const bool first_wave = blockIdx.x == 0 && wave == 0;
+    if (first_wave) b.report(p);
     int S = b.total(), active = b.active(), longest = b.longest(), block = 0, before = 0;
     for (int i = 1; i < n_blocks; ++i) {
         Block x;
         x.load(p, i, lane, t0, t1);
+        if (first_wave) x.report(p);
         S += x.total();
         active += x.active();
         longest = max(longest, x.longest());

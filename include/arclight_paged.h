@@ -95,7 +95,8 @@ int al_paged_append_f32(const al_paged_append_args * args);
  *   sinks   f32 [Hq], or data NULL
  * Token t < counts[s] sees cells c < lens[s] - counts[s] + 1 + t. Rows of
  * tokens t >= counts[s] are left as they were (counts[s] = 0: an empty slot
- * of the batch). A row that sees no cell is zero, with or without a sink
+ * of the batch, whose length is not looked at; a negative count is recorded
+ * as an error, and the slot is empty too). A row that sees no cell is zero, with or without a sink
  * (al_fattn_f16 gives NaN without one). The logits are scale * q . k, or
  * logit_softcap * tanh(scale * q . k / logit_softcap) when logit_softcap is
  * not 0. What cells that a row does not see hold, NaN and infinities too,
@@ -105,7 +106,8 @@ int al_paged_append_f32(const al_paged_append_args * args);
  * P / 32 below 2^31 (AL_ERR_UNSUPPORTED otherwise). dst may not overlap q.
  * Queries and probabilities are carried as pairs of f16, so that results are
  * those of f32 arithmetic (relative error about 1e-6), unlike al_fattn_f16's.
- * A sequence with an error that the kernel records has NaN rows.
+ * A sequence whose length or count is recorded as an error has NaN rows, and
+ * so have all rows that see a cell of a page outside the pool.
  * workspace: device scratch (al_paged_fattn_workspace_bytes), NULL: the
  * library's own for (current device, stream), as al_fattn_f16: then one
  * eager call of the same shapes has to come before a capture. Calls and
