@@ -182,18 +182,18 @@ __device__ __forceinline__ char * record(const P & p, const int unit, const int 
 __device__ __forceinline__ float grow(const float a, const float b) { return a == b ? 1.0f : exp_fast(a - b); }
 
 // Factor of a row's sums, with the sink as one more logit without a value: 0
-// for a row that saw nothing.
+// for a row that sees nothing, NaN where all logits are -inf.
 template <typename P>
-__device__ __forceinline__ float row_factor(const P & p, const float M, float L, const int head) {
+__device__ __forceinline__ float row_factor(const P & p, const float M, float L, const int head, const bool sees) {
     L *= 1.0f / kPScale;
     float up = 1.0f / kPScale;
     if (p.sinks) {
         const float sink = p.sinks[head], top = fmaxf(M, sink);
         const float e = grow(M, top);
         up *= e;
-        L = L * e + grow(sink, top);
+        L = L * e + (sink == -AL_INF ? 0.0f : grow(sink, top));
     }
-    return L == 0.0f ? 0.0f : up / L;
+    return L == 0.0f ? sees ? __builtin_nanf("") : 0.0f : up / L;
 }
 
 // The kernel's arguments as memory, to be loaded where they are used: held in
@@ -447,9 +447,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
 #pragma unroll
                 for (int j = 0; j < 8; ++j) acc[j] *= f;
             }
+            // (a row that has met no logit but -inf, as products that overflow
+            // give it, has m = -inf still: their weights are 0, not e^(-inf + inf))
+            const float from = m == -AL_INF ? 0.0f : m;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float e = exp_fast(x[i] - m) * kPScale;
+                float e = exp_fast(x[i] - from) * kPScale;
                 if (masked && c0 + i >= limit) e = 0.0f;
                 l += e;
                 const _Float16 hi = (_Float16) e;
@@ -566,7 +569,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
             float f = 1.0f;
             if (whole) {
                 const int head = h * ep.G + gr - tok * ep.G;
-                f = row_factor(ep, M, L, head);
+                f = row_factor(ep, M, L, head, w.len - w.count + 1 + tok > 0);
                 d = (float *) (ep.dst + (int64_t) seq * ep.d_nb3 + (int64_t) tok * ep.d_nb2 + (int64_t) head * ep.d_nb1) + dim;
             } else {
                 d = (float *) rec + row * 128 + dim;
@@ -653,7 +656,8 @@ __device__ __forceinline__ void join_row(const PagedFattnParams & p, const int2 
     }
     if (!mine || half) return;
     const int head = h * p.G + gr - t * p.G;
-    const float f = row_factor(p, M, L, head);
+    const SeqWork w = seq_work(p, p.lens[seq], count);
+    const float f = row_factor(p, M, L, head, w.len - w.count + 1 + t > 0);
     *(float4 *) ((float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) head * p.d_nb1) + 4 * d4) =
         float4{o.x * f, o.y * f, o.z * f, o.w * f};
 }

@@ -1,0 +1,96 @@
+"""Errors and values that test_gpu_paged.py does not give the attention: counts
+below zero, in every block of 64 slots; logits of -inf."""
+import math
+
+import numpy as np
+import pytest
+
+from arclight_amd import abi
+from tests import paged_cases as P
+from tests.test_gpu_paged import MARK, _attend, _case, _check, _put
+
+pytestmark = pytest.mark.gpu
+D = 128
+
+
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("n, slot", [(1, 0), (4, 2), (4, 3), (70, 3), (70, 66), (200, 199)])
+def test_negative_counts_are_reported(gpu, n, slot, T):
+    """A slot with a negative count is recorded and has no rows; the others
+    are right. (One slot: no sequence has work at all.)"""
+    from arclight_amd import _lib, device, fattn, paged
+    _case(f"paged attention, a negative count in slot {slot} of {n}, T={T}")
+    rng = np.random.default_rng(30 + n + slot)
+    lens = [int(x) for x in rng.integers(T, 40, n)]
+    counts = [T] * n
+    counts[slot] = -3
+    pool = P.Pool(rng, lens, 2, 16)
+    q = rng.standard_normal((n, T, 8, D)).astype(np.float32)
+    out = _put(np.full(q.shape, MARK, np.float32))
+    call = paged.AttentionCall(pool.device(), _put(q), _put(np.array(lens, np.int32)), out, counts=_put(np.array(counts, np.int32)),
+                               scale=1 / math.sqrt(D))
+    call.run()
+    device.synchronize()
+    with pytest.raises(_lib.ArclightError) as e:
+        fattn.device_errors()
+    assert e.value.status == abi.AL_ERR_INVALID and "-3 new tokens" in str(e.value)
+    fattn.device_errors()                                              # reported once
+    got = out.numpy(np.float32)
+    assert np.all(got[slot] == MARK)
+    keep = [s for s in range(n) if s != slot]
+    if keep:
+        ref = P.attention(pool, q, lens, [max(c, 0) for c in counts], 1 / math.sqrt(D))
+        _check(got[keep], (ref[0][keep], ref[1][keep]), f"slot {slot} of {n}")
+
+
+@pytest.mark.parametrize("T, Hq, Hkv", [(1, 8, 2), (3, 8, 2), (1, 16, 16), (20, 4, 4)])
+@pytest.mark.parametrize("n", [1, 33, 300, 5000])
+@pytest.mark.parametrize("sinks", [None, 0.5])
+def test_logits_that_overflow(gpu, n, T, Hq, Hkv, sinks):
+    """Finite queries and keys whose products are below float32's range: those
+    cells' weights are 0 wherever they lie, whole tiles and workgroups' parts
+    among them; a row that sees nothing else is NaN, or 0 beside a sink.
+
+    All other logits are 0, their probabilities 1 and their sums exact; what is
+    left are the additions of values in chains (n 2^-23 of the mean size at the
+    most: the matrix cores may cut instead of round), the sink's e^0.5 (2^-21)
+    and a quotient and a product (2^-22)."""
+    _case(f"paged attention, logits below the range, {n} cells, T={T}, sinks={sinks}")
+    rng = np.random.default_rng(n + T)
+    n = max(n, T)
+    low = np.ones(n, bool)                                          # cells whose logits are -inf
+    low[2 * n // 3::3] = False
+    lens = [n, n, 7 + T]
+    pool = P.Pool(rng, [1], Hkv, 16)
+    per = (n + 15) // 16
+    pool.n_pages, pool.max_pages = 3 * per + 3, per + 3
+    pool.table = np.full((3, pool.max_pages), -7, np.int32)
+    order = rng.permutation(pool.n_pages)
+    for s in range(3):
+        need = (lens[s] + 15) // 16
+        pool.table[s, :need], order = order[:need], order[need:]
+    pool.k = np.zeros((pool.n_pages, 16, Hkv, D), np.float16)
+    pool.v = rng.standard_normal(pool.k.shape).astype(np.float16)
+    cells = [low, np.ones(n, bool), np.zeros(lens[2], bool)]        # some, all, none
+    for s, x in enumerate(cells):
+        for c in np.flatnonzero(x):
+            pool.k[pool.table[s, c // 16], c % 16, :, 3] = -6e4
+    q = np.zeros((3, T, Hq, D), np.float32)
+    q[..., 3] = 1e36
+    q[..., 5] = 1.0                                                # (its keys are 0)
+    with np.errstate(all="ignore"):
+        got = _attend(pool, q, lens, sinks=None if sinks is None else [sinks] * Hq, scale=1.0)
+    for s in range(3):
+        v = pool.cells(pool.v, s, lens[s])
+        for t in range(T):
+            sees = lens[s] - T + 1 + t
+            own = ~cells[s][:sees]
+            for h in range(Hq):
+                g = got[s, t, h].astype(np.float64)
+                if not own.any():
+                    assert np.all(np.isnan(g)) if sinks is None else np.all(g == 0), (s, t, h)
+                    continue
+                vv = v[:sees, h // (Hq // Hkv)][own]
+                total = len(vv) + (0.0 if sinks is None else math.exp(sinks))
+                tol = np.abs(vv).sum(0) / total * (len(vv) * 2.0 ** -23 + 2.0 ** -20)
+                assert np.all(np.abs(g - vv.sum(0) / total) <= tol), (s, t, h)
