@@ -8,7 +8,9 @@
  * server's batch do:
  *     y[t] = base[t] + s_a B_a (A_a x[t]),   a = ids[t]   (a < 0: base[t])
  * with the adapters resident in slots of one size, their ranks their own.
- * Both products are those of f32 arithmetic.
+ * Both products are those of f32 arithmetic for finite operands: a row whose x
+ * is not finite, or whose adapter's weights in use are not, may be NaN where
+ * f32 arithmetic gives an infinity.
  *
  * All data pointers are device pointers of the current device; no pointer is
  * kept after a call returns. Error convention as arclight_fattn.h. Calls

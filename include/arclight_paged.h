@@ -105,7 +105,11 @@ int al_paged_append_f32(const al_paged_append_args * args);
  * 2^22, n_seq 65535, T G / 64 Hkv 65535; T G^2 is below 2^32, n_seq max_pages
  * P / 32 below 2^31 (AL_ERR_UNSUPPORTED otherwise). dst may not overlap q.
  * Queries and probabilities are carried as pairs of f16, so that results are
- * those of f32 arithmetic (relative error about 1e-6), unlike al_fattn_f16's.
+ * those of f32 arithmetic (relative error about 1e-6), unlike al_fattn_f16's,
+ * for finite operands: a row that sees a key which is not finite, and the dim
+ * of a value which is not, may be NaN where f32 arithmetic gives an infinity
+ * or the cell no weight. (al_paged_append_f32 stores what lies beyond f16's
+ * range, 65504, as an infinity.)
  * A sequence whose length or count is recorded as an error has NaN rows, and
  * so have all rows that see a cell of a page outside the pool.
  * workspace: device scratch (al_paged_fattn_workspace_bytes), NULL: the

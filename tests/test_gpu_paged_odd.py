@@ -1,5 +1,6 @@
 """Errors and values that test_gpu_paged.py does not give the attention: counts
-below zero, in every block of 64 slots; logits of -inf."""
+below zero, in every block of 64 slots; logits of -inf; keys and values that are
+not finite, for the rows that see them."""
 import math
 
 import numpy as np
@@ -94,3 +95,54 @@ def test_logits_that_overflow(gpu, n, T, Hq, Hkv, sinks):
                 total = len(vv) + (0.0 if sinks is None else math.exp(sinks))
                 tol = np.abs(vv).sum(0) / total * (len(vv) * 2.0 ** -23 + 2.0 ** -20)
                 assert np.all(np.abs(g - vv.sum(0) / total) <= tol), (s, t, h)
+
+
+@pytest.mark.parametrize("T, Hq, Hkv", [(1, 32, 8), (3, 32, 8), (6, 64, 8), (20, 4, 4)])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_odd_values_reach_the_rows_that_see_them(gpu, value, T, Hq, Hkv):
+    """Values that are not finite, in a cell that all tokens see, one that some
+    see and the last one: not finite in their dims of the rows that see them,
+    which are right in all other dims, as the other rows are in all."""
+    _case(f"paged attention, values of {value} that rows see, T={T}")
+    rng = np.random.default_rng(31)
+    lens = [T, 60, 97, 700]
+    pool = P.Pool(rng, lens, Hkv, 16)
+    odd = {}
+    for s, n in enumerate(lens):
+        for c, d in ((n - 1, 5), (n - T // 2 - 1, 40), (max(n - T - 9, 0), 77)):
+            pool.v[pool.table[s, c // 16], c % 16, :, d::64] = value
+            odd.setdefault((s, c), []).append(d)
+    finite = pool.v.copy()
+    pool.v[~np.isfinite(pool.v)] = 0
+    q = (rng.standard_normal((4, T, Hq, D)) * 0.5).astype(np.float32)   # (no weight is lost to 0)
+    out, bound = P.attention(pool, q, lens, [T] * 4, 1 / math.sqrt(D))
+    pool.v = finite
+    got = _attend(pool, q, lens)
+    reached = np.zeros(got.shape, bool)
+    for (s, c), dims in odd.items():
+        for t in range(T):
+            if c < lens[s] - T + 1 + t:
+                for d in dims:
+                    reached[s, t, :, d::64] = True
+    assert not np.any(np.isfinite(got[reached]))
+    _check(got[~reached], (out[~reached], bound[~reached]), f"value {value}")
+
+
+@pytest.mark.parametrize("T, Hq, Hkv", [(1, 32, 8), (6, 64, 8)])
+def test_nan_keys_reach_the_rows_that_see_them(gpu, T, Hq, Hkv):
+    _case(f"paged attention, NaN keys that rows see, T={T}")
+    rng = np.random.default_rng(32)
+    lens = [60, 700]
+    pool = P.Pool(rng, lens, Hkv, 16)
+    at = [(s, n - T // 2 - 1) for s, n in enumerate(lens)]
+    q = (rng.standard_normal((2, T, Hq, D)) * 2).astype(np.float32)
+    out, bound = P.attention(pool, q, lens, [T] * 2, 1 / math.sqrt(D))
+    for s, c in at:
+        pool.k[pool.table[s, c // 16], c % 16, :, 9] = np.nan
+    got = _attend(pool, q, lens)
+    for s, c in at:
+        sees = [c < lens[s] - T + 1 + t for t in range(T)]
+        assert np.all(np.isnan(got[s][sees]))
+        other = [not x for x in sees]
+        if any(other):
+            _check(got[s][other], (out[s][other], bound[s][other]), f"sequence {s}")
