@@ -20,6 +20,7 @@
 #include "fattn_kernels.hpp"
 #include "kv_write.hpp"
 #include "runtime.hpp"
+#include "workspace_growth.hpp"
 
 namespace {
 
@@ -136,16 +137,14 @@ static int library_workspace(size_t bytes, void * stream, void ** ptr) {
     std::lock_guard<std::mutex> lk(g_mu);
     Workspace & w = st->ws[stream];
     if (w.bytes < bytes) {
-        // room for any prefill call (at most one 128-row record a CU, 17 MB)
-        // and any one-stream decode call, so that those never grow it (a
-        // growth waits for the device and fails inside a capture)
-        // A graph captured on the stream goes on using the smaller one, which
-        // is kept; a new one is at least twice its size, so that those kept
-        // are less than the one in use.
-        const size_t sz = std::max({bytes, 2 * w.bytes, (size_t) 20 << 20});
         void * next = nullptr;
-        hipError_t e = hipMalloc(&next, sz);
-        if (e != hipSuccess) return al_fail(AL_ERR_HIP, "hipMalloc(workspace %zu bytes): %s", sz, hipGetErrorString(e));
+        hipError_t e = hipSuccess;
+        const size_t sz = grow_workspace(bytes, w.bytes, [&](size_t n) {
+            e = hipMalloc(&next, n);
+            if (e != hipSuccess) (void) hipGetLastError();        // not left for the next launch to find
+            return e == hipSuccess;
+        });
+        if (sz == 0) return al_fail(AL_ERR_HIP, "hipMalloc(workspace %zu bytes): %s", bytes, hipGetErrorString(e));
         e = hipMemset(next, 0, sz);
         if (e == hipSuccess) e = hipDeviceSynchronize();       // zeroed before the stream's kernels use it
         if (e != hipSuccess) {
