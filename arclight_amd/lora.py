@@ -68,8 +68,11 @@ class ProjectCall(_Call):
 
 def apply(ad, x, ids, base, y=None, stream=None):
     """Enqueues y = base + the adapters' products; returns y (allocated when
-    None; base itself may be given)."""
+    None; base itself may be given). base None: y's own content, and then y has
+    to be given."""
     if y is None:
+        if base is None:
+            raise ValueError("without base the products are added to y, which has to be given")
         y = DeviceTensor.empty((x.shape[0], ad.N), np.float32)
     ApplyCall(ad, x, ids, base, y, stream).run()
     return y
