@@ -259,7 +259,7 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     if (base.type != AL_TYPE_F32 || base.ne[0] != N || base.ne[1] != T || base.ne[2] != 1 || base.ne[3] != 1 || base.nb[0] != 4 ||
         ((uintptr_t) base.data & 3u) || base.nb[1] % 4)
         return al_fail(AL_ERR_INVALID, "lora: base must be f32 [N, T]");
-    if (T > 0 && (base.data != y.data || base.nb[1] != y.nb[1])) {
+    if (T > 0 && (base.data != y.data || (T > 1 && base.nb[1] != y.nb[1]))) {
         const uintptr_t b0 = (uintptr_t) base.data, b1 = b0 + (uint64_t) (T - 1) * base.nb[1] + (uint64_t) N * 4;
         const uintptr_t y0 = (uintptr_t) y.data, y1 = y0 + (uint64_t) (T - 1) * y.nb[1] + (uint64_t) N * 4;
         // rows side by side, as columns of one wider matrix, are apart too
