@@ -125,6 +125,13 @@ int al_device_lds_per_block(int * bytes) {
     return AL_OK;
 }
 
+// What the workspaces go by: the stream's handle, but for hipStreamPerThread,
+// which names another stream in each thread.
+static void * stream_key(void * stream) {
+    static thread_local char own;
+    return stream == (void *) hipStreamPerThread ? &own : stream;
+}
+
 // Library-owned workspace of (current device, stream), zero-filled when
 // (re)allocated. The kernels leave the counter region zeroed after every
 // call. One workspace per stream: calls on one stream are ordered, so they
@@ -135,7 +142,7 @@ static int library_workspace(size_t bytes, void * stream, void ** ptr) {
     const int rc = device_state(&dev, &st);
     if (rc != AL_OK) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
-    Workspace & w = st->ws[stream];
+    Workspace & w = st->ws[stream_key(stream)];
     if (w.bytes < bytes) {
         void * next = nullptr;
         hipError_t e = hipSuccess;
@@ -176,7 +183,7 @@ int al_library_operands(size_t bytes, void * stream, void ** ptr) {
     if (rc != AL_OK) return rc;
     if (bytes > kOperandBytes) return al_fail(AL_ERR_WORKSPACE, "operands of %zu bytes > %zu", bytes, kOperandBytes);
     std::lock_guard<std::mutex> lk(g_mu);
-    void *& own = st->ws[stream].operands;
+    void *& own = st->ws[stream_key(stream)].operands;
     if (!own) {
         hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
         hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
@@ -199,7 +206,7 @@ extern "C" int al_fattn_release_stream(void * stream) {
     const int rc = device_state(&dev, &st);
     if (rc != AL_OK) return rc;
     std::lock_guard<std::mutex> lk(g_mu);
-    auto it = st->ws.find(stream);
+    auto it = st->ws.find(stream_key(stream));
     if (it == st->ws.end()) return AL_OK;
     Workspace & w = it->second;
     if (w.ptr || w.operands) {

@@ -92,8 +92,9 @@ typedef struct al_tensor {
  * when the node carries them: al_fattn_apply_node_hints below.)
  *
  * workspace: device scratch for split-KV partials. NULL lets the library use
- * its own buffer for the current device and args->stream (allocated on first
- * use; a larger one when needed, beside which those before it are kept for the
+ * its own buffer for the current device and args->stream (that of the calling
+ * thread for hipStreamPerThread; allocated on first use; a larger one when
+ * needed, beside which those before it are kept for the
  * graphs that use them; freed by al_fattn_release_stream; a graph
  * captured on a stream uses that stream's, so the stream needs one eager call
  * of the same shapes before the capture: allocating inside a capture fails;
@@ -184,7 +185,8 @@ int al_fattn_apply_node_hints(al_fattn_args * args, const int32_t * op_params);
  * graph replayed on the stream may still use it). No counterpart in the
  * reference (its op uses per-thread scratch of the graph's work buffer,
  * nnml/src/ops/arm/arm.cpp:2299-2302). A later call allocates again. AL_OK
- * when the stream has none.
+ * when the stream has none. A thread that ends gives its hipStreamPerThread's
+ * back before.
  */
 int al_fattn_release_stream(void * stream);
 
