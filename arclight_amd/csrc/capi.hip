@@ -166,11 +166,19 @@ static int library_workspace(size_t bytes, void * stream, void ** ptr) {
     return AL_OK;
 }
 
-int al_library_workspace(size_t bytes, void * stream, void ** ptr) {
-    void * base = nullptr;
-    const int rc = library_workspace(kFattnCounterBytes + bytes, stream, &base);
-    if (rc == AL_OK) *ptr = (char *) base + kFattnCounterBytes;
-    return rc;
+size_t al_workspace_bytes(size_t records) { return kFattnCounterBytes + records; }
+
+int al_workspace_records(const char * what, size_t bytes, void * workspace, uint64_t workspace_bytes, void * stream, void ** ptr) {
+    const size_t need = al_workspace_bytes(bytes);
+    if (!workspace) {
+        const int rc = library_workspace(need, stream, &workspace);
+        if (rc != AL_OK) return rc;
+    } else if (workspace_bytes < need || ((uintptr_t) workspace & 15u)) {
+        return al_fail(AL_ERR_WORKSPACE, "%s: workspace %llu bytes (16-byte aligned) < %zu needed", what,
+                       (unsigned long long) workspace_bytes, need);
+    }
+    *ptr = (char *) workspace + kFattnCounterBytes;
+    return AL_OK;
 }
 
 // One for each stream, as above. Of one size, so that none grows, and without

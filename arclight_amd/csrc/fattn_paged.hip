@@ -814,7 +814,7 @@ extern "C" uint64_t al_paged_fattn_workspace_bytes(const al_paged_fattn_args * a
     int n_cu = 0;
     Plan pl;
     if (al_device_cu_count(&n_cu) != AL_OK || make_plan(a, n_cu, &pl) != AL_OK) return 0;
-    return pl.empty ? 0 : pl.bytes;
+    return pl.empty ? 0 : al_workspace_bytes(pl.bytes);
 }
 
 extern "C" int al_paged_fattn_f16(const al_paged_fattn_args * a) {
@@ -827,15 +827,8 @@ extern "C" int al_paged_fattn_f16(const al_paged_fattn_args * a) {
     if (rc == AL_OK) rc = make_plan(a, n_cu, &pl);
     if (rc == AL_OK) rc = al_device_error_flag(&pl.p.c.err);
     if (rc != AL_OK) return rc;
-    if (a->workspace) {
-        if (a->workspace_bytes < pl.bytes || ((uintptr_t) a->workspace & 15u))
-            return al_fail(AL_ERR_WORKSPACE, "paged_fattn: workspace %llu bytes (16-byte aligned) < %zu needed",
-                           (unsigned long long) a->workspace_bytes, pl.bytes);
-        pl.p.info = (int2 *) a->workspace;
-    } else {
-        rc = al_library_workspace(pl.bytes, a->stream, (void **) &pl.p.info);
-        if (rc != AL_OK) return rc;
-    }
+    rc = al_workspace_records("paged_fattn", pl.bytes, a->workspace, a->workspace_bytes, a->stream, (void **) &pl.p.info);
+    if (rc != AL_OK) return rc;
     pl.p.part = (float *) ((char *) pl.p.info + pl.info_bytes);
     const hipError_t e = launch(pl.p, (hipStream_t) a->stream);
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "paged_fattn: launch");

@@ -344,16 +344,9 @@ int run(const al_lora_args * g, bool project) {
     if (rc == AL_OK) rc = make_plan(g, project, n_cu, &pl);
     if (rc == AL_OK) rc = al_device_error_flag(&pl.p.err);
     if (rc != AL_OK) return rc;
-    const size_t need = pl.v_bytes + pl.g_bytes + pl.q_bytes;
-    void * ws = g->workspace;
-    if (ws) {
-        if (g->workspace_bytes < need || ((uintptr_t) ws & 15u))
-            return al_fail(AL_ERR_WORKSPACE, "lora: workspace %llu bytes (16-byte aligned) < %zu needed",
-                           (unsigned long long) g->workspace_bytes, need);
-    } else {
-        rc = al_library_workspace(need, g->stream, &ws);
-        if (rc != AL_OK) return rc;
-    }
+    void * ws = nullptr;
+    rc = al_workspace_records("lora", pl.v_bytes + pl.g_bytes + pl.q_bytes, g->workspace, g->workspace_bytes, g->stream, &ws);
+    if (rc != AL_OK) return rc;
     pl.p.v = (float *) ws;
     pl.p.groups = (int32_t *) ((char *) ws + pl.v_bytes);
     const hipStream_t st = (hipStream_t) g->stream;
@@ -381,5 +374,5 @@ extern "C" uint64_t al_lora_workspace_bytes(const al_lora_args * args) {
     int n_cu = 0;
     Plan pl;
     if (al_device_cu_count(&n_cu) != AL_OK || make_plan(args, args && args->w.data != nullptr, n_cu, &pl) != AL_OK) return 0;
-    return pl.empty ? 0 : pl.v_bytes + pl.g_bytes + pl.q_bytes;
+    return pl.empty ? 0 : al_workspace_bytes(pl.v_bytes + pl.g_bytes + pl.q_bytes);
 }

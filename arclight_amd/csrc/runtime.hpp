@@ -13,10 +13,13 @@ int al_device_cu_count(int * n_cu);
 int al_device_lds_per_block(int * bytes);
 int al_device_error_flag(int ** flag);   // its words: device_errors.hpp
 
-// Records of a call with no workspace of its own: `bytes` of the library's
-// workspace of (current device, stream), behind its counters. No initial
-// value; calls on one stream share it.
-int al_library_workspace(size_t bytes, void * stream, void ** ptr);
+// Where a call's `bytes` of records lie: in the caller's workspace, or (NULL) in
+// the library's of (current device, stream). No initial value; calls on one
+// stream share it. They lie behind the counters that every workspace begins
+// with, which al_fattn_f16 carries from call to call, so that any calls may
+// share one. what: the caller's name.
+size_t al_workspace_bytes(size_t records);      // of a workspace with so many of records
+int al_workspace_records(const char * what, size_t bytes, void * workspace, uint64_t workspace_bytes, void * stream, void ** ptr);
 
 // The quantized activations of the Q4_0 projection: memory of (current device,
 // stream) apart from its workspace, kOperandBytes whatever `bytes` (64 tokens

@@ -53,7 +53,8 @@ extern "C" {
  * workspace: device scratch (al_lora_workspace_bytes), NULL: the library's
  * own for (current device, stream), as al_fattn_f16: then one eager call of
  * the same shapes has to come before a capture. Calls and replays that share
- * a workspace must be ordered on one stream. It needs no initial value.
+ * a workspace must be ordered on one stream. It needs no initial value; its
+ * first 256 KiB are not touched, so that it may also be al_fattn_f16's.
  */
 typedef struct al_lora_args {
     al_tensor a;

@@ -116,7 +116,8 @@ int al_paged_append_f32(const al_paged_append_args * args);
  * library's own for (current device, stream), as al_fattn_f16: then one
  * eager call of the same shapes has to come before a capture. Calls and
  * replays that share a workspace must be ordered on one stream. A workspace
- * needs no initial value.
+ * needs no initial value; its first 256 KiB are not touched, so that it may
+ * also be al_fattn_f16's, whose counters those are.
  */
 typedef struct al_paged_fattn_args {
     al_tensor q;
