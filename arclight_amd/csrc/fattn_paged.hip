@@ -45,8 +45,10 @@
 //
 // What bounds it: the cells' bytes, and for small calls the chain lengths ->
 // page numbers -> keys -> scores -> values, then the join. Measured, 8 KV heads
-// of 4 query heads each: one sequence of 700 cells 9.5 us, 24 of 1400 to 4000
-// 50.8 us, 100000 cells (64 query heads) 79 us, 5.2 TB/s.
+// of 4 query heads each: one sequence of 700 cells 9.4 us, 24 of 1400 to 4000
+// 51.1 us, 100000 cells (64 query heads) 79 us, 5.2 TB/s. Prompts are bound
+// elsewhere: every wave reads its 16 KB of a tile through the L1 and turns V
+// itself (4 prompts of 2048 tokens, 32 heads over 8: 749 us, 184 TFLOP/s).
 
 #include <hip/hip_runtime.h>
 

@@ -16,8 +16,8 @@
 // Two launches: the first product into the workspace, K split over workgroups
 // where there are few rows, then the second, which sums the parts, for a slice
 // of the outputs. (Beside the Q4_0 projection: parts of its launches.) 300 rows
-// of 2048 -> 8192 in the order of their requests, ranks to 64: 13.6 us;
-// shuffled over 12 adapters 17.4, as a group of rows then is of 5 on average.
+// of 2560 -> 4096 in the order of their requests, ranks to 64: 13.4 us; shuffled
+// over 12 adapters 21.2, as a group of rows then is of 5 on average.
 
 #include <hip/hip_runtime.h>
 
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(64 * shrink_waves<RT>(), RT == 8 ? 2 : 4) void lora
 // another: 70 us instead of 55, then, for 8000 rows of 4096 outputs; several slices to
 // a workgroup gained nothing). VEC: rows of y and base in whole 16 bytes;
 // SPLIT: v in parts.
-// Measured there, rank 16: 51.7 us, 5.1 TB/s, what a copy reaches.
+// Measured there, rank 16: 51.7 us, 5.1 TB/s (a plain copy: 5.5 at the best).
 template <int RT, bool VEC, bool SPLIT>
 __device__ __forceinline__ void expand_group(const LoraParams & p, const Rows & rows, float (*v)[RT * 16 + 4]) {
     constexpr int kPiece = RT == 1 ? 16 : 32;                          // ranks of a lane's load of B: 4 or 8 in each quarter
@@ -286,8 +286,9 @@ int make_plan(const al_lora_args * g, bool project, int n_cu, Plan * out) {
     // adapter's first, 17th ... row work. Of more, groups are picked out of 64
     // rows at a time or of 256, which costs more for a small batch in the order
     // of its requests and saves half the groups of a shuffled one (us, ordered
-    // and shuffled over 12 adapters: 300 rows 13.5, 17.4 with 64, 15.6, 16.1
-    // with 256; 500 18.0, 21.7 and 16.6, 17.8; 2000 35.2, 61.4 and 35.4, 43.2).
+    // and shuffled over 12 adapters of ranks 8 to 64, 2560 -> 4096: 300 rows
+    // 13.5, 21.2 with 64, 18.9, 20.6 with 256; 500 16.8, 26.4 and 17.1, 22.2;
+    // 2000 37, 68 and 38, 47).
     // They have at least 4 or 16 groups, which p.slots workgroups share, an odd
     // number, as workgroups go to the 8 XCDs in turn and the last slots have
     // little to do (8000 rows with 4, 5, 8 for 64 rows: 93, 86, 97). Many

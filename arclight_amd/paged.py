@@ -10,7 +10,8 @@ row for each token, q (T, Hq, 128) and k, v (T, Hkv, 128) f32, with its
 position and its sequence (negative: a padding row); attention takes q
 (n_seq, T, Hq, 128) f32, the last T tokens (or counts[s] of them) of each
 sequence's lens[s] cells. A decode step's rows are the same in both, one
-token for each sequence.
+token for each sequence. norm=False rotates the rows as they are, without q_w
+and k_w.
 
 AppendCall and AttentionCall hold a call's argument structure, as a C host
 does, to run it any number of times over the same buffers.

@@ -104,6 +104,11 @@ int al_paged_append_f32(const al_paged_append_args * args);
  * Hq is a multiple of Hkv, G = Hq / Hkv. T is at most 2^16, Hq 4096, T Hq
  * 2^22, n_seq 65535, T G / 64 Hkv 65535; T G^2 is below 2^32, n_seq max_pages
  * P / 32 below 2^31 (AL_ERR_UNSUPPORTED otherwise). dst may not overlap q.
+ * T decides how the launch shares out the card, for every sequence: single
+ * tokens beside a prompt are right, but slow. They belong in two calls over the
+ * same buffers, one with T = 1 (views with ne = 1 there), each with a count of 0
+ * for the other's sequences. 63 sequences of 4000 cells with one token and a
+ * prompt of 2048, 32 heads over 8: 6.7 ms in one call, 0.2 + 0.2 ms in two.
  * Queries and probabilities are carried as pairs of f16, so that results are
  * those of f32 arithmetic (relative error about 1e-6), unlike al_fattn_f16's,
  * for finite operands: a row that sees a key which is not finite, and the dim

@@ -146,3 +146,27 @@ def test_nan_keys_reach_the_rows_that_see_them(gpu, T, Hq, Hkv):
         other = [not x for x in sees]
         if any(other):
             _check(got[s][other], (out[s][other], bound[s][other]), f"sequence {s}")
+
+
+def test_prompts_and_single_tokens_in_two_calls(gpu):
+    """A step of prompts and single tokens over one pair of padded buffers: a
+    call with T = 1 views and one of all T, each with counts of 0 for the
+    other's sequences, write each its own rows, and what one call of all gives
+    to the same bound."""
+    from arclight_amd import device, fattn, paged
+    _case("paged attention, prompts and single tokens in two calls")
+    rng = np.random.default_rng(33)
+    lens, counts, T, Hq, Hkv = [400, 50, 90, 1, 700, 64], [1, 50, 1, 1, 1, 30], 50, 8, 2
+    pool = P.Pool(rng, lens, Hkv, 16)
+    q = (rng.standard_normal((6, T, Hq, D)) * 2).astype(np.float32)
+    ref = P.attention(pool, q, lens, counts, 1 / math.sqrt(D))
+    cache, dq, out, dl = pool.device(), _put(q), _put(np.full(q.shape, MARK, np.float32)), _put(np.array(lens, np.int32))
+    view = lambda t: device.DeviceTensor(t.buf, abi.AL_TYPE_F32, (6, 1, Hq, D), (T * Hq * D * 4, Hq * D * 4, D * 4, 4))  # noqa: E731
+    one = [int(c == 1) for c in counts]
+    more = [0 if c == 1 else c for c in counts]
+    paged.attention(cache, view(dq), dl, view(out), counts=_put(np.array(one, np.int32)), scale=1 / math.sqrt(D))
+    paged.attention(cache, dq, dl, out, counts=_put(np.array(more, np.int32)), scale=1 / math.sqrt(D))
+    device.synchronize()
+    fattn.device_errors()
+    _check(out.numpy(np.float32), ref, "two calls")
+    _check(_attend(pool, q, lens, counts), ref, "one call")
