@@ -72,7 +72,8 @@ std::vector<DeviceState> g_dev;
 
 }  // namespace
 
-// Kernel-recorded error flags (al_device_errors), one copy per GPU.
+// Kernel-recorded error flags (al_device_errors), one copy per GPU, zero when it
+// is loaded: nothing is enqueued on first use, which may be inside a capture.
 static __device__ __align__(256) int g_err_flags[64];
 
 static int device_state(int * dev_out, DeviceState ** st_out) {
@@ -89,8 +90,6 @@ static int device_state(int * dev_out, DeviceState ** st_out) {
         if (e != hipSuccess) return al_hip_fail(e, "hipDeviceGetAttribute");
         e = hipGetSymbolAddress((void **) &st.err, HIP_SYMBOL(g_err_flags));
         if (e != hipSuccess) return al_hip_fail(e, "hipGetSymbolAddress(error flags)");
-        e = hipMemset(st.err, 0, sizeof(g_err_flags));
-        if (e != hipSuccess) return al_hip_fail(e, "hipMemset(error flags)");
         st.init = true;
     }
     *dev_out = dev;
