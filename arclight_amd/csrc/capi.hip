@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <deque>
 #include <map>
 #include <mutex>
 #include <string>
@@ -68,7 +69,7 @@ struct DeviceState {
 };
 
 std::mutex g_mu;
-std::vector<DeviceState> g_dev;
+std::deque<DeviceState> g_dev;       // (whose elements stay where they are when it grows)
 
 }  // namespace
 
