@@ -84,6 +84,15 @@ SIGNATURES = {
     "al_paged_append_f32": (_I, [ctypes.POINTER(abi.AlPagedAppendArgs)]),
     "al_paged_fattn_f16": (_I, [ctypes.POINTER(abi.AlPagedFattnArgs)]),
     "al_paged_fattn_workspace_bytes": (_U64, [ctypes.POINTER(abi.AlPagedFattnArgs)]),
+    "al_paged_fattn_sees_f16": (_I, [ctypes.POINTER(abi.AlPagedFattnArgs), ctypes.POINTER(abi.AlPagedSees)]),
+    "al_paged_fattn_sees_workspace_bytes": (_U64, [ctypes.POINTER(abi.AlPagedFattnArgs), ctypes.POINTER(abi.AlPagedSees)]),
+    "al_paged_append_cells_f32": (_I, [ctypes.POINTER(abi.AlPagedAppendArgs), ctypes.POINTER(abi.AlTensor)]),
+    "al_paged_keep_f16": (_I, [ctypes.POINTER(abi.AlPagedKeepArgs)]),
+    "al_paged_copy_f16": (_I, [ctypes.POINTER(abi.AlPagedCopyArgs)]),
+    # include/arclight_draft.h
+    "al_draft_tree_i32": (_I, [ctypes.POINTER(abi.AlDraftTreeArgs)]),
+    "al_draft_verify_f32": (_I, [ctypes.POINTER(abi.AlDraftVerifyArgs)]),
+    "al_draft_verify_workspace_bytes": (_U64, [ctypes.POINTER(abi.AlDraftVerifyArgs)]),
     # include/arclight_lora.h
     "al_lora_f32": (_I, [ctypes.POINTER(abi.AlLoraArgs)]),
     "al_mul_mat_q4_0_lora_f32": (_I, [ctypes.POINTER(abi.AlLoraArgs)]),

@@ -190,6 +190,66 @@ class AlPagedFattnArgs(ctypes.Structure):
     ]
 
 
+class AlPagedSees(ctypes.Structure):
+    """al_paged_sees."""
+    _fields_ = [
+        ("window", ctypes.c_int32),
+        ("first", ctypes.c_int32),
+        ("bits", AlTensor),
+        ("pos", AlTensor),
+    ]
+
+
+class AlPagedLayers(ctypes.Structure):
+    """al_paged_layers."""
+    _fields_ = [
+        ("k_pool", AlTensor), ("v_pool", AlTensor),
+        ("k", ctypes.POINTER(ctypes.c_void_p)),
+        ("v", ctypes.POINTER(ctypes.c_void_p)),
+        ("n_layers", ctypes.c_int32),
+    ]
+
+
+class AlPagedKeepArgs(ctypes.Structure):
+    """al_paged_keep_args."""
+    _fields_ = [
+        ("layers", AlPagedLayers),
+        ("table", AlTensor), ("lens", AlTensor), ("counts", AlTensor), ("path", AlTensor), ("kept", AlTensor),
+        ("lens_out", AlTensor),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class AlPagedCopyArgs(ctypes.Structure):
+    """al_paged_copy_args."""
+    _fields_ = [
+        ("layers", AlPagedLayers),
+        ("src", AlTensor), ("dst", AlTensor), ("cells", AlTensor),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+# include/arclight_draft.h
+class AlDraftTreeArgs(ctypes.Structure):
+    """al_draft_tree_args."""
+    _fields_ = [
+        ("parents", AlTensor), ("lens", AlTensor), ("counts", AlTensor),
+        ("pos", AlTensor), ("cells", AlTensor), ("seq", AlTensor), ("bits", AlTensor),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class AlDraftVerifyArgs(ctypes.Structure):
+    """al_draft_verify_args."""
+    _fields_ = [
+        ("target", AlTensor), ("draft", AlTensor), ("tokens", AlTensor), ("parents", AlTensor), ("counts", AlTensor),
+        ("accept", AlTensor), ("sample", AlTensor), ("path", AlTensor), ("kept", AlTensor), ("next", AlTensor),
+        ("stream", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 # include/arclight_lora.h
 class AlLoraArgs(ctypes.Structure):
     """al_lora_args."""

@@ -12,10 +12,15 @@ enum DeviceErrorWord {
     kErrMerge = 2,
     kErrPaged = 4,                              // [5]: a PagedError, [6]: its value
     kErrLora = 8,                               // [9]: the adapter
-    kErrWords = 12
+    kErrDraft = 12,                             // [13]: a DraftError, [14]: its value
+    kErrWords = 16
 };
 
-enum PagedError { kPagedBadPage = 1, kPagedBadLength = 2, kPagedBadCount = 3, kPagedBadSeq = 4, kPagedBadPos = 5 };
+enum PagedError {
+    kPagedBadPage = 1, kPagedBadLength = 2, kPagedBadCount = 3, kPagedBadSeq = 4, kPagedBadPos = 5, kPagedBadCell = 6, kPagedBadPath = 7,
+    kPagedBadKept = 8, kPagedBadCopy = 9, kPagedBadCells = 10
+};
+enum DraftError { kDraftBadParent = 1, kDraftBadCount = 2, kDraftBadToken = 3, kDraftBadRow = 4 };
 
 inline std::string paged_error_text(const int what, const int value) {
     const std::string v = std::to_string(value);
@@ -24,14 +29,29 @@ inline std::string paged_error_text(const int what, const int value) {
         case kPagedBadLength: return "a length of " + v + " cells is not within the table";
         case kPagedBadCount:  return "a sequence with " + v + " new tokens";
         case kPagedBadSeq:    return "a token of sequence " + v + ", which the table does not have";
+        case kPagedBadCell:   return "a token of cell " + v + ", which is not within the table";
+        case kPagedBadPath:   return "new token " + v + " is not one that can be kept in its place of the path";
+        case kPagedBadKept:   return "a path of " + v + " tokens, more or fewer than there can be";
+        case kPagedBadCopy:   return "page " + v + " of a copy is not in the pool";
+        case kPagedBadCells:  return "a copy of " + v + " cells of a page";
         default:              return "a token at position " + v + ", which is not within the table";
+    }
+}
+
+inline std::string draft_error_text(const int what, const int value) {
+    const std::string v = std::to_string(value);
+    switch (what) {
+        case kDraftBadParent: return "a node whose parent is " + v + ", which does not come before it";
+        case kDraftBadCount:  return "a tree of " + v + " nodes, more or fewer than there can be";
+        case kDraftBadToken:  return "a node of token " + v + ", which the vocabulary does not have";
+        default:              return "sequence " + v + " has no probabilities to draw from";
     }
 }
 
 // The status for the recorded words, and in `text` every kind of error among
 // them, as all are cleared together. A merge that gave up is the library's own
-// failure and keeps its status beside errors of the paged cache or the
-// adapters, which are the caller's.
+// failure and keeps its status beside errors of the paged cache, the adapters
+// or drafts, which are the caller's.
 inline int device_error_status(const int (&w)[kErrWords], std::string & text) {
     text.clear();
     auto add = [&](const std::string & s) { text += (text.empty() ? "" : "; ") + s; };
@@ -39,6 +59,7 @@ inline int device_error_status(const int (&w)[kErrWords], std::string & text) {
     if (w[kErrMerge]) add("fattn: a merging workgroup gave up waiting for the other splits' records");
     if (w[kErrPaged]) add("paged cache: " + paged_error_text(w[kErrPaged + 1], w[kErrPaged + 2]));
     if (w[kErrLora]) add("lora: a row of adapter " + std::to_string(w[kErrLora + 1]) + ", which is not there or whose rank does not fit");
+    if (w[kErrDraft]) add("draft: " + draft_error_text(w[kErrDraft + 1], w[kErrDraft + 2]));
     if (text.empty()) return AL_OK;
     return w[kErrMerge] && !w[kErrSetRows] ? AL_ERR_HIP : AL_ERR_INVALID;
 }

@@ -1,0 +1,586 @@
+// Trees of drafted tokens (include/arclight_draft.h), for gfx950: positions,
+// cells and the bits of what each node sees from the parents, and verification
+// against the target's probabilities.
+//
+// Tree. A wave takes 64 nodes of a tree, a lane each, which goes up its parents
+// in LDS: the steps are its depth, and as a parent's number is smaller the words
+// of its bits come one after another from the last to the first.
+//
+// Verification. Accept and reject take a few numbers of each node (its
+// parent's p and q at its token), gathered by a workgroup into LDS; the walk down
+// the tree is then ballots over the nodes. The token that follows is drawn from
+// one row of V: the row's weights are summed in 64 bits by workgroups of kChunk
+// each, and a last workgroup for each sequence finds the chunk in which the sum
+// passes sample times the whole, and the token in it. Every sum is taken in one
+// fixed order, so that equal inputs give equal tokens.
+//
+// Where several children of a node were drawn from a draft's row, what is left
+// after each rejection has to be normalised before the next child is tried: a
+// sum over the row within the walk, which a workgroup for each sequence then
+// does in a launch of its own.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "../../include/arclight_draft.h"
+#include "device_errors.hpp"
+#include "kernel_args.hpp"
+#include "runtime.hpp"
+
+namespace {
+
+constexpr int kMaxNodes = 1024;
+constexpr int kThreads = 256;
+constexpr int kEach = 8;                        // a thread's tokens of a chunk
+constexpr int kChunk = kThreads * kEach;
+
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ void draft_error(int * err, const int what, const int value) {
+    if (atomicCAS(err + kErrDraft, 0, 1) == 0) {
+        err[kErrDraft + 1] = what;
+        err[kErrDraft + 2] = value;
+    }
+}
+
+struct TreeParams {
+    const int32_t * parents;  int64_t par_nb1;  // sequence, in entries
+    const int32_t * lens;
+    const int32_t * counts;                     // or null
+    int32_t * pos;    int64_t pos_nb1;          // each or null
+    int32_t * cells;  int64_t cells_nb1;
+    int32_t * seq;    int64_t seq_nb1;
+    int32_t * bits;   int64_t b_nb1, b_nb2;
+    int32_t T, words;
+    int * err;
+};
+
+// Grid: 64 nodes, sequences.
+__global__ __launch_bounds__(64) void draft_tree_kernel(const TreeParams p) {
+    __shared__ int32_t par[kMaxNodes];
+    prefetch_params(p);
+    const int s = blockIdx.y, lane = threadIdx.x, t = blockIdx.x * 64 + lane;
+    const int len = p.lens[s], raw = p.counts ? p.counts[s] : p.T;
+    const bool ok = raw >= 0 && raw <= p.T && raw <= len;
+    const int count = ok ? raw : 0;
+    if (!ok && t == 0) draft_error(p.err, kDraftBadCount, raw);
+    const int last = min((int) blockIdx.x * 64 + 63, count - 1);         // no lane comes past it
+    for (int u = lane; u <= last; u += 64) {
+        int x = p.parents[(int64_t) s * p.par_nb1 + u];
+        if (x >= u) {
+            if (u == t) draft_error(p.err, kDraftBadParent, x);
+            x = -1;
+        }
+        par[u] = x;
+    }
+    __syncthreads();
+    if (t >= p.T) return;
+    int depth = -1;
+    int32_t * words = p.bits + (int64_t) s * p.b_nb2 + (int64_t) t * p.b_nb1;
+    int w = p.words - 1;
+    uint32_t word = 0;
+    if (t < count)
+        for (int u = t; u >= 0; u = par[u], ++depth) {
+            if (p.bits)
+                for (; w > u >> 5; --w, word = 0) words[w] = (int32_t) word;
+            word |= 1u << (u & 31);
+        }
+    if (p.bits)
+        for (; w >= 0; --w, word = 0) words[w] = (int32_t) word;
+    if (p.pos) p.pos[(int64_t) s * p.pos_nb1 + t] = t < count ? len - count + depth : 0;
+    if (p.cells) p.cells[(int64_t) s * p.cells_nb1 + t] = t < count ? len - count + t : 0;
+    if (p.seq) p.seq[(int64_t) s * p.seq_nb1 + t] = t < count ? s : -1;
+}
+
+struct VerifyParams {
+    const char * target;  int64_t t_nb1, t_nb2; // node, sequence, in bytes
+    const char * draft;   int64_t d_nb1, d_nb2; // or null
+    const int32_t * tokens;   int64_t tok_nb1;  // sequence, in entries
+    const int32_t * parents;  int64_t par_nb1;  // or null
+    const int32_t * counts;                     // or null
+    const float * accept;     int64_t acc_nb1;
+    const float * sample;
+    int32_t * path;           int64_t path_nb1;
+    int32_t * kept;
+    int32_t * next;
+    int2 * state;                               // [sequence]: the last accepted node (-1: none), its rejected children
+    double * norms;                             // [sequence][T]: with siblings of a draft, the sums after each rejection
+    double2 * sums;                             // [sequence][chunk]: of what is left, of the row itself
+    int32_t T, V, chunks, walked;               // walked: state and norms are there
+    int * err;
+};
+
+__device__ __forceinline__ float weight(const float x) { return x > 0.0f ? x : 0.0f; }
+
+// What m rejections of children drawn from q leave of p, before it is
+// normalised: norms[i] is the sum after rejection i + 1.
+__device__ __forceinline__ double left_of(const double p, const double q, const int m, const double * norms) {
+    double f = p;
+    for (int i = 0; i < m; ++i) f = fmax((i ? f / norms[i - 1] : f) - q, 0.0);
+    return f;
+}
+
+// Sums of the workgroup's lanes, in a fixed order; every thread gets them.
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
+    return x;
+}
+__device__ __forceinline__ double block_sum(double x, double * lds) {
+    x = wave_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = lds[0];
+#pragma unroll
+    for (int i = 1; i < kThreads / 64; ++i) x += lds[i];
+    return x;
+}
+
+struct WalkLds {
+    int32_t par[kMaxNodes];                     // -1: nobody's child
+    int32_t tok[kMaxNodes];
+    float p[kMaxNodes], q[kMaxNodes], r[kMaxNodes];
+    int32_t path[kMaxNodes];
+    double red[kThreads / 64];
+};
+
+struct Walked {
+    int v, m;                                   // as VerifyParams::state
+    int kept;
+};
+
+__device__ __forceinline__ int nodes_of(const VerifyParams & p, const int s, const bool report) {
+    const int raw = p.counts ? p.counts[s] : p.T;
+    const bool ok = raw >= 0 && raw <= p.T;
+    if (!ok && report) draft_error(p.err, kDraftBadCount, raw);
+    return ok ? raw : 0;
+}
+
+// The parent of node u, -1 where it is nobody's child.
+__device__ __forceinline__ int parent_of(const VerifyParams & p, const int s, const int u, const int token, const bool report) {
+    const int par = p.parents ? p.parents[(int64_t) s * p.par_nb1 + u] : u - 1;
+    if (par >= u) {
+        if (report) draft_error(p.err, kDraftBadParent, par);
+        return -1;
+    }
+    if (par >= 0 && (uint32_t) token >= (uint32_t) p.V) {
+        if (report) draft_error(p.err, kDraftBadToken, token);
+        return -1;
+    }
+    return par;
+}
+
+// The walk down the tree, by every wave of a workgroup alike. NORMS: with a
+// draft whose nodes can have several children; norms: of this sequence.
+template <bool NORMS>
+__device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, const int count, const bool report, WalkLds & x, double * norms) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const char * target = p.target + (int64_t) s * p.t_nb2;
+    const char * draft = p.draft ? p.draft + (int64_t) s * p.d_nb2 : nullptr;
+    for (int u = tid; u < count; u += kThreads) {
+        const int tok = u ? p.tokens[(int64_t) s * p.tok_nb1 + u] : 0;
+        const int par = parent_of(p, s, u, tok, report);
+        const float r = p.accept[(int64_t) s * p.acc_nb1 + u];
+        x.par[u] = par;
+        x.tok[u] = tok;
+        x.r[u] = r;
+        x.p[u] = par >= 0 ? weight(*(const float *) (target + (int64_t) par * p.t_nb1 + (int64_t) tok * 4)) : 0.0f;
+        x.q[u] = par >= 0 && draft ? weight(*(const float *) (draft + (int64_t) par * p.d_nb1 + (int64_t) tok * 4)) : 1.0f;
+    }
+    __syncthreads();
+    Walked at = {count > 0 ? 0 : -1, 0, count > 0};
+    if (tid == 0) x.path[0] = 0;
+    while (at.v >= 0) {
+        // the children of v in their order
+        double mass = 1.0;
+        bool nothing = false;
+        int m = 0, found = -1, first = -1;
+        for (int base = (at.v + 1) & ~63; base < count && found < 0; base += 64) {
+            const int u = base + lane;
+            uint64_t todo = __ballot(u > at.v && u < count && x.par[min(u, count - 1)] == at.v);
+            for (; todo && found < 0; todo &= todo - 1) {
+                const int c = base + __builtin_ctzll(todo), tok = x.tok[c];
+                if (first < 0) first = c;
+                bool pass;
+                if (!p.draft) {
+                    // a token that was rejected already has nothing left
+                    bool twice = false;
+                    for (int b = first & ~63; m > 0 && b < c; b += 64) {
+                        const int e = b + lane;
+                        twice |= __any(e >= first && e < c && x.par[min(e, count - 1)] == at.v && x.tok[min(e, count - 1)] == tok);
+                    }
+                    const double pc = x.p[c];
+                    pass = !twice && pc > 0.0 && (double) x.r[c] * mass < pc;
+                    if (!pass && !twice) mass -= pc;
+                } else {
+                    double pc = x.p[c];
+                    const double qc = x.q[c];
+                    if (NORMS && m > 0) {
+                        // the sum of what the last rejection left
+                        if (!nothing) {
+                            const char * pr = target + (int64_t) at.v * p.t_nb1;
+                            const char * qr = draft + (int64_t) at.v * p.d_nb1;
+                            double sum = 0.0;
+                            for (int y = tid; y < p.V; y += kThreads)
+                                sum += left_of(weight(*(const float *) (pr + (int64_t) y * 4)), weight(*(const float *) (qr + (int64_t) y * 4)), m, norms);
+                            sum = block_sum(sum, x.red);
+                            nothing = !(sum > 0.0 && sum < __builtin_inf());
+                            if (tid == 0) norms[m - 1] = sum;
+                            __syncthreads();
+                        }
+                        pc = nothing ? 0.0 : left_of(pc, qc, m, norms) / norms[m - 1];
+                    }
+                    pass = pc > 0.0 && (double) x.r[c] * qc < pc;
+                }
+                if (pass) found = c;
+                else ++m;
+            }
+        }
+        if (found < 0) {
+            at.m = nothing ? 0 : m;
+            break;
+        }
+        at.v = found;
+        if (tid == 0) x.path[at.kept] = found;
+        ++at.kept;
+    }
+    __syncthreads();
+    return at;
+}
+
+__device__ __forceinline__ void write_path(const VerifyParams & p, const int s, const Walked & at, const WalkLds & x) {
+    for (int i = threadIdx.x; i < p.T; i += kThreads) p.path[(int64_t) s * p.path_nb1 + i] = i < at.kept ? x.path[i] : -1;
+    if (threadIdx.x == 0) {
+        p.kept[s] = at.kept;
+        p.state[s] = int2{at.v, at.m};
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyParams p) {
+    __shared__ WalkLds x;
+    const int s = blockIdx.x;
+    const int count = nodes_of(p, s, threadIdx.x == 0);
+    const Walked at = walk<true>(p, s, count, true, x, p.norms + (int64_t) s * p.T);
+    write_path(p, s, at, x);
+}
+
+// What is left of the last accepted node's row, kEach tokens from `first` on.
+// gone: the tokens of the chunk that were rejected, a bit each.
+__device__ __forceinline__ void row_weights(const VerifyParams & p, const int s, const Walked & at, const double * norms, const int first,
+                                            const uint32_t * gone, double (&left)[kEach], double (&own)[kEach]) {
+    const char * pr = p.target + (int64_t) s * p.t_nb2 + (int64_t) at.v * p.t_nb1 + (int64_t) first * 4;
+    const char * qr = p.draft + (int64_t) s * p.d_nb2 + (int64_t) at.v * p.d_nb1 + (int64_t) first * 4;
+    const bool drafted = p.draft && at.m > 0;
+    float a[kEach], b[kEach];
+    if (first + kEach <= p.V) {
+#pragma unroll
+        for (int j = 0; j < kEach; j += 4) {
+            const float4u x = *(const float4u *) (pr + 4 * j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[j + e] = x[e];
+        }
+        if (drafted) {
+#pragma unroll
+            for (int j = 0; j < kEach; j += 4) {
+                const float4u x = *(const float4u *) (qr + 4 * j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) b[j + e] = x[e];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            a[j] = first + j < p.V ? *(const float *) (pr + 4 * j) : 0.0f;
+            b[j] = drafted && first + j < p.V ? *(const float *) (qr + 4 * j) : 0.0f;
+        }
+    }
+    const uint32_t out = p.draft ? 0u : gone[threadIdx.x * kEach / 32] >> (threadIdx.x * kEach % 32);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        own[j] = weight(a[j]);
+        left[j] = drafted ? left_of(own[j], weight(b[j]), at.m, norms) : out >> j & 1 ? 0.0 : own[j];
+    }
+}
+
+// The tokens of a chunk that the last accepted node's children had, without a draft.
+__device__ __forceinline__ void rejected(const VerifyParams & p, const int s, const Walked & at, const int count, const int chunk, uint32_t * gone) {
+    for (int i = threadIdx.x; i < kChunk / 32; i += kThreads) gone[i] = 0;
+    __syncthreads();
+    if (!p.draft)
+        for (int u = at.v + 1 + threadIdx.x; u < count; u += kThreads) {
+            const int tok = p.tokens[(int64_t) s * p.tok_nb1 + u];
+            if (parent_of(p, s, u, tok, false) == at.v && tok / kChunk == chunk) atomicOr(gone + tok % kChunk / 32, 1u << (tok % 32));
+        }
+    __syncthreads();
+}
+
+// Grid: chunks, sequences.
+__global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyParams p) {
+    __shared__ WalkLds x;
+    __shared__ uint32_t gone[kChunk / 32];
+    prefetch_params(p);
+    const int s = blockIdx.y, chunk = blockIdx.x;
+    const bool first = chunk == 0;
+    Walked at;
+    int count = 0;
+    if (p.walked) {
+        const int2 st = p.state[s];
+        at = {st.x, st.y, 0};
+        count = nodes_of(p, s, false);
+    } else {
+        count = nodes_of(p, s, first && threadIdx.x == 0);
+        at = walk<false>(p, s, count, first, x, nullptr);
+        if (first) write_path(p, s, at, x);
+    }
+    if (at.v < 0) return;
+    rejected(p, s, at, count, chunk, gone);
+    double left[kEach], own[kEach], a = 0.0, b = 0.0;
+    row_weights(p, s, at, p.norms + (int64_t) s * p.T, chunk * kChunk + threadIdx.x * kEach, gone, left, own);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) a += left[j], b += own[j];
+    a = block_sum(a, x.red);
+    b = block_sum(b, x.red);
+    if (threadIdx.x == 0) p.sums[(int64_t) s * p.chunks + chunk] = double2{a, b};
+}
+
+// Sum of the workgroup's values before this thread's, and of all.
+__device__ __forceinline__ double block_before(const double x, double & all, double * lds) {
+    double y = x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        const double o = __shfl_up(y, i);
+        if (lane >= i) y += o;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = y;
+    double before = __shfl_up(y, 1);
+    if (lane == 0) before = 0.0;
+    __syncthreads();
+    double from = 0.0;
+    all = 0.0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+        if (i == wave) from = all;
+        all += lds[i];
+    }
+    return from + before;
+}
+
+// Grid: sequences.
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParams p) {
+    __shared__ double lds[kThreads / 64];
+    __shared__ uint32_t gone[kChunk / 32];
+    __shared__ int s_at, s_last;
+    __shared__ double s_before;
+    prefetch_params(p);
+    const int s = blockIdx.x, tid = threadIdx.x;
+    const int2 st = p.state[s];
+    const Walked at = {st.x, st.y, 0};
+    if (at.v < 0) {
+        if (tid == 0) p.next[s] = -1;
+        return;
+    }
+    // the chunk: each thread some that follow one another
+    const double2 * sums = p.sums + (int64_t) s * p.chunks;
+    const int each = (p.chunks + kThreads - 1) / kThreads, c0 = min(tid * each, p.chunks), c1 = min(c0 + each, p.chunks);
+    double a = 0.0, b = 0.0, total, own_total;
+    for (int c = c0; c < c1; ++c) a += sums[c].x, b += sums[c].y;
+    double before = block_before(a, total, lds);
+    const double own_before = block_before(b, own_total, lds);
+    const bool own = !(total > 0.0);
+    if (own) total = own_total, before = own_before;
+    if (!(total > 0.0 && total < __builtin_inf())) {
+        if (tid == 0) {
+            draft_error(p.err, kDraftBadRow, s);
+            p.next[s] = -1;
+        }
+        return;
+    }
+    const double goal = (double) p.sample[s] * total;
+    if (tid == 0) s_at = INT32_MAX, s_last = -1;
+    __syncthreads();
+    // the first chunk that goes past the goal; else the last that holds any
+    int hit = -1, last = -1;
+    double hit_before = 0.0, last_before = 0.0;
+    for (int c = c0; c < c1; ++c) {
+        const double w = own ? sums[c].y : sums[c].x;
+        if (w > 0.0) {
+            last = c;
+            last_before = before;
+            if (hit < 0 && before + w > goal) hit = c, hit_before = before;
+        }
+        before += w;
+    }
+    if (hit >= 0) atomicMin(&s_at, hit);
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    const int chunk = s_at == INT32_MAX ? s_last : s_at;
+    if (chunk >= c0 && chunk < c1) s_before = s_at == INT32_MAX ? last_before : hit_before;
+    __syncthreads();
+    const double from = s_before;
+    if (tid == 0) s_at = INT32_MAX, s_last = -1;
+    // the token in it
+    rejected(p, s, at, nodes_of(p, s, false), chunk, gone);
+    const int first = chunk * kChunk + tid * kEach;
+    double left[kEach], row[kEach], mine = 0.0, all;
+    row_weights(p, s, at, p.norms + (int64_t) s * p.T, first, gone, left, row);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        if (own) left[j] = row[j];
+        mine += left[j];
+    }
+    double run = from + block_before(mine, all, lds);
+    hit = last = -1;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        run += left[j];
+        if (left[j] > 0.0) {
+            last = first + j;
+            if (hit < 0 && run > goal) hit = first + j;
+        }
+    }
+    if (hit >= 0) atomicMin(&s_at, hit);
+    if (last >= 0) atomicMax(&s_last, last);
+    __syncthreads();
+    if (tid == 0) p.next[s] = s_at == INT32_MAX ? s_last : s_at;
+}
+
+bool index(const al_tensor & t, const int64_t n) {
+    return t.data && t.type == AL_TYPE_I32 && t.ne[0] == n && t.ne[1] == 1 && t.ne[2] == 1 && t.ne[3] == 1 && t.nb[0] == 4 &&
+           ((uintptr_t) t.data & 3u) == 0;
+}
+
+// [T, n_seq] of 32-bit values
+bool nodes(const al_tensor & t, const int type, const int64_t T, const int64_t n) {
+    return t.data && t.type == type && t.ne[0] == T && t.ne[1] == n && t.ne[2] == 1 && t.ne[3] == 1 && t.nb[0] == 4 && t.nb[1] % 4 == 0 &&
+           ((uintptr_t) t.data & 3u) == 0;
+}
+
+int64_t entries(const uint64_t bytes) { return (int64_t) (bytes / 4); }
+
+struct VerifyPlan {
+    VerifyParams p;
+    int64_t n_seq = 0;
+    size_t norms_at = 0, sums_at = 0, bytes = 0;
+};
+
+int make_plan(const al_draft_verify_args * a, VerifyPlan * out) {
+    if (!a) return al_fail(AL_ERR_INVALID, "draft_verify: null arguments");
+    const al_tensor & t = a->target;
+    if (!t.data) return al_fail(AL_ERR_INVALID, "draft_verify: target is required");
+    const int64_t V = t.ne[0], T = t.ne[1], n = t.ne[2];
+    auto rows = [&](const al_tensor & x) {
+        return x.type == AL_TYPE_F32 && x.ne[0] == V && x.ne[1] == T && x.ne[2] == n && x.ne[3] == 1 && x.nb[0] == 4 && x.nb[1] % 4 == 0 &&
+               x.nb[2] % 4 == 0 && ((uintptr_t) x.data & 3u) == 0;
+    };
+    if (V < 1 || T < 0 || n < 0 || !rows(t) || (a->draft.data && !rows(a->draft)))
+        return al_fail(AL_ERR_INVALID, "draft_verify: target and draft must be f32 [V, T, n_seq]");
+    if (!nodes(a->tokens, AL_TYPE_I32, T, n) || !nodes(a->path, AL_TYPE_I32, T, n) || !nodes(a->accept, AL_TYPE_F32, T, n) ||
+        (a->parents.data && !nodes(a->parents, AL_TYPE_I32, T, n)))
+        return al_fail(AL_ERR_INVALID, "draft_verify: tokens, parents and path must be i32 [T, n_seq], accept f32 [T, n_seq]");
+    al_tensor u = a->sample;
+    if (u.type != AL_TYPE_F32) return al_fail(AL_ERR_INVALID, "draft_verify: sample must be f32 [n_seq]");
+    u.type = AL_TYPE_I32;
+    if (!index(u, n) || !index(a->kept, n) || !index(a->next, n) || (a->counts.data && !index(a->counts, n)))
+        return al_fail(AL_ERR_INVALID, "draft_verify: sample, counts, kept and next must be [n_seq], i32 but for sample");
+    if (V > (1 << 24) || T > kMaxNodes || n > 65535) return al_fail(AL_ERR_UNSUPPORTED, "draft_verify: sizes out of range");
+    VerifyPlan pl;
+    VerifyParams & p = pl.p;
+    memset(&p, 0, sizeof(p));
+    p.target = (const char *) t.data; p.t_nb1 = (int64_t) t.nb[1]; p.t_nb2 = (int64_t) t.nb[2];
+    p.draft = (const char *) a->draft.data; p.d_nb1 = (int64_t) a->draft.nb[1]; p.d_nb2 = (int64_t) a->draft.nb[2];
+    p.tokens = (const int32_t *) a->tokens.data; p.tok_nb1 = entries(a->tokens.nb[1]);
+    p.parents = (const int32_t *) a->parents.data; p.par_nb1 = entries(a->parents.nb[1]);
+    p.counts = (const int32_t *) a->counts.data;
+    p.accept = (const float *) a->accept.data; p.acc_nb1 = entries(a->accept.nb[1]);
+    p.sample = (const float *) a->sample.data;
+    p.path = (int32_t *) a->path.data; p.path_nb1 = entries(a->path.nb[1]);
+    p.kept = (int32_t *) a->kept.data;
+    p.next = (int32_t *) a->next.data;
+    p.T = (int32_t) T; p.V = (int32_t) V;
+    p.chunks = (int32_t) ((V + kChunk - 1) / kChunk);
+    // only siblings of a draft's tokens need sums within the walk
+    p.walked = p.draft && p.parents && T > 2;
+    pl.n_seq = n;
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    pl.norms_at = up((size_t) n * sizeof(int2));
+    pl.sums_at = pl.norms_at + (p.walked ? up((size_t) n * T * sizeof(double)) : 0);
+    pl.bytes = pl.sums_at + (size_t) n * p.chunks * sizeof(double2);
+    *out = pl;
+    return AL_OK;
+}
+
+}  // namespace
+
+extern "C" int al_draft_tree_i32(const al_draft_tree_args * a) {
+    if (!a) return al_fail(AL_ERR_INVALID, "draft_tree: null arguments");
+    const int64_t T = a->parents.ne[0], n = a->parents.ne[1];
+    if (T < 0 || n < 0 || !nodes(a->parents, AL_TYPE_I32, T, n)) return al_fail(AL_ERR_INVALID, "draft_tree: parents must be i32 [T, n_seq]");
+    if (!index(a->lens, n) || (a->counts.data && !index(a->counts, n)))
+        return al_fail(AL_ERR_INVALID, "draft_tree: lens and counts must be i32 [n_seq]");
+    for (const al_tensor * t : {&a->pos, &a->cells, &a->seq})
+        if (t->data && !nodes(*t, AL_TYPE_I32, T, n)) return al_fail(AL_ERR_INVALID, "draft_tree: pos, cells and seq must be i32 [T, n_seq]");
+    const al_tensor & b = a->bits;
+    if (b.data && (b.type != AL_TYPE_I32 || b.ne[0] < (T + 31) / 32 || b.ne[1] != T || b.ne[2] != n || b.ne[3] != 1 || b.nb[0] != 4 || b.nb[1] % 4 ||
+                   b.nb[2] % 4 || ((uintptr_t) b.data & 3u)))
+        return al_fail(AL_ERR_INVALID, "draft_tree: bits must be i32 [words, T, n_seq], 32 nodes to a word");
+    if (T > kMaxNodes || n > 65535 || (b.data && b.ne[0] > (1 << 16))) return al_fail(AL_ERR_UNSUPPORTED, "draft_tree: sizes out of range");
+    if (T == 0 || n == 0) return AL_OK;
+    TreeParams p;
+    memset(&p, 0, sizeof(p));
+    p.parents = (const int32_t *) a->parents.data; p.par_nb1 = entries(a->parents.nb[1]);
+    p.lens = (const int32_t *) a->lens.data;
+    p.counts = (const int32_t *) a->counts.data;
+    p.pos = (int32_t *) a->pos.data; p.pos_nb1 = entries(a->pos.nb[1]);
+    p.cells = (int32_t *) a->cells.data; p.cells_nb1 = entries(a->cells.nb[1]);
+    p.seq = (int32_t *) a->seq.data; p.seq_nb1 = entries(a->seq.nb[1]);
+    p.bits = (int32_t *) b.data; p.b_nb1 = entries(b.nb[1]); p.b_nb2 = entries(b.nb[2]);
+    p.T = (int32_t) T;
+    p.words = b.data ? (int32_t) b.ne[0] : 0;
+    const int rc = al_device_error_flag(&p.err);
+    if (rc != AL_OK) return rc;
+    const dim3 grid((unsigned) ((T + 63) / 64), (unsigned) n);
+    hipLaunchKernelGGL(draft_tree_kernel, grid, dim3(64), 0, (hipStream_t) a->stream, p);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? AL_OK : al_hip_fail(e, "draft_tree: launch");
+}
+
+extern "C" uint64_t al_draft_verify_workspace_bytes(const al_draft_verify_args * a) {
+    VerifyPlan pl;
+    return make_plan(a, &pl) != AL_OK || pl.n_seq == 0 ? 0 : al_workspace_bytes(pl.bytes);
+}
+
+extern "C" int al_draft_verify_f32(const al_draft_verify_args * a) {
+    VerifyPlan pl;
+    int rc = make_plan(a, &pl);
+    if (rc != AL_OK || pl.n_seq == 0) return rc;
+    VerifyParams & p = pl.p;
+    rc = al_device_error_flag(&p.err);
+    if (rc != AL_OK) return rc;
+    char * at = nullptr;
+    rc = al_workspace_records("draft_verify", pl.bytes, a->workspace, a->workspace_bytes, a->stream, (void **) &at);
+    if (rc != AL_OK) return rc;
+    p.state = (int2 *) at;
+    p.norms = (double *) (at + pl.norms_at);
+    p.sums = (double2 *) (at + pl.sums_at);
+    const hipStream_t st = (hipStream_t) a->stream;
+    const unsigned n = (unsigned) pl.n_seq;
+    hipError_t e = hipSuccess;
+    if (p.walked) {
+        hipLaunchKernelGGL(verify_walk_kernel, dim3(n), dim3(kThreads), 0, st, p);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess) {
+        hipLaunchKernelGGL(verify_sums_kernel, dim3((unsigned) p.chunks, n), dim3(kThreads), 0, st, p);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess) {
+        hipLaunchKernelGGL(verify_pick_kernel, dim3(n), dim3(kThreads), 0, st, p);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess ? AL_OK : al_hip_fail(e, "draft_verify: launch");
+}

@@ -83,6 +83,15 @@ struct PagedFattnParams {
     int32_t target, long_target;                        // workgroups of a unit (head, row group), those that long sequences use
     int32_t row_waves;                                  // join: waves of a row
     float scale, softcap;
+    static constexpr bool kSees = false;
+};
+
+// The same with a rule for what a token sees (al_paged_sees).
+struct PagedSeesParams : PagedFattnParams {
+    int32_t window, first;                              // window 0: none
+    const int32_t * bits;  int64_t b_nb1, b_nb2;        // or null; token, sequence, in words
+    const int32_t * pos;   int64_t p_nb1;               // or null; sequence
+    static constexpr bool kSees = true;
 };
 
 template <int CTRL, int ROW_MASK>
@@ -120,7 +129,8 @@ struct SeqWork {
     }
 };
 
-__device__ __forceinline__ SeqWork seq_work(const PagedFattnParams & p, const int len, const int count) {
+template <typename P>
+__device__ __forceinline__ SeqWork seq_work(const P & p, const int len, const int count) {
     SeqWork w;
     w.len = min(max(len, 0), p.c.max_pages * p.c.page_size);
     w.count = min(max(count, 0), p.T);
@@ -128,10 +138,79 @@ __device__ __forceinline__ SeqWork seq_work(const PagedFattnParams & p, const in
     return w;
 }
 
+// The cells that tokens t0 to t1 of a sequence see, as a whole: those before
+// `limit` (-1: there are no such tokens), but none from p.first to `low`.
+struct Span {
+    int limit, low;
+    // Tiles without such a cell, and the first of them.
+    __device__ __forceinline__ int gap(const int first) const { return max(low / kTile - gap_at(first), 0); }
+    __device__ __forceinline__ int gap_at(const int first) const { return (min(first, low) + kTile - 1) / kTile; }
+};
+
+template <typename P>
+__device__ __forceinline__ Span span_of(const P & p, const SeqWork & w, const int t0, const int t1) {
+    Span a = {w.limit(t0, t1), 0};
+    if constexpr (P::kSees) {
+        if (p.bits && a.limit >= 0) a.limit = w.len;                   // of nodes each may see any
+        if (p.window) a.low = min(max(w.len - w.count + (p.bits ? 0 : t0) + 1 - p.window, 0), max(a.limit - 1, 0));
+    }
+    return a;
+}
+
 // Tiles of a sequence in the row of all tiles: one at least, so that rows that
 // see nothing are written too.
-__device__ __forceinline__ int tiles_of(const int limit) {
-    return limit < 0 ? 0 : max(1, (limit + kTile - 1) / kTile);
+template <typename P>
+__device__ __forceinline__ int tiles_of(const P & p, const Span a) {
+    int gap = 0;
+    if constexpr (P::kSees) gap = a.gap(p.first);
+    return a.limit < 0 ? 0 : max(1, (a.limit + kTile - 1) / kTile - gap);
+}
+
+// The first k of 8 cells, a bit each.
+__device__ __forceinline__ uint32_t upto8(const int k) { return (1u << min(max(k, 0), 8)) - 1; }
+// Of cells c0 to c0 + 7: those before `limit` that are not from `first` to `low`.
+__device__ __forceinline__ uint32_t span8(const int c0, const int limit, const int low, const int first) {
+    return upto8(limit - c0) & (~upto8(low - c0) | upto8(first - c0));
+}
+
+// Of nodes u0 to u0 + 7 (u0 may be negative) those that a token sees, whose
+// words are `words`, among the sequence's first `count`.
+__device__ __forceinline__ uint32_t nodes8(const int32_t * words, const int u0, const int count) {
+    if (u0 <= -8 || u0 >= count) return 0;
+    const int u = max(u0, 0), i = u >> 5, last = (count - 1) >> 5;
+    const uint64_t two = (uint32_t) words[i] | (uint64_t) (uint32_t) words[min(i + 1, last)] << 32;
+    return (uint32_t) (two >> (u & 31)) << (u - u0) & upto8(count - u0);
+}
+
+// The same, without those that lie before the token's window and are not among
+// the first cells either; pos: the nodes' positions.
+__device__ __forceinline__ uint32_t nodes8(const PagedSeesParams & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
+                                           const int low) {
+    uint32_t m = nodes8(words, u0, count);
+    if (p.window)
+        for (uint32_t rest = m; rest; rest &= rest - 1) {
+            const int at = pos[u0 + __builtin_ctz(rest)];
+            if (at < low && at >= p.first) m &= ~(rest & -rest);
+        }
+    return m;
+}
+
+// Whether token t of sequence s sees a cell at all.
+template <typename P>
+__device__ __forceinline__ bool sees_any(const P & p, const SeqWork & w, const int s, const int t) {
+    const int begin = w.len - w.count;
+    if constexpr (P::kSees) {
+        if (p.bits) {
+            const int32_t * words = p.bits + (int64_t) s * p.b_nb2 + (int64_t) t * p.b_nb1;
+            const int32_t * pos = p.pos + (int64_t) s * p.p_nb1;
+            const int low = p.window ? pos[t] + 1 - p.window : 0;
+            if (begin > 0 && (begin > low || p.first > 0)) return true;
+            for (int u = max(-begin, 0); u < w.count; u += 8)
+                if (nodes8(p, words, pos, u, w.count, low)) return true;
+            return false;
+        }
+    }
+    return begin + 1 + t > 0;
 }
 
 // S tiles cut into W parts, the first S % W of them one tile longer: the first
@@ -149,12 +228,13 @@ struct Parts {
 // Sequences 64 b .. 64 b + 63, one to a lane.
 struct Block {
     int len, count, tiles, upto;                // as read; tiles, and those of all sequences up to this one
-    __device__ __forceinline__ void load(const PagedFattnParams & p, const int b, const int lane, const int t0, const int t1) {
+    template <typename P>
+    __device__ __forceinline__ void load(const P & p, const int b, const int lane, const int t0, const int t1) {
         const int s = 64 * b + lane;
         const bool in = s < p.c.n_seq;
         len = in ? p.lens[s] : 0;
         count = !in ? 0 : p.counts ? p.counts[s] : p.T;
-        tiles = in ? tiles_of(seq_work(p, len, count).limit(t0, t1)) : 0;
+        tiles = in ? tiles_of(p, span_of(p, seq_work(p, len, count), t0, t1)) : 0;
         upto = wave_scan(tiles);
     }
     // A negative count makes an empty slot, which no workgroup comes to.
@@ -185,33 +265,37 @@ __device__ __forceinline__ float grow(const float a, const float b) { return a =
 
 // Factor of a row's sums, with the sink as one more logit without a value: 0
 // for a row that sees nothing, NaN where all logits are -inf.
-template <typename P>
-__device__ __forceinline__ float row_factor(const P & p, const float M, float L, const int head, const bool sees) {
+// p: the arguments, a: the same, to be loaded where they are used.
+template <typename P, typename A>
+__device__ __forceinline__ float row_factor(const P & p, const A & a, const SeqWork & w, const int s, const int t, const float M, float L,
+                                            const int head) {
     L *= 1.0f / kPScale;
     float up = 1.0f / kPScale;
-    if (p.sinks) {
-        const float sink = p.sinks[head], top = fmaxf(M, sink);
+    if (a.sinks) {
+        const float sink = a.sinks[head], top = fmaxf(M, sink);
         const float e = grow(M, top);
         up *= e;
         L = L * e + (sink == -AL_INF ? 0.0f : grow(sink, top));
     }
-    return L == 0.0f ? sees ? __builtin_nanf("") : 0.0f : up / L;
+    return L == 0.0f ? sees_any(p, w, s, t) ? __builtin_nanf("") : 0.0f : up / L;
 }
 
 // The kernel's arguments as memory, to be loaded where they are used: held in
 // scalar registers from the start, those that only a piece's beginning and end
 // use displace what the loop over the cells needs.
-__device__ __forceinline__ const __attribute__((address_space(4))) PagedFattnParams & arguments() {
-    auto a = (const __attribute__((address_space(4))) PagedFattnParams *) __builtin_amdgcn_kernarg_segment_ptr();
+template <typename P>
+__device__ __forceinline__ const __attribute__((address_space(4))) P & arguments() {
+    auto a = (const __attribute__((address_space(4))) P *) __builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(a));
     return *a;
 }
 
 // ROWT: row tiles of 16 query rows that the waves take side by side (1, 2 or
 // 4); the tiles of cells go round the waves of a row tile. CAP: logits
-// soft-capped.
-template <int ROWT, bool CAP>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const PagedFattnParams p) {
+// soft-capped. P: PagedFattnParams, or PagedSeesParams for tokens that see
+// other cells than all before them.
+template <int ROWT, bool CAP, typename P>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) {
     constexpr int kCellWaves = kWaves / ROWT;
     __shared__ __attribute__((aligned(16))) float o_lds[kWaves][16][132];
     __shared__ float ml_lds[kWaves][16][2];
@@ -292,7 +376,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         const int first = at - base, end = min(tiles, stop - base);
         at = base + end;
         const bool whole = first == 0 && end == tiles;
-        const auto & ap = arguments();
+        const auto & ap = arguments<P>();
         if (threadIdx.x == 0) {
             if (first == 0)
                 ap.info[(int64_t) unit * ap.c.n_seq + seq] =
@@ -300,8 +384,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
             if (w.bad) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         bool bad = w.bad;
-        const int seen = w.limit(wt0, wt1);                        // cells that the wave's last row sees
-        const int least = max(w.len - w.count + 1 + wt0, 0);       // cells that all its rows see
+        const Span wave_span = span_of(p, w, wt0, wt1);
+        const int seen = wave_span.limit;                          // cells that the wave's last row sees
+        int least = max(w.len - w.count + 1 + wt0, 0);             // cells that all its rows see
+        // Of a rule: the tiles that the group leaves out, and where the last of
+        // the rows' windows begins.
+        int gap = 0, gap_at = 0, low_last = 0, first_cells = 0;
+        const int begin = w.len - w.count;
+        if constexpr (P::kSees) {
+            const Span all = span_of(p, w, t0, t1);
+            first_cells = p.first;
+            gap = all.gap(p.first);
+            gap_at = all.gap_at(p.first);
+            if (p.bits) least = max(begin, 0);
+            if (p.window) low_last = (p.bits ? w.len : begin + 1 + min(wt1, w.count - 1)) - p.window;
+        }
+        auto tile_at = [&](const int i) { return P::kSees && i >= gap_at ? i + gap : i; };
 
         // Pages of a tile's cells: K by lanes n (group n / 4), V by lanes g.
         // Cells past the last group that the wave sees are taken from that one.
@@ -311,9 +409,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         };
         const int32_t * table = p.c.table + (int64_t) seq * p.c.t_nb1;
         const uint32_t last_group = (uint32_t) max(seen - 1, 0) / 8;
-        auto look_up = [&](const int tile) {
+        auto look_up = [&](const int i) {
             Where a;
-            const uint32_t kg = min((uint32_t) tile * 4 + (n >> 2), last_group), vg = min((uint32_t) tile * 4 + g, last_group);
+            const int tile = tile_at(i);
+            uint32_t kg = min((uint32_t) tile * 4 + (n >> 2), last_group), vg = min((uint32_t) tile * 4 + g, last_group);
+            if constexpr (P::kSees) {                                  // and those that no window has from the first that one has
+                const int low = wave_span.low, from = (p.first + 7) >> 3;
+                if ((int) kg >= from) kg = max((int) kg, low >> 3);
+                if ((int) vg >= from) vg = max((int) vg, low >> 3);
+            }
             const uint32_t kp = page_of_group(p.c, kg), vp = page_of_group(p.c, vg);
             a.k_page = table[kp];
             a.v_page = table[vp];
@@ -347,13 +451,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         const int r = r0 + n, t = token_of(p, min(r, p.R - 1));
         const bool valid = r < p.R && t < w.count;
         const int limit = valid ? w.len - w.count + 1 + t : seen;
+        // its window's beginning, the words of the nodes that it sees
+        int low = 0;
+        const int32_t * words = nullptr;
+        const int32_t * node_pos = nullptr;
+        bool bad_row = false;
+        if constexpr (P::kSees) {
+            int at = begin + t;
+            if (p.bits) {
+                words = p.bits + (int64_t) seq * p.b_nb2 + (int64_t) (valid ? t : 0) * p.b_nb1;
+                node_pos = p.pos + (int64_t) seq * p.p_nb1;
+                if (p.window && valid) {
+                    at = node_pos[t];
+                    bad_row = at < begin || at >= w.len;
+                    if (bad_row && g == 0) paged_error(p.c, kPagedBadPos, at);
+                }
+            }
+            if (p.window && valid && !bad_row) low = at + 1 - p.window;
+        }
+        // Of cells c0 to c0 + 7: those that this lane's row sees.
+        auto sees8 = [&](const int c0) {
+            if constexpr (P::kSees) {
+                if (p.bits) return span8(c0, begin, low, p.first) | nodes8(p, words, node_pos, c0 - begin, w.count, low);
+                return span8(c0, limit, low, p.first);
+            } else return upto8(limit - c0);
+        };
         half8 q_hi[4], q_lo[4];
         float fac, m = -AL_INF, l = 0.0f;
         floatx4 acc[8];
         // Everything that the first tile needs goes out before anything is
         // computed: pages, query rows, then K and V (a wave without a tile
         // loads another wave's and uses none of it).
-        const int wave_end = min(end, seen > 0 ? (seen + kTile - 1) / kTile : 0);
+        const int wave_end = min(end, seen > 0 ? (seen + kTile - 1) / kTile - gap : 0);
         const bool has = first + cw < wave_end;
         int tile = has ? first + cw : max(wave_end - 1, 0);
         const Where here = look_up(tile);
@@ -423,10 +552,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
                 for (int e = 0; e < 2; ++e) s[e] = mfma_16x16x32(k[e][kk], q_hi[kk], s[e]);
         };
         half8 p_hi, p_lo;
+        // Whether some row does not see all of a tile.
+        auto partly = [&](const int tile) {
+            return (tile + 1) * kTile > least || (P::kSees && tile * kTile < low_last && (tile + 1) * kTile > first_cells);
+        };
         // Probabilities of the tile against the rows' running maxima.
         auto softmax = [&](const int tile) {
             const int c0 = tile * kTile + 8 * g;
-            const bool masked = (tile + 1) * kTile > least;          // some row does not see all of it
+            const bool masked = partly(tile);
+            uint32_t sees = 0xffu;
+            if constexpr (P::kSees) {
+                if (masked) sees = sees8(c0);
+            }
+            auto hidden = [&](const int i) { return P::kSees ? !(sees >> i & 1) : c0 + i >= limit; };
             float x[8];
             float top = -AL_INF;
 #pragma unroll
@@ -437,7 +575,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (c0 + i >= limit) x[i] = -AL_INF;
+                    if (hidden(i)) x[i] = -AL_INF;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
@@ -455,7 +593,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float e = exp_fast(x[i] - from) * kPScale;
-                if (masked && c0 + i >= limit) e = 0.0f;
+                if (masked && hidden(i)) e = 0.0f;
                 l += e;
                 const _Float16 hi = (_Float16) e;
                 p_hi[i] = hi;
@@ -468,16 +606,27 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         // see one get NaN in its dim, found by a product of ones.
         auto product = [&](const int tile) {
             const int c0 = tile * kTile + 8 * g;
-            if ((tile + 1) * kTile > seen) {
+            bool differ = least < seen && (tile + 1) * kTile > least;   // (one token: never)
+            uint32_t some = 0xffu, all = upto8(least - c0);          // cells that some, that all rows see
+            if constexpr (P::kSees) {
+                if (partly(tile)) {
+                    some = span8(c0, seen, wave_span.low, p.first);
+                    all = span8(c0, least, low_last, p.first);
+                    differ = true;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (!(some >> i & 1)) v[i] = u32x4{0, 0, 0, 0};
+                }
+            } else if ((tile + 1) * kTile > seen) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (c0 + i >= seen) v[i] = u32x4{0, 0, 0, 0};
             }
-            if (least < seen && (tile + 1) * kTile > least) {        // (one token: never)
+            if (differ) {
                 uint32_t odd[2] = {0, 0};                            // bit 8 (i % 4) + j of word i / 4: cell i, dim j
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (c0 + i >= least)
+                    if (P::kSees ? (some & ~all) >> i & 1 : c0 + i >= least)
 #pragma unroll
                         for (int d = 0; d < 4; ++d) {
                             if ((v[i][d] & 0x7c00u) == 0x7c00u) odd[i / 4] |= 1u << (8 * (i % 4) + 2 * d), v[i][d] &= 0xffff0000u;
@@ -485,9 +634,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
                         }
                 }
                 if (__any((odd[0] | odd[1]) != 0)) {
+                    const uint32_t mine = P::kSees ? sees8(c0) : 0;
                     half8 sees;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sees[i] = c0 + i < limit ? (_Float16) 1.0f : (_Float16) 0.0f;
+                    for (int i = 0; i < 8; ++i) sees[i] = (P::kSees ? mine >> i & 1 : c0 + i < limit) ? (_Float16) 1.0f : (_Float16) 0.0f;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         half8 a;
@@ -518,14 +668,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
                 const Where after = look_up(tile + 2 * kCellWaves);
                 scores();
                 load_k(next, true);
-                softmax(tile);
-                product(tile);
+                softmax(tile_at(tile));
+                product(tile_at(tile));
                 load_v(next, true);
                 next = after;
             }
             scores();
-            softmax(tile);
-            product(tile);
+            softmax(tile_at(tile));
+            product(tile_at(tile));
         }
 
         // join the row tile's waves: maxima and sums, then the rescaled outputs
@@ -533,7 +683,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
         const bool any_bad = __any(bad);
         if (any_bad && lane == 0 && !w.bad) paged_error(p.c, kPagedBadPage, seq);
         l = colsum4(l);
-        if (any_bad) l = __builtin_nanf("");
+        if (any_bad || bad_row) l = __builtin_nanf("");
         if (g == 0) {
             ml_lds[wave][n][0] = m;
             ml_lds[wave][n][1] = l;
@@ -551,7 +701,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
             }
         }
         __syncthreads();
-        const auto & ep = arguments();
+        const auto & ep = arguments<P>();
         char * rec = record(ep, unit, wg, first == 0 ? 1 : 0);
         for (int item = threadIdx.x; item < 16 * ROWT * 16; item += 64 * kWaves) {
             const int row = item >> 4, dim = (item & 15) * 8;        // of the group
@@ -571,7 +721,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
             float f = 1.0f;
             if (whole) {
                 const int head = h * ep.G + gr - tok * ep.G;
-                f = row_factor(ep, M, L, head, w.len - w.count + 1 + tok > 0);
+                f = row_factor(p, ep, w, seq, tok, M, L, head);
                 d = (float *) (ep.dst + (int64_t) seq * ep.d_nb3 + (int64_t) tok * ep.d_nb2 + (int64_t) head * ep.d_nb1) + dim;
             } else {
                 d = (float *) rec + row * 128 + dim;
@@ -588,7 +738,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const Paged
 // p.row_waves waves (1 or kWaves) take it, the halves of a wave every second
 // piece, 4 dims to a lane; all loads of 8 of a half's pieces are in flight
 // together.
-__device__ __forceinline__ void join_row(const PagedFattnParams & p, const int2 info, const int unit, const int seq, const int count,
+template <typename P>
+__device__ __forceinline__ void join_row(const P & p, const int2 info, const int unit, const int seq, const int count,
                                          const int row, float (*o_lds)[132]) {
     const int lane = threadIdx.x & 63, half = lane >> 5, d4 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -659,13 +810,14 @@ __device__ __forceinline__ void join_row(const PagedFattnParams & p, const int2 
     if (!mine || half) return;
     const int head = h * p.G + gr - t * p.G;
     const SeqWork w = seq_work(p, p.lens[seq], count);
-    const float f = row_factor(p, M, L, head, w.len - w.count + 1 + t > 0);
+    const float f = row_factor(p, p, w, seq, t, M, L, head);
     *(float4 *) ((float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) head * p.d_nb1) + 4 * d4) =
         float4{o.x * f, o.y * f, o.z * f, o.w * f};
 }
 
 // Workgroups (rows, sequence, unit); few of them where most have nothing to join.
-__global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(const PagedFattnParams p) {
+template <typename P>
+__global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(const P p) {
     __shared__ __attribute__((aligned(16))) float o_lds[kWaves][132];
     prefetch_params(p);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -680,7 +832,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(const PagedFatt
 }
 
 struct Plan {
-    PagedFattnParams p;
+    PagedSeesParams p;                                  // (without a rule: its PagedFattnParams)
     bool empty = false;
     size_t info_bytes = 0, bytes = 0;                   // of the info, of it and the records
 };
@@ -691,7 +843,37 @@ bool aligned16(const al_tensor & t, int from) {
     return ((uintptr_t) t.data & 15u) == 0;
 }
 
-int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
+// The rule's operands, checked, in p; *tiles: at most so many of a sequence's
+// tiles are seen.
+int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n_seq, int64_t * tiles) {
+    if (r->window < 0 || r->first < 0)
+        return al_fail(AL_ERR_INVALID, "paged_fattn: a window of %d cells and %d first ones", r->window, r->first);
+    // (positions are below 2^30: a longer window is all of them)
+    p->window = std::min(r->window, 1 << 30);
+    p->first = p->window ? std::min(r->first, 1 << 30) : 0;
+    if (r->bits.data) {
+        const al_tensor & b = r->bits;
+        if (b.type != AL_TYPE_I32 || b.ne[0] < (T + 31) / 32 || b.ne[1] != T || b.ne[2] != n_seq || b.ne[3] != 1 || b.nb[0] != 4 || b.nb[1] % 4 ||
+            b.nb[2] % 4 || ((uintptr_t) b.data & 3u))
+            return al_fail(AL_ERR_INVALID, "paged_fattn: bits must be i32 [words, T, n_seq], 32 tokens to a word");
+        p->bits = (const int32_t *) b.data; p->b_nb1 = (int64_t) (b.nb[1] / 4); p->b_nb2 = (int64_t) (b.nb[2] / 4);
+    }
+    if (r->pos.data) {
+        const al_tensor & t = r->pos;
+        if (!r->bits.data) return al_fail(AL_ERR_INVALID, "paged_fattn: positions without bits");
+        if (t.type != AL_TYPE_I32 || t.ne[0] != T || t.ne[1] != n_seq || t.ne[2] != 1 || t.ne[3] != 1 || t.nb[0] != 4 || t.nb[1] % 4 ||
+            ((uintptr_t) t.data & 3u))
+            return al_fail(AL_ERR_INVALID, "paged_fattn: positions must be i32 [T, n_seq]");
+        p->pos = (const int32_t *) t.data; p->p_nb1 = (int64_t) (t.nb[1] / 4);
+    } else if (r->bits.data && r->window) {
+        return al_fail(AL_ERR_INVALID, "paged_fattn: bits and a window need positions");
+    }
+    if (p->window)
+        *tiles = std::min(*tiles, ((int64_t) p->first + kTile - 1) / kTile + ((int64_t) p->window + T + kTile - 1) / kTile + 1);
+    return AL_OK;
+}
+
+int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_cu, Plan * out) {
     if (!a) return al_fail(AL_ERR_INVALID, "paged_fattn: null arguments");
     const al_tensor &q = a->q, &d = a->dst;
     if (!q.data || !d.data || !a->lens.data) return al_fail(AL_ERR_INVALID, "paged_fattn: q, dst and lens are required");
@@ -704,7 +886,7 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     if (q.nb[0] != 4 || d.nb[0] != 4 || !aligned16(q, 1) || !aligned16(d, 1))
         return al_fail(AL_ERR_INVALID, "paged_fattn: q and dst rows must be contiguous and 16-byte aligned");
     Plan pl;
-    PagedFattnParams & p = pl.p;
+    PagedSeesParams & p = pl.p;
     memset(&p, 0, sizeof(p));
     int rc = paged_pools("paged_fattn", &a->k_pool, &a->v_pool, &a->table, &p.c);
     if (rc != AL_OK) return rc;
@@ -734,7 +916,10 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     p.row_groups = (p.R + rows - 1) / rows;
     const int64_t units = (int64_t) p.row_groups * Hkv;
     if (units > 65535) return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
-    const int64_t most = n_seq * std::max<int64_t>(1, ((int64_t) p.c.max_pages * p.c.page_size + kTile - 1) / kTile);   // tiles there can be
+    int64_t tiles = std::max<int64_t>(1, ((int64_t) p.c.max_pages * p.c.page_size + kTile - 1) / kTile);
+    if (rule) rc = make_rule(rule, &p, T, n_seq, &tiles);
+    if (rc != AL_OK) return rc;
+    const int64_t most = n_seq * tiles;                                                                                 // tiles there can be
     if (most > INT32_MAX) return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
     // One workgroup a CU, 48 to 64 KB of its waves' loads in flight: more only
     // lengthen the queues (us with one / two / four: 24 sequences to 4000 cells
@@ -756,14 +941,15 @@ int make_plan(const al_paged_fattn_args * a, int n_cu, Plan * out) {
     return AL_OK;
 }
 
-template <int ROWT>
-void launch(const PagedFattnParams & p, hipStream_t st) {
+template <int ROWT, typename P>
+void launch(const P & p, hipStream_t st) {
     const dim3 grid((unsigned) (p.target * p.row_groups * p.Hkv));
-    if (p.softcap != 0.0f) hipLaunchKernelGGL((paged_fattn_kernel<ROWT, true>), grid, dim3(64 * kWaves), 0, st, p);
-    else                   hipLaunchKernelGGL((paged_fattn_kernel<ROWT, false>), grid, dim3(64 * kWaves), 0, st, p);
+    if (p.softcap != 0.0f) hipLaunchKernelGGL((paged_fattn_kernel<ROWT, true, P>), grid, dim3(64 * kWaves), 0, st, p);
+    else                   hipLaunchKernelGGL((paged_fattn_kernel<ROWT, false, P>), grid, dim3(64 * kWaves), 0, st, p);
 }
 
-hipError_t launch(const PagedFattnParams & p, hipStream_t st) {
+template <typename P>
+hipError_t launch(const P & p, hipStream_t st) {
     switch (p.row_tiles) {
         case 1: launch<1>(p, st); break;
         case 2: launch<2>(p, st); break;
@@ -776,7 +962,7 @@ hipError_t launch(const PagedFattnParams & p, hipStream_t st) {
     const int64_t pairs = (int64_t) p.c.n_seq * p.row_groups * p.Hkv;
     const int side = (int) std::max<int64_t>(1, std::min<int64_t>((rows + kWaves - 1) / kWaves, 2048 / pairs));
     const dim3 grid((unsigned) (p.row_waves == 1 ? side : rows), (unsigned) p.c.n_seq, (unsigned) (p.row_groups * p.Hkv));
-    hipLaunchKernelGGL(paged_join_kernel, grid, dim3(64 * kWaves), 0, st, p);
+    hipLaunchKernelGGL((paged_join_kernel<P>), grid, dim3(64 * kWaves), 0, st, p);
     return hipGetLastError();
 }
 
@@ -812,26 +998,44 @@ int paged_pools(const char * what, const al_tensor * k, const al_tensor * v, con
     return AL_OK;
 }
 
-extern "C" uint64_t al_paged_fattn_workspace_bytes(const al_paged_fattn_args * a) {
+namespace {
+
+uint64_t workspace_bytes(const al_paged_fattn_args * a, const al_paged_sees * rule) {
     int n_cu = 0;
     Plan pl;
-    if (al_device_cu_count(&n_cu) != AL_OK || make_plan(a, n_cu, &pl) != AL_OK) return 0;
+    if (al_device_cu_count(&n_cu) != AL_OK || make_plan(a, rule, n_cu, &pl) != AL_OK) return 0;
     return pl.empty ? 0 : al_workspace_bytes(pl.bytes);
 }
 
-extern "C" int al_paged_fattn_f16(const al_paged_fattn_args * a) {
+int attend(const al_paged_fattn_args * a, const al_paged_sees * rule) {
     // the arguments first: refusals need no device
     Plan pl;
-    int rc = make_plan(a, 1, &pl);
+    int rc = make_plan(a, rule, 1, &pl);
     if (rc != AL_OK || pl.empty) return rc;
     int n_cu = 0;
     rc = al_device_cu_count(&n_cu);
-    if (rc == AL_OK) rc = make_plan(a, n_cu, &pl);
+    if (rc == AL_OK) rc = make_plan(a, rule, n_cu, &pl);
     if (rc == AL_OK) rc = al_device_error_flag(&pl.p.c.err);
     if (rc != AL_OK) return rc;
     rc = al_workspace_records("paged_fattn", pl.bytes, a->workspace, a->workspace_bytes, a->stream, (void **) &pl.p.info);
     if (rc != AL_OK) return rc;
     pl.p.part = (float *) ((char *) pl.p.info + pl.info_bytes);
-    const hipError_t e = launch(pl.p, (hipStream_t) a->stream);
+    const hipStream_t st = (hipStream_t) a->stream;
+    // (a rule that leaves nothing out is none)
+    const hipError_t e = pl.p.window || pl.p.bits ? launch(pl.p, st) : launch<PagedFattnParams>(pl.p, st);
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "paged_fattn: launch");
+}
+
+}  // namespace
+
+extern "C" uint64_t al_paged_fattn_workspace_bytes(const al_paged_fattn_args * a) { return workspace_bytes(a, nullptr); }
+
+extern "C" int al_paged_fattn_f16(const al_paged_fattn_args * a) { return attend(a, nullptr); }
+
+extern "C" uint64_t al_paged_fattn_sees_workspace_bytes(const al_paged_fattn_args * a, const al_paged_sees * sees) {
+    return sees ? workspace_bytes(a, sees) : 0;
+}
+
+extern "C" int al_paged_fattn_sees_f16(const al_paged_fattn_args * a, const al_paged_sees * sees) {
+    return sees ? attend(a, sees) : al_fail(AL_ERR_INVALID, "paged_fattn: null rule");
 }

@@ -46,6 +46,7 @@ struct AppendParams {
     char * q_out;    int64_t o_nb1, o_nb2;
     const int32_t * pos;
     const int32_t * seq;
+    const int32_t * cells;                       // or null: pos
     int32_t T, Hq, Hkv, norm;
     int32_t yq, yk;                              // blocks of 8 heads of q, of k (and v)
     float eps;
@@ -53,7 +54,7 @@ struct AppendParams {
 };
 
 // Cell of token t, or -1 when it has none that can be written.
-__device__ __forceinline__ int64_t cell_of(const PagedPools & c, const int s, const int pos, const bool report, int & page) {
+__device__ __forceinline__ int64_t cell_of(const PagedPools & c, const int s, const int pos, const bool report, const bool own_cell, int & page) {
     const bool seq_ok = s < c.n_seq;
     const bool pos_ok = pos >= 0 && pos < c.max_pages * c.page_size;
     int pg = -1, at = 0;
@@ -63,7 +64,7 @@ __device__ __forceinline__ int64_t cell_of(const PagedPools & c, const int s, co
         pg = c.table[(int64_t) s * c.t_nb1 + i];
     }
     const bool ok = (uint32_t) pg < (uint32_t) c.n_pages;
-    if (!ok && report) paged_error(c, !seq_ok ? kPagedBadSeq : !pos_ok ? kPagedBadPos : kPagedBadPage, !seq_ok ? s : !pos_ok ? pos : s);
+    if (!ok && report) paged_error(c, !seq_ok ? kPagedBadSeq : !pos_ok ? (own_cell ? kPagedBadCell : kPagedBadPos) : kPagedBadPage, !seq_ok ? s : !pos_ok ? pos : s);
     page = pg;
     return ok ? at : -1;
 }
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(const AppendP
     if (s < 0) return;                                                   // wave-uniform: a row of no sequence
     int page = 0;
     int64_t cell = 0;
-    if (kind != 0) cell = cell_of(p.c, s, pos, lane == 0 && h == 0, page);
+    if (kind != 0) cell = cell_of(p.c, s, p.cells ? p.cells[t] : pos, lane == 0 && h == 0, p.cells != nullptr, page);
 
     if (kind != 2) {
         float lo[8], hi[8], wl[8], wh[8];
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(const AppendP
     }
 }
 
-int make_params(const al_paged_append_args * a, AppendParams * out, int * mode, bool * empty) {
+int make_params(const al_paged_append_args * a, const al_tensor * cells, AppendParams * out, int * mode, bool * empty) {
     if (!a) return al_fail(AL_ERR_INVALID, "paged_append: null arguments");
     AppendParams p;
     memset(&p, 0, sizeof(p));
@@ -169,6 +170,7 @@ int make_params(const al_paged_append_args * a, AppendParams * out, int * mode, 
         return al_fail(AL_ERR_INVALID, "paged_append: q and q_out must be f32 [128, Hq, T]");
     auto index = [&](const al_tensor & t) { return t.data && t.type == AL_TYPE_I32 && t.ne[0] == T && t.nb[0] == 4 && ((uintptr_t) t.data & 3u) == 0; };
     if (!index(a->pos) || !index(a->seq)) return al_fail(AL_ERR_INVALID, "paged_append: pos and seq must be i32 [T]");
+    if (cells && !index(*cells)) return al_fail(AL_ERR_INVALID, "paged_append: cells must be i32 [T]");
     auto weight = [](const al_tensor & t) { return !t.data || (t.type == AL_TYPE_F32 && t.ne[0] >= 128 && t.nb[0] == 4 && ((uintptr_t) t.data & 3u) == 0); };
     if (!weight(a->q_w) || !weight(a->k_w)) return al_fail(AL_ERR_INVALID, "paged_append: q_w and k_w must be f32 [128]");
     if (!a->norm && (a->q_w.data || a->k_w.data)) return al_fail(AL_ERR_INVALID, "paged_append: norm weights without the norm");
@@ -183,6 +185,7 @@ int make_params(const al_paged_append_args * a, AppendParams * out, int * mode, 
     p.q_out = (char *) a->q_out.data; p.o_nb1 = a->q_out.nb[1]; p.o_nb2 = a->q_out.nb[2];
     p.pos = (const int32_t *) a->pos.data;
     p.seq = (const int32_t *) a->seq.data;
+    p.cells = cells ? (const int32_t *) cells->data : nullptr;
     p.T = (int32_t) T; p.Hq = (int32_t) Hq; p.Hkv = (int32_t) Hkv; p.norm = a->norm != 0;
     p.yq = (int32_t) ((Hq + kRows - 1) / kRows);
     p.yk = (int32_t) ((Hkv + kRows - 1) / kRows);
@@ -192,13 +195,11 @@ int make_params(const al_paged_append_args * a, AppendParams * out, int * mode, 
     return AL_OK;
 }
 
-}  // namespace
-
-extern "C" int al_paged_append_f32(const al_paged_append_args * a) {
+int append(const al_paged_append_args * a, const al_tensor * cells) {
     AppendParams p;
     int mode = 0;
     bool empty = false;
-    int rc = make_params(a, &p, &mode, &empty);
+    int rc = make_params(a, cells, &p, &mode, &empty);
     if (rc != AL_OK || empty) return rc;
     rc = al_device_error_flag(&p.c.err);
     if (rc != AL_OK) return rc;
@@ -211,4 +212,12 @@ extern "C" int al_paged_append_f32(const al_paged_append_args * a) {
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "paged_append: launch");
+}
+
+}  // namespace
+
+extern "C" int al_paged_append_f32(const al_paged_append_args * a) { return append(a, nullptr); }
+
+extern "C" int al_paged_append_cells_f32(const al_paged_append_args * a, const al_tensor * cells) {
+    return cells ? append(a, cells) : al_fail(AL_ERR_INVALID, "paged_append: null cells");
 }

@@ -1,6 +1,7 @@
 /*
  * arclight_paged.h - C ABI of a paged f16 KV cache: appending a batch's keys
- * and values to it, and attention of each sequence's new tokens over it.
+ * and values to it, attention of each sequence's new tokens over it, and cells
+ * moved and copied in it.
  *
  * The ring of arclight_kv.h gives a sequence one range of cells, as the
  * reference's llm_kv_cache does. A server of many requests keeps their cells
@@ -144,6 +145,115 @@ int al_paged_fattn_f16(const al_paged_fattn_args * args);
 
 /* Bytes of a caller's workspace for these arguments; 0 for refused ones. */
 uint64_t al_paged_fattn_workspace_bytes(const al_paged_fattn_args * args);
+
+/*
+ * Which cells a token sees, where that is not all before it: layers with a
+ * window, and trees of drafted tokens.
+ *   window  positions that a token sees, its own among them (0: all)
+ *   first   cells at the beginning that stay visible behind a window
+ *   bits    i32 ne = [words, T, n_seq], nb0 = 4: bit u % 32 of word u / 32 of
+ *           token t is set where t sees new token u (its own is u = t); words
+ *           is (T + 31) / 32 or more, bits from counts[s] on are not looked at
+ *           (data NULL: those up to and with itself)
+ *   pos     i32 ne = [T, n_seq], nb0 = 4: the new tokens' positions (data NULL:
+ *           the cells that they lie in). With bits and a window they are
+ *           required, without bits refused.
+ * With n = lens[s], b = n - counts[s] and p the token's position (pos[t][s],
+ * without positions b + t), token t sees cell c of those before the new ones
+ * (c < b) if c > p - window or c < first, and new token u (cell b + u) if its
+ * bit is set (without bits: u <= t) and its position is above p - window or
+ * below first. Positions have to lie in b to n - 1 where a window needs them:
+ * the rows of others are recorded as errors and NaN.
+ * Pages are looked up for every new cell, for the first cells, and from the
+ * first window's beginning on: the lowest of the tokens', with bits that of a
+ * token at position b. What the table says of other pages is not looked at, so
+ * that they may have been freed.
+ */
+typedef struct al_paged_sees {
+    int32_t   window;
+    int32_t   first;
+    al_tensor bits;
+    al_tensor pos;
+} al_paged_sees;
+
+/* al_paged_fattn_f16 of what `sees` says instead of all cells before a token.
+ * Its cost goes by the cells that are seen, not by the sequences' lengths. */
+int al_paged_fattn_sees_f16(const al_paged_fattn_args * args, const al_paged_sees * sees);
+
+/* Bytes of a caller's workspace for these arguments; 0 for refused ones. */
+uint64_t al_paged_fattn_sees_workspace_bytes(const al_paged_fattn_args * args, const al_paged_sees * sees);
+
+/*
+ * al_paged_append_f32 of rows whose cells are not their positions, as those of
+ * a drafted tree are not: row t goes to cell cells[t] (i32 [T], device) of its
+ * sequence, rotated by pos[t], which may be any value then.
+ */
+int al_paged_append_cells_f32(const al_paged_append_args * args, const al_tensor * cells);
+
+/*
+ * Pools of all layers, for calls that move cells in every layer at once:
+ * k and v are host arrays of n_layers device pointers, each a pool of the
+ * shape and strides of k_pool and v_pool (whose own data is not used). The
+ * arrays are read before the call returns. n_layers is at most 65535.
+ */
+typedef struct al_paged_layers {
+    al_tensor k_pool;
+    al_tensor v_pool;
+    void * const * k;
+    void * const * v;
+    int32_t n_layers;
+} al_paged_layers;
+
+/*
+ * Arguments of al_paged_keep_f16: of the last counts[s] cells of each sequence
+ * those of an accepted path are kept, in the path's order, behind the cells
+ * before them: cell b + path[i] goes to cell b + i for i < kept[s], with
+ * b = lens[s] - counts[s].
+ *   table     i32 [max_pages, n_seq]
+ *   lens      i32 [n_seq], counts i32 [n_seq] (data NULL: T each)
+ *   path      i32 ne = [T, n_seq], nb0 = 4: rising, path[i] >= i
+ *   kept      i32 [n_seq], 0 to counts[s]
+ *   lens_out  i32 [n_seq], the new lengths b + kept[s] (data NULL: none). May
+ *             not overlap the other operands.
+ * A path[i] below i or at counts[s] or more, or a page outside the pool, is
+ * recorded as an error and the cell is not moved; a sequence whose length
+ * (0 to max_pages P), count (0 to T and the length) or kept is wrong is recorded,
+ * and its cells and length stay as they are. Pages that hold moved cells may not be
+ * shared with another sequence. T is at most 2^16, n_seq 65535.
+ */
+typedef struct al_paged_keep_args {
+    al_paged_layers layers;
+    al_tensor table;
+    al_tensor lens;
+    al_tensor counts;
+    al_tensor path;
+    al_tensor kept;
+    al_tensor lens_out;
+    void *    stream;
+} al_paged_keep_args;
+
+int al_paged_keep_f16(const al_paged_keep_args * args);
+
+/*
+ * Arguments of al_paged_copy_f16: page src[i] copied into page dst[i], or its
+ * first cells[i] cells, for n pairs: the last, partly filled page of a
+ * sequence that is forked, or pages brought together.
+ *   src, dst  i32 [n], device; a pair with a negative src or dst is left out
+ *   cells     i32 [n], device, 0 to P (data NULL: P)
+ * No page may be the dst of two pairs, nor dst of one and src of another (a
+ * page copied into itself is left alone). A page outside the pool and a count
+ * of cells that does not fit are recorded as errors, and the pair is left out.
+ * n is at most 65535.
+ */
+typedef struct al_paged_copy_args {
+    al_paged_layers layers;
+    al_tensor src;
+    al_tensor dst;
+    al_tensor cells;
+    void *    stream;
+} al_paged_copy_args;
+
+int al_paged_copy_f16(const al_paged_copy_args * args);
 
 #ifdef __cplusplus
 }
