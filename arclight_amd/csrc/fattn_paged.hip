@@ -55,240 +55,12 @@
 #include <algorithm>
 #include <cstring>
 
-#include "../../include/arclight_paged.h"
-#include "device_common.hpp"
-#include "kernel_args.hpp"
-#include "paged.hpp"
+#include "fattn_paged.hpp"
 #include "runtime.hpp"
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kTile = 32;                       // cells of a wave's step
-constexpr int kMinTiles = 4;                    // least tiles of a part: one for each wave
-constexpr int kWhole = 16;                      // sequences of up to so many tiles are not cut
-constexpr float kPScale = 16384.0f;             // probabilities: 2^14 p stays normal in f16 down to p = 2^-28
-
-struct PagedFattnParams {
-    PagedPools c;
-    const char * q;  int64_t q_nb1, q_nb2, q_nb3;       // token, head, sequence
-    char * dst;      int64_t d_nb1, d_nb2, d_nb3;       // head, token, sequence
-    const int32_t * lens;
-    const int32_t * counts;                             // or null
-    const float * sinks;                                // or null
-    int2 * info;                                        // [unit][n_seq]: first workgroup of the sequence, pieces
-    float * part;                                       // records [unit][workgroup][2]: rows x 128 sums, rows x {m, l}
-    int32_t T, G, Hkv, R, row_groups, row_tiles;        // row tiles of 16 in a group
-    uint32_t g_magic;                                   // ceil(2^32 / G) (0 for 1)
-    int32_t target, long_target;                        // workgroups of a unit (head, row group), those that long sequences use
-    int32_t row_waves;                                  // join: waves of a row
-    float scale, softcap;
-    static constexpr bool kSees = false;
-};
-
-// The same with a rule for what a token sees (al_paged_sees).
-struct PagedSeesParams : PagedFattnParams {
-    int32_t window, first;                              // window 0: none
-    const int32_t * bits;  int64_t b_nb1, b_nb2;        // or null; token, sequence, in words
-    const int32_t * pos;   int64_t p_nb1;               // or null; sequence
-    static constexpr bool kSees = true;
-};
-
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ int dpp_add(const int x) {
-    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
-}
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ int dpp_max(const int x) {                 // (of values that are not negative)
-    return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false));
-}
-// Sum of the lanes up to and with this one (DPP: within rows of 16, then the
-// rows' last lanes into those after them).
-__device__ __forceinline__ int wave_scan(int x) {
-    x = dpp_add<0x111, 0xf>(x);
-    x = dpp_add<0x112, 0xf>(x);
-    x = dpp_add<0x114, 0xf>(x);
-    x = dpp_add<0x118, 0xf>(x);
-    x = dpp_add<0x142, 0xa>(x);
-    x = dpp_add<0x143, 0xc>(x);
-    return x;
-}
-
-template <typename P>
-__device__ __forceinline__ int token_of(const P & p, const int r) {
-    return p.G == 1 ? r : (int) __umulhi((uint32_t) r, p.g_magic);
-}
-
-// What a row group has to do for a sequence, t0 and t1 its first and last token.
-struct SeqWork {
-    int len, count;                             // cells (within the table), new tokens
-    bool bad;
-    // cells that the group's last row sees, -1 if it has no row
-    __device__ __forceinline__ int limit(const int t0, const int t1) const {
-        return count > t0 ? min(max(len - count + 1 + min(t1, count - 1), 0), len) : -1;
-    }
-};
-
-template <typename P>
-__device__ __forceinline__ SeqWork seq_work(const P & p, const int len, const int count) {
-    SeqWork w;
-    w.len = min(max(len, 0), p.c.max_pages * p.c.page_size);
-    w.count = min(max(count, 0), p.T);
-    w.bad = len != w.len || count != w.count;
-    return w;
-}
-
-// The cells that tokens t0 to t1 of a sequence see, as a whole: those before
-// `limit` (-1: there are no such tokens), but none from p.first to `low`.
-struct Span {
-    int limit, low;
-    // Tiles without such a cell, and the first of them.
-    __device__ __forceinline__ int gap(const int first) const { return max(low / kTile - gap_at(first), 0); }
-    __device__ __forceinline__ int gap_at(const int first) const { return (min(first, low) + kTile - 1) / kTile; }
-};
-
-template <typename P>
-__device__ __forceinline__ Span span_of(const P & p, const SeqWork & w, const int t0, const int t1) {
-    Span a = {w.limit(t0, t1), 0};
-    if constexpr (P::kSees) {
-        if (p.bits && a.limit >= 0) a.limit = w.len;                   // of nodes each may see any
-        if (p.window) a.low = min(max(w.len - w.count + (p.bits ? 0 : t0) + 1 - p.window, 0), max(a.limit - 1, 0));
-    }
-    return a;
-}
-
-// Tiles of a sequence in the row of all tiles: one at least, so that rows that
-// see nothing are written too.
-template <typename P>
-__device__ __forceinline__ int tiles_of(const P & p, const Span a) {
-    int gap = 0;
-    if constexpr (P::kSees) gap = a.gap(p.first);
-    return a.limit < 0 ? 0 : max(1, (a.limit + kTile - 1) / kTile - gap);
-}
-
-// The first k of 8 cells, a bit each.
-__device__ __forceinline__ uint32_t upto8(const int k) { return (1u << min(max(k, 0), 8)) - 1; }
-// Of cells c0 to c0 + 7: those before `limit` that are not from `first` to `low`.
-__device__ __forceinline__ uint32_t span8(const int c0, const int limit, const int low, const int first) {
-    return upto8(limit - c0) & (~upto8(low - c0) | upto8(first - c0));
-}
-
-// Of nodes u0 to u0 + 7 (u0 may be negative) those that a token sees, whose
-// words are `words`, among the sequence's first `count`.
-__device__ __forceinline__ uint32_t nodes8(const int32_t * words, const int u0, const int count) {
-    if (u0 <= -8 || u0 >= count) return 0;
-    const int u = max(u0, 0), i = u >> 5, last = (count - 1) >> 5;
-    const uint64_t two = (uint32_t) words[i] | (uint64_t) (uint32_t) words[min(i + 1, last)] << 32;
-    return (uint32_t) (two >> (u & 31)) << (u - u0) & upto8(count - u0);
-}
-
-// The same, without those that lie before the token's window and are not among
-// the first cells either; pos: the nodes' positions.
-__device__ __forceinline__ uint32_t nodes8(const PagedSeesParams & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
-                                           const int low) {
-    uint32_t m = nodes8(words, u0, count);
-    if (p.window)
-        for (uint32_t rest = m; rest; rest &= rest - 1) {
-            const int at = pos[u0 + __builtin_ctz(rest)];
-            if (at < low && at >= p.first) m &= ~(rest & -rest);
-        }
-    return m;
-}
-
-// Whether token t of sequence s sees a cell at all.
-template <typename P>
-__device__ __forceinline__ bool sees_any(const P & p, const SeqWork & w, const int s, const int t) {
-    const int begin = w.len - w.count;
-    if constexpr (P::kSees) {
-        if (p.bits) {
-            const int32_t * words = p.bits + (int64_t) s * p.b_nb2 + (int64_t) t * p.b_nb1;
-            const int32_t * pos = p.pos + (int64_t) s * p.p_nb1;
-            const int low = p.window ? pos[t] + 1 - p.window : 0;
-            if (begin > 0 && (begin > low || p.first > 0)) return true;
-            for (int u = max(-begin, 0); u < w.count; u += 8)
-                if (nodes8(p, words, pos, u, w.count, low)) return true;
-            return false;
-        }
-    }
-    return begin + 1 + t > 0;
-}
-
-// S tiles cut into W parts, the first S % W of them one tile longer: the first
-// tile of a part, and the part that holds a tile.
-struct Parts {
-    int each, longer;
-    __device__ __forceinline__ Parts(const int S, const int W) : each(S / W), longer(S - S / W * W) {}
-    __device__ __forceinline__ int begin(const int w) const { return w * each + min(w, longer); }
-    __device__ __forceinline__ int of(const int x) const {
-        const int y = x - longer * (each + 1);
-        return y < 0 ? x / (each + 1) : longer + y / each;
-    }
-};
-
-// Sequences 64 b .. 64 b + 63, one to a lane.
-struct Block {
-    int len, count, tiles, upto;                // as read; tiles, and those of all sequences up to this one
-    template <typename P>
-    __device__ __forceinline__ void load(const P & p, const int b, const int lane, const int t0, const int t1) {
-        const int s = 64 * b + lane;
-        const bool in = s < p.c.n_seq;
-        len = in ? p.lens[s] : 0;
-        count = !in ? 0 : p.counts ? p.counts[s] : p.T;
-        tiles = in ? tiles_of(p, span_of(p, seq_work(p, len, count), t0, t1)) : 0;
-        upto = wave_scan(tiles);
-    }
-    // A negative count makes an empty slot, which no workgroup comes to.
-    __device__ __forceinline__ void report(const PagedFattnParams & p) const {
-        if (count < 0) paged_error(p.c, kPagedBadCount, count);
-    }
-    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
-    __device__ __forceinline__ int active() const { return __builtin_popcountll(__ballot(tiles > 0)); }
-    __device__ __forceinline__ int longest() const {
-        int x = tiles;
-        x = dpp_max<0x111, 0xf>(x);
-        x = dpp_max<0x112, 0xf>(x);
-        x = dpp_max<0x114, 0xf>(x);
-        x = dpp_max<0x118, 0xf>(x);
-        x = dpp_max<0x142, 0xa>(x);
-        x = dpp_max<0x143, 0xc>(x);
-        return __builtin_amdgcn_readlane(x, 63);
-    }
-};
-
-template <typename P>
-__device__ __forceinline__ char * record(const P & p, const int unit, const int wg, const int slot) {
-    return (char *) p.part + (((int64_t) unit * p.target + wg) * 2 + slot) * (16 * p.row_tiles) * 130 * 4;
-}
-
-// e^(a - b) for running maxima a <= b, 1 where they are equal (both -inf too).
-__device__ __forceinline__ float grow(const float a, const float b) { return a == b ? 1.0f : exp_fast(a - b); }
-
-// Factor of a row's sums, with the sink as one more logit without a value: 0
-// for a row that sees nothing, NaN where all logits are -inf.
-// p: the arguments, a: the same, to be loaded where they are used.
-template <typename P, typename A>
-__device__ __forceinline__ float row_factor(const P & p, const A & a, const SeqWork & w, const int s, const int t, const float M, float L,
-                                            const int head) {
-    L *= 1.0f / kPScale;
-    float up = 1.0f / kPScale;
-    if (a.sinks) {
-        const float sink = a.sinks[head], top = fmaxf(M, sink);
-        const float e = grow(M, top);
-        up *= e;
-        L = L * e + (sink == -AL_INF ? 0.0f : grow(sink, top));
-    }
-    return L == 0.0f ? sees_any(p, w, s, t) ? __builtin_nanf("") : 0.0f : up / L;
-}
-
-// The kernel's arguments as memory, to be loaded where they are used: held in
-// scalar registers from the start, those that only a piece's beginning and end
-// use displace what the loop over the cells needs.
-template <typename P>
-__device__ __forceinline__ const __attribute__((address_space(4))) P & arguments() {
-    auto a = (const __attribute__((address_space(4))) P *) __builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(a));
-    return *a;
-}
+using namespace paged_fattn;
 
 // ROWT: row tiles of 16 query rows that the waves take side by side (1, 2 or
 // 4); the tiles of cells go round the waves of a row tile. CAP: logits
@@ -314,51 +86,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
     // this workgroup's part of all tiles
     const int n_blocks = (p.c.n_seq + 63) / 64;
     Block b;
-    b.load(p, 0, lane, t0, t1);
-    const bool first_wave = blockIdx.x == 0 && wave == 0;
-    if (first_wave) b.report(p);
-    int S = b.total(), active = b.active(), longest = b.longest(), block = 0, before = 0;
-    for (int i = 1; i < n_blocks; ++i) {
-        Block x;
-        x.load(p, i, lane, t0, t1);
-        if (first_wave) x.report(p);
-        S += x.total();
-        active += x.active();
-        longest = max(longest, x.longest());
-    }
-    // Several sequences of up to kWhole tiles each are left whole, one or some to
-    // a workgroup: equal parts cut them at places of their own, and a second
-    // piece costs a workgroup more than the rounds that the cut saves (us, cut
-    // and whole: 4 sequences of up to 200 cells 13.4, 10.1, 64 of 100 16.4, 11.5,
-    // 10 of 500 14.1, 12.3; whole up to 32 tiles: 128 of 700 56.4, 60.2). Else
-    // kMinTiles a workgroup at least, or a sequence; p.target workgroups for
-    // sequences of up to 16 tiles on average, p.long_target for longer ones.
-    const bool cut = longest > kWhole || active == 1;
-    const int W = cut ? min(S > 16 * active ? p.long_target : p.target, max((S + kMinTiles - 1) / kMinTiles, active)) : min(p.target, active);
-    if (wg >= W) return;
-    const Parts parts(S, W);
-    int at = parts.begin(wg), stop = parts.begin(wg + 1);
-    if (!cut) {
-        const Parts seqs(active, W);
-        auto tile_of = [&](int i) {                                    // first tile of the i-th sequence that has any
-            Block x = b;
-            for (int k = 0, tiles = 0;;) {
-                const uint64_t mask = __ballot(x.tiles > 0);
-                const int have = __builtin_popcountll(mask);
-                if (i < have) {
-                    const int nth = __builtin_amdgcn_mbcnt_hi((uint32_t) (mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) mask, 0));
-                    const int l = __builtin_ctzll(__ballot(x.tiles > 0 && nth == i));
-                    return tiles + __builtin_amdgcn_readlane(x.upto, l) - __builtin_amdgcn_readlane(x.tiles, l);
-                }
-                i -= have;
-                tiles += x.total();
-                if (++k == n_blocks) return tiles;
-                x.load(p, k, lane, t0, t1);
-            }
-        };
-        at = tile_of(seqs.begin(wg));
-        stop = tile_of(seqs.begin(wg + 1));
-    }
+    MyPart part;
+    if (!find_part(p, wg, lane, t0, t1, blockIdx.x == 0 && wave == 0, b, part)) return;
+    const Parts & parts = part.parts;
+    int at = part.at, block = 0, before = 0;
+    const int stop = part.stop;
 
     while (at < stop) {
         // the sequence that holds tile `at`
@@ -394,8 +126,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         if constexpr (P::kSees) {
             const Span all = span_of(p, w, t0, t1);
             first_cells = p.first;
-            gap = all.gap(p.first);
-            gap_at = all.gap_at(p.first);
+            gap = all.gap(p);
+            gap_at = all.gap_at(p);
             if (p.bits) least = max(begin, 0);
             if (p.window) low_last = (p.bits ? w.len : begin + 1 + min(wt1, w.count - 1)) - p.window;
         }
@@ -482,7 +214,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         // Everything that the first tile needs goes out before anything is
         // computed: pages, query rows, then K and V (a wave without a tile
         // loads another wave's and uses none of it).
-        const int wave_end = min(end, seen > 0 ? (seen + kTile - 1) / kTile - gap : 0);
+        const int wave_end = min(end, seen > 0 ? (seen + P::kTile - 1) / P::kTile - gap : 0);
         const bool has = first + cw < wave_end;
         int tile = has ? first + cw : max(wave_end - 1, 0);
         const Where here = look_up(tile);
@@ -554,11 +286,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         half8 p_hi, p_lo;
         // Whether some row does not see all of a tile.
         auto partly = [&](const int tile) {
-            return (tile + 1) * kTile > least || (P::kSees && tile * kTile < low_last && (tile + 1) * kTile > first_cells);
+            return (tile + 1) * P::kTile > least || (P::kSees && tile * P::kTile < low_last && (tile + 1) * P::kTile > first_cells);
         };
         // Probabilities of the tile against the rows' running maxima.
         auto softmax = [&](const int tile) {
-            const int c0 = tile * kTile + 8 * g;
+            const int c0 = tile * P::kTile + 8 * g;
             const bool masked = partly(tile);
             uint32_t sees = 0xffu;
             if constexpr (P::kSees) {
@@ -605,8 +337,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         // are not finite of cells that some row does not see; the rows that do
         // see one get NaN in its dim, found by a product of ones.
         auto product = [&](const int tile) {
-            const int c0 = tile * kTile + 8 * g;
-            bool differ = least < seen && (tile + 1) * kTile > least;   // (one token: never)
+            const int c0 = tile * P::kTile + 8 * g;
+            bool differ = least < seen && (tile + 1) * P::kTile > least;   // (one token: never)
             uint32_t some = 0xffu, all = upto8(least - c0);          // cells that some, that all rows see
             if constexpr (P::kSees) {
                 if (partly(tile)) {
@@ -617,7 +349,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
                     for (int i = 0; i < 8; ++i)
                         if (!(some >> i & 1)) v[i] = u32x4{0, 0, 0, 0};
                 }
-            } else if ((tile + 1) * kTile > seen) {
+            } else if ((tile + 1) * P::kTile > seen) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (c0 + i >= seen) v[i] = u32x4{0, 0, 0, 0};
@@ -693,7 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             float M = m;
 #pragma unroll
             for (int i = 0; i < kCellWaves; ++i) M = fmaxf(M, ml_lds[rt * kCellWaves + i][n][0]);
-            const float f = grow(m, M);
+            const float f = grow<P>(m, M);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 *(float4 *) &o_lds[wave][n][8 * (4 * g + i)] = float4{acc[0][i] * f, acc[1][i] * f, acc[2][i] * f, acc[3][i] * f};
@@ -713,7 +445,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             for (int i = 1; i < kCellWaves; ++i) M = fmaxf(M, ml_lds[w0 + i][rr][0]);
 #pragma unroll
             for (int i = 0; i < kCellWaves; ++i) {
-                L += ml_lds[w0 + i][rr][1] * grow(ml_lds[w0 + i][rr][0], M);
+                L += ml_lds[w0 + i][rr][1] * grow<P>(ml_lds[w0 + i][rr][0], M);
 #pragma unroll
                 for (int d = 0; d < 8; ++d) o[d] += o_lds[w0 + i][rr][dim + d];
             }
@@ -734,106 +466,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
     }
 }
 
-// A row of the group, joined from the pieces of a sequence that has several.
-// p.row_waves waves (1 or kWaves) take it, the halves of a wave every second
-// piece, 4 dims to a lane; all loads of 8 of a half's pieces are in flight
-// together.
-template <typename P>
-__device__ __forceinline__ void join_row(const P & p, const int2 info, const int unit, const int seq, const int count,
-                                         const int row, float (*o_lds)[132]) {
-    const int lane = threadIdx.x & 63, half = lane >> 5, d4 = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rows = 16 * p.row_tiles, row_waves = p.row_waves;
-    const int h = unit % p.Hkv, gr = unit / p.Hkv * rows + row, t = token_of(p, min(gr, p.R - 1));
-    const bool mine = gr < p.R && t < min(count, p.T);
-    float M = -AL_INF, L = 0.0f;
-    float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (mine) {
-        for (int i0 = row_waves == 1 ? 0 : 16 * wave; i0 < info.y; i0 += 16 * row_waves) {
-            float2 ml[8];
-            float4 x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int c = min(i0 + 2 * i + half, info.y - 1);
-                const char * rec = record(p, unit, info.x + c, c == 0 ? 1 : 0);
-                ml[i] = *(const float2 *) ((const float *) rec + rows * 128 + row * 2);
-                x[i] = *(const float4 *) ((const float *) rec + row * 128 + 4 * d4);
-            }
-            asm volatile("" ::: "memory");
-            float top = M;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i0 + 2 * i + half < info.y) top = fmaxf(top, ml[i].x);
-            const float f = grow(M, top);
-            L *= f; o.x *= f; o.y *= f; o.z *= f; o.w *= f;
-            M = top;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i0 + 2 * i + half < info.y) {
-                    const float e = grow(ml[i].x, M);
-                    L += ml[i].y * e;
-                    o.x += x[i].x * e; o.y += x[i].y * e; o.z += x[i].z * e; o.w += x[i].w * e;
-                }
-        }
-    }
-    // the wave's halves, then the row's waves
-    {
-        const float M2 = __shfl_xor(M, 32), L2 = __shfl_xor(L, 32);
-        const float4 o2 = {__shfl_xor(o.x, 32), __shfl_xor(o.y, 32), __shfl_xor(o.z, 32), __shfl_xor(o.w, 32)};
-        const float top = fmaxf(M, M2), f = grow(M, top), f2 = grow(M2, top);
-        M = top;
-        L = half ? L2 * f2 + L * f : L * f + L2 * f2;
-        o = half ? float4{o2.x * f2 + o.x * f, o2.y * f2 + o.y * f, o2.z * f2 + o.z * f, o2.w * f2 + o.w * f}
-                 : float4{o.x * f + o2.x * f2, o.y * f + o2.y * f2, o.z * f + o2.z * f2, o.w * f + o2.w * f2};
-    }
-    if (row_waves > 1) {
-        if (half == 0) {
-            *(float4 *) &o_lds[wave][4 * d4] = o;
-            if (d4 == 0) o_lds[wave][128] = M, o_lds[wave][129] = L;
-        }
-        __syncthreads();
-        if (wave) return;
-        float top = M;
-#pragma unroll
-        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, o_lds[i][128]);
-        L = 0.0f;
-        o = float4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            const float f = grow(o_lds[i][128], top);
-            const float4 x = *(const float4 *) &o_lds[i][4 * d4];
-            L += o_lds[i][129] * f;
-            o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
-        }
-        M = top;
-    }
-    if (!mine || half) return;
-    const int head = h * p.G + gr - t * p.G;
-    const SeqWork w = seq_work(p, p.lens[seq], count);
-    const float f = row_factor(p, p, w, seq, t, M, L, head);
-    *(float4 *) ((float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) head * p.d_nb1) + 4 * d4) =
-        float4{o.x * f, o.y * f, o.z * f, o.w * f};
-}
-
-// Workgroups (rows, sequence, unit); few of them where most have nothing to join.
-template <typename P>
-__global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(const P p) {
-    __shared__ __attribute__((aligned(16))) float o_lds[kWaves][132];
-    prefetch_params(p);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rows = min(16 * p.row_tiles, p.R), seq = blockIdx.y, unit = blockIdx.z;
-    const int2 info = p.info[(int64_t) unit * p.c.n_seq + seq];
-    const int count = p.counts ? p.counts[seq] : p.T;
-    // (no row of the group: nothing was written to info)
-    if (min(count, p.T) <= token_of(p, unit / p.Hkv * (16 * p.row_tiles)) || info.y < 2) return;
-    if (p.row_waves > 1) join_row(p, info, unit, seq, count, blockIdx.x, o_lds);
-    else
-        for (int row = blockIdx.x * kWaves + wave; row < rows; row += gridDim.x * kWaves) join_row(p, info, unit, seq, count, row, o_lds);
-}
-
 struct Plan {
     PagedSeesParams p;                                  // (without a rule: its PagedFattnParams)
     bool empty = false;
+    bool many = false;                                  // by the kernel of many query rows
     size_t info_bytes = 0, bytes = 0;                   // of the info, of it and the records
 };
 
@@ -845,7 +481,7 @@ bool aligned16(const al_tensor & t, int from) {
 
 // The rule's operands, checked, in p; *tiles: at most so many of a sequence's
 // tiles are seen.
-int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n_seq, int64_t * tiles) {
+int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n_seq, int64_t tile, int64_t * tiles) {
     if (r->window < 0 || r->first < 0)
         return al_fail(AL_ERR_INVALID, "paged_fattn: a window of %d cells and %d first ones", r->window, r->first);
     // (positions are below 2^30: a longer window is all of them)
@@ -869,8 +505,14 @@ int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n
         return al_fail(AL_ERR_INVALID, "paged_fattn: bits and a window need positions");
     }
     if (p->window)
-        *tiles = std::min(*tiles, ((int64_t) p->first + kTile - 1) / kTile + ((int64_t) p->window + T + kTile - 1) / kTile + 1);
+        *tiles = std::min(*tiles, ((int64_t) p->first + tile - 1) / tile + ((int64_t) p->window + T + tile - 1) / tile + 1);
     return AL_OK;
+}
+
+// Whether a call with a rule goes to the kernel of many query rows.
+bool many_rows(const PagedFattnParams & p) {
+    constexpr int64_t kStride = 1 << 29;                 // (its loads' offsets within 4 cells have 32 bits)
+    return p.R > 64 && p.c.k_nb1 < kStride && p.c.v_nb1 < kStride;
 }
 
 int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_cu, Plan * out) {
@@ -911,13 +553,16 @@ int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_c
     p.T = (int32_t) T; p.G = (int32_t) (Hq / Hkv); p.Hkv = (int32_t) Hkv;
     p.R = p.T * p.G;
     p.g_magic = p.G > 1 ? (uint32_t) (((1ull << 32) + (uint64_t) p.G - 1) / (uint64_t) p.G) : 0u;
-    p.row_tiles = p.R <= 16 ? 1 : p.R <= 32 ? 2 : 4;
+    pl.many = rule && many_rows(p);
+    p.row_tiles = pl.many ? PagedRowsParams::kRows / 16 : p.R <= 16 ? 1 : p.R <= 32 ? 2 : 4;
     const int rows = 16 * p.row_tiles;
     p.row_groups = (p.R + rows - 1) / rows;
     const int64_t units = (int64_t) p.row_groups * Hkv;
     if (units > 65535) return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
-    int64_t tiles = std::max<int64_t>(1, ((int64_t) p.c.max_pages * p.c.page_size + kTile - 1) / kTile);
-    if (rule) rc = make_rule(rule, &p, T, n_seq, &tiles);
+    const int tile = pl.many ? PagedRowsParams::kTile : PagedFattnParams::kTile;
+    const int min_tiles = pl.many ? PagedRowsParams::kMinTiles : PagedFattnParams::kMinTiles;
+    int64_t tiles = std::max<int64_t>(1, ((int64_t) p.c.max_pages * p.c.page_size + tile - 1) / tile);
+    if (rule) rc = make_rule(rule, &p, T, n_seq, tile, &tiles);
     if (rc != AL_OK) return rc;
     const int64_t most = n_seq * tiles;                                                                                 // tiles there can be
     if (most > INT32_MAX) return al_fail(AL_ERR_UNSUPPORTED, "paged_fattn: sizes out of range");
@@ -928,7 +573,7 @@ int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_c
     // sequences 48.5 / 47.1 / 50.0), and for many short sequences, whose ends
     // are not hidden (96 to 300 cells 30.8 / 24.9, 128 to 700 57.2 / 57.2).
     const int64_t per_cu = n_cu / std::max<int64_t>(1, units);
-    const int64_t useful = std::max(n_seq, (most + kMinTiles - 1) / kMinTiles);
+    const int64_t useful = std::max(n_seq, (most + min_tiles - 1) / min_tiles);
     p.target = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * n_cu / std::max<int64_t>(1, units), useful));
     p.long_target = p.row_tiles == 1 ? (int32_t) std::max<int64_t>(1, std::min<int64_t>(per_cu, p.target)) : p.target;
     // few sequences have many pieces each
@@ -956,14 +601,7 @@ hipError_t launch(const P & p, hipStream_t st) {
         default: launch<4>(p, st); break;
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.target == 1) return e;                    // one workgroup a unit: no pieces
-    const int rows = std::min(16 * p.row_tiles, p.R);
-    // (all rows side by side: 98 sequences of one tile, 56 rows, 24.6 us in all instead of 20.7)
-    const int64_t pairs = (int64_t) p.c.n_seq * p.row_groups * p.Hkv;
-    const int side = (int) std::max<int64_t>(1, std::min<int64_t>((rows + kWaves - 1) / kWaves, 2048 / pairs));
-    const dim3 grid((unsigned) (p.row_waves == 1 ? side : rows), (unsigned) p.c.n_seq, (unsigned) (p.row_groups * p.Hkv));
-    hipLaunchKernelGGL((paged_join_kernel<P>), grid, dim3(64 * kWaves), 0, st, p);
-    return hipGetLastError();
+    return e == hipSuccess ? launch_join(p, st) : e;
 }
 
 }  // namespace
@@ -1000,7 +638,10 @@ int paged_pools(const char * what, const al_tensor * k, const al_tensor * v, con
 
 namespace {
 
+bool leaves_nothing_out(const al_paged_sees & r) { return r.window == 0 && r.first >= 0 && !r.bits.data && !r.pos.data; }
+
 uint64_t workspace_bytes(const al_paged_fattn_args * a, const al_paged_sees * rule) {
+    if (rule && leaves_nothing_out(*rule)) rule = nullptr;
     int n_cu = 0;
     Plan pl;
     if (al_device_cu_count(&n_cu) != AL_OK || make_plan(a, rule, n_cu, &pl) != AL_OK) return 0;
@@ -1008,6 +649,7 @@ uint64_t workspace_bytes(const al_paged_fattn_args * a, const al_paged_sees * ru
 }
 
 int attend(const al_paged_fattn_args * a, const al_paged_sees * rule) {
+    if (rule && leaves_nothing_out(*rule)) rule = nullptr;
     // the arguments first: refusals need no device
     Plan pl;
     int rc = make_plan(a, rule, 1, &pl);
@@ -1021,8 +663,14 @@ int attend(const al_paged_fattn_args * a, const al_paged_sees * rule) {
     if (rc != AL_OK) return rc;
     pl.p.part = (float *) ((char *) pl.p.info + pl.info_bytes);
     const hipStream_t st = (hipStream_t) a->stream;
-    // (a rule that leaves nothing out is none)
-    const hipError_t e = pl.p.window || pl.p.bits ? launch(pl.p, st) : launch<PagedFattnParams>(pl.p, st);
+    hipError_t e;
+    if (pl.many) {
+        PagedRowsParams p;
+        static_cast<PagedSeesParams &>(p) = pl.p;
+        e = launch_rows(p, st);
+    } else {
+        e = rule ? launch(pl.p, st) : launch<PagedFattnParams>(pl.p, st);
+    }
     return e == hipSuccess ? AL_OK : al_hip_fail(e, "paged_fattn: launch");
 }
 
