@@ -453,7 +453,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             float f = 1.0f;
             if (whole) {
                 const int head = h * ep.G + gr - tok * ep.G;
-                f = row_factor(p, ep, w, seq, tok, M, L, head);
+                f = row_factor<P>(ep, w, seq, tok, M, L, head);
                 d = (float *) (ep.dst + (int64_t) seq * ep.d_nb3 + (int64_t) tok * ep.d_nb2 + (int64_t) head * ep.d_nb1) + dim;
             } else {
                 d = (float *) rec + row * 128 + dim;
@@ -511,8 +511,9 @@ int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n
 
 // Whether a call with a rule goes to the kernel of many query rows.
 bool many_rows(const PagedFattnParams & p) {
-    constexpr int64_t kStride = 1 << 29;                 // (its loads' offsets within 4 cells have 32 bits)
-    return p.R > 64 && p.c.k_nb1 < kStride && p.c.v_nb1 < kStride;
+    // (it counts bytes within a page, and from page to page, in 32 bits)
+    constexpr int64_t kMost = 0xffffffffll;
+    return p.R > 64 && p.c.page_size * p.c.k_nb1 <= kMost && p.c.page_size * p.c.v_nb1 <= kMost && p.c.k_nb3 <= kMost && p.c.v_nb3 <= kMost;
 }
 
 int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_cu, Plan * out) {

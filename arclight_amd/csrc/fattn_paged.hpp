@@ -78,8 +78,8 @@ __device__ __forceinline__ int wave_scan(int x) {
     return x;
 }
 
-template <typename P>
-__device__ __forceinline__ int token_of(const P & p, const int r) {
+template <typename A>
+__device__ __forceinline__ int token_of(const A & p, const int r) {
     return p.G == 1 ? r : (int) __umulhi((uint32_t) r, p.g_magic);
 }
 
@@ -150,7 +150,8 @@ __device__ __forceinline__ uint32_t nodes8(const int32_t * words, const int u0, 
 
 // The same, without those that lie before the token's window and are not among
 // the first cells either; pos: the nodes' positions.
-__device__ __forceinline__ uint32_t nodes8(const PagedSeesParams & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
+template <typename A>
+__device__ __forceinline__ uint32_t nodes8(const A & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
                                            const int low) {
     uint32_t m = nodes8(words, u0, count);
     if (p.window)
@@ -162,8 +163,8 @@ __device__ __forceinline__ uint32_t nodes8(const PagedSeesParams & p, const int3
 }
 
 // Whether token t of sequence s sees a cell at all.
-template <typename P>
-__device__ __forceinline__ bool sees_any(const P & p, const SeqWork & w, const int s, const int t) {
+template <typename P, typename A>
+__device__ __forceinline__ bool sees_any(const A & p, const SeqWork & w, const int s, const int t) {
     const int begin = w.len - w.count;
     if constexpr (P::kSees) {
         if (p.bits) {
@@ -221,8 +222,8 @@ struct Block {
     }
 };
 
-template <typename P>
-__device__ __forceinline__ char * record(const P & p, const int unit, const int wg, const int slot) {
+template <typename A>
+__device__ __forceinline__ char * record(const A & p, const int unit, const int wg, const int slot) {
     return (char *) p.part + (((int64_t) unit * p.target + wg) * 2 + slot) * (16 * p.row_tiles) * 130 * 4;
 }
 
@@ -234,9 +235,9 @@ __device__ __forceinline__ float grow(const float a, const float b) {
 
 // Factor of a row's sums, with the sink as one more logit without a value: 0
 // for a row that sees nothing, NaN where all logits are -inf.
-// p: the arguments, a: the same, to be loaded where they are used.
+// a: the arguments, of type P.
 template <typename P, typename A>
-__device__ __forceinline__ float row_factor(const P & p, const A & a, const SeqWork & w, const int s, const int t, const float M, float L,
+__device__ __forceinline__ float row_factor(const A & a, const SeqWork & w, const int s, const int t, const float M, float L,
                                             const int head) {
     float up = P::kLog2 ? 1.0f : 1.0f / kPScale;
     L *= up;
@@ -246,7 +247,7 @@ __device__ __forceinline__ float row_factor(const P & p, const A & a, const SeqW
         up *= e;
         L = L * e + (sink == -AL_INF ? 0.0f : grow<P>(sink, top));
     }
-    return L == 0.0f ? sees_any(p, w, s, t) ? __builtin_nanf("") : 0.0f : up / L;
+    return L == 0.0f ? sees_any<P>(a, w, s, t) ? __builtin_nanf("") : 0.0f : up / L;
 }
 
 // The kernel's arguments as memory, to be loaded where they are used: held in
@@ -394,7 +395,7 @@ __device__ __forceinline__ void join_row(const P & p, const int2 info, const int
     if (!mine || half) return;
     const int head = h * p.G + gr - t * p.G;
     const SeqWork w = seq_work(p, p.lens[seq], count);
-    const float f = row_factor(p, p, w, seq, t, M, L, head);
+    const float f = row_factor<P>(p, w, seq, t, M, L, head);
     *(float4 *) ((float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) head * p.d_nb1) + 4 * d4) =
         float4{o.x * f, o.y * f, o.z * f, o.w * f};
 }

@@ -43,16 +43,30 @@ namespace paged_fattn {
 
 namespace {
 
-using fattn::dma16;
 using fattn::half4;
 using fattn::int4v;
 using fattn::lds_addr;
-using fattn::lds_read_tr16;
+using fattn_prefill::float2v;
 using fattn_prefill::floatx16;
+using fattn_prefill::half2v;
 using fattn_prefill::mfma32;
 using fattn_prefill::pair_max;
 using fattn_prefill::pair_sum;
 using fattn_prefill::wait_vm;
+
+// LDS by address.
+template <typename T>
+__device__ __forceinline__ T lds_at(const uint32_t at) { return *(const __attribute__((address_space(3))) T *) (uintptr_t) at; }
+__device__ __forceinline__ half4 read_tr16(const uint32_t at) {
+    return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((fattn::lds_short4v *) (uintptr_t) at));
+}
+// x - (a half of) hi
+__device__ __forceinline__ float rest(const half2v hi, const int half, const float x) {
+    float y;
+    if (half) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(hi), "v"(x));
+    else      asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(y) : "v"(hi), "v"(x));
+    return y;
+}
 
 constexpr int kTileBytes = PagedRowsParams::kTile * 256;
 constexpr float kBelow = 8.0f, kOutgrown = 14.0f;        // log2: the reference below the maximum, a score that moves it
@@ -63,7 +77,8 @@ __device__ __forceinline__ uint64_t upto64(const int k) { return k <= 0 ? 0ull :
 __device__ __forceinline__ uint64_t span64(const int c0, const int limit, const int low, const int first) {
     return upto64(limit - c0) & (~upto64(low - c0) | upto64(first - c0));
 }
-__device__ __forceinline__ uint64_t nodes64(const PagedSeesParams & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
+template <typename A>
+__device__ __forceinline__ uint64_t nodes64(const A & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
                                             const int low) {
     if (u0 <= -64 || u0 >= count) return 0;
     const int u = max(u0, 0), i = u >> 5, last = (count - 1) >> 5, sh = u & 31;
@@ -79,11 +94,21 @@ __device__ __forceinline__ uint64_t nodes64(const PagedSeesParams & p, const int
     return m;
 }
 
-// A descriptor of `bytes` from memory that the wave addresses alike in every lane.
-__device__ __forceinline__ int4v uniform_desc(const char * base, const uint32_t bytes) {
-    const uint64_t a = (uint64_t) base;
-    return int4v{__builtin_amdgcn_readfirstlane((int) (uint32_t) a), __builtin_amdgcn_readfirstlane((int) (uint32_t) (a >> 32)),
-                 __builtin_amdgcn_readfirstlane((int) bytes), 0x00020000};
+// 16 bytes a lane from page + at + lane_at into LDS at `to` + 16 * lane, without
+// passing registers. page, at and to are the wave's. (M0 carries the LDS address;
+// nothing else in this kernel uses it.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_lds(const int4v page, const uint32_t at, const uint32_t lane_at, const uint32_t to) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 :
+                 : "v"(lane_at), "s"(page), "s"(at), "s"(to)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ int4v page_desc(const char * head, const uint32_t page, const uint32_t nb3) {
+    const uint64_t a = (uint64_t) head + (uint64_t) page * nb3;
+    return int4v{(int) (uint32_t) a, (int) (uint32_t) (a >> 32), -1, 0x00020000};
 }
 
 // CAP: logits soft-capped.
@@ -113,7 +138,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
     if (tid < 128) odd[tid] = 0;
     if (tid == 0) any_odd = any_bad = 0;
 
-    const uint32_t k_nb1 = (uint32_t) p.c.k_nb1, v_nb1 = (uint32_t) p.c.v_nb1, lds0 = lds_addr(lds);
+    const uint32_t k_nb1 = (uint32_t) p.c.k_nb1, k_nb3 = (uint32_t) p.c.k_nb3, v_nb1 = (uint32_t) p.c.v_nb1, v_nb3 = (uint32_t) p.c.v_nb3, lds0 = lds_addr(lds);
     // this lane's offset within 4 cells of K (their place among 16 cells) and of V
     uint32_t k_lane[4];
 #pragma unroll
@@ -122,9 +147,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
     const char * k_head = p.c.k + (int64_t) head * p.c.k_nb2;
     const char * v_head = p.c.v + (int64_t) head * p.c.v_nb2;
     // operand reads: K of cell lr, V as 4 x 16 pieces
-    const int k_at = lr * 256 + ((h ^ (lr & 15)) << 4);
+    // (the permutation's bits are flipped in the address: a tile begins at a
+    // multiple of its size)
     const int s16 = lane & 15, v_sw = s16 >> 2;
-    const int v_at = (4 * h + v_sw) * 256 + ((2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1)) << 4) + (s16 & 1) * 8;
+    const uint32_t k_at = lds0 + lr * 256 + ((h ^ (lr & 15)) << 4);
+    const uint32_t v_at = lds0 + kTileBytes + (((4 * h + v_sw) * 256 + ((2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1)) << 4) + (s16 & 1) * 8) ^ (64 * v_sw));
 
     while (at < stop) {
         // the sequence that holds tile `at`
@@ -142,8 +169,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         const int first = at - base, end = min(tiles, stop - base);
         at = base + end;
         const bool whole = first == 0 && end == tiles;
+        const auto & ap = arguments<P>();
         if (tid == 0) {
-            if (first == 0) p.info[(int64_t) unit * p.c.n_seq + seq] = int2{wg, whole ? 1 : part.parts.of(base + tiles - 1) - wg + 1};
+            if (first == 0) ap.info[(int64_t) unit * ap.c.n_seq + seq] = int2{wg, whole ? 1 : part.parts.of(base + tiles - 1) - wg + 1};
             if (w.bad) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         const int begin = w.len - w.count;
@@ -151,73 +179,79 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         const Span group = span_of(p, w, t0, t1), mine = span_of(p, w, wt0, wt1);
         const int gap = group.gap(p), gap_at = group.gap_at(p);
         auto tile_at = [&](const int i) { return i >= gap_at ? i + gap : i; };
+        // Tiles that some row does not see all of: from `from` on, and from `a` to `b`.
+        struct Edges {
+            int from, a, b;
+            __device__ __forceinline__ bool has(const int tile) const { return tile >= from || (tile >= a && tile < b); }
+        };
+        auto edges_of = [&](const int least, const int low) {
+            return Edges{least / P::kTile, p.first / P::kTile, (max(low, 0) + P::kTile - 1) / P::kTile};
+        };
+        // cells that all rows from a token on see, and the last window's beginning
         auto least_of = [&](const int first_token) { return p.bits ? max(begin, 0) : max(begin + 1 + first_token, 0); };
         auto low_of = [&](const int last_token) {
             return p.window ? (p.bits ? w.len : begin + 1 + min(last_token, w.count - 1)) - p.window : 0;
         };
-        auto partly = [&](const int tile, const int least, const int low) {
-            return (tile + 1) * P::kTile > least || (tile * P::kTile < low && (tile + 1) * P::kTile > p.first);
-        };
-        const int least = least_of(t0), low_last = low_of(t1), my_least = least_of(wt0), my_low_last = low_of(wt1);
+        const Edges edges = edges_of(least_of(t0), low_of(t1)), my_edges = edges_of(least_of(wt0), low_of(wt1));
         const int tiles_end = group.limit > 0 ? end : first;             // (nothing is seen: no tile)
 
-        // Pages of this wave's 16 cells of a tile, two groups of 8, those past
-        // the last that the group sees taken from that one, those before the
+        // Where this wave's 16 cells of 32 tiles lie, two groups of 8 to a tile:
+        // lane 2 (i % 32) + e that of group e of tile i. Groups past the last
+        // that the group of rows sees are taken from that one, those before the
         // first window from its.
         struct Where {
-            int page[2], cell[2];
+            uint32_t page, k, v;                                         // bytes in the page
         };
-        const int32_t * table = p.c.table + (int64_t) seq * p.c.t_nb1;
-        const int last_group = max(group.limit - 1, 0) / 8, from = (p.first + 7) >> 3, low_group = group.low >> 3;
         bool bad = false;
-        auto look_up = [&](const int i) {
-            Where a;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                int g = min(tile_at(i) * 8 + 2 * wave + e, last_group);
-                if (g >= from) g = max(g, low_group);
-                const int pg = (int) page_of_group(p.c, (uint32_t) g);
-                a.page[e] = ld_uniform(table + pg);
-                a.cell[e] = (g - pg * p.c.groups) * 8;
-            }
-            return a;
+        auto look_up = [&](const int i) {                                // of tiles i / 32 * 32 on
+            const int last_group = max(group.limit - 1, 0) / 8, from = (ap.first + 7) >> 3;
+            const int of = min(i / 32 * 32 + (lane >> 1), tiles_end - 1);
+            int g = min((of >= gap_at ? of + gap : of) * 8 + 2 * wave + (lane & 1), last_group);
+            if (g >= from) g = max(g, group.low >> 3);
+            const int pg = (int) page_of_group(p.c, (uint32_t) g);
+            const int page = ap.c.table[(int64_t) seq * ap.c.t_nb1 + pg];
+            const bool ok = (uint32_t) page < (uint32_t) ap.c.n_pages;
+            bad |= !ok && of >= first;
+            const uint32_t cell = (uint32_t) (g - pg * p.c.groups) * 8;
+            return Where{ok ? (uint32_t) page : 0u, cell * k_nb1, cell * v_nb1};
         };
-        auto load = [&](const Where & a, const int buf) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const bool ok = (uint32_t) a.page[e] < (uint32_t) p.c.n_pages;
-                bad |= !ok;
-                const int pg = ok ? a.page[e] : 0;
-                const char * k = k_head + pg * p.c.k_nb3 + a.cell[e] * p.c.k_nb1;
-                const char * v = v_head + pg * p.c.v_nb3 + a.cell[e] * p.c.v_nb1;
-                const uint32_t to = lds0 + (uint32_t) (buf * 2 * kTileBytes + (16 * wave + 8 * e) * 256);
-#pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    dma16(uniform_desc(k + 4 * f * p.c.k_nb1, 3 * k_nb1 + 256), k_lane[2 * e + f], to + 1024 * f);
-                    dma16(uniform_desc(v + 4 * f * p.c.v_nb1, 3 * v_nb1 + 256), v_lane, to + kTileBytes + 1024 * f);
-                }
+        // One of the 8 instructions that load tile i: cells 8 e + 4 f on of this
+        // wave's, K or V.
+        int4v desc[2];
+        auto load = [&](const Where & a, const int i, const int buf, const int q) {
+            const int e = q >> 2, v = q >> 1 & 1, f = q & 1, from = 2 * (i & 31) + e;
+            if ((q & 3) == 0) {
+                const uint32_t pg = (uint32_t) __builtin_amdgcn_readlane((int) a.page, from);
+                desc[0] = page_desc(k_head, pg, k_nb3);
+                desc[1] = page_desc(v_head, pg, v_nb3);
             }
+            load_lds(desc[v], (uint32_t) __builtin_amdgcn_readlane((int) (v ? a.v : a.k), from) + 4 * f * (v ? v_nb1 : k_nb1),
+                     v ? v_lane : k_lane[2 * e + f], lds0 + (uint32_t) (buf * 2 * kTileBytes + v * kTileBytes + (16 * wave + 8 * e + 4 * f) * 256));
         };
-        Where next;
-        if (first < tiles_end) {
-            load(look_up(first), 0);
-            next = look_up(min(first + 1, tiles_end - 1));
-        }
 
-        // This lane's query row: its operands times a power of two that brings
-        // the largest value to [2^11, 2^12), the scores' factor, what it sees
+        // This lane's query row, loaded while the first pages are looked up
         const int r = r0 + lr, t = token_of(p, min(r, p.R - 1));
         const bool valid = r < p.R && t < w.count;
-        half8 q_hi[8], q_lo[8];
-        float fac;
+        Where where = {0, 0, 0};
+        if (first < tiles_end) where = look_up(first);
+        float4 x[8][2];
         {
-            const float * qr = (const float *) (p.q + (int64_t) seq * p.q_nb3 + (int64_t) (valid ? t : 0) * p.q_nb1 +
-                                                (int64_t) (head * p.G + (valid ? r - t * p.G : 0)) * p.q_nb2) + 8 * h;
-            float4 x[8][2];
+            const float * qr = (const float *) (ap.q + (int64_t) seq * ap.q_nb3 + (int64_t) (valid ? t : 0) * ap.q_nb1 +
+                                                (int64_t) (head * ap.G + (valid ? r - t * ap.G : 0)) * ap.q_nb2) + 8 * h;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) x[ks][e] = *(const float4 *) (qr + 16 * ks + 4 * e);
+        }
+        asm volatile("" ::: "memory");
+        if (first < tiles_end)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) load(where, first, 0, q);
+        // its operands times a power of two that brings the largest value to
+        // [2^11, 2^12), and the scores' factor
+        half8 q_hi[8], q_lo[8];
+        float fac;
+        {
             float top = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
@@ -250,6 +284,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
                 }
             }
         }
+        // what it sees
         const int limit = valid ? begin + 1 + t : group.limit;
         int low = 0;
         const int32_t * words = nullptr;
@@ -257,21 +292,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         bool bad_row = false;
         {
             int place = begin + t;
-            if (p.bits) {
-                words = p.bits + (int64_t) seq * p.b_nb2 + (int64_t) (valid ? t : 0) * p.b_nb1;
-                node_pos = p.pos + (int64_t) seq * p.p_nb1;
-                if (p.window && valid) {
+            if (ap.bits) {
+                words = ap.bits + (int64_t) seq * ap.b_nb2 + (int64_t) (valid ? t : 0) * ap.b_nb1;
+                node_pos = ap.pos + (int64_t) seq * ap.p_nb1;
+                if (ap.window && valid) {
                     place = node_pos[t];
                     bad_row = place < begin || place >= w.len;
                     if (bad_row && h == 0) paged_error(p.c, kPagedBadPos, place);
                 }
             }
-            if (p.window && valid && !bad_row) low = place + 1 - p.window;
+            if (ap.window && valid && !bad_row) low = place + 1 - ap.window;
         }
         // Of the 64 cells from c0 on: those that this lane's row sees.
         auto sees64 = [&](const int c0) {
-            if (p.bits) return span64(c0, begin, low, p.first) | nodes64(p, words, node_pos, c0 - begin, w.count, low);
-            return span64(c0, limit, low, p.first);
+            const auto & sp = arguments<P>();
+            if (sp.bits) return span64(c0, begin, low, sp.first) | nodes64(sp, words, node_pos, c0 - begin, w.count, low);
+            return span64(c0, limit, low, sp.first);
         };
 
         floatx16 o[4];
@@ -283,15 +319,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
             const int buf = (i - first) & 1, tile = tile_at(i), c0 = tile * P::kTile;
             wait_vm<0>();
             __syncthreads();                                             // the tile is there, the other buffer free
-            if (i + 1 < tiles_end) {
-                load(next, buf ^ 1);
-                next = look_up(min(i + 2, tiles_end - 1));
-            }
-            const char * k_tile = lds + buf * 2 * kTileBytes;
+            const bool more = i + 1 < tiles_end;                         // (loaded beside the scores)
+            if (more && ((i + 1) & 31) == 0) where = look_up(i + 1);
             char * v_tile = lds + buf * 2 * kTileBytes + kTileBytes;
-            const bool edge = partly(tile, least, low_last);             // some row of the group does not see all of it
+            const bool edge = edges.has(tile);                           // some row of the group does not see all of it
             if (edge) {
-                const uint64_t some = span64(c0, group.limit, group.low, p.first), all = span64(c0, least, low_last, p.first);
+                const uint64_t some = span64(c0, group.limit, group.low, ap.first), all = span64(c0, least_of(t0), low_of(t1), ap.first);
                 const int c = tid >> 2;
                 if (!(all >> c & 1)) {
                     const bool none = !(some >> c & 1);
@@ -319,17 +352,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
                 __syncthreads();
             }
             const bool work = has_rows && c0 < mine.limit && !(c0 >= p.first && c0 + P::kTile <= mine.low);
+            if (!work && more)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) load(where, i + 1, buf ^ 1, q);
             if (work) {
+                // scores: K's operands read one step ahead, an instruction of
+                // the next tile's loads a step
                 floatx16 s[2] = {floatx16{}, floatx16{}};
+                half8 k[2][2];
+                const uint32_t kx = k_at + buf * 2 * kTileBytes;
+                auto k_read = [&](const int ks) {
+#pragma unroll
+                    for (int cb = 0; cb < 2; ++cb) k[ks & 1][cb] = as_half8(lds_at<u32x4>((kx ^ (ks << 5)) + 32 * 256 * cb));
+                };
+                k_read(0);
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
-                    half8 k[2];
+                    if (ks + 1 < 8) k_read(ks + 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int cb = 0; cb < 2; ++cb) k[cb] = as_half8(*(const u32x4 *) (k_tile + 32 * 256 * cb + (k_at ^ (ks << 5))));
+                    for (int cb = 0; cb < 2; ++cb) s[cb] = mfma32(k[ks & 1][cb], q_lo[ks], s[cb]);
+                    if (more) load(where, i + 1, buf ^ 1, ks);
 #pragma unroll
-                    for (int cb = 0; cb < 2; ++cb) s[cb] = mfma32(k[cb], q_lo[ks], s[cb]);
-#pragma unroll
-                    for (int cb = 0; cb < 2; ++cb) s[cb] = mfma32(k[cb], q_hi[ks], s[cb]);
+                    for (int cb = 0; cb < 2; ++cb) s[cb] = mfma32(k[ks & 1][cb], q_hi[ks], s[cb]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 float f = fac;
                 if constexpr (CAP) {
@@ -339,7 +385,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
 #pragma unroll
                         for (int v = 0; v < 16; ++v) s[cb][v] = tanhf(s[cb][v] * fac);
                 }
-                if (partly(tile, my_least, my_low_last)) {
+                if (my_edges.has(tile)) {
                     uint64_t sees = valid ? sees64(c0) : ~0ull;
                     sees >>= 4 * h;
 #pragma unroll
@@ -360,29 +406,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
 #pragma unroll
                     for (int db = 0; db < 4; ++db) o[db] *= g;
                 }
+                // probabilities and products, 16 cells (kk) and 32 dims (db) a
+                // step: a step's V is read one step ahead, and beside its two
+                // products a quarter of the next 16 cells' probabilities is made
                 const float ref = m == -AL_INF ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float sum[2] = {0.0f, 0.0f};
+                half8 p_hi[2], p_lo[2], v[2];
+                const uint32_t vx = v_at + buf * 2 * kTileBytes;
+                auto v_read = [&](const int step) {
+                    const uint32_t x = (vx ^ (64 * (step & 3))) + 16 * 256 * (step >> 2);
+                    const half4 a = read_tr16(x), c = read_tr16(x + 8 * 256);
+                    v[step & 1] = half8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+                };
+                auto probabilities = [&](const int kk, const int e) {    // of slots e and e + 1
+                    float x[2];
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    half8 p_hi, p_lo;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][8 * (kk & 1) + e], f, -ref));
-                        sum[e & 3] += x;
-                        const _Float16 hi = (_Float16) x;
-                        p_hi[e] = hi;
-                        p_lo[e] = (_Float16) (x - (float) hi);
+                    for (int u = 0; u < 2; ++u) {
+                        x[u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][8 * (kk & 1) + e + u], f, -ref));
+                        sum[u] += x[u];
                     }
+                    half2v hi = __builtin_convertvector(float2v{x[0], x[1]}, half2v);
+                    asm volatile("" : "+v"(hi));                         // (kept in this step)
+                    half2v lo = __builtin_convertvector(float2v{rest(hi, 0, x[0]), rest(hi, 1, x[1])}, half2v);
+                    asm volatile("" : "+v"(lo));
 #pragma unroll
-                    for (int db = 0; db < 4; ++db) {
-                        const char * x = v_tile + ((v_at ^ (64 * v_sw)) ^ (64 * db)) + 16 * 256 * kk;
-                        const half4 a = lds_read_tr16(x), c = lds_read_tr16(x + 8 * 256);
-                        const half8 v = {a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
-                        o[db] = mfma32(v, p_lo, o[db]);
-                        o[db] = mfma32(v, p_hi, o[db]);
+                    for (int u = 0; u < 2; ++u) {
+                        p_hi[kk & 1][e + u] = hi[u];
+                        p_lo[kk & 1][e + u] = lo[u];
                     }
+                };
+                v_read(0);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) probabilities(0, e);
+#pragma unroll
+                for (int step = 0; step < 16; ++step) {
+                    const int kk = step >> 2, db = step & 3;
+                    if (step + 1 < 16) v_read(step + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    o[db] = mfma32(v[step & 1], p_lo[kk & 1], o[db]);
+                    if (kk < 3) probabilities(kk + 1, 2 * db);
+                    o[db] = mfma32(v[step & 1], p_hi[kk & 1], o[db]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l += sum[0] + sum[1];
             }
             if (edge && any_odd) {                                       // (written before the barrier above)
                 if (work) {
@@ -413,7 +479,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
             }
         }
 
-        if (bad && lane == 0) {
+        if (__any(bad) && lane == 0) {
             any_bad = 1;
             if (!w.bad) paged_error(p.c, kPagedBadPage, seq);
         }
@@ -421,14 +487,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         l = pair_sum(l);
         if (any_bad || w.bad || bad_row) l = __builtin_nanf("");
         if (valid) {
-            float f = 1.0f;
+            const auto & ep = arguments<P>();
+            float factor = 1.0f;
             float * d;
             if (whole) {
-                const int hq = head * p.G + r - t * p.G;
-                f = row_factor(p, p, w, seq, t, m, l, hq);
-                d = (float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) hq * p.d_nb1);
+                const int hq = head * ep.G + r - t * ep.G;
+                factor = row_factor<P>(ep, w, seq, t, m, l, hq);
+                d = (float *) (ep.dst + (int64_t) seq * ep.d_nb3 + (int64_t) t * ep.d_nb2 + (int64_t) hq * ep.d_nb1);
             } else {
-                float * rec = (float *) record(p, unit, wg, first == 0 ? 1 : 0);
+                float * rec = (float *) record(ep, unit, wg, first == 0 ? 1 : 0);
                 d = rec + (r - group0) * 128;
                 if (h == 0) *(float2 *) (rec + P::kRows * 128 + (r - group0) * 2) = float2{m, l};
             }
@@ -436,12 +503,64 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
             for (int db = 0; db < 4; ++db)
 #pragma unroll
                 for (int bq = 0; bq < 4; ++bq)
-                    *(float4 *) (d + 32 * db + 8 * bq + 4 * h) = float4{o[db][4 * bq] * f, o[db][4 * bq + 1] * f, o[db][4 * bq + 2] * f, o[db][4 * bq + 3] * f};
+                    *(float4 *) (d + 32 * db + 8 * bq + 4 * h) =
+                        float4{o[db][4 * bq] * factor, o[db][4 * bq + 1] * factor, o[db][4 * bq + 2] * factor, o[db][4 * bq + 3] * factor};
         }
         if (at < stop) {
             __syncthreads();                                             // the LDS is free for the next piece
             if (tid == 0) any_bad = 0;
         }
+    }
+}
+
+// The join of sequences with few pieces each: half a wave to a row, 4 dims to a
+// lane, the loads of 4 pieces in flight together. Workgroups (rows, sequence,
+// unit). (A wave to a row, its halves every second piece, as the join of few
+// rows has it: 28 us instead of JOINUS for 11 trees of up to 488 rows.)
+__global__ __launch_bounds__(64 * kWaves) void paged_join_rows_kernel(const PagedRowsParams p) {
+    using P = PagedRowsParams;
+    prefetch_params(p);
+    const int seq = blockIdx.y, unit = blockIdx.z, d4 = threadIdx.x & 31;
+    const int2 info = p.info[(int64_t) unit * p.c.n_seq + seq];
+    const int count = min(p.counts ? p.counts[seq] : p.T, p.T), len = p.lens[seq];
+    const int head = unit % p.Hkv, group0 = unit / p.Hkv * P::kRows;
+    // (no row of the group: nothing was written to info)
+    if (count <= token_of(p, group0) || info.y < 2) return;
+    const SeqWork w = seq_work(p, len, count);
+    const int end = min(P::kRows, min(p.R, count * p.G) - group0);
+    for (int row = blockIdx.x * (2 * kWaves) + (threadIdx.x >> 5); row < end; row += gridDim.x * (2 * kWaves)) {
+        float M = -AL_INF, L = 0.0f;
+        float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = 0; i0 < info.y; i0 += 4) {
+            float2 ml[4];
+            float4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = min(i0 + i, info.y - 1);
+                const float * rec = (const float *) record(p, unit, info.x + c, c == 0 ? 1 : 0);
+                ml[i] = *(const float2 *) (rec + P::kRows * 128 + row * 2);
+                x[i] = *(const float4 *) (rec + row * 128 + 4 * d4);
+            }
+            asm volatile("" ::: "memory");
+            float top = M;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i0 + i < info.y) top = fmaxf(top, ml[i].x);
+            const float f = grow<P>(M, top);
+            L *= f; o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+            M = top;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i0 + i < info.y) {
+                    const float e = grow<P>(ml[i].x, M);
+                    L += ml[i].y * e;
+                    o.x += x[i].x * e; o.y += x[i].y * e; o.z += x[i].z * e; o.w += x[i].w * e;
+                }
+        }
+        const int gr = group0 + row, t = token_of(p, gr), hq = head * p.G + gr - t * p.G;
+        const float f = row_factor<P>(p, w, seq, t, M, L, hq);
+        *(float4 *) ((float *) (p.dst + (int64_t) seq * p.d_nb3 + (int64_t) t * p.d_nb2 + (int64_t) hq * p.d_nb1) + 4 * d4) =
+            float4{o.x * f, o.y * f, o.z * f, o.w * f};
     }
 }
 
@@ -451,8 +570,13 @@ hipError_t launch_rows(const PagedRowsParams & p, hipStream_t st) {
     const dim3 grid((unsigned) (p.target * p.row_groups * p.Hkv));
     if (p.softcap != 0.0f) hipLaunchKernelGGL(paged_rows_kernel<true>, grid, dim3(64 * kWaves), 0, st, p);
     else                   hipLaunchKernelGGL(paged_rows_kernel<false>, grid, dim3(64 * kWaves), 0, st, p);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? launch_join(p, st) : e;
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.target == 1) return e;
+    if (p.row_waves > 1) return launch_join(p, st);
+    const int64_t pairs = (int64_t) p.c.n_seq * p.row_groups * p.Hkv;
+    const int side = (int) std::max<int64_t>(1, std::min<int64_t>(PagedRowsParams::kRows / (2 * kWaves), 4096 / pairs));
+    hipLaunchKernelGGL(paged_join_rows_kernel, dim3((unsigned) side, (unsigned) p.c.n_seq, (unsigned) (p.row_groups * p.Hkv)), dim3(64 * kWaves), 0, st, p);
+    return hipGetLastError();
 }
 
 }  // namespace paged_fattn
