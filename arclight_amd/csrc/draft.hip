@@ -9,7 +9,7 @@
 // Verification. Accept and reject take a few numbers of each node (its
 // parent's p and q at its token), gathered by a workgroup into LDS; the walk down
 // the tree is then ballots over the nodes. The token that follows is drawn from
-// one row of V: the row's weights are summed in 64 bits by workgroups of kChunk
+// one row of V: the row's weights are summed in 64 bits by waves, kChunk tokens
 // each, and a last workgroup for each sequence finds the chunk in which the sum
 // passes sample times the whole, and the token in it. Every sum is taken in one
 // fixed order, so that equal inputs give equal tokens.
@@ -33,9 +33,11 @@ namespace {
 
 constexpr int kMaxNodes = 1024;
 constexpr int kThreads = 256;
-constexpr int kEach = 8;                        // a thread's tokens of a chunk
-constexpr int kChunk = kThreads * kEach;
+constexpr int kWaves = kThreads / 64;
+constexpr int kEach = 8;                        // a lane's tokens of a chunk
+constexpr int kChunk = 64 * kEach;              // tokens that a wave sums
 
+typedef double pair64 __attribute__((ext_vector_type(2)));
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ void draft_error(int * err, const int what, const int value) {
@@ -107,7 +109,7 @@ struct VerifyParams {
     int32_t * next;
     int2 * state;                               // [sequence]: the last accepted node (-1: none), its rejected children
     double * norms;                             // [sequence][T]: with siblings of a draft, the sums after each rejection
-    double2 * sums;                             // [sequence][chunk]: of what is left, of the row itself
+    pair64 * sums;                             // [sequence][chunk]: of what is left, of the row itself
     int32_t T, V, chunks, walked;               // walked: state and norms are there
     int * err;
 };
@@ -135,7 +137,7 @@ __device__ __forceinline__ double block_sum(double x, double * lds) {
     __syncthreads();
     x = lds[0];
 #pragma unroll
-    for (int i = 1; i < kThreads / 64; ++i) x += lds[i];
+    for (int i = 1; i < kWaves; ++i) x += lds[i];
     return x;
 }
 
@@ -144,7 +146,7 @@ struct WalkLds {
     int32_t tok[kMaxNodes];
     float p[kMaxNodes], q[kMaxNodes], r[kMaxNodes];
     int32_t path[kMaxNodes];
-    double red[kThreads / 64];
+    double red[kWaves];
 };
 
 struct Walked {
@@ -181,9 +183,9 @@ __device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, cons
     const char * target = p.target + (int64_t) s * p.t_nb2;
     const char * draft = p.draft ? p.draft + (int64_t) s * p.d_nb2 : nullptr;
     for (int u = tid; u < count; u += kThreads) {
+        const float r = p.accept[(int64_t) s * p.acc_nb1 + u];
         const int tok = u ? p.tokens[(int64_t) s * p.tok_nb1 + u] : 0;
         const int par = parent_of(p, s, u, tok, report);
-        const float r = p.accept[(int64_t) s * p.acc_nb1 + u];
         x.par[u] = par;
         x.tok[u] = tok;
         x.r[u] = r;
@@ -267,132 +269,180 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyParam
     write_path(p, s, at, x);
 }
 
-// What is left of the last accepted node's row, kEach tokens from `first` on.
-// gone: the tokens of the chunk that were rejected, a bit each.
-__device__ __forceinline__ void row_weights(const VerifyParams & p, const int s, const Walked & at, const double * norms, const int first,
-                                            const uint32_t * gone, double (&left)[kEach], double (&own)[kEach]) {
+// A thread's tokens of the last accepted node's rows, as they are: 0 past the
+// last one.
+struct Row {
+    float p[kEach], q[kEach];
+};
+__device__ __forceinline__ Row load_row(const VerifyParams & p, const int s, const Walked & at, const int first) {
+    Row x;
+    const bool drafted = p.draft && at.m > 0;
     const char * pr = p.target + (int64_t) s * p.t_nb2 + (int64_t) at.v * p.t_nb1 + (int64_t) first * 4;
     const char * qr = p.draft + (int64_t) s * p.d_nb2 + (int64_t) at.v * p.d_nb1 + (int64_t) first * 4;
-    const bool drafted = p.draft && at.m > 0;
-    float a[kEach], b[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) x.p[j] = x.q[j] = 0.0f;
     if (first + kEach <= p.V) {
 #pragma unroll
         for (int j = 0; j < kEach; j += 4) {
-            const float4u x = *(const float4u *) (pr + 4 * j);
+            const float4u y = *(const float4u *) (pr + 4 * j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a[j + e] = x[e];
+            for (int e = 0; e < 4; ++e) x.p[j + e] = y[e];
         }
         if (drafted) {
 #pragma unroll
             for (int j = 0; j < kEach; j += 4) {
-                const float4u x = *(const float4u *) (qr + 4 * j);
+                const float4u y = *(const float4u *) (qr + 4 * j);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) b[j + e] = x[e];
+                for (int e = 0; e < 4; ++e) x.q[j + e] = y[e];
             }
         }
-    } else {
+    } else if (first < p.V) {
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            a[j] = first + j < p.V ? *(const float *) (pr + 4 * j) : 0.0f;
-            b[j] = drafted && first + j < p.V ? *(const float *) (qr + 4 * j) : 0.0f;
-        }
+        for (int j = 0; j < kEach; ++j)
+            if (first + j < p.V) {
+                x.p[j] = *(const float *) (pr + 4 * j);
+                if (drafted) x.q[j] = *(const float *) (qr + 4 * j);
+            }
     }
-    const uint32_t out = p.draft ? 0u : gone[threadIdx.x * kEach / 32] >> (threadIdx.x * kEach % 32);
+    return x;
+}
+
+// What is left of them, and they themselves. gone: the tokens of the chunk that
+// were rejected, a bit each.
+__device__ __forceinline__ void row_weights(const VerifyParams & p, const Walked & at, const double * norms, const Row & x, const uint32_t * gone,
+                                            double (&left)[kEach], double (&own)[kEach]) {
+    const bool drafted = p.draft && at.m > 0;
+    const int lane = threadIdx.x & 63;
+    const uint32_t out = p.draft ? 0u : gone[lane * kEach / 32] >> (lane * kEach % 32);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-        own[j] = weight(a[j]);
-        left[j] = drafted ? left_of(own[j], weight(b[j]), at.m, norms) : out >> j & 1 ? 0.0 : own[j];
+        own[j] = weight(x.p[j]);
+        left[j] = drafted ? left_of(own[j], weight(x.q[j]), at.m, norms) : out >> j & 1 ? 0.0 : own[j];
     }
 }
 
-// The tokens of a chunk that the last accepted node's children had, without a draft.
-__device__ __forceinline__ void rejected(const VerifyParams & p, const int s, const Walked & at, const int count, const int chunk, uint32_t * gone) {
-    for (int i = threadIdx.x; i < kChunk / 32; i += kThreads) gone[i] = 0;
-    __syncthreads();
-    if (!p.draft)
-        for (int u = at.v + 1 + threadIdx.x; u < count; u += kThreads) {
-            const int tok = p.tokens[(int64_t) s * p.tok_nb1 + u];
-            if (parent_of(p, s, u, tok, false) == at.v && tok / kChunk == chunk) atomicOr(gone + tok % kChunk / 32, 1u << (tok % 32));
-        }
-    __syncthreads();
+// Waits for this wave's LDS accesses, and keeps those after it behind them.
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-// Grid: chunks, sequences.
+// The tokens of a chunk that the last accepted node's children had, without a
+// draft, by one wave.
+__device__ __forceinline__ void rejected(const WalkLds & x, const Walked & at, const int count, const int chunk, uint32_t * gone) {
+    const int lane = threadIdx.x & 63;
+    wave_lds();
+    if (lane < kChunk / 32) gone[lane] = 0;
+    wave_lds();
+    for (int u = at.v + 1 + lane; u < count; u += 64)
+        if (x.par[u] == at.v && x.tok[u] / kChunk == chunk) atomicOr(gone + x.tok[u] % kChunk / 32, 1u << (x.tok[u] % 32));
+    wave_lds();
+}
+
+// Grid: workgroups of a sequence, sequences. A wave takes the chunks that follow
+// its number in steps of all of the sequence's waves, each loaded while the one
+// before is summed.
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyParams p) {
     __shared__ WalkLds x;
-    __shared__ uint32_t gone[kChunk / 32];
+    __shared__ uint32_t gone[kWaves][kChunk / 32];
     prefetch_params(p);
-    const int s = blockIdx.y, chunk = blockIdx.x;
-    const bool first = chunk == 0;
+    const int s = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool first = blockIdx.x == 0;
     Walked at;
     int count = 0;
     if (p.walked) {
         const int2 st = p.state[s];
         at = {st.x, st.y, 0};
-        count = nodes_of(p, s, false);
     } else {
         count = nodes_of(p, s, first && threadIdx.x == 0);
         at = walk<false>(p, s, count, first, x, nullptr);
         if (first) write_path(p, s, at, x);
     }
     if (at.v < 0) return;
-    rejected(p, s, at, count, chunk, gone);
-    double left[kEach], own[kEach], a = 0.0, b = 0.0;
-    row_weights(p, s, at, p.norms + (int64_t) s * p.T, chunk * kChunk + threadIdx.x * kEach, gone, left, own);
+    const int step = gridDim.x * kWaves;
+    int chunk = blockIdx.x * kWaves + wave;
+    Row row = load_row(p, s, at, chunk * kChunk + lane * kEach);
+    for (; chunk < p.chunks; chunk += step) {
+        const Row next = load_row(p, s, at, (chunk + step) * kChunk + lane * kEach);
+        if (!p.draft) rejected(x, at, count, chunk, gone[wave]);         // (the walk was this workgroup's own)
+        double left[kEach], own[kEach], a = 0.0, b = 0.0;
+        row_weights(p, at, p.norms + (int64_t) s * p.T, row, gone[wave], left, own);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) a += left[j], b += own[j];
-    a = block_sum(a, x.red);
-    b = block_sum(b, x.red);
-    if (threadIdx.x == 0) p.sums[(int64_t) s * p.chunks + chunk] = double2{a, b};
+        for (int j = 0; j < kEach; ++j) a += left[j], b += own[j];
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if (lane == 0) p.sums[(int64_t) s * p.chunks + chunk] = pair64{a, b};
+        row = next;
+    }
 }
 
-// Sum of the workgroup's values before this thread's, and of all.
-__device__ __forceinline__ double block_before(const double x, double & all, double * lds) {
-    double y = x;
+// Sums of the workgroup's pairs before this thread's, and of all.
+__device__ __forceinline__ pair64 block_before(const pair64 v, pair64 & all, pair64 * lds) {
+    double a = v.x, b = v.y;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 1; i < 64; i *= 2) {
-        const double o = __shfl_up(y, i);
-        if (lane >= i) y += o;
+        const double oa = __shfl_up(a, i), ob = __shfl_up(b, i);
+        if (lane >= i) a += oa, b += ob;
     }
+    pair64 before = {__shfl_up(a, 1), __shfl_up(b, 1)};
+    if (lane == 0) before = pair64{0.0, 0.0};
     __syncthreads();
-    if (lane == 63) lds[wave] = y;
-    double before = __shfl_up(y, 1);
-    if (lane == 0) before = 0.0;
+    if (lane == 63) lds[wave] = pair64{a, b};
     __syncthreads();
-    double from = 0.0;
-    all = 0.0;
+    pair64 from = {0.0, 0.0};
+    all = pair64{0.0, 0.0};
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
         if (i == wave) from = all;
-        all += lds[i];
+        all.x += lds[i].x;
+        all.y += lds[i].y;
     }
-    return from + before;
+    return pair64{from.x + before.x, from.y + before.y};
 }
 
-// Grid: sequences.
+// Grid: sequences. What does not depend on the state is loaded with it; one
+// load, of the chunk, follows. (Nothing is gathered by atomics on one word: 256
+// of them took 4.4 us.)
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParams p) {
-    __shared__ double lds[kThreads / 64];
+    __shared__ pair64 lds[kWaves];
     __shared__ uint32_t gone[kChunk / 32];
-    __shared__ int s_at, s_last;
-    __shared__ double s_before;
+    __shared__ int s_hit[kWaves], s_last[kWaves];
+    __shared__ double s_hit_before[kWaves], s_last_before[kWaves];
     prefetch_params(p);
-    const int s = blockIdx.x, tid = threadIdx.x;
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // the chunks: each thread some that follow one another, the first kHeld of
+    // them at once
+    constexpr int kHeld = 4;
+    const pair64 * sums = p.sums + (int64_t) s * p.chunks;
+    const int each = (p.chunks + kThreads - 1) / kThreads, c0 = min(tid * each, p.chunks), c1 = min(c0 + each, p.chunks);
+    pair64 held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = sums[min(c0 + i, p.chunks - 1)];
+    const float u = p.sample[s];
     const int2 st = p.state[s];
+    // the node of this thread (of trees of up to kThreads)
+    const bool node = !p.draft && tid < p.T && tid > 0;
+    const int tok = node ? p.tokens[(int64_t) s * p.tok_nb1 + tid] : 0;
+    const int par = node ? parent_of(p, s, tid, tok, false) : -1;
+    const int count = nodes_of(p, s, false);
+    if (tid < kChunk / 32) gone[tid] = 0;
     const Walked at = {st.x, st.y, 0};
     if (at.v < 0) {
         if (tid == 0) p.next[s] = -1;
         return;
     }
-    // the chunk: each thread some that follow one another
-    const double2 * sums = p.sums + (int64_t) s * p.chunks;
-    const int each = (p.chunks + kThreads - 1) / kThreads, c0 = min(tid * each, p.chunks), c1 = min(c0 + each, p.chunks);
-    double a = 0.0, b = 0.0, total, own_total;
-    for (int c = c0; c < c1; ++c) a += sums[c].x, b += sums[c].y;
-    double before = block_before(a, total, lds);
-    const double own_before = block_before(b, own_total, lds);
-    const bool own = !(total > 0.0);
-    if (own) total = own_total, before = own_before;
+    auto sum_of = [&](const int c) {
+        const int i = c - c0;
+        return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : i == 3 ? held[3] : sums[c];
+    };
+    pair64 part = {0.0, 0.0}, whole;
+    for (int c = c0; c < c1; ++c) part += sum_of(c);
+    const pair64 ahead = block_before(part, whole, lds);
+    // where nothing is left the row itself
+    const bool own = !(whole.x > 0.0);
+    const double total = own ? whole.y : whole.x;
+    double before = own ? ahead.y : ahead.x;
     if (!(total > 0.0 && total < __builtin_inf())) {
         if (tid == 0) {
             draft_error(p.err, kDraftBadRow, s);
@@ -400,41 +450,62 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParam
         }
         return;
     }
-    const double goal = (double) p.sample[s] * total;
-    if (tid == 0) s_at = INT32_MAX, s_last = -1;
-    __syncthreads();
+    const double goal = (double) u * total;
     // the first chunk that goes past the goal; else the last that holds any
-    int hit = -1, last = -1;
-    double hit_before = 0.0, last_before = 0.0;
-    for (int c = c0; c < c1; ++c) {
-        const double w = own ? sums[c].y : sums[c].x;
-        if (w > 0.0) {
-            last = c;
-            last_before = before;
-            if (hit < 0 && before + w > goal) hit = c, hit_before = before;
+    {
+        int hit = -1, last = -1;
+        double hit_before = 0.0, last_before = 0.0;
+        for (int c = c0; c < c1; ++c) {
+            const pair64 x = sum_of(c);
+            const double w = own ? x.y : x.x;
+            if (w > 0.0) {
+                last = c;
+                last_before = before;
+                if (hit < 0 && before + w > goal) hit = c, hit_before = before;
+            }
+            before += w;
         }
-        before += w;
+        const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
+        if (hits ? lane == __builtin_ctzll(hits) : lane == 0) s_hit[wave] = hit, s_hit_before[wave] = hit_before;
+        if (lasts ? lane == 63 - __builtin_clzll(lasts) : lane == 0) s_last[wave] = last, s_last_before[wave] = last_before;
     }
-    if (hit >= 0) atomicMin(&s_at, hit);
-    if (last >= 0) atomicMax(&s_last, last);
     __syncthreads();
-    const int chunk = s_at == INT32_MAX ? s_last : s_at;
-    if (chunk >= c0 && chunk < c1) s_before = s_at == INT32_MAX ? last_before : hit_before;
+    int chunk = -1, last_chunk = -1;
+    double from = 0.0, last_from = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (chunk < 0 && s_hit[i] >= 0) chunk = s_hit[i], from = s_hit_before[i];
+        if (s_last[i] >= 0) last_chunk = s_last[i], last_from = s_last_before[i];
+    }
+    if (chunk < 0) chunk = last_chunk, from = last_from;
+    // the token in it: by the first wave, once the rejected ones are known
+    Row row;
+    const int first = chunk * kChunk + lane * kEach;
+    if (wave == 0) row = load_row(p, s, at, first);
+    if (tid < count && par == at.v && tok / kChunk == chunk) atomicOr(gone + tok % kChunk / 32, 1u << (tok % 32));
+    if (!p.draft)
+        for (int v = kThreads + tid; v < count; v += kThreads) {
+            const int x = p.tokens[(int64_t) s * p.tok_nb1 + v];
+            if (parent_of(p, s, v, x, false) == at.v && x / kChunk == chunk) atomicOr(gone + x % kChunk / 32, 1u << (x % 32));
+        }
     __syncthreads();
-    const double from = s_before;
-    if (tid == 0) s_at = INT32_MAX, s_last = -1;
-    // the token in it
-    rejected(p, s, at, nodes_of(p, s, false), chunk, gone);
-    const int first = chunk * kChunk + tid * kEach;
-    double left[kEach], row[kEach], mine = 0.0, all;
-    row_weights(p, s, at, p.norms + (int64_t) s * p.T, first, gone, left, row);
+    if (wave) return;
+    double left[kEach], weights[kEach], sum = 0.0;
+    row_weights(p, at, p.norms + (int64_t) s * p.T, row, gone, left, weights);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-        if (own) left[j] = row[j];
-        mine += left[j];
+        if (own) left[j] = weights[j];
+        sum += left[j];
     }
-    double run = from + block_before(mine, all, lds);
-    hit = last = -1;
+    double upto = sum;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        const double o = __shfl_up(upto, i);
+        if (lane >= i) upto += o;
+    }
+    double run = __shfl_up(upto, 1);
+    run = from + (lane == 0 ? 0.0 : run);
+    int hit = -1, last = -1;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         run += left[j];
@@ -443,10 +514,12 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParam
             if (hit < 0 && run > goal) hit = first + j;
         }
     }
-    if (hit >= 0) atomicMin(&s_at, hit);
-    if (last >= 0) atomicMax(&s_last, last);
-    __syncthreads();
-    if (tid == 0) p.next[s] = s_at == INT32_MAX ? s_last : s_at;
+    const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
+    if (hits) {
+        if (lane == __builtin_ctzll(hits)) p.next[s] = hit;
+    } else if (lasts && lane == 63 - __builtin_clzll(lasts)) {
+        p.next[s] = last;
+    }
 }
 
 bool index(const al_tensor & t, const int64_t n) {
@@ -509,7 +582,7 @@ int make_plan(const al_draft_verify_args * a, VerifyPlan * out) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     pl.norms_at = up((size_t) n * sizeof(int2));
     pl.sums_at = pl.norms_at + (p.walked ? up((size_t) n * T * sizeof(double)) : 0);
-    pl.bytes = pl.sums_at + (size_t) n * p.chunks * sizeof(double2);
+    pl.bytes = pl.sums_at + (size_t) n * p.chunks * sizeof(pair64);
     *out = pl;
     return AL_OK;
 }
@@ -559,14 +632,16 @@ extern "C" int al_draft_verify_f32(const al_draft_verify_args * a) {
     int rc = make_plan(a, &pl);
     if (rc != AL_OK || pl.n_seq == 0) return rc;
     VerifyParams & p = pl.p;
-    rc = al_device_error_flag(&p.err);
+    int n_cu = 0;
+    rc = al_device_cu_count(&n_cu);
+    if (rc == AL_OK) rc = al_device_error_flag(&p.err);
     if (rc != AL_OK) return rc;
     char * at = nullptr;
     rc = al_workspace_records("draft_verify", pl.bytes, a->workspace, a->workspace_bytes, a->stream, (void **) &at);
     if (rc != AL_OK) return rc;
     p.state = (int2 *) at;
     p.norms = (double *) (at + pl.norms_at);
-    p.sums = (double2 *) (at + pl.sums_at);
+    p.sums = (pair64 *) (at + pl.sums_at);
     const hipStream_t st = (hipStream_t) a->stream;
     const unsigned n = (unsigned) pl.n_seq;
     hipError_t e = hipSuccess;
@@ -575,7 +650,9 @@ extern "C" int al_draft_verify_f32(const al_draft_verify_args * a) {
         e = hipGetLastError();
     }
     if (e == hipSuccess) {
-        hipLaunchKernelGGL(verify_sums_kernel, dim3((unsigned) p.chunks, n), dim3(kThreads), 0, st, p);
+        // four workgroups a CU walk the tree, and take the chunks between them
+        const unsigned side = (unsigned) std::max<int64_t>(1, std::min<int64_t>((p.chunks + kWaves - 1) / kWaves, 4ll * n_cu / n));
+        hipLaunchKernelGGL(verify_sums_kernel, dim3(side, n), dim3(kThreads), 0, st, p);
         e = hipGetLastError();
     }
     if (e == hipSuccess) {

@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBatch = 8;                       // 16-byte pieces of a thread in flight
+constexpr int kCopyGroups = 4096;               // workgroups that copy pages, if there are so many pieces
 constexpr int kPath = 64;                       // entries of a path looked up together
 constexpr int kLayers = 64;                     // layers of a launch: pointers among its arguments
 
@@ -54,7 +55,7 @@ struct CopyParams {
     const int32_t * src;
     const int32_t * dst;
     const int32_t * cells;                      // or null
-    int32_t Hkv, blocks;                        // workgroups of a page in one pool
+    int32_t Hkv, blocks;                        // workgroups of a page in one pool, which take its pieces in turn
     int32_t heads_first;                        // a head's cells lie closer than a cell's heads
     LayerPools layers;
 };
@@ -144,25 +145,26 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(const CopyParams p
         return;
     }
     const bool v = (int) blockIdx.x >= p.blocks;
-    const int at = ((int) blockIdx.x - (v ? p.blocks : 0)) * (kThreads * kBatch) + tid;
     const int units = cells * p.Hkv * 16;
-    if (at >= units || src == dst) return;
+    if (src == dst) return;
     const int64_t nb1 = v ? p.c.v_nb1 : p.c.k_nb1, nb2 = v ? p.c.v_nb2 : p.c.k_nb2, nb3 = v ? p.c.v_nb3 : p.c.k_nb3;
     char * pool = layer_pool<CopyParams>(blockIdx.y, v);
     const char * from = pool + src * nb3;
     char * to = pool + dst * nb3;
-    u32x4 x[kBatch];
-    int64_t off[kBatch];
     const uint32_t inner = p.heads_first ? cells : p.Hkv;
+    for (int at = ((int) blockIdx.x - (v ? p.blocks : 0)) * (kThreads * kBatch) + tid; at < units; at += p.blocks * (kThreads * kBatch)) {
+        u32x4 x[kBatch];
+        int64_t off[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-        const uint32_t u = min(at + j * kThreads, units - 1), row = u >> 4, o = row / inner, in = row - o * inner;
-        off[j] = (p.heads_first ? in : o) * nb1 + (p.heads_first ? o : in) * nb2 + (u & 15) * 16;
-        x[j] = *(const u32x4 *) (from + off[j]);
+        for (int j = 0; j < kBatch; ++j) {
+            const uint32_t u = min(at + j * kThreads, units - 1), row = u >> 4, o = row / inner, in = row - o * inner;
+            off[j] = (p.heads_first ? in : o) * nb1 + (p.heads_first ? o : in) * nb2 + (u & 15) * 16;
+            x[j] = *(const u32x4 *) (from + off[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (at + j * kThreads < units) *(u32x4 *) (to + off[j]) = x[j];
     }
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-        if (at + j * kThreads < units) *(u32x4 *) (to + off[j]) = x[j];
 }
 
 bool index(const al_tensor & t, const int64_t n) {
@@ -264,7 +266,8 @@ extern "C" int al_paged_copy_f16(const al_paged_copy_args * a) {
     p.src = (const int32_t *) a->src.data;
     p.dst = (const int32_t *) a->dst.data;
     p.cells = (const int32_t *) a->cells.data;
-    p.blocks = (int32_t) ((units + kThreads * kBatch - 1) / (kThreads * kBatch));
+    const int64_t most = (units + kThreads * kBatch - 1) / (kThreads * kBatch), launched = 2 * n * std::min(kLayers, a->layers.n_layers);
+    p.blocks = (int32_t) std::max<int64_t>(1, std::min(most, (kCopyGroups + launched - 1) / launched));
     p.heads_first = p.c.k_nb1 < p.c.k_nb2;
     rc = al_device_error_flag(&p.c.err);
     if (rc != AL_OK) return rc;
