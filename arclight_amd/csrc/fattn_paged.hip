@@ -509,11 +509,16 @@ int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n
     return AL_OK;
 }
 
-// Whether a call with a rule goes to the kernel of many query rows.
+// Whether a call with a rule goes to the kernel of many query rows: for more
+// than 64 of a KV head, and for more than 32 of several sequences (us, this
+// kernel and that one, trees over 3000 cells of 8 heads: 40 rows of one sequence
+// 18.5, 20.0, of 8 37.2, 34.3, 64 rows of one 21.0, 23.1, of 8 42.7, 35.5, of 30
+// 113, 81.6, 100 rows of one over 6000 cells 33, 27).
 bool many_rows(const PagedFattnParams & p) {
     // (it counts bytes within a page, and from page to page, in 32 bits)
     constexpr int64_t kMost = 0xffffffffll;
-    return p.R > 64 && p.c.page_size * p.c.k_nb1 <= kMost && p.c.page_size * p.c.v_nb1 <= kMost && p.c.k_nb3 <= kMost && p.c.v_nb3 <= kMost;
+    return p.R > (p.c.n_seq > 1 ? 32 : 64) && p.c.page_size * p.c.k_nb1 <= kMost && p.c.page_size * p.c.v_nb1 <= kMost && p.c.k_nb3 <= kMost &&
+           p.c.v_nb3 <= kMost;
 }
 
 int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_cu, Plan * out) {

@@ -52,7 +52,10 @@ struct PagedSeesParams : PagedFattnParams {
 struct PagedRowsParams : PagedSeesParams {
     static constexpr bool kLog2 = true;
     static constexpr int kTile = 64;
-    static constexpr int kMinTiles = 1;
+    // (us with parts of 1, 2, 3, 4 tiles at least: a tree of 26 nodes over 2000
+    // cells 23.1, 21.9, 20.4, 22.0, 2 prompts of 40 over windows of 1024 29.1,
+    // 27.8, 24.8, 32.4, one of 500 30.6, 29.6, 29.1, 26.6)
+    static constexpr int kMinTiles = 3;
     static constexpr int kWhole = 8;
     static constexpr int kRows = 128;                   // of a group
 };

@@ -59,15 +59,16 @@ class DeviceTensor:
         numpy axis of nnml dim i (default: reversed, i.e. contiguous nnml)."""
         self.buf = buf
         self.type = typ
-        self.shape = tuple(int(x) for x in shape)
+        self.shape = tuple(map(int, shape))
         esz = abi.TYPE_SIZES[typ]
         if strides is None:
-            strides = []
-            acc = esz
-            for d in reversed(self.shape):
-                strides.insert(0, acc)
+            strides, acc = [], esz
+            for d in self.shape[::-1]:
+                strides.append(acc)
                 acc *= d
-        self.strides = tuple(int(x) for x in strides)
+            self.strides = tuple(strides[::-1])
+        else:
+            self.strides = tuple(map(int, strides))
         self.offset = int(offset)
         nd = len(self.shape)
         self.axes = tuple(axes) if axes is not None else tuple(range(nd - 1, -1, -1)) + tuple(range(nd, 4))

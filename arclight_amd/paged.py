@@ -128,14 +128,13 @@ def _layers(caches):
     caches = list(caches)
     if not caches:
         raise ValueError("no layers")
-    like = caches[0]
-    for c in caches:
-        if any(getattr(c, x).shape != getattr(like, x).shape or getattr(c, x).strides != getattr(like, x).strides for x in ("k", "v")) or \
-                c.heads_first != like.heads_first:
-            raise ValueError("the layers' pools have to be of one shape, with the same strides")
+    like = [(c.k.shape, c.k.strides, c.v.shape, c.v.strides, c.heads_first) for c in caches]
+    if any(x != like[0] for x in like):
+        raise ValueError("the layers' pools have to be of one shape, with the same strides")
     r = abi.AlPagedLayers()
-    r.k_pool, r.v_pool = like.pool_descs()
-    k, v = ((ctypes.c_void_p * len(caches))(*(getattr(c, x).ptr for c in caches)) for x in ("k", "v"))
+    r.k_pool, r.v_pool = caches[0].pool_descs()
+    pointers = ctypes.c_void_p * len(caches)
+    k, v = pointers(*[c.k.ptr for c in caches]), pointers(*[c.v.ptr for c in caches])
     r.k, r.v, r.n_layers = k, v, len(caches)
     return r, (caches, k, v)
 
