@@ -581,13 +581,20 @@ int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_c
     const int64_t per_cu = n_cu / std::max<int64_t>(1, units);
     const int64_t useful = std::max(n_seq, (most + min_tiles - 1) / min_tiles);
     p.target = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * n_cu / std::max<int64_t>(1, units), useful));
+    // Where the row groups alone fill the card twice over, a workgroup takes whole
+    // sequences, one or some: nothing to join, and many short workgroups rather
+    // than a round of long ones and a part of another (us, all of a unit's
+    // sequences by one workgroup, and so: two prompts of 1000 over windows of 1024
+    // 62.9, 60.1, of 4000 280.0, 279.1).
+    p.whole = pl.many && 2 * n_cu <= 2 * units;
+    if (p.whole) p.target = (int32_t) std::min<int64_t>(n_seq, std::max<int64_t>(1, 8192 / units));
     p.long_target = p.row_tiles == 1 ? (int32_t) std::max<int64_t>(1, std::min<int64_t>(per_cu, p.target)) : p.target;
     // few sequences have many pieces each
     p.row_waves = p.long_target > 16 * n_seq ? kWaves : 1;
     p.scale = a->scale;
     p.softcap = a->logit_softcap;
     pl.info_bytes = ((size_t) units * n_seq * sizeof(int2) + 255) / 256 * 256;
-    pl.bytes = pl.info_bytes + (p.target > 1 ? (size_t) units * p.target * 2 * rows * 130 * 4 : 0);     // one workgroup a unit: no pieces
+    pl.bytes = pl.info_bytes + (p.target > 1 && !p.whole ? (size_t) units * p.target * 2 * rows * 130 * 4 : 0);     // one workgroup a unit: no pieces
     *out = pl;
     return AL_OK;
 }

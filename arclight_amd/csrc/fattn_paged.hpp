@@ -45,6 +45,7 @@ struct PagedSeesParams : PagedFattnParams {
     int32_t window, first;                              // window 0: none
     const int32_t * bits;  int64_t b_nb1, b_nb2;        // or null; token, sequence, in words
     const int32_t * pos;   int64_t p_nb1;               // or null; sequence
+    int32_t whole;                                      // sequences are not cut, however long
     static constexpr bool kSees = true;
 };
 
@@ -292,7 +293,8 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int l
     // 10 of 500 14.1, 12.3; whole up to 32 tiles: 128 of 700 56.4, 60.2). Else
     // kMinTiles a workgroup at least, or a sequence; p.target workgroups for
     // sequences of up to 16 tiles on average, p.long_target for longer ones.
-    const bool cut = longest > P::kWhole || active == 1;
+    bool cut = longest > P::kWhole || active == 1;
+    if constexpr (P::kSees) cut &= !p.whole;
     const int W = cut ? min(S > 16 * active ? p.long_target : p.target, max((S + P::kMinTiles - 1) / P::kMinTiles, active)) : min(p.target, active);
     if (wg >= W) return false;
     m.parts = Parts(S, W);
