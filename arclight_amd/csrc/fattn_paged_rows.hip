@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
             fac = fabsf(p.scale) * down;
             fac = CAP ? fac / p.softcap : fac * kLog2e;
             // (a factor of 0 would make NaN of the -inf of hidden cells)
-            if (!CAP) fac = fmaxf(fac, 1.17549435e-38f);
+            if (!CAP && fac < 1.17549435e-38f) fac = 1.17549435e-38f;
             if (p.scale == 0.0f) up = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {

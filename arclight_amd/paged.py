@@ -146,6 +146,8 @@ class KeepCall:
     def __init__(self, caches, lens, counts, path, kept, lens_out=None, stream=None):
         a = self.args = abi.AlPagedKeepArgs()
         a.layers, pools = _layers(caches)
+        if pools[0][0].table is None:
+            raise ValueError("the sequences' table is missing")
         a.table, a.lens, a.path, a.kept = pools[0][0].table.desc(), lens.desc(), path.desc(), kept.desc()
         if counts is not None:
             a.counts = counts.desc()
