@@ -18,6 +18,12 @@
 // after each rejection has to be normalised before the next child is tried: a
 // sum over the row within the walk, which a workgroup for each sequence then
 // does in a launch of its own.
+//
+// What bounds them: chains of loads. The tables of one tree of 26 nodes or of 50
+// of up to 200 take 3.7 us, a launch and two loads in series. Verification is two
+// launches, count and nodes -> their p -> the row -> its sums, and sums -> the
+// chunk: one tree of 26 nodes over 32003 tokens 9.4 us, 30 chains with a draft's
+// rows of 128000 (31 MB) 14.2, 20 trees of 40 nodes over 152000 (12 MB) 13.8.
 
 #include <hip/hip_runtime.h>
 

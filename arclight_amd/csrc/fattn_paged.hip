@@ -49,6 +49,14 @@
 // 51.1 us, 100000 cells (64 query heads) 79 us, 5.2 TB/s. Prompts are bound
 // elsewhere: every wave reads its 16 KB of a tile through the L1 and turns V
 // itself (4 prompts of 2048 tokens, 32 heads over 8: 749 us, 184 TFLOP/s).
+//
+// Calls with a rule (al_paged_sees: windows with first cells, trees) take the
+// same code with PagedSeesParams: tiles that no row of the group sees are left
+// out of the row of tiles, those that some row does not see all of are masked by
+// a bit for each of a lane's 8 cells, and pages outside of what is seen are not
+// looked up. Many query rows go to the kernel of fattn_paged_rows.hip. Measured:
+// one token over a window of 1024 10.6 us, 30 over windows of 4096 90.3 us (5.6
+// TB/s), 64 of 1024 55.3.
 
 #include <hip/hip_runtime.h>
 

@@ -23,16 +23,30 @@
 // maximum is still carried.
 //
 // Tiles go from memory into LDS directly (buffer_load ... lds), one tile ahead,
-// each wave a quarter, its pages looked up another tile ahead by scalar loads.
-// A tile is [cell][128] with 16-byte pieces permuted within a cell so that the
-// operand reads are free of bank conflicts: piece j of K's cell c at j ^ (c &
-// 15), of V's at j ^ 4 (c & 3). Two workgroups to a CU: while one waits for its
-// scores' exponentials the other has the matrix cores.
+// each wave a quarter: one of its 8 instructions beside every second pair of the
+// first products (8 in a row took 0.6 us of a tile's 3), by page numbers that a
+// vector load finds for 32 tiles at once. A tile is [cell][128] with 16-byte
+// pieces permuted within a cell so that the operand reads are free of bank
+// conflicts: piece j of K's cell c at j ^ (c & 15), of V's at j ^ 4 (c & 3). The
+// probabilities of 16 cells are made beside the products of the 16 before. Two
+// workgroups to a CU, each wave with half of a SIMD's registers.
 //
 // Tiles that some row does not see all of are masked value by value; V of cells
 // that no row sees is cleared there (0 times NaN is not 0), and so are single
 // values that are not finite: the rows that do see them get NaN in their dim,
 // found by a product of ones.
+//
+// What bounds it: the matrix cores, each product taken twice, which are busy half
+// of the time over a launch and run at 1.9 GHz under this load; what else there
+// is are a tile's barrier (0.24 us of 3), the query rows' way into registers (3 us
+// a sequence and workgroup) and parts of tiles that are hidden. Measured, 32 heads
+// over 8: two prompts of 4000 over windows of 1000 280 us, 470 TFLOP/s by the
+// cells that are seen, 940 as executed (a plain f16 product of 8192^3 runs at
+// 1250, products from registers alone at 1400 to 1550); 11 trees of 31 to 61 nodes
+// over 2000 to 6000 cells, 64 heads, 168 us. (The next tile's scores beside this
+// one's probabilities, tiles of 32 cells in a ring of four: 330 us instead of 294,
+// for twice the barriers; of 64 cells it does not fit the registers. Rows stored
+// through LDS: no gain.)
 
 #include <hip/hip_runtime.h>
 
@@ -60,7 +74,8 @@ __device__ __forceinline__ T lds_at(const uint32_t at) { return *(const __attrib
 __device__ __forceinline__ half4 read_tr16(const uint32_t at) {
     return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((fattn::lds_short4v *) (uintptr_t) at));
 }
-// x - (a half of) hi
+// x - (a half of) hi. hi is made of x in an instruction between, so x, an
+// exponential, is never read here by the instruction right after it.
 __device__ __forceinline__ float rest(const half2v hi, const int half, const float x) {
     float y;
     if (half) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(hi), "v"(x));
