@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
     const int n_blocks = (p.c.n_seq + 63) / 64;
     Block b;
     MyPart part;
-    if (!find_part(p, wg, lane, t0, t1, blockIdx.x == 0 && wave == 0, b, part)) return;
+    if (!find_part(p, wg, p.target, p.long_target, lane, t0, t1, blockIdx.x == 0 && wave == 0, b, part)) return;
     const Parts & parts = part.parts;
     int at = part.at, block = 0, before = 0;
     const int stop = part.stop;
@@ -688,6 +688,7 @@ int attend(const al_paged_fattn_args * a, const al_paged_sees * rule) {
     if (pl.many) {
         PagedRowsParams p;
         static_cast<PagedSeesParams &>(p) = pl.p;
+        p.shared = p.counts && !p.whole && p.target > 1 && p.row_groups > 1 && p.row_groups * ((p.c.n_seq + 63) / 64) <= PagedRowsParams::kShared;
         e = launch_rows(p, st);
     } else {
         e = rule ? launch(pl.p, st) : launch<PagedFattnParams>(pl.p, st);

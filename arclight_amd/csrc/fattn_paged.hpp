@@ -59,6 +59,8 @@ struct PagedRowsParams : PagedSeesParams {
     static constexpr int kMinTiles = 3;
     static constexpr int kWhole = 8;
     static constexpr int kRows = 128;                   // of a group
+    static constexpr int kShared = 8;                   // row groups times blocks of 64 sequences whose tiles are counted
+    int32_t shared;                                     // a head's workgroups go to its row groups by their tiles
 };
 hipError_t launch_rows(const PagedRowsParams & p, hipStream_t stream);
 
@@ -271,9 +273,11 @@ struct MyPart {
 };
 
 // Finds it, false if there is none; b: sequences 0 to 63. report: record counts
-// that are wrong. t0, t1: the group's first and last token.
+// that are wrong. t0, t1: the group's first and last token; target, long_target:
+// the unit's workgroups, and those that long sequences use.
 template <typename P>
-__device__ __forceinline__ bool find_part(const P & p, const int wg, const int lane, const int t0, const int t1, const bool report, Block & b, MyPart & m) {
+__device__ __forceinline__ bool find_part(const P & p, const int wg, const int target, const int long_target, const int lane, const int t0, const int t1,
+                                          const bool report, Block & b, MyPart & m) {
     const int n_blocks = (p.c.n_seq + 63) / 64;
     b.load(p, 0, lane, t0, t1);
     if (report) b.report(p);
@@ -291,8 +295,8 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int l
     // piece costs a workgroup more than the rounds that the cut saves (us, cut
     // and whole: 4 sequences of up to 200 cells 13.4, 10.1, 64 of 100 16.4, 11.5,
     // 10 of 500 14.1, 12.3; whole up to 32 tiles: 128 of 700 56.4, 60.2). Else
-    // kMinTiles a workgroup at least, or a sequence; p.target workgroups for
-    // sequences of up to 16 tiles on average, p.long_target for longer ones.
+    // kMinTiles a workgroup at least, or a sequence; `target` workgroups for
+    // sequences of up to 16 tiles on average, `long_target` for longer ones.
     bool cut = longest > P::kWhole || active == 1;
     if constexpr (P::kSees) {
         // Nor are sequences cut that are about as long as one another, as those
@@ -302,9 +306,9 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int l
         // 81.6, 33 of 4096 104, 135).
         auto fills = [&](const int places) { return active <= places && 10 * active >= 9 * places; };
         const bool even = (int64_t) longest * active * 8 <= (int64_t) S * 9;
-        cut &= !p.whole && !(even && (fills(p.long_target) || fills(p.target)));
+        cut &= !p.whole && !(even && (fills(long_target) || fills(target)));
     }
-    const int W = cut ? min(S > 16 * active ? p.long_target : p.target, max((S + P::kMinTiles - 1) / P::kMinTiles, active)) : min(p.target, active);
+    const int W = cut ? min(S > 16 * active ? long_target : target, max((S + P::kMinTiles - 1) / P::kMinTiles, active)) : min(target, active);
     if (wg >= W) return false;
     m.parts = Parts(S, W);
     m.at = m.parts.begin(wg);

@@ -40,13 +40,14 @@
 // of the time over a launch and run at 1.9 GHz under this load; what else there
 // is are a tile's barrier (0.24 us of 3), the query rows' way into registers (3 us
 // a sequence and workgroup) and parts of tiles that are hidden. Measured, 32 heads
-// over 8: two prompts of 4000 over windows of 1000 280 us, 470 TFLOP/s by the
-// cells that are seen, 940 as executed (a plain f16 product of 8192^3 runs at
-// 1250, products from registers alone at 1400 to 1550); 11 trees of 31 to 61 nodes
-// over 2000 to 6000 cells, 64 heads, 168 us. (The next tile's scores beside this
-// one's probabilities, tiles of 32 cells in a ring of four: 330 us instead of 294,
-// for twice the barriers; of 64 cells it does not fit the registers. Rows stored
-// through LDS: no gain.)
+// over 8: two prompts of 4000 over windows of 1000 275 to 294 us on three cards,
+// 450 to 480 TFLOP/s by the cells that are seen, twice that as executed (a plain
+// f16 product of 8192^3 runs at 1250 to 1300, products from registers alone at
+// 1400 to 1550), one of 4096 over windows of 8192 558; 11 trees of 31 to 61 nodes
+// over 2000 to 6000 cells, 64 heads, 163 to 176 us. (The next tile's scores beside
+// this one's probabilities, tiles of 32 cells in a ring of four: 330 us instead of
+// 294, for twice the barriers; of 64 cells it does not fit the registers. Rows
+// stored through LDS, waves' priorities raised for the products: no gain.)
 
 #include <hip/hip_runtime.h>
 
@@ -126,6 +127,50 @@ __device__ __forceinline__ int4v page_desc(const char * head, const uint32_t pag
     return int4v{(int) (uint32_t) a, (int) (uint32_t) (a >> 32), -1, 0x00020000};
 }
 
+// Of a KV head's workgroups each row group gets a share by its tiles, one at
+// least, where sequences differ in their groups: those of few rows are not in
+// the last ones (us, equal shares and so: 4 prompts of 1 to 200 tokens over
+// windows of 1024 33.4, 24.1, 8 trees of 30 to 60 nodes over 4000 cells 67.9, 62.5,
+// 11 of 31 to 61 over up to 6000, 64 heads, 165.5, 162.6). Changes this
+// workgroup's unit, its number within it, the unit's workgroups, and what brings
+// the number to its record among the head's.
+__device__ __forceinline__ void share(const PagedRowsParams & p, const int lane, int & unit, int & wg, int & target, int & records) {
+    const int n_blocks = (p.c.n_seq + 63) / 64, last = token_of(p, (p.row_groups - 1) * PagedRowsParams::kRows);
+    bool fewer = false;
+    for (int k = 0; k < n_blocks; ++k) {
+        const int s = 64 * k + lane, count = s < p.c.n_seq ? p.counts[s] : 0;
+        fewer |= count > 0 && count <= last;
+    }
+    if (!__any(fewer)) return;
+    const int head = blockIdx.x % p.Hkv, places = p.row_groups * p.target, place = blockIdx.x / p.Hkv;
+    int tiles = 0;                                                       // lane g: tiles of group g
+    float total = 0.0f;
+    for (int k = 0; k < n_blocks; ++k)
+        for (int g = 0; g < p.row_groups; ++g) {
+            const int r = g * PagedRowsParams::kRows;
+            Block x;
+            x.load(p, k, lane, token_of(p, r), token_of(p, min(r + PagedRowsParams::kRows, p.R) - 1));
+            const int S = x.total();
+            if (lane == g) tiles += S;
+            total += (float) S;
+        }
+    const float each = (float) places / fmaxf(total, 1.0f);
+    float upto = 0.0f;
+    int start = 0, stop = 0, g = 0;
+    for (;; ++g) {
+        upto += (float) __builtin_amdgcn_readlane(tiles, g);
+        const int after = p.row_groups - 1 - g;
+        stop = min(max(__builtin_amdgcn_readfirstlane((int) (upto * each + 0.5f)), start + 1), places - after);
+        if (after == 0) stop = places;
+        if (place < stop || after == 0) break;
+        start = stop;
+    }
+    unit = g * p.Hkv + head;
+    wg = place - start;
+    target = stop - start;
+    records = head * places + start - unit * p.target;
+}
+
 // CAP: logits soft-capped.
 template <bool CAP>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedRowsParams p) {
@@ -136,8 +181,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
     prefetch_params(p);
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, lr = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // the heads of the same cells next to one another in the grid
-    const int units = p.row_groups * p.Hkv, unit = blockIdx.x % units, wg = blockIdx.x / units;
+    // The heads of the same cells next to one another in the grid, and the last
+    // row groups first: those of a prompt's beginning see the fewest cells and end
+    // the launch (us, first groups first: two prompts of 4000 over windows of 1000
+    // 301, 294).
+    const int units = p.row_groups * p.Hkv;
+    int unit = units - 1 - (int) (blockIdx.x % units), wg = blockIdx.x / units, target = p.target, records = 0;
+    if (p.shared) share(p, lane, unit, wg, target, records);
     const int head = unit % p.Hkv, group0 = unit / p.Hkv * P::kRows;
     // tokens of the group, and of the wave's rows (none past the last row)
     const int t0 = token_of(p, group0), t1 = token_of(p, min(group0 + P::kRows, p.R) - 1);
@@ -147,7 +197,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
     const int n_blocks = (p.c.n_seq + 63) / 64;
     Block b;
     MyPart part;
-    if (!find_part(p, wg, lane, t0, t1, blockIdx.x == 0 && wave == 0, b, part)) return;
+    if (!find_part(p, wg, target, target, lane, t0, t1, blockIdx.x == 0 && wave == 0, b, part)) return;
     int at = part.at, block = 0, before = 0;
     const int stop = part.stop;
     if (tid < 128) odd[tid] = 0;
@@ -186,7 +236,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         const bool whole = first == 0 && end == tiles;
         const auto & ap = arguments<P>();
         if (tid == 0) {
-            if (first == 0) ap.info[(int64_t) unit * ap.c.n_seq + seq] = int2{wg, whole ? 1 : part.parts.of(base + tiles - 1) - wg + 1};
+            if (first == 0) ap.info[(int64_t) unit * ap.c.n_seq + seq] = int2{wg + records, whole ? 1 : part.parts.of(base + tiles - 1) - wg + 1};
             if (w.bad) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         const int begin = w.len - w.count;
@@ -510,7 +560,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
                 factor = row_factor<P>(ep, w, seq, t, m, l, hq);
                 d = (float *) (ep.dst + (int64_t) seq * ep.d_nb3 + (int64_t) t * ep.d_nb2 + (int64_t) hq * ep.d_nb1);
             } else {
-                float * rec = (float *) record(ep, unit, wg, first == 0 ? 1 : 0);
+                float * rec = (float *) record(ep, unit, wg + records, first == 0 ? 1 : 0);
                 d = rec + (r - group0) * 128;
                 if (h == 0) *(float2 *) (rec + P::kRows * 128 + (r - group0) * 2) = float2{m, l};
             }

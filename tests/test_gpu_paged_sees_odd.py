@@ -270,6 +270,60 @@ def test_many_sequences_of_many_rows(gpu, n, T, Hq, Hkv, window):
         assert np.all(a[s, counts[s]:] == MARK) and np.linalg.norm(a[s, :counts[s]] - b[s, :counts[s]]) <= 2e-5 * np.linalg.norm(b[s, :counts[s]]), s
 
 
+SHARES = [                                                              # tokens, heads, new tokens of each sequence, cells before them at most
+    (100, 16, 4, [100, 1, 7, 33], 2500),
+    (100, 16, 4, [9, 0, 32, 20], 2500),                                 # the last row groups have no rows
+    (300, 4, 1, [5], 4000),
+    (300, 4, 1, [300], 4000),
+    (70, 8, 4, [70, 0, 0, 0, 0, 0, 0, 64], 1500),
+    (40, 8, 1, [0] * 30 + [40] + [1] * 60 + [17] * 20, 300),            # two blocks of sequences, three row groups
+    (130, 8, 8, [0, 0, 0], 900),
+]
+
+
+@pytest.mark.parametrize("i", range(len(SHARES)))
+@pytest.mark.parametrize("window, first", [(0, 0), (700, 3)])
+def test_row_groups_of_sequences_that_differ(gpu, i, window, first):
+    """Sequences of few rows beside those of many: the row groups' shares of the
+    card, and pieces of several groups' sequences, in a call and replayed with
+    the counts the other way round."""
+    from arclight_amd import device, fattn, paged
+    T, Hq, Hkv, counts, before = SHARES[i]
+    _case(f"counts {counts} of {T}, window {window}")
+    rng = np.random.default_rng(i)
+    n = len(counts)
+    begin = [int(x) for x in rng.integers(before // 2, before, n)]
+    pool = P.Pool(rng, [b + max(c, e) for b, c, e in zip(begin, counts, counts[::-1])], Hkv, 16)
+    q = rng.standard_normal((n, T, Hq, D)).astype(np.float32) * 2
+    bits = np.zeros((T, (T + 31) // 32), np.uint32)
+    for t, u in zip(*np.nonzero(np.tril(rng.random((T, T)) < 0.7) | np.eye(T, dtype=bool))):
+        bits[t, u // 32] |= np.uint32(1 << (u % 32))
+    bits = bits.view(np.int32)
+    buf = {"lens": _put(np.zeros(n, np.int32)), "counts": _put(np.zeros(n, np.int32)), "pos": _put(np.zeros((n, T), np.int32)),
+           "out": _put(np.zeros(q.shape, np.float32))}
+    st = device.Stream()
+    call = paged.AttentionCall(pool.device(), _put(q), buf["lens"], buf["out"], counts=buf["counts"], scale=SCALE, stream=st, window=window,
+                               first=first, bits=_put(np.ascontiguousarray(np.broadcast_to(bits, (n, *bits.shape)))), pos=buf["pos"] if window else None)
+    graph = None
+    for step in range(3):
+        c = counts[::-1] if step == 1 else counts
+        lens = [x + k for x, k in zip(begin, c)]
+        pos = np.array(begin, np.int32)[:, None] + np.arange(T, dtype=np.int32)          # as in a chain
+        for name, x in (("lens", lens), ("counts", c), ("pos", pos)):
+            buf[name].buf.upload(np.array(x, np.int32))
+        buf["out"].buf.upload(np.full(q.shape, MARK, np.float32))
+        device.synchronize()
+        if step == 1:
+            graph = device.Graph(st, call.run)
+        graph.launch(st) if graph else call.run()
+        device.synchronize()
+        fattn.device_errors()
+        sees = [C.visible(m, k, T, window, first, bits, x if window else None) for m, k, x in zip(lens, c, pos)]
+        _check(buf["out"].numpy(np.float32), C.attention(pool, q, lens, c, SCALE, sees), f"step {step}")
+    graph.destroy()
+    st.destroy()
+
+
 @pytest.mark.parametrize("what", ["few rows", "many rows", "verification"])
 def test_a_workspaces_counters_are_left_alone(gpu, what):
     from arclight_amd import device, draft, fattn, paged
