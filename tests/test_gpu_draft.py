@@ -329,3 +329,53 @@ def test_verify_replayed(gpu, drafted):
         _verify(h["target"], h["tokens"], h["accept"], h["sample"], h["parents"], stream=st)
     graph.destroy()
     st.destroy()
+
+
+def test_two_threads_with_streams_of_their_own(gpu):
+    """Verification and attention of trees by two threads at once, on streams of
+    their own and the library's workspaces: each call's results are those of the
+    same call alone, bit for bit."""
+    import threading
+
+    from arclight_amd import device, draft, paged
+    from tests import paged_cases as P
+    _case("two threads")
+    rng = np.random.default_rng(12)
+    n, T, V, Hq, Hkv = 4, 30, 5000, 16, 4
+    lens = [900, 30, 2100, 333]
+    pool = P.Pool(rng, lens, Hkv, 16)
+    cache, dl = pool.device(), _put(np.array(lens, np.int32))
+    work = []
+    for _ in range(2):
+        parents = np.stack([C.random_tree(rng, T) for _ in range(n)])
+        target = _probabilities(rng, n, T, V)
+        tokens = _put(rng.integers(0, V, (n, T)).astype(np.int32))
+        st = device.Stream()
+        path, kept, nxt = (_put(np.zeros(s, np.int32)) for s in ((n, T), (n,), (n,)))
+        v = draft.VerifyCall(_put(target.astype(np.float32)), tokens, _put(rng.random((n, T)).astype(np.float32)), _put(rng.random(n).astype(np.float32)),
+                             path, kept, nxt, parents=_put(parents.astype(np.int32)), stream=st)
+        q, out = _put(rng.standard_normal((n, T, Hq, 128)).astype(np.float32)), _put(np.zeros((n, T, Hq, 128), np.float32))
+        bits = np.stack([C.tree(p, m, T)[3] for p, m in zip(parents, lens)])
+        a = paged.AttentionCall(cache, q, dl, out, scale=0.09, bits=_put(bits), stream=st)
+        v.run(), a.run()
+        _sync()
+        work.append((st, v, a, (path, kept, nxt, out), [x.numpy(t) for x, t in zip((path, kept, nxt, out), (np.int32,) * 3 + (np.float32,))]))
+    wrong = []
+
+    def run(st, v, a, outs, want):
+        try:
+            for _ in range(40):
+                v.run(), a.run()
+        except Exception as e:                                          # noqa: BLE001 (shown by the main thread)
+            wrong.append(e)
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    _sync()
+    assert not wrong, wrong
+    for st, _, _, outs, want in work:
+        for x, w in zip(outs, want):
+            assert np.array_equal(x.numpy(w.dtype), w)
+        st.destroy()
