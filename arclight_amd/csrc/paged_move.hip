@@ -237,11 +237,14 @@ extern "C" int al_paged_keep_f16(const al_paged_keep_args * a) {
         return al_fail(AL_ERR_INVALID, "paged_keep: lens, counts, kept and lens_out must be i32 [n_seq]");
     if (T > (1 << 16) || n_seq > 65535) return al_fail(AL_ERR_UNSUPPORTED, "paged_keep: sizes out of range");
     const size_t bytes = (size_t) n_seq * 4;
-    if (a->lens_out.data)
-        for (const al_tensor * x : {&a->lens, &a->kept, &a->counts})
-            if (x->data && overlap(a->lens_out.data, bytes, x->data, bytes))
-                return al_fail(AL_ERR_INVALID, "paged_keep: lens_out overlaps an operand");
     if (n_seq == 0) return AL_OK;
+    if (a->lens_out.data) {
+        bool bad = false;
+        for (const al_tensor * x : {&a->lens, &a->kept, &a->counts}) bad |= x->data && overlap(a->lens_out.data, bytes, x->data, bytes);
+        for (const al_tensor * x : {&a->path, &a->table})
+            bad |= overlap(a->lens_out.data, bytes, x->data, (size_t) (n_seq - 1) * x->nb[1] + (size_t) x->ne[0] * 4);
+        if (bad) return al_fail(AL_ERR_INVALID, "paged_keep: lens_out overlaps an operand");
+    }
     p.lens = (const int32_t *) a->lens.data;
     p.counts = (const int32_t *) a->counts.data;
     p.path = (const int32_t *) t.data; p.p_nb1 = (int64_t) (t.nb[1] / 4);

@@ -79,6 +79,7 @@ int al_draft_tree_i32(const al_draft_tree_args * args);
  *            on, -1 behind them
  *   kept     i32 [n_seq]: how many they are, the root among them
  *   next     i32 [n_seq]: the token that follows the last of them
+ * path, kept and next may not overlap one another or another operand.
  * From node v = 0 on, with p = p_0 = target row v: the children of v are tried in
  * their order. Child u of token x is accepted if accept[u] q(x) < p_i(x) and
  * p_i(x) > 0, and becomes v; else the next one is tried with p_(i+1). Without a

@@ -58,3 +58,42 @@ def test_layers_that_do_not_go_together():
             paged.KeepCall(caches, None, None, None, None)
     with pytest.raises(ValueError, match="table"):
         paged.KeepCall([a, a], None, None, None, None)
+
+
+@pytest.mark.parametrize("entry, names", [("al_draft_tree_i32", ("pos", "cells", "seq", "bits")), ("al_draft_verify_f32", ("path", "kept", "next"))])
+def test_outputs_that_are_other_operands(entry, names):
+    """Each operand at an address of its own, but one that two share (of memory
+    that refused calls never touch)."""
+    import ctypes
+
+    from arclight_amd import _lib
+    from tests.test_draft_refusals import tree_args, verify_args
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    lib = _lib.load()
+    for i, out in enumerate(names):
+        a = tree_args() if entry == "al_draft_tree_i32" else verify_args()
+        operands = [n for n, t in a._fields_ if t is abi.AlTensor and getattr(a, n).data]
+        for j, n in enumerate(operands):
+            getattr(a, n).data = 0x10000 * (j + 1)
+        other = next(n for n in operands[i:] + operands if n not in names[:i + 1])
+        getattr(a, out).data = getattr(a, other).data
+        assert getattr(lib, entry)(ctypes.byref(a)) == abi.AL_ERR_INVALID
+        assert "another operand's memory" in lib.al_last_error().decode()
+
+
+def test_new_lengths_inside_the_path_or_the_table():
+    import ctypes
+
+    from arclight_amd import _lib
+    from tests.test_draft_refusals import keep_args
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    lib = _lib.load()
+    for name in ("path", "table"):
+        a = keep_args()
+        getattr(a, name).data = 0x70000
+        for at in (0x70000 - 8, 0x70000 + 4 * (5 if name == "table" else 9) * 3 - 4):
+            a.lens_out.data = at
+            assert lib.al_paged_keep_f16(ctypes.byref(a)) == abi.AL_ERR_INVALID
+            assert "overlaps" in lib.al_last_error().decode()
