@@ -167,18 +167,12 @@ __device__ __forceinline__ int nodes_of(const VerifyParams & p, const int s, con
     return ok ? raw : 0;
 }
 
-// The parent of node u, -1 where it is nobody's child.
-__device__ __forceinline__ int parent_of(const VerifyParams & p, const int s, const int u, const int token, const bool report) {
-    const int par = p.parents ? p.parents[(int64_t) s * p.par_nb1 + u] : u - 1;
-    if (par >= u) {
-        if (report) draft_error(p.err, kDraftBadParent, par);
-        return -1;
-    }
-    if (par >= 0 && (uint32_t) token >= (uint32_t) p.V) {
-        if (report) draft_error(p.err, kDraftBadToken, token);
-        return -1;
-    }
-    return par;
+// The parent of node u, -1 where it is nobody's child; up: as it was given.
+__device__ __forceinline__ int valid_parent(const VerifyParams & p, const int u, const int up, const int token) {
+    return up < u && (uint32_t) token < (uint32_t) p.V ? max(up, -1) : -1;
+}
+__device__ __forceinline__ int parent_of(const VerifyParams & p, const int s, const int u, const int token) {
+    return valid_parent(p, u, p.parents ? p.parents[(int64_t) s * p.par_nb1 + u] : u - 1, token);
 }
 
 // The walk down the tree, by every wave of a workgroup alike. NORMS: with a
@@ -188,15 +182,23 @@ __device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, cons
     const int tid = threadIdx.x, lane = tid & 63;
     const char * target = p.target + (int64_t) s * p.t_nb2;
     const char * draft = p.draft ? p.draft + (int64_t) s * p.d_nb2 : nullptr;
-    for (int u = tid; u < count; u += kThreads) {
+    // (all T places are read, so that nothing waits for the count)
+    for (int u = tid; u < p.T; u += kThreads) {
         const float r = p.accept[(int64_t) s * p.acc_nb1 + u];
         const int tok = u ? p.tokens[(int64_t) s * p.tok_nb1 + u] : 0;
-        const int par = parent_of(p, s, u, tok, report);
+        const int up = p.parents ? p.parents[(int64_t) s * p.par_nb1 + u] : u - 1;
+        const int par = valid_parent(p, u, up, tok);
+        float pu = 0.0f, qu = 1.0f;
+        if (par >= 0) {
+            pu = *(const float *) (target + (int64_t) par * p.t_nb1 + (int64_t) tok * 4);
+            if (draft) qu = *(const float *) (draft + (int64_t) par * p.d_nb1 + (int64_t) tok * 4);
+        }
+        if (report && u < count && up >= 0 && par < 0) draft_error(p.err, up >= u ? kDraftBadParent : kDraftBadToken, up >= u ? up : tok);
         x.par[u] = par;
         x.tok[u] = tok;
         x.r[u] = r;
-        x.p[u] = par >= 0 ? weight(*(const float *) (target + (int64_t) par * p.t_nb1 + (int64_t) tok * 4)) : 0.0f;
-        x.q[u] = par >= 0 && draft ? weight(*(const float *) (draft + (int64_t) par * p.d_nb1 + (int64_t) tok * 4)) : 1.0f;
+        x.p[u] = weight(pu);
+        x.q[u] = weight(qu);
     }
     __syncthreads();
     Walked at = {count > 0 ? 0 : -1, 0, count > 0};
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParam
     // the node of this thread (of trees of up to kThreads)
     const bool node = !p.draft && tid < p.T && tid > 0;
     const int tok = node ? p.tokens[(int64_t) s * p.tok_nb1 + tid] : 0;
-    const int par = node ? parent_of(p, s, tid, tok, false) : -1;
+    const int par = node ? parent_of(p, s, tid, tok) : -1;
     const int count = nodes_of(p, s, false);
     if (tid < kChunk / 32) gone[tid] = 0;
     const Walked at = {st.x, st.y, 0};
@@ -492,7 +494,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParam
     if (!p.draft)
         for (int v = kThreads + tid; v < count; v += kThreads) {
             const int x = p.tokens[(int64_t) s * p.tok_nb1 + v];
-            if (parent_of(p, s, v, x, false) == at.v && x / kChunk == chunk) atomicOr(gone + x % kChunk / 32, 1u << (x % 32));
+            if (parent_of(p, s, v, x) == at.v && x / kChunk == chunk) atomicOr(gone + x % kChunk / 32, 1u << (x % 32));
         }
     __syncthreads();
     if (wave) return;

@@ -379,3 +379,26 @@ def test_two_threads_with_streams_of_their_own(gpu):
         for x, w in zip(outs, want):
             assert np.array_equal(x.numpy(w.dtype), w)
         st.destroy()
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+@pytest.mark.parametrize("T", [9, 300])
+def test_nodes_behind_the_count_hold_anything(gpu, T, drafted):
+    """Tokens, parents and numbers of nodes that are not there: not followed, and
+    nothing recorded."""
+    _case(f"verification, nodes behind the count, T={T}, drafted={drafted}")
+    rng = np.random.default_rng(T)
+    n, V = 6, 700
+    target = _probabilities(rng, n, T, V)
+    drafts = _probabilities(rng, n, T, V) if drafted else None
+    parents = np.stack([C.random_tree(rng, T, 0.6) for _ in range(n)])
+    tokens = _children(rng, target, parents, drafts)
+    accept, sample, counts = rng.random((n, T)), rng.random(n), np.array([0, 1, 2, T // 2, T - 1, T])
+    for s, c in enumerate(counts):
+        parents[s, c:] = rng.choice([-2 ** 31, -9, T, 2 ** 31 - 1, c, 0], T - c)
+        tokens[s, c:] = rng.choice([-2 ** 31, -1, V, 2 ** 31 - 1, 3], T - c)
+        accept[s, c:] = rng.choice([np.nan, np.inf, -1.0, 0.5], T - c)
+    got = _verify(target, tokens, accept, sample, parents, counts, drafts)
+    some = counts > 0
+    _same([x[some] for x in got], target[some], tokens[some], accept[some], sample[some], parents[some], counts[some], None if drafts is None else drafts[some])
+    assert got[1][0] == 0 and got[2][0] == -1 and np.all(got[0][0] == -1)
