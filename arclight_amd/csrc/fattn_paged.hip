@@ -136,8 +136,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             first_cells = p.first;
             gap = all.gap(p);
             gap_at = all.gap_at(p);
-            if (p.bits) least = max(begin, 0);
-            if (p.window) low_last = (p.bits ? w.len : begin + 1 + min(wt1, w.count - 1)) - p.window;
+            if (has_bits(p)) least = max(begin, 0);
+            low_last = (has_bits(p) ? w.len : begin + 1 + min(wt1, w.count - 1)) - p.window;
         }
         auto tile_at = [&](const int i) { return P::kSees && i >= gap_at ? i + gap : i; };
 
@@ -198,21 +198,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         bool bad_row = false;
         if constexpr (P::kSees) {
             int at = begin + t;
-            if (p.bits) {
+            if (has_bits(p)) {
                 words = p.bits + (int64_t) seq * p.b_nb2 + (int64_t) (valid ? t : 0) * p.b_nb1;
                 node_pos = p.pos + (int64_t) seq * p.p_nb1;
-                if (p.window && valid) {
+                if (p.pos && valid) {
                     at = node_pos[t];
                     bad_row = at < begin || at >= w.len;
                     if (bad_row && g == 0) paged_error(p.c, kPagedBadPos, at);
                 }
             }
-            if (p.window && valid && !bad_row) low = at + 1 - p.window;
+            if (valid && !bad_row) low = at + 1 - p.window;
         }
         // Of cells c0 to c0 + 7: those that this lane's row sees.
         auto sees8 = [&](const int c0) {
             if constexpr (P::kSees) {
-                if (p.bits) return span8(c0, begin, low, p.first) | nodes8(p, words, node_pos, c0 - begin, w.count, low);
+                if (has_bits(p)) return span8(c0, begin, low, p.first) | nodes8(p, words, node_pos, c0 - begin, w.count, low);
                 return span8(c0, limit, low, p.first);
             } else return upto8(limit - c0);
         };
@@ -340,6 +340,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
                 p_lo[i] = (_Float16) (e - (float) hi);
             }
         };
+        // (the wave's rows see the same cells)
+        const bool one_token = !(has_bits(p)) && wt0 >= min(wt1, w.count - 1);
         // o += P V of the tile. Cells past the wave's last are stale memory:
         // zeroed, as 0 times NaN is not 0. So are, one by one, the values that
         // are not finite of cells that some row does not see; the rows that do
@@ -352,7 +354,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
                 if (partly(tile)) {
                     some = span8(c0, seen, wave_span.low, p.first);
                     all = span8(c0, least, low_last, p.first);
-                    differ = true;
+                    differ = !one_token;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (!(some >> i & 1)) v[i] = u32x4{0, 0, 0, 0};
@@ -493,8 +495,8 @@ int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n
     if (r->window < 0 || r->first < 0)
         return al_fail(AL_ERR_INVALID, "paged_fattn: a window of %d cells and %d first ones", r->window, r->first);
     // (positions are below 2^30: a longer window is all of them)
-    p->window = std::min(r->window, 1 << 30);
-    p->first = p->window ? std::min(r->first, 1 << 30) : 0;
+    p->window = r->window ? std::min(r->window, 1 << 30) : 1 << 30;
+    p->first = r->window ? std::min(r->first, 1 << 30) : 0;
     if (r->bits.data) {
         const al_tensor & b = r->bits;
         if (b.type != AL_TYPE_I32 || b.ne[0] < (T + 31) / 32 || b.ne[1] != T || b.ne[2] != n_seq || b.ne[3] != 1 || b.nb[0] != 4 || b.nb[1] % 4 ||
@@ -508,11 +510,11 @@ int make_rule(const al_paged_sees * r, PagedSeesParams * p, int64_t T, int64_t n
         if (t.type != AL_TYPE_I32 || t.ne[0] != T || t.ne[1] != n_seq || t.ne[2] != 1 || t.ne[3] != 1 || t.nb[0] != 4 || t.nb[1] % 4 ||
             ((uintptr_t) t.data & 3u))
             return al_fail(AL_ERR_INVALID, "paged_fattn: positions must be i32 [T, n_seq]");
-        p->pos = (const int32_t *) t.data; p->p_nb1 = (int64_t) (t.nb[1] / 4);
+        if (r->window) p->pos = (const int32_t *) t.data, p->p_nb1 = (int64_t) (t.nb[1] / 4);
     } else if (r->bits.data && r->window) {
         return al_fail(AL_ERR_INVALID, "paged_fattn: bits and a window need positions");
     }
-    if (p->window)
+    if (r->window)
         *tiles = std::min(*tiles, ((int64_t) p->first + tile - 1) / tile + ((int64_t) p->window + T + tile - 1) / tile + 1);
     return AL_OK;
 }
@@ -690,6 +692,10 @@ int attend(const al_paged_fattn_args * a, const al_paged_sees * rule) {
         static_cast<PagedSeesParams &>(p) = pl.p;
         p.shared = p.counts && !p.whole && p.target > 1 && p.row_groups > 1 && p.row_groups * ((p.c.n_seq + 63) / 64) <= PagedRowsParams::kShared;
         e = launch_rows(p, st);
+    } else if (rule && !pl.p.bits) {
+        PagedWindowParams p;
+        static_cast<PagedSeesParams &>(p) = pl.p;
+        e = launch(p, st);
     } else {
         e = rule ? launch(pl.p, st) : launch<PagedFattnParams>(pl.p, st);
     }

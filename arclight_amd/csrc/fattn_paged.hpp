@@ -34,6 +34,7 @@ struct PagedFattnParams {
     float scale, softcap;
 
     static constexpr bool kSees = false;                // a rule beside the lengths
+    static constexpr bool kBits = false;                // it may have bits
     static constexpr bool kLog2 = false;                // maxima in log2 units, weights unscaled
     static constexpr int kTile = 32;                    // cells of a tile, the units that work is shared out in
     static constexpr int kMinTiles = 4;                 // least tiles of a part: one for each wave
@@ -42,11 +43,18 @@ struct PagedFattnParams {
 
 // The same with a rule for what a token sees (al_paged_sees).
 struct PagedSeesParams : PagedFattnParams {
-    int32_t window, first;                              // window 0: none
+    int32_t window, first;                              // no window: 2^30, which no cell lies before
     const int32_t * bits;  int64_t b_nb1, b_nb2;        // or null; token, sequence, in words
-    const int32_t * pos;   int64_t p_nb1;               // or null; sequence
+    const int32_t * pos;   int64_t p_nb1;               // or null; sequence (with bits and a window)
     int32_t whole;                                      // sequences are not cut, however long
     static constexpr bool kSees = true;
+    static constexpr bool kBits = true;
+};
+
+// Windows alone: a launch begins with an empty instruction cache, and code that
+// a call steps over costs it too (us, one token over a window of 1024 WINDOWONE).
+struct PagedWindowParams : PagedSeesParams {
+    static constexpr bool kBits = false;
 };
 
 // The same for the kernel of many query rows (fattn_paged_rows.hip).
@@ -89,6 +97,13 @@ __device__ __forceinline__ int token_of(const A & p, const int r) {
     return p.G == 1 ? r : (int) __umulhi((uint32_t) r, p.g_magic);
 }
 
+// Whether the call's rule has bits (a constant for kernels without).
+template <typename P>
+__device__ __forceinline__ bool has_bits(const P & p) {
+    if constexpr (P::kBits) return p.bits != nullptr;
+    else return false;
+}
+
 // What a row group has to do for a sequence, t0 and t1 its first and last token.
 struct SeqWork {
     int len, count;                             // cells (within the table), new tokens
@@ -123,8 +138,9 @@ template <typename P>
 __device__ __forceinline__ Span span_of(const P & p, const SeqWork & w, const int t0, const int t1) {
     Span a = {w.limit(t0, t1), 0};
     if constexpr (P::kSees) {
-        if (p.bits && a.limit >= 0) a.limit = w.len;                   // of nodes each may see any
-        if (p.window) a.low = min(max(w.len - w.count + (p.bits ? 0 : t0) + 1 - p.window, 0), max(a.limit - 1, 0));
+        const bool bits = has_bits(p);
+        if (bits && a.limit >= 0) a.limit = w.len;                     // of nodes each may see any
+        a.low = min(max(w.len - w.count + (bits ? 0 : t0) + 1 - p.window, 0), max(a.limit - 1, 0));
     }
     return a;
 }
@@ -160,7 +176,7 @@ template <typename A>
 __device__ __forceinline__ uint32_t nodes8(const A & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
                                            const int low) {
     uint32_t m = nodes8(words, u0, count);
-    if (p.window)
+    if (p.pos)
         for (uint32_t rest = m; rest; rest &= rest - 1) {
             const int at = pos[u0 + __builtin_ctz(rest)];
             if (at < low && at >= p.first) m &= ~(rest & -rest);
@@ -172,11 +188,11 @@ __device__ __forceinline__ uint32_t nodes8(const A & p, const int32_t * words, c
 template <typename P, typename A>
 __device__ __forceinline__ bool sees_any(const A & p, const SeqWork & w, const int s, const int t) {
     const int begin = w.len - w.count;
-    if constexpr (P::kSees) {
+    if constexpr (P::kBits) {
         if (p.bits) {
             const int32_t * words = p.bits + (int64_t) s * p.b_nb2 + (int64_t) t * p.b_nb1;
             const int32_t * pos = p.pos + (int64_t) s * p.p_nb1;
-            const int low = p.window ? pos[t] + 1 - p.window : 0;
+            const int low = p.pos ? pos[t] + 1 - p.window : 0;
             if (begin > 0 && (begin > low || p.first > 0)) return true;
             for (int u = max(-begin, 0); u < w.count; u += 8)
                 if (nodes8(p, words, pos, u, w.count, low)) return true;

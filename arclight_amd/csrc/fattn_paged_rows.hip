@@ -102,7 +102,7 @@ __device__ __forceinline__ uint64_t nodes64(const A & p, const int32_t * words, 
     const uint64_t third = (uint32_t) words[min(i + 2, last)];
     uint64_t m = (sh ? two >> sh | third << (64 - sh) : two) << (u - u0) & upto64(count - u0);
     // (positions of nodes are within a window that is as long as the tree)
-    if (p.window && p.window < count)
+    if (p.pos && p.window < count)
         for (uint64_t rest = m; rest; rest &= rest - 1) {
             const int at = pos[u0 + __builtin_ctzll(rest)];
             if (at < low && at >= p.first) m &= ~(rest & -rest);
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         // cells that all rows from a token on see, and the last window's beginning
         auto least_of = [&](const int first_token) { return p.bits ? max(begin, 0) : max(begin + 1 + first_token, 0); };
         auto low_of = [&](const int last_token) {
-            return p.window ? (p.bits ? w.len : begin + 1 + min(last_token, w.count - 1)) - p.window : 0;
+            return (p.bits ? w.len : begin + 1 + min(last_token, w.count - 1)) - p.window;
         };
         const Edges edges = edges_of(least_of(t0), low_of(t1)), my_edges = edges_of(least_of(wt0), low_of(wt1));
         const int tiles_end = group.limit > 0 ? end : first;             // (nothing is seen: no tile)
@@ -364,13 +364,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
             if (ap.bits) {
                 words = ap.bits + (int64_t) seq * ap.b_nb2 + (int64_t) (valid ? t : 0) * ap.b_nb1;
                 node_pos = ap.pos + (int64_t) seq * ap.p_nb1;
-                if (ap.window && valid) {
+                if (ap.pos && valid) {
                     place = node_pos[t];
                     bad_row = place < begin || place >= w.len;
                     if (bad_row && h == 0) paged_error(p.c, kPagedBadPos, place);
                 }
             }
-            if (ap.window && valid && !bad_row) low = place + 1 - ap.window;
+            if (valid && !bad_row) low = place + 1 - ap.window;
         }
         // Of the 64 cells from c0 on: those that this lane's row sees.
         auto sees64 = [&](const int c0) {
