@@ -137,9 +137,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             gap = all.gap(p);
             gap_at = all.gap_at(p);
             if (has_bits(p)) least = max(begin, 0);
-            low_last = (has_bits(p) ? w.len : begin + 1 + min(wt1, w.count - 1)) - p.window;
+            if constexpr (P::kWindow) low_last = (has_bits(p) ? w.len : begin + 1 + min(wt1, w.count - 1)) - p.window;
         }
-        auto tile_at = [&](const int i) { return P::kSees && i >= gap_at ? i + gap : i; };
+        auto tile_at = [&](const int i) { return P::kWindow && i >= gap_at ? i + gap : i; };
 
         // Pages of a tile's cells: K by lanes n (group n / 4), V by lanes g.
         // Cells past the last group that the wave sees are taken from that one.
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             Where a;
             const int tile = tile_at(i);
             uint32_t kg = min((uint32_t) tile * 4 + (n >> 2), last_group), vg = min((uint32_t) tile * 4 + g, last_group);
-            if constexpr (P::kSees) {                                  // and those that no window has from the first that one has
+            if constexpr (P::kWindow) {                                // and those that no window has from the first that one has
                 const int low = wave_span.low, from = (p.first + 7) >> 3;
                 if ((int) kg >= from) kg = max((int) kg, low >> 3);
                 if ((int) vg >= from) vg = max((int) vg, low >> 3);
@@ -200,18 +200,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             int at = begin + t;
             if (has_bits(p)) {
                 words = p.bits + (int64_t) seq * p.b_nb2 + (int64_t) (valid ? t : 0) * p.b_nb1;
-                node_pos = p.pos + (int64_t) seq * p.p_nb1;
-                if (p.pos && valid) {
+                if (P::kWindow && p.pos) node_pos = p.pos + (int64_t) seq * p.p_nb1;
+                if (node_pos && valid) {
                     at = node_pos[t];
                     bad_row = at < begin || at >= w.len;
                     if (bad_row && g == 0) paged_error(p.c, kPagedBadPos, at);
                 }
             }
-            if (valid && !bad_row) low = at + 1 - p.window;
+            if (P::kWindow && valid && !bad_row) low = at + 1 - p.window;
         }
         // Of cells c0 to c0 + 7: those that this lane's row sees.
         auto sees8 = [&](const int c0) {
-            if constexpr (P::kSees) {
+            if constexpr (!P::kWindow && P::kBits) return upto8(begin - c0) | nodes8(p, words, nullptr, c0 - begin, w.count, 0);
+            else if constexpr (P::kSees) {
                 if (has_bits(p)) return span8(c0, begin, low, p.first) | nodes8(p, words, node_pos, c0 - begin, w.count, low);
                 return span8(c0, limit, low, p.first);
             } else return upto8(limit - c0);
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         half8 p_hi, p_lo;
         // Whether some row does not see all of a tile.
         auto partly = [&](const int tile) {
-            return (tile + 1) * P::kTile > least || (P::kSees && tile * P::kTile < low_last && (tile + 1) * P::kTile > first_cells);
+            return (tile + 1) * P::kTile > least || (P::kWindow && tile * P::kTile < low_last && (tile + 1) * P::kTile > first_cells);
         };
         // Probabilities of the tile against the rows' running maxima.
         auto softmax = [&](const int tile) {
@@ -352,8 +353,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             uint32_t some = 0xffu, all = upto8(least - c0);          // cells that some, that all rows see
             if constexpr (P::kSees) {
                 if (partly(tile)) {
-                    some = span8(c0, seen, wave_span.low, p.first);
-                    all = span8(c0, least, low_last, p.first);
+                    some = P::kWindow ? span8(c0, seen, wave_span.low, p.first) : upto8(seen - c0);
+                    all = P::kWindow ? span8(c0, least, low_last, p.first) : upto8(least - c0);
                     differ = !one_token;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
@@ -692,10 +693,11 @@ int attend(const al_paged_fattn_args * a, const al_paged_sees * rule) {
         static_cast<PagedSeesParams &>(p) = pl.p;
         p.shared = p.counts && !p.whole && p.target > 1 && p.row_groups > 1 && p.row_groups * ((p.c.n_seq + 63) / 64) <= PagedRowsParams::kShared;
         e = launch_rows(p, st);
-    } else if (rule && !pl.p.bits) {
-        PagedWindowParams p;
-        static_cast<PagedSeesParams &>(p) = pl.p;
-        e = launch(p, st);
+    } else if (rule && (!pl.p.bits || !pl.p.pos)) {
+        PagedWindowParams w;
+        PagedTreeParams t;
+        static_cast<PagedSeesParams &>(w) = static_cast<PagedSeesParams &>(t) = pl.p;
+        e = pl.p.bits ? launch(t, st) : launch(w, st);
     } else {
         e = rule ? launch(pl.p, st) : launch<PagedFattnParams>(pl.p, st);
     }

@@ -34,7 +34,8 @@ struct PagedFattnParams {
     float scale, softcap;
 
     static constexpr bool kSees = false;                // a rule beside the lengths
-    static constexpr bool kBits = false;                // it may have bits
+    static constexpr bool kBits = false;                // it may have bits,
+    static constexpr bool kWindow = false;              // or a window
     static constexpr bool kLog2 = false;                // maxima in log2 units, weights unscaled
     static constexpr int kTile = 32;                    // cells of a tile, the units that work is shared out in
     static constexpr int kMinTiles = 4;                 // least tiles of a part: one for each wave
@@ -49,12 +50,19 @@ struct PagedSeesParams : PagedFattnParams {
     int32_t whole;                                      // sequences are not cut, however long
     static constexpr bool kSees = true;
     static constexpr bool kBits = true;
+    static constexpr bool kWindow = true;
 };
 
-// Windows alone: a launch begins with an empty instruction cache, and code that
-// a call steps over costs it too (us, one token over a window of 1024 WINDOWONE).
+// Windows alone, and trees alone: a launch begins with an empty instruction
+// cache, and code that a call steps over costs it too (us with the code of both,
+// with one's own: one token over a window of 1024 11.5, 10.1, 10 sequences of 6
+// 25.9, 24.7, a tree of 26 nodes over 2000 cells 20.1, 19.5, of 10 over 3000 18.9,
+// 17.9).
 struct PagedWindowParams : PagedSeesParams {
     static constexpr bool kBits = false;
+};
+struct PagedTreeParams : PagedSeesParams {
+    static constexpr bool kWindow = false;
 };
 
 // The same for the kernel of many query rows (fattn_paged_rows.hip).
@@ -69,6 +77,12 @@ struct PagedRowsParams : PagedSeesParams {
     static constexpr int kRows = 128;                   // of a group
     static constexpr int kShared = 8;                   // row groups times blocks of 64 sequences whose tiles are counted
     int32_t shared;                                     // a head's workgroups go to its row groups by their tiles
+};
+struct PagedRowsWindowParams : PagedRowsParams {
+    static constexpr bool kBits = false;
+};
+struct PagedRowsTreeParams : PagedRowsParams {
+    static constexpr bool kWindow = false;
 };
 hipError_t launch_rows(const PagedRowsParams & p, hipStream_t stream);
 
@@ -131,7 +145,7 @@ struct Span {
     template <typename P>
     __device__ __forceinline__ int gap_at(const P & p) const { return (min(p.first, low) + P::kTile - 1) / P::kTile; }
     template <typename P>
-    __device__ __forceinline__ int gap(const P & p) const { return max(low / P::kTile - gap_at(p), 0); }
+    __device__ __forceinline__ int gap(const P & p) const { return P::kWindow ? max(low / P::kTile - gap_at(p), 0) : 0; }
 };
 
 template <typename P>
@@ -140,7 +154,7 @@ __device__ __forceinline__ Span span_of(const P & p, const SeqWork & w, const in
     if constexpr (P::kSees) {
         const bool bits = has_bits(p);
         if (bits && a.limit >= 0) a.limit = w.len;                     // of nodes each may see any
-        a.low = min(max(w.len - w.count + (bits ? 0 : t0) + 1 - p.window, 0), max(a.limit - 1, 0));
+        if constexpr (P::kWindow) a.low = min(max(w.len - w.count + (bits ? 0 : t0) + 1 - p.window, 0), max(a.limit - 1, 0));
     }
     return a;
 }
@@ -176,7 +190,7 @@ template <typename A>
 __device__ __forceinline__ uint32_t nodes8(const A & p, const int32_t * words, const int32_t * pos, const int u0, const int count,
                                            const int low) {
     uint32_t m = nodes8(words, u0, count);
-    if (p.pos)
+    if (pos)
         for (uint32_t rest = m; rest; rest &= rest - 1) {
             const int at = pos[u0 + __builtin_ctz(rest)];
             if (at < low && at >= p.first) m &= ~(rest & -rest);
@@ -191,8 +205,8 @@ __device__ __forceinline__ bool sees_any(const A & p, const SeqWork & w, const i
     if constexpr (P::kBits) {
         if (p.bits) {
             const int32_t * words = p.bits + (int64_t) s * p.b_nb2 + (int64_t) t * p.b_nb1;
-            const int32_t * pos = p.pos + (int64_t) s * p.p_nb1;
-            const int low = p.pos ? pos[t] + 1 - p.window : 0;
+            const int32_t * pos = P::kWindow && p.pos ? p.pos + (int64_t) s * p.p_nb1 : nullptr;
+            const int low = pos ? pos[t] + 1 - p.window : 0;
             if (begin > 0 && (begin > low || p.first > 0)) return true;
             for (int u = max(-begin, 0); u < w.count; u += 8)
                 if (nodes8(p, words, pos, u, w.count, low)) return true;

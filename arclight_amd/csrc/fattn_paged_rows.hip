@@ -102,7 +102,7 @@ __device__ __forceinline__ uint64_t nodes64(const A & p, const int32_t * words, 
     const uint64_t third = (uint32_t) words[min(i + 2, last)];
     uint64_t m = (sh ? two >> sh | third << (64 - sh) : two) << (u - u0) & upto64(count - u0);
     // (positions of nodes are within a window that is as long as the tree)
-    if (p.pos && p.window < count)
+    if (pos && p.window < count)
         for (uint64_t rest = m; rest; rest &= rest - 1) {
             const int at = pos[u0 + __builtin_ctzll(rest)];
             if (at < low && at >= p.first) m &= ~(rest & -rest);
@@ -134,8 +134,9 @@ __device__ __forceinline__ int4v page_desc(const char * head, const uint32_t pag
 // 11 of 31 to 61 over up to 6000, 64 heads, 165.5, 162.6). Changes this
 // workgroup's unit, its number within it, the unit's workgroups, and what brings
 // the number to its record among the head's.
-__device__ __forceinline__ void share(const PagedRowsParams & p, const int lane, int & unit, int & wg, int & target, int & records) {
-    const int n_blocks = (p.c.n_seq + 63) / 64, last = token_of(p, (p.row_groups - 1) * PagedRowsParams::kRows);
+template <typename P>
+__device__ __forceinline__ void share(const P & p, const int lane, int & unit, int & wg, int & target, int & records) {
+    const int n_blocks = (p.c.n_seq + 63) / 64, last = token_of(p, (p.row_groups - 1) * P::kRows);
     bool fewer = false;
     for (int k = 0; k < n_blocks; ++k) {
         const int s = 64 * k + lane, count = s < p.c.n_seq ? p.counts[s] : 0;
@@ -147,9 +148,9 @@ __device__ __forceinline__ void share(const PagedRowsParams & p, const int lane,
     float total = 0.0f;
     for (int k = 0; k < n_blocks; ++k)
         for (int g = 0; g < p.row_groups; ++g) {
-            const int r = g * PagedRowsParams::kRows;
+            const int r = g * P::kRows;
             Block x;
-            x.load(p, k, lane, token_of(p, r), token_of(p, min(r + PagedRowsParams::kRows, p.R) - 1));
+            x.load(p, k, lane, token_of(p, r), token_of(p, min(r + P::kRows, p.R) - 1));
             const int S = x.total();
             if (lane == g) tiles += S;
             total += (float) S;
@@ -171,10 +172,9 @@ __device__ __forceinline__ void share(const PagedRowsParams & p, const int lane,
     records = head * places + start - unit * p.target;
 }
 
-// CAP: logits soft-capped.
-template <bool CAP>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedRowsParams p) {
-    using P = PagedRowsParams;
+// CAP: logits soft-capped. P: PagedRowsParams, or with a window or bits alone.
+template <bool CAP, typename P>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const P p) {
     __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];  // K and V of two tiles
     __shared__ uint64_t odd[128];                   // of each dim, the tile's cells whose value is not finite
     __shared__ int any_odd, any_bad;
@@ -243,19 +243,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         // what the group sees, what the wave sees, what all of the group's or the wave's rows see
         const Span group = span_of(p, w, t0, t1), mine = span_of(p, w, wt0, wt1);
         const int gap = group.gap(p), gap_at = group.gap_at(p);
-        auto tile_at = [&](const int i) { return i >= gap_at ? i + gap : i; };
+        auto tile_at = [&](const int i) { return P::kWindow && i >= gap_at ? i + gap : i; };
         // Tiles that some row does not see all of: from `from` on, and from `a` to `b`.
         struct Edges {
             int from, a, b;
-            __device__ __forceinline__ bool has(const int tile) const { return tile >= from || (tile >= a && tile < b); }
+            __device__ __forceinline__ bool has(const int tile) const { return tile >= from || (P::kWindow && tile >= a && tile < b); }
         };
         auto edges_of = [&](const int least, const int low) {
             return Edges{least / P::kTile, p.first / P::kTile, (max(low, 0) + P::kTile - 1) / P::kTile};
         };
         // cells that all rows from a token on see, and the last window's beginning
-        auto least_of = [&](const int first_token) { return p.bits ? max(begin, 0) : max(begin + 1 + first_token, 0); };
+        auto least_of = [&](const int first_token) { return has_bits(p) ? max(begin, 0) : max(begin + 1 + first_token, 0); };
         auto low_of = [&](const int last_token) {
-            return (p.bits ? w.len : begin + 1 + min(last_token, w.count - 1)) - p.window;
+            return P::kWindow ? (has_bits(p) ? w.len : begin + 1 + min(last_token, w.count - 1)) - p.window : 0;
         };
         const Edges edges = edges_of(least_of(t0), low_of(t1)), my_edges = edges_of(least_of(wt0), low_of(wt1));
         const int tiles_end = group.limit > 0 ? end : first;             // (nothing is seen: no tile)
@@ -271,8 +271,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         auto look_up = [&](const int i) {                                // of tiles i / 32 * 32 on
             const int last_group = max(group.limit - 1, 0) / 8, from = (ap.first + 7) >> 3;
             const int of = min(i / 32 * 32 + (lane >> 1), tiles_end - 1);
-            int g = min((of >= gap_at ? of + gap : of) * 8 + 2 * wave + (lane & 1), last_group);
-            if (g >= from) g = max(g, group.low >> 3);
+            int g = min(tile_at(of) * 8 + 2 * wave + (lane & 1), last_group);
+            if (P::kWindow && g >= from) g = max(g, group.low >> 3);
             const int pg = (int) page_of_group(p.c, (uint32_t) g);
             const uint32_t cell = (uint32_t) (g - pg * p.c.groups) * 8;
             return Where{(uint32_t) ap.c.table[(int64_t) seq * ap.c.t_nb1 + pg], cell * k_nb1, cell * v_nb1};
@@ -361,21 +361,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
         bool bad_row = false;
         {
             int place = begin + t;
-            if (ap.bits) {
+            if (P::kBits && ap.bits) {
                 words = ap.bits + (int64_t) seq * ap.b_nb2 + (int64_t) (valid ? t : 0) * ap.b_nb1;
-                node_pos = ap.pos + (int64_t) seq * ap.p_nb1;
-                if (ap.pos && valid) {
+                if (P::kWindow && ap.pos) node_pos = ap.pos + (int64_t) seq * ap.p_nb1;
+                if (node_pos && valid) {
                     place = node_pos[t];
                     bad_row = place < begin || place >= w.len;
                     if (bad_row && h == 0) paged_error(p.c, kPagedBadPos, place);
                 }
             }
-            if (valid && !bad_row) low = place + 1 - ap.window;
+            if (P::kWindow && valid && !bad_row) low = place + 1 - ap.window;
         }
         // Of the 64 cells from c0 on: those that this lane's row sees.
         auto sees64 = [&](const int c0) {
             const auto & sp = arguments<P>();
-            if (sp.bits) return span64(c0, begin, low, sp.first) | nodes64(sp, words, node_pos, c0 - begin, w.count, low);
+            if constexpr (!P::kWindow) return upto64(begin - c0) | nodes64(sp, words, nullptr, c0 - begin, w.count, 0);
+            if (P::kBits && sp.bits) return span64(c0, begin, low, sp.first) | nodes64(sp, words, node_pos, c0 - begin, w.count, low);
             return span64(c0, limit, low, sp.first);
         };
 
@@ -396,7 +397,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
             char * v_tile = lds + buf * 2 * kTileBytes + kTileBytes;
             const bool edge = edges.has(tile);                           // some row of the group does not see all of it
             if (edge) {
-                const uint64_t some = span64(c0, group.limit, group.low, ap.first), all = span64(c0, least_of(t0), low_of(t1), ap.first);
+                const uint64_t some = P::kWindow ? span64(c0, group.limit, group.low, ap.first) : upto64(group.limit - c0);
+                const uint64_t all = P::kWindow ? span64(c0, least_of(t0), low_of(t1), ap.first) : upto64(least_of(t0) - c0);
                 const int c = tid >> 2;
                 if (!(all >> c & 1)) {
                     const bool none = !(some >> c & 1);
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const PagedR
                 }
                 __syncthreads();
             }
-            const bool work = has_rows && c0 < mine.limit && !(c0 >= p.first && c0 + P::kTile <= mine.low);
+            const bool work = has_rows && c0 < mine.limit && !(P::kWindow && c0 >= p.first && c0 + P::kTile <= mine.low);
             if (!work && more)
 #pragma unroll
                 for (int q = 0; q < 8; ++q) load(where, i + 1, buf ^ 1, q);
@@ -640,10 +642,19 @@ __global__ __launch_bounds__(64 * kWaves) void paged_join_rows_kernel(const Page
 
 }  // namespace
 
-hipError_t launch_rows(const PagedRowsParams & p, hipStream_t st) {
+template <typename P>
+void launch(const PagedRowsParams & all, hipStream_t st) {
+    P p;
+    static_cast<PagedRowsParams &>(p) = all;
     const dim3 grid((unsigned) (p.target * p.row_groups * p.Hkv));
-    if (p.softcap != 0.0f) hipLaunchKernelGGL(paged_rows_kernel<true>, grid, dim3(64 * kWaves), 0, st, p);
-    else                   hipLaunchKernelGGL(paged_rows_kernel<false>, grid, dim3(64 * kWaves), 0, st, p);
+    if (p.softcap != 0.0f) hipLaunchKernelGGL((paged_rows_kernel<true, P>), grid, dim3(64 * kWaves), 0, st, p);
+    else                   hipLaunchKernelGGL((paged_rows_kernel<false, P>), grid, dim3(64 * kWaves), 0, st, p);
+}
+
+hipError_t launch_rows(const PagedRowsParams & p, hipStream_t st) {
+    if (!p.bits) launch<PagedRowsWindowParams>(p, st);
+    else if (!p.pos) launch<PagedRowsTreeParams>(p, st);
+    else launch<PagedRowsParams>(p, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.target == 1 || p.whole) return e;           // no pieces
     if (p.row_waves > 1) return launch_join(p, st);
