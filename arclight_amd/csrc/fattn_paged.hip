@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
 
     while (at < stop) {
         // the sequence that holds tile `at`
-        while (at >= before + b.total()) {
+        while (__builtin_expect(at >= before + b.total(), 0)) {
             before += b.total();
             if (++block >= n_blocks) return;                         // (lengths that change meanwhile: not without an end)
             b.load(p, block, lane, t0, t1);
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
             if (first == 0)
                 ap.info[(int64_t) unit * ap.c.n_seq + seq] =
                     int2{wg, whole ? 1 : parts.of(base + tiles - 1) - wg + 1};
-            if (w.bad) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
+            if (__builtin_expect(w.bad, 0)) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         bool bad = w.bad;
         const Span wave_span = span_of(p, w, wt0, wt1);
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
                 if (node_pos && valid) {
                     at = node_pos[t];
                     bad_row = at < begin || at >= w.len;
-                    if (bad_row && g == 0) paged_error(p.c, kPagedBadPos, at);
+                    if (__builtin_expect(bad_row && g == 0, 0)) paged_error(p.c, kPagedBadPos, at);
                 }
             }
             if (P::kWindow && valid && !bad_row) low = at + 1 - p.window;
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
                 for (int i = 0; i < 8; ++i)
                     if (c0 + i >= seen) v[i] = u32x4{0, 0, 0, 0};
             }
-            if (differ) {
+            if (__builtin_expect(differ, P::kBits)) {
                 uint32_t odd[2] = {0, 0};                            // bit 8 (i % 4) + j of word i / 4: cell i, dim j
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         // join the row tile's waves: maxima and sums, then the rescaled outputs
         // through LDS
         const bool any_bad = __any(bad);
-        if (any_bad && lane == 0 && !w.bad) paged_error(p.c, kPagedBadPage, seq);
+        if (__builtin_expect(any_bad && lane == 0 && !w.bad, 0)) paged_error(p.c, kPagedBadPage, seq);
         l = colsum4(l);
         if (any_bad || bad_row) l = __builtin_nanf("");
         if (g == 0) {

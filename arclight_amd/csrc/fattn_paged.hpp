@@ -242,7 +242,7 @@ struct Block {
     }
     // A negative count makes an empty slot, which no workgroup comes to.
     __device__ __forceinline__ void report(const PagedFattnParams & p) const {
-        if (count < 0) paged_error(p.c, kPagedBadCount, count);
+        if (__builtin_expect(count < 0, 0)) paged_error(p.c, kPagedBadCount, count);
     }
     __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
     __device__ __forceinline__ int active() const { return __builtin_popcountll(__ballot(tiles > 0)); }
@@ -312,7 +312,7 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
     b.load(p, 0, lane, t0, t1);
     if (report) b.report(p);
     int S = b.total(), active = b.active(), longest = b.longest();
-    for (int i = 1; i < n_blocks; ++i) {
+    for (int i = 1; __builtin_expect(i < n_blocks, 0); ++i) {
         Block x;
         x.load(p, i, lane, t0, t1);
         if (report) x.report(p);
@@ -343,7 +343,7 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
     m.parts = Parts(S, W);
     m.at = m.parts.begin(wg);
     m.stop = m.parts.begin(wg + 1);
-    if (!cut) {
+    if (__builtin_expect(!cut, 0)) {
         const Parts seqs(active, W);
         auto tile_of = [&](int i) {                                    // first tile of the i-th sequence that has any
             Block x = b;

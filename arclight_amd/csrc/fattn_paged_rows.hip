@@ -187,7 +187,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const P p) {
     // 301, 294).
     const int units = p.row_groups * p.Hkv;
     int unit = units - 1 - (int) (blockIdx.x % units), wg = blockIdx.x / units, target = p.target, records = 0;
-    if (p.shared) share(p, lane, unit, wg, target, records);
+    if (__builtin_expect(p.shared, 0)) share(p, lane, unit, wg, target, records);
     const int head = unit % p.Hkv, group0 = unit / p.Hkv * P::kRows;
     // tokens of the group, and of the wave's rows (none past the last row)
     const int t0 = token_of(p, group0), t1 = token_of(p, min(group0 + P::kRows, p.R) - 1);
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const P p) {
 
     while (at < stop) {
         // the sequence that holds tile `at`
-        while (at >= before + b.total()) {
+        while (__builtin_expect(at >= before + b.total(), 0)) {
             before += b.total();
             if (++block >= n_blocks) return;                         // (lengths that change meanwhile: not without an end)
             b.load(p, block, lane, t0, t1);
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const P p) {
         const auto & ap = arguments<P>();
         if (tid == 0) {
             if (first == 0) ap.info[(int64_t) unit * ap.c.n_seq + seq] = int2{wg + records, whole ? 1 : part.parts.of(base + tiles - 1) - wg + 1};
-            if (w.bad) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
+            if (__builtin_expect(w.bad, 0)) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         const int begin = w.len - w.count;
         // what the group sees, what the wave sees, what all of the group's or the wave's rows see
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const P p) {
                 if (node_pos && valid) {
                     place = node_pos[t];
                     bad_row = place < begin || place >= w.len;
-                    if (bad_row && h == 0) paged_error(p.c, kPagedBadPos, place);
+                    if (__builtin_expect(bad_row && h == 0, 0)) paged_error(p.c, kPagedBadPos, place);
                 }
             }
             if (P::kWindow && valid && !bad_row) low = place + 1 - ap.window;
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const P p) {
                 }
                 l += sum[0] + sum[1];
             }
-            if (edge && any_odd) {                                       // (written before the barrier above)
+            if (__builtin_expect(edge && any_odd, 0)) {                                       // (written before the barrier above)
                 if (work) {
                     const uint64_t sees = (valid ? sees64(c0) : 0ull) >> (4 * h);
 #pragma unroll
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(const P p) {
             }
         }
 
-        if (__any(bad) && lane == 0) {
+        if (__builtin_expect(__any(bad) && lane == 0, 0)) {
             any_bad = 1;
             if (!w.bad) paged_error(p.c, kPagedBadPage, seq);
         }
