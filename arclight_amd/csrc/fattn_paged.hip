@@ -532,6 +532,22 @@ bool many_rows(const PagedFattnParams & p) {
            p.c.v_nb3 <= kMost;
 }
 
+// Whether a call with a rule has so little to do that each row tile of 16 is a
+// group of its own, its workgroups' waves side by side over cells: few rounds and
+// small records, though the groups load the same cells. By the rows times the
+// cells that there can be (the table's, or the window's), up to 20 K a CU, or 48 K
+// where the other choice is two or four row tiles of a workgroup. (us, the other
+// choice and so, 32 heads over 8: a tree of 26 nodes over 300 cells 18.9, 12.8, 2000
+// 19.5, 16.7, 8000 29.9, 30.6, 20000 41.7, 56.5, 4 of 12 over 1500 23.8, 20.5, 4 of 26
+// 29.3, 29.0, 8 of 26 over 500 29.6, 31.0, 40 tokens over a window of 1024 23.2, 14.2;
+// two and four row tiles: a tree of 16 over 20000 39.6, 35.6, 8 of 8 over 3000 29.3,
+// 26.8, 30 of 8 80.1, 81.4, 60 of 8 tokens over windows of 1024 73.5, 90.2.)
+bool few_row_cells(const PagedFattnParams & p, const al_paged_sees & r, const int n_cu) {
+    double cells = (double) p.c.max_pages * p.c.page_size;
+    if (r.window > 0) cells = std::min(cells, (double) r.window + std::max(r.first, 0) + p.T);
+    return cells * p.R * p.Hkv * p.c.n_seq <= (many_rows(p) ? 20.0 : 48.0) * 1024 * n_cu;
+}
+
 int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_cu, Plan * out) {
     if (!a) return al_fail(AL_ERR_INVALID, "paged_fattn: null arguments");
     const al_tensor &q = a->q, &d = a->dst;
@@ -570,8 +586,9 @@ int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_c
     p.T = (int32_t) T; p.G = (int32_t) (Hq / Hkv); p.Hkv = (int32_t) Hkv;
     p.R = p.T * p.G;
     p.g_magic = p.G > 1 ? (uint32_t) (((1ull << 32) + (uint64_t) p.G - 1) / (uint64_t) p.G) : 0u;
-    pl.many = rule && many_rows(p);
-    p.row_tiles = pl.many ? PagedRowsParams::kRows / 16 : p.R <= 16 ? 1 : p.R <= 32 ? 2 : 4;
+    const bool few = rule && few_row_cells(p, *rule, n_cu);
+    pl.many = rule && !few && many_rows(p);
+    p.row_tiles = pl.many ? PagedRowsParams::kRows / 16 : p.R <= 16 || few ? 1 : p.R <= 32 ? 2 : 4;
     const int rows = 16 * p.row_tiles;
     p.row_groups = (p.R + rows - 1) / rows;
     const int64_t units = (int64_t) p.row_groups * Hkv;
