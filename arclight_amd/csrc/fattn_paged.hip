@@ -535,17 +535,21 @@ bool many_rows(const PagedFattnParams & p) {
 // Whether a call with a rule has so little to do that each row tile of 16 is a
 // group of its own, its workgroups' waves side by side over cells: few rounds and
 // small records, though the groups load the same cells. By the rows times the
-// cells that there can be (the table's, or the window's), up to 20 K a CU, or 48 K
-// where the other choice is two or four row tiles of a workgroup. (us, the other
-// choice and so, 32 heads over 8: a tree of 26 nodes over 300 cells 18.9, 12.8, 2000
-// 19.5, 16.7, 8000 29.9, 30.6, 20000 41.7, 56.5, 4 of 12 over 1500 23.8, 20.5, 4 of 26
-// 29.3, 29.0, 8 of 26 over 500 29.6, 31.0, 40 tokens over a window of 1024 23.2, 14.2;
-// two and four row tiles: a tree of 16 over 20000 39.6, 35.6, 8 of 8 over 3000 29.3,
-// 26.8, 30 of 8 80.1, 81.4, 60 of 8 tokens over windows of 1024 73.5, 90.2.)
+// cells that there can be (the table's, or the window's) for each CU, and by the
+// pairs of a group and a sequence, which are one workgroup's at least.
+// us, the other choice and so, 32 heads over 8 but where they are of all kinds: for
+// the kernel of many rows a tree of 26 nodes over 300 cells 18.9, 12.8, 2000 19.5,
+// 16.7, 8000 (26 K a CU) 29.9, 30.6, 4 of 12 over 1500 23.8, 20.5, 40 tokens over a
+// window of 1024 23.2, 14.2, 15 trees of 52 rows over 384 (480 pairs) 22.0, 18.9, 4 of
+// 368 over 144 (736) 21.4, 23.3, 14 of 364 over 96 (2576) 26.5, 58; for two and four row
+// tiles a tree of 16 over 20000 (39 K) 39.6, 35.6, 10 of 28 rows over 512 17.4, 13.8, 9
+// of 21 over 4000 (23 K) 33.7, 37.3, 46 of 32 over 48 (368) 12.5, 14.1.
 bool few_row_cells(const PagedFattnParams & p, const al_paged_sees & r, const int n_cu) {
     double cells = (double) p.c.max_pages * p.c.page_size;
     if (r.window > 0) cells = std::min(cells, (double) r.window + std::max(r.first, 0) + p.T);
-    return cells * p.R * p.Hkv * p.c.n_seq <= (many_rows(p) ? 20.0 : 48.0) * 1024 * n_cu;
+    const bool many = many_rows(p);
+    const double pairs = (double) ((p.R + 15) / 16) * p.Hkv * p.c.n_seq;
+    return pairs <= (many ? 2 : 1) * n_cu && cells * p.R * p.Hkv * p.c.n_seq <= (many ? 16.0 : p.c.n_seq == 1 ? 48.0 : 8.0) * 1024 * n_cu;
 }
 
 int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_cu, Plan * out) {

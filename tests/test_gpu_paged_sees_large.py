@@ -1,7 +1,7 @@
 """Windows and trees over the paged cache, the same tests as
 test_gpu_paged_sees.py and test_gpu_paged_sees_odd.py at sizes whose rows times
-cells are beyond what goes to the kernel of few rows (5.2 million on 256 CUs):
-all of these run the kernel of many rows."""
+cells (5.2 million and more) are beyond what goes to the kernel of few rows: all
+of these run the kernel of many rows."""
 import numpy as np
 import pytest
 
