@@ -51,12 +51,14 @@
 // itself (4 prompts of 2048 tokens, 32 heads over 8: 749 us, 184 TFLOP/s).
 //
 // Calls with a rule (al_paged_sees: windows with first cells, trees) take the
-// same code with PagedSeesParams: tiles that no row of the group sees are left
-// out of the row of tiles, those that some row does not see all of are masked by
-// a bit for each of a lane's 8 cells, and pages outside of what is seen are not
-// looked up. Many query rows go to the kernel of fattn_paged_rows.hip. Measured:
-// one token over a window of 1024 10.6 us, 30 over windows of 4096 90.3 us (5.6
-// TB/s), 64 of 1024 55.3.
+// same code with PagedSeesParams, or its parts for windows or trees alone: tiles
+// that no row of the group sees are left out of the row of tiles, those that some
+// row does not see all of are masked by a bit for each of a lane's 8 cells, and
+// pages outside of what is seen are not looked up. With little to do every 16 rows
+// are a group of their own (few_row_cells), and many query rows go to the kernel of
+// fattn_paged_rows.hip. Measured, 32 heads over 8: one token over a window of 1024
+// 10.1 us, 30 over windows of 4096 90.3 us (5.6 TB/s), 64 of 1024 55.5, a tree of 26
+// nodes over 2000 cells 16.5.
 
 #include <hip/hip_runtime.h>
 
@@ -540,7 +542,8 @@ bool many_rows(const PagedFattnParams & p) {
 // us, the other choice and so, 32 heads over 8 but where they are of all kinds: for
 // the kernel of many rows a tree of 26 nodes over 300 cells 18.9, 12.8, 2000 19.5,
 // 16.7, 8000 (26 K a CU) 29.9, 30.6, 4 of 12 over 1500 23.8, 20.5, 40 tokens over a
-// window of 1024 23.2, 14.2, 15 trees of 52 rows over 384 (480 pairs) 22.0, 18.9, 4 of
+// window of 1024 23.2, 14.2, 128 (18 K) 28.2, 20.3, 200 (30 K) 34.4, 28.0, a tree of 100
+// over 2000 (26 K) 32.8, 29.2, of 50 over 5000 (31 K) 30.4, 34.5, 15 trees of 52 rows over 384 (480 pairs) 22.0, 18.9, 4 of
 // 368 over 144 (736) 21.4, 23.3, 14 of 364 over 96 (2576) 26.5, 58; for two and four row
 // tiles a tree of 16 over 20000 (39 K) 39.6, 35.6, 10 of 28 rows over 512 17.4, 13.8, 9
 // of 21 over 4000 (23 K) 33.7, 37.3, 46 of 32 over 48 (368) 12.5, 14.1.
@@ -549,7 +552,8 @@ bool few_row_cells(const PagedFattnParams & p, const al_paged_sees & r, const in
     if (r.window > 0) cells = std::min(cells, (double) r.window + std::max(r.first, 0) + p.T);
     const bool many = many_rows(p);
     const double pairs = (double) ((p.R + 15) / 16) * p.Hkv * p.c.n_seq;
-    return pairs <= (many ? 2 : 1) * n_cu && cells * p.R * p.Hkv * p.c.n_seq <= (many ? 16.0 : p.c.n_seq == 1 ? 48.0 : 8.0) * 1024 * n_cu;
+    const double most = many ? (p.c.n_seq > 1 ? 16.0 : r.bits.data ? 28.0 : 32.0) : p.c.n_seq > 1 ? 8.0 : 48.0;
+    return pairs <= (many ? 2 : 1) * n_cu && cells * p.R * p.Hkv * p.c.n_seq <= most * 1024 * n_cu;
 }
 
 int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_cu, Plan * out) {
@@ -609,7 +613,8 @@ int make_plan(const al_paged_fattn_args * a, const al_paged_sees * rule, int n_c
     // 51.3 / 52.6 / 54.6, 100000 cells of 64 heads 79.4 / 81.7 / 85.7, 8000 cells
     // 13.2 / 14.2 / 13.9). Two where row tiles share the loads (verify of 10
     // sequences 48.5 / 47.1 / 50.0), and for many short sequences, whose ends
-    // are not hidden (96 to 300 cells 30.8 / 24.9, 128 to 700 57.2 / 57.2).
+    // are not hidden (96 to 300 cells 30.8 / 24.9, 128 to 700 57.2 / 57.2). Row
+    // tiles that are groups have one (a tree of 26 nodes over 2000 cells 16.8 / 19.0).
     const int64_t per_cu = n_cu / std::max<int64_t>(1, units);
     const int64_t useful = std::max(n_seq, (most + min_tiles - 1) / min_tiles);
     p.target = (int32_t) std::max<int64_t>(1, std::min<int64_t>(2 * n_cu / std::max<int64_t>(1, units), useful));

@@ -40,11 +40,11 @@
 // of the time over a launch and run at 1.9 GHz under this load; what else there
 // is are a tile's barrier (0.24 us of 3), the query rows' way into registers (3 us
 // a sequence and workgroup) and parts of tiles that are hidden. Measured, 32 heads
-// over 8: two prompts of 4000 over windows of 1000 275 to 294 us on three cards,
-// 450 to 480 TFLOP/s by the cells that are seen, twice that as executed (a plain
+// over 8: two prompts of 4000 over windows of 1000 270 to 292 us on several cards,
+// 450 to 485 TFLOP/s by the cells that are seen, twice that as executed (a plain
 // f16 product of 8192^3 runs at 1250 to 1300, products from registers alone at
 // 1400 to 1550), one of 4096 over windows of 8192 558; 11 trees of 31 to 61 nodes
-// over 2000 to 6000 cells, 64 heads, 163 to 176 us. (The next tile's scores beside
+// over 2000 to 6000 cells, 64 heads, 160 to 172 us. (The next tile's scores beside
 // this one's probabilities, tiles of 32 cells in a ring of four: 330 us instead of
 // 294, for twice the barriers; of 64 cells it does not fit the registers. Rows
 // stored through LDS, waves' priorities raised for the products: no gain.)

@@ -1,7 +1,7 @@
 """Windows and trees over the paged cache, the same tests as
 test_gpu_paged_sees.py and test_gpu_paged_sees_odd.py at sizes whose rows times
-cells (5.2 million and more) are beyond what goes to the kernel of few rows: all
-of these run the kernel of many rows."""
+cells, or pairs of 16 rows and a sequence, are beyond what goes to the kernel of
+few rows: all of these run the kernel of many rows."""
 import numpy as np
 import pytest
 
