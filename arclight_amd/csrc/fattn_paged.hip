@@ -98,7 +98,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
     Block b;
     MyPart part;
     if (!find_part(p, wg, p.target, p.long_target, lane, t0, t1, blockIdx.x == 0 && wave == 0, b, part)) return;
-    const Parts & parts = part.parts;
     int at = part.at, block = 0, before = 0;
     const int stop = part.stop;
 
@@ -122,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         if (threadIdx.x == 0) {
             if (first == 0)
                 ap.info[(int64_t) unit * ap.c.n_seq + seq] =
-                    int2{wg, whole ? 1 : parts.of(base + tiles - 1) - wg + 1};
+                    int2{wg, whole ? 1 : part.pieces(base, tiles, wg)};
             if (__builtin_expect(w.bad, 0)) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         bool bad = w.bad;

@@ -48,6 +48,7 @@ struct PagedSeesParams : PagedFattnParams {
     const int32_t * bits;  int64_t b_nb1, b_nb2;        // or null; token, sequence, in words
     const int32_t * pos;   int64_t p_nb1;               // or null; sequence (with bits and a window)
     int32_t whole;                                      // sequences are not cut, however long
+    static constexpr int kPiece = 16;                   // tiles that a workgroup could do instead of beginning a second piece
     static constexpr bool kSees = true;
     static constexpr bool kBits = true;
     static constexpr bool kWindow = true;
@@ -74,6 +75,7 @@ struct PagedRowsParams : PagedSeesParams {
     // 27.8, 24.8, 32.4, one of 500 30.6, 29.6, 29.1, 26.6)
     static constexpr int kMinTiles = 3;
     static constexpr int kWhole = 8;
+    static constexpr int kPiece = 8;
     static constexpr int kRows = 128;                   // of a group
     static constexpr int kShared = 8;                   // row groups times blocks of 64 sequences whose tiles are counted
     int32_t shared;                                     // a head's workgroups go to its row groups by their tiles
@@ -300,6 +302,12 @@ __device__ __forceinline__ const __attribute__((address_space(4))) P & arguments
 struct MyPart {
     Parts parts{0, 1};
     int at, stop;
+    int each = 0;                               // workgroups of every sequence (0: equal parts of them all)
+    // Pieces of a sequence of `tiles` tiles from `base` on that is not whole,
+    // whose first one is workgroup wg's.
+    __device__ __forceinline__ int pieces(const int base, const int tiles, const int wg) const {
+        return each ? min(tiles, each) : parts.of(base + tiles - 1) - wg + 1;
+    }
 };
 
 // Finds it, false if there is none; b: sequences 0 to 63. report: record counts
@@ -327,7 +335,7 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
     // 10 of 500 14.1, 12.3; whole up to 32 tiles: 128 of 700 56.4, 60.2). Else
     // kMinTiles a workgroup at least, or a sequence; `target` workgroups for
     // sequences of up to 16 tiles on average, `long_target` for longer ones.
-    bool cut = longest > P::kWhole || active == 1;
+    bool cut = longest > P::kWhole || active == 1, even = false;
     if constexpr (P::kSees) {
         // Nor are sequences cut that are about as long as one another, as those
         // are that a window is shorter than, where one each is what the card
@@ -335,15 +343,25 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
         // 63.6, 55.2, 29 of 1000 33.0, 29.3; where it holds more, 40 of 2048 71.9,
         // 81.6, 33 of 4096 104, 135).
         auto fills = [&](const int places) { return active <= places && 10 * active >= 9 * places; };
-        const bool even = (int64_t) longest * active * 8 <= (int64_t) S * 9;
+        even = (int64_t) longest * active * 8 <= (int64_t) S * 9;
         cut &= !p.whole && !(even && (fills(long_target) || fills(target)));
     }
-    const int W = cut ? min(S > 16 * active ? long_target : target, max((S + P::kMinTiles - 1) / P::kMinTiles, active)) : min(target, active);
+    int W = cut ? min(S > 16 * active ? long_target : target, max((S + P::kMinTiles - 1) / P::kMinTiles, active)) : min(target, active);
+    if constexpr (P::kSees) {
+        // Else each of such sequences has workgroups of its own, where equal parts
+        // of them all are not shorter by more than what a second piece costs (us,
+        // equal parts of all and so: 8 windows of 1024 16.3, 14.3, 5 of 600 14.2,
+        // 11.8, 20 of 1024 22.4, 21.5, 10 of 6 tokens 22.9, 20.4, 4 of 6 17.8, 14.1).
+        if (cut && even && active > 1 && active <= W && longest <= W / active * (S / W + P::kPiece)) {
+            m.each = W / active;
+            W = m.each * active;
+        }
+    }
     if (wg >= W) return false;
     m.parts = Parts(S, W);
     m.at = m.parts.begin(wg);
     m.stop = m.parts.begin(wg + 1);
-    if (__builtin_expect(!cut, 0)) {
+    if (__builtin_expect(!cut || m.each, 0)) {
         const Parts seqs(active, W);
         auto tile_of = [&](int i) {                                    // first tile of the i-th sequence that has any
             Block x = b;
@@ -361,8 +379,15 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
                 x.load(p, k, lane, t0, t1);
             }
         };
-        m.at = tile_of(seqs.begin(wg));
-        m.stop = tile_of(seqs.begin(wg + 1));
+        if (m.each) {
+            const int i = wg / m.each, j = wg - i * m.each, base = tile_of(i);
+            const Parts own(tile_of(i + 1) - base, m.each);
+            m.at = base + own.begin(j);
+            m.stop = base + own.begin(j + 1);
+        } else {
+            m.at = tile_of(seqs.begin(wg));
+            m.stop = tile_of(seqs.begin(wg + 1));
+        }
     }
     return true;
 }

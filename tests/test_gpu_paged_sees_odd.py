@@ -324,6 +324,25 @@ def test_row_groups_of_sequences_that_differ(gpu, i, window, first):
     st.destroy()
 
 
+LONGER = [(2, [], 300), (5, [0], 400), (8, [3, 7], 130), (11, [], 1000), (70, [0, 5, *range(12, 64), 65], 200)]
+
+
+@pytest.mark.parametrize("n, gone, window, T, Hq, Hkv", [(*x, *y) for x in LONGER for y in ((1, 16, 8), (5, 16, 2))] + [(*x, 150, 96, 4) for x in LONGER[:3]])
+def test_windows_that_all_sequences_are_longer_than(gpu, n, gone, window, T, Hq, Hkv):
+    """Sequences that see as many cells as one another, with empty slots between
+    them: each has workgroups of its own."""
+    _case(f"{n} sequences beyond windows of {window}, T={T}")
+    rng = np.random.default_rng(n + T)
+    lens = [window + T + int(x) for x in rng.integers(0, 90, n)]
+    counts = [T] * n
+    for s in gone:
+        lens[s], counts[s] = (0 if s % 2 else 40), 0
+    pool = P.Pool(rng, lens, Hkv, 16)
+    q = (rng.standard_normal((n, T, Hq, D)) * 2).astype(np.float32)
+    got = _attend(pool, q, lens, counts, window=window, first=2)
+    _check(got, C.attention(pool, q, lens, counts, SCALE, [C.visible(m, c, T, window, 2) for m, c in zip(lens, counts)]), "windows")
+
+
 @pytest.mark.parametrize("what", ["few rows", "many rows", "verification"])
 def test_a_workspaces_counters_are_left_alone(gpu, what):
     from arclight_amd import device, draft, fattn, paged
