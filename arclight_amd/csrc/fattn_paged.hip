@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_fattn_kernel(const P p) 
         if (threadIdx.x == 0) {
             if (first == 0)
                 ap.info[(int64_t) unit * ap.c.n_seq + seq] =
-                    int2{wg, whole ? 1 : part.pieces(base, tiles, wg)};
+                    int2{wg, whole ? 1 : part.pieces(base, tiles, wg, l64)};
             if (__builtin_expect(w.bad, 0)) paged_error(p.c, raw_len != w.len ? kPagedBadLength : kPagedBadCount, raw_len != w.len ? raw_len : raw_count);
         }
         bool bad = w.bad;

@@ -302,11 +302,12 @@ __device__ __forceinline__ const __attribute__((address_space(4))) P & arguments
 struct MyPart {
     Parts parts{0, 1};
     int at, stop;
-    int each = 0;                               // workgroups of every sequence (0: equal parts of them all)
-    // Pieces of a sequence of `tiles` tiles from `base` on that is not whole,
-    // whose first one is workgroup wg's.
-    __device__ __forceinline__ int pieces(const int base, const int tiles, const int wg) const {
-        return each ? min(tiles, each) : parts.of(base + tiles - 1) - wg + 1;
+    bool apart = false;                         // each sequence has workgroups of its own
+    int each = 0;                               // then: those of this lane's
+    // Pieces of a sequence of `tiles` tiles from `base` on, lane l's, that is not
+    // whole and whose first one is workgroup wg's.
+    __device__ __forceinline__ int pieces(const int base, const int tiles, const int wg, const int l) const {
+        return apart ? min(tiles, __builtin_amdgcn_readlane(each, l)) : parts.of(base + tiles - 1) - wg + 1;
     }
 };
 
@@ -335,7 +336,7 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
     // 10 of 500 14.1, 12.3; whole up to 32 tiles: 128 of 700 56.4, 60.2). Else
     // kMinTiles a workgroup at least, or a sequence; `target` workgroups for
     // sequences of up to 16 tiles on average, `long_target` for longer ones.
-    bool cut = longest > P::kWhole || active == 1, even = false;
+    bool cut = longest > P::kWhole || active == 1;
     if constexpr (P::kSees) {
         // Nor are sequences cut that are about as long as one another, as those
         // are that a window is shorter than, where one each is what the card
@@ -343,25 +344,38 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
         // 63.6, 55.2, 29 of 1000 33.0, 29.3; where it holds more, 40 of 2048 71.9,
         // 81.6, 33 of 4096 104, 135).
         auto fills = [&](const int places) { return active <= places && 10 * active >= 9 * places; };
-        even = (int64_t) longest * active * 8 <= (int64_t) S * 9;
+        const bool even = (int64_t) longest * active * 8 <= (int64_t) S * 9;
         cut &= !p.whole && !(even && (fills(long_target) || fills(target)));
     }
-    int W = cut ? min(S > 16 * active ? long_target : target, max((S + P::kMinTiles - 1) / P::kMinTiles, active)) : min(target, active);
+    const int W = cut ? min(S > 16 * active ? long_target : target, max((S + P::kMinTiles - 1) / P::kMinTiles, active)) : min(target, active);
     if constexpr (P::kSees) {
-        // Else each of such sequences has workgroups of its own, where equal parts
-        // of them all are not shorter by more than what a second piece costs (us,
-        // equal parts of all and so: 8 windows of 1024 16.3, 14.3, 5 of 600 14.2,
-        // 11.8, 20 of 1024 22.4, 21.5, 10 of 6 tokens 22.9, 20.4, 4 of 6 17.8, 14.1).
-        if (cut && even && active > 1 && active <= W && longest <= W / active * (S / W + P::kPiece)) {
-            m.each = W / active;
-            W = m.each * active;
+        // Else each sequence has workgroups of its own, by its tiles, where equal
+        // parts of them all are not shorter by more than what a second piece costs
+        // (us, equal parts of all and so: 8 windows of 1024 16.3, 14.3, 5 of 600
+        // 14.2, 11.8, 20 of 1024 22.4, 21.5, 10 of 6 tokens 22.9, 20.4, 4 of 6 17.8,
+        // 14.1, 8 trees of 8 nodes over up to 3000 cells 29.6, 25.7, 3 of 12 over 1000
+        // 19.0, 14.6, 12 of 30 over 2000 45.5, 41.5; 12 windows of 2048 25.1, 25.7).
+        if (cut && active > 1 && n_blocks == 1) {
+            m.each = b.tiles > 0 ? max((int) ((float) b.tiles * (float) W / (float) S), 1) : 0;
+            const int upto = wave_scan(m.each);
+            if (__builtin_amdgcn_readlane(upto, 63) <= W && !__any(b.tiles > m.each * (S / W + P::kPiece))) {
+                m.apart = true;
+                const uint64_t mask = __ballot(wg < upto);
+                if (!mask) return false;
+                const int l = __builtin_ctzll(mask), n = __builtin_amdgcn_readlane(b.tiles, l), k = __builtin_amdgcn_readlane(m.each, l);
+                const int base = __builtin_amdgcn_readlane(b.upto, l) - n, j = wg - (__builtin_amdgcn_readlane(upto, l) - k);
+                const Parts own(n, k);
+                m.at = base + own.begin(j);
+                m.stop = base + own.begin(j + 1);
+                return m.at < m.stop;
+            }
         }
     }
     if (wg >= W) return false;
     m.parts = Parts(S, W);
     m.at = m.parts.begin(wg);
     m.stop = m.parts.begin(wg + 1);
-    if (__builtin_expect(!cut || m.each, 0)) {
+    if (__builtin_expect(!cut, 0)) {
         const Parts seqs(active, W);
         auto tile_of = [&](int i) {                                    // first tile of the i-th sequence that has any
             Block x = b;
@@ -379,15 +393,8 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
                 x.load(p, k, lane, t0, t1);
             }
         };
-        if (m.each) {
-            const int i = wg / m.each, j = wg - i * m.each, base = tile_of(i);
-            const Parts own(tile_of(i + 1) - base, m.each);
-            m.at = base + own.begin(j);
-            m.stop = base + own.begin(j + 1);
-        } else {
-            m.at = tile_of(seqs.begin(wg));
-            m.stop = tile_of(seqs.begin(wg + 1));
-        }
+        m.at = tile_of(seqs.begin(wg));
+        m.stop = tile_of(seqs.begin(wg + 1));
     }
     return true;
 }
