@@ -177,7 +177,9 @@ typedef struct al_paged_sees {
 } al_paged_sees;
 
 /* al_paged_fattn_f16 of what `sees` says instead of all cells before a token.
- * Its cost goes by the cells that are seen, not by the sequences' lengths. */
+ * Its cost goes by the cells that are seen, not by the sequences' lengths. (For
+ * small calls of several query rows the table's width, max_pages, is what the
+ * kernel is chosen by.) */
 int al_paged_fattn_sees_f16(const al_paged_fattn_args * args, const al_paged_sees * sees);
 
 /* Bytes of a caller's workspace for these arguments; 0 for refused ones. */
