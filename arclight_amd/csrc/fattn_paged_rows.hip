@@ -112,11 +112,14 @@ __device__ __forceinline__ uint64_t nodes64(const A & p, const int32_t * words, 
 
 // 16 bytes a lane from page + at + lane_at into LDS at `to` + 16 * lane, without
 // passing registers. page, at and to are the wave's. (M0 carries the LDS address;
-// nothing else in this kernel uses it.)
+// nothing else in this kernel uses it.) A scalar register that a vector
+// instruction wrote, as readlane writes `at` or brings back a spilled one, may be
+// read by a vector memory instruction 5 wait states later, which the compiler does
+// not see to within an asm statement: the move to M0 and four of s_nop.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds(const int4v page, const uint32_t at, const uint32_t lane_at, const uint32_t to) {
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                  :
                  : "v"(lane_at), "s"(page), "s"(at), "s"(to)
                  : "memory", "m0");
