@@ -176,10 +176,13 @@ __global__ __launch_bounds__(WS * 64) void fattn_decode_kernel(const FattnParams
         const uint32_t base = ring + (uint32_t) (u * STAGE);
         // the stage's V rows, then its K rows (grouped by tensor: 0.3-0.4 µs
         // per launch faster at 32K than K and V alternating, measured)
+        uint32_t kat[4], vat[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dma16(vd, vofs + (uint32_t) (4 * i) * v_nb1 + dj[i], base + (uint32_t) (4096 + i * 1024));
+        for (int i = 0; i < 4; ++i) vat[i] = vofs + (uint32_t) (4 * i) * v_nb1 + dj[i];
+        dma16x4(vd, vat, base + 4096u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dma16(kd, kofs + (uint32_t) (4 * i) * k_nb1 + dj[i], base + (uint32_t) (i * 1024));
+        for (int i = 0; i < 4; ++i) kat[i] = kofs + (uint32_t) (4 * i) * k_nb1 + dj[i];
+        dma16x4(kd, kat, base);
         if constexpr (MASK == 1) dma16(md, msrc + cs * 2, base + 8192u);
     };
 

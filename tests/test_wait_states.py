@@ -87,3 +87,25 @@ def test_the_check_finds_what_it_looks_for():
 
 def test_rows_of_the_paged_cache():
     assert not faults("paged_rows_kernel")
+
+
+def test_every_kernel():
+    assert not faults("")
+
+
+def test_loads_into_lds_keep_the_distance_themselves():
+    """Whatever the compiler puts before them: a move to M0 and the waits, then
+    loads that go on by the same registers."""
+    n = 0
+    for name, body in code_object.functions().items():
+        for k, x in enumerate(body):
+            if not x.op.startswith("buffer_load") or not re.search(r"\blds$", x.args):
+                continue
+            passed, j = 0, k
+            while body[j].op.startswith(("buffer_load", "s_nop")) or body[j].args.startswith("m0, m0,"):
+                passed += states(body[j]) if j < k else 0
+                assert j == k or scalars(body[j].args) <= scalars(x.args), name
+                j -= 1
+            assert body[j].op == "s_mov_b32" and body[j].args.startswith("m0,") and passed + 1 >= NEEDED, name
+            n += 1
+    assert n > 1000
