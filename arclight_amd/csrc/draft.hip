@@ -33,6 +33,7 @@
 #include "../../include/arclight_draft.h"
 #include "device_errors.hpp"
 #include "kernel_args.hpp"
+#include "overlap.hpp"
 #include "runtime.hpp"
 
 namespace {
@@ -541,16 +542,6 @@ bool nodes(const al_tensor & t, const int type, const int64_t T, const int64_t n
            ((uintptr_t) t.data & 3u) == 0;
 }
 
-// Whether one of the first `outs` operands begins where another one does.
-// (Strided ones may lie in one another's gaps.)
-template <int N>
-bool shared(const al_tensor * const (&x)[N], const int outs) {
-    for (int i = 0; i < outs; ++i)
-        for (int j = i + 1; j < N; ++j)
-            if (x[i]->data && x[i]->data == x[j]->data) return true;
-    return false;
-}
-
 int64_t entries(const uint64_t bytes) { return (int64_t) (bytes / 4); }
 
 struct VerifyPlan {
@@ -579,7 +570,7 @@ int make_plan(const al_draft_verify_args * a, VerifyPlan * out) {
     if (!index(u, n) || !index(a->kept, n) || !index(a->next, n) || (a->counts.data && !index(a->counts, n)))
         return al_fail(AL_ERR_INVALID, "draft_verify: sample, counts, kept and next must be [n_seq], i32 but for sample");
     if (V > (1 << 24) || T > kMaxNodes || n > 65535) return al_fail(AL_ERR_UNSUPPORTED, "draft_verify: sizes out of range");
-    if (shared({&a->path, &a->kept, &a->next, &a->target, &a->draft, &a->tokens, &a->parents, &a->counts, &a->accept, &a->sample}, 3) && T > 0 && n > 0)
+    if (outputs_overlap({&a->path, &a->kept, &a->next, &a->target, &a->draft, &a->tokens, &a->parents, &a->counts, &a->accept, &a->sample}, 3))
         return al_fail(AL_ERR_INVALID, "draft_verify: path, kept and next may not be another operand's memory");
     VerifyPlan pl;
     VerifyParams & p = pl.p;
@@ -622,7 +613,7 @@ extern "C" int al_draft_tree_i32(const al_draft_tree_args * a) {
                    b.nb[2] % 4 || ((uintptr_t) b.data & 3u)))
         return al_fail(AL_ERR_INVALID, "draft_tree: bits must be i32 [words, T, n_seq], 32 nodes to a word");
     if (T > kMaxNodes || n > 65535 || (b.data && b.ne[0] > (1 << 16))) return al_fail(AL_ERR_UNSUPPORTED, "draft_tree: sizes out of range");
-    if (shared({&a->pos, &a->cells, &a->seq, &a->bits, &a->parents, &a->lens, &a->counts}, 4) && T > 0 && n > 0)
+    if (outputs_overlap({&a->pos, &a->cells, &a->seq, &a->bits, &a->parents, &a->lens, &a->counts}, 4))
         return al_fail(AL_ERR_INVALID, "draft_tree: pos, cells, seq and bits may not be another operand's memory");
     if (T == 0 || n == 0) return AL_OK;
     TreeParams p;
