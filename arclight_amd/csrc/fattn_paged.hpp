@@ -321,7 +321,8 @@ __device__ __forceinline__ bool find_part(const P & p, const int wg, const int t
     b.load(p, 0, lane, t0, t1);
     if (report) b.report(p);
     int S = b.total(), active = b.active(), longest = b.longest();
-    for (int i = 1; __builtin_expect(i < n_blocks, 0); ++i) {
+    // (said to be unlikely, this loop leaves the kernels 20 bytes of private memory)
+    for (int i = 1; i < n_blocks; ++i) {
         Block x;
         x.load(p, i, lane, t0, t1);
         if (report) x.report(p);
