@@ -17,7 +17,9 @@
 // Where several children of a node were drawn from a draft's row, what is left
 // after each rejection has to be normalised before the next child is tried: a
 // sum over the row within the walk, which a workgroup for each sequence then
-// does in a launch of its own.
+// does in a launch of its own. It keeps what is left of the row in memory from one
+// rejection to the next, as a node's rejections cost their square if each begins
+// from the row again.
 //
 // What bounds them: chains of loads. The tables of one tree of 26 nodes or of 50
 // of up to 200 take 3.7 us, a launch and two loads in series. Verification is two
@@ -115,21 +117,14 @@ struct VerifyParams {
     int32_t * kept;
     int32_t * next;
     int2 * state;                               // [sequence]: the last accepted node (-1: none), its rejected children
-    double * norms;                             // [sequence][T]: with siblings of a draft, the sums after each rejection
+    double * rest;                              // [sequence][V]: of three siblings of a draft and more, what all rejections but the last left
+    double * norm;                              // [sequence]: of two and more, its sum
     pair64 * sums;                             // [sequence][chunk]: of what is left, of the row itself
-    int32_t T, V, chunks, walked;               // walked: state and norms are there
+    int32_t T, V, chunks, walked;               // walked: state, rest and norm are there
     int * err;
 };
 
 __device__ __forceinline__ float weight(const float x) { return x > 0.0f ? x : 0.0f; }
-
-// What m rejections of children drawn from q leave of p, before it is
-// normalised: norms[i] is the sum after rejection i + 1.
-__device__ __forceinline__ double left_of(const double p, const double q, const int m, const double * norms) {
-    double f = p;
-    for (int i = 0; i < m; ++i) f = fmax((i ? f / norms[i - 1] : f) - q, 0.0);
-    return f;
-}
 
 // Sums of the workgroup's lanes, in a fixed order; every thread gets them.
 __device__ __forceinline__ double wave_sum(double x) {
@@ -146,6 +141,43 @@ __device__ __forceinline__ double block_sum(double x, double * lds) {
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) x += lds[i];
     return x;
+}
+
+// What is left of a token's p, q in the draft's row, by two rejections of children
+// drawn from it. norm: the sum of what the first left of all.
+__device__ __forceinline__ double left_by_one(const double p, const double q) { return fmax(p - q, 0.0); }
+__device__ __forceinline__ double left_by_two(const double p, const double q, const double norm) { return fmax(left_by_one(p, q) / norm - q, 0.0); }
+
+// Rejection m of a child of node v drawn from its row q, by a workgroup: the sum of
+// what it leaves of p, which every thread gets, and from the second on that itself,
+// before it is normalised, to p.rest. norm: the sum of what rejection m - 1 left. M:
+// 1, 2, or 3 for all behind. A thread's tokens are its own in all rejections; others
+// read them behind block_sum's barriers.
+template <int M>
+__device__ __forceinline__ double reject(const VerifyParams & p, const int s, const int v, const double norm, double * lds) {
+    constexpr int kHeld = 8;                                             // a thread's loads in flight, of each row
+    const float * pr = (const float *) (p.target + (int64_t) s * p.t_nb2 + (int64_t) v * p.t_nb1);
+    const float * qr = (const float *) (p.draft + (int64_t) s * p.d_nb2 + (int64_t) v * p.d_nb1);
+    double * rest = p.rest + (int64_t) s * p.V;
+    double sum = 0.0;
+    for (int y0 = threadIdx.x; y0 < p.V; y0 += kThreads * kHeld) {
+        double f[kHeld];
+        float q[kHeld];
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int y = min(y0 + j * kThreads, p.V - 1);
+            f[j] = M < 3 ? (double) weight(pr[y]) : rest[y];
+            q[j] = weight(qr[y]);
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (y0 + j * kThreads < p.V) {
+                const double left = M == 1 ? left_by_one(f[j], q[j]) : M == 2 ? left_by_two(f[j], q[j], norm) : fmax(f[j] / norm - q[j], 0.0);
+                if (M > 1) rest[y0 + j * kThreads] = left;
+                sum += left;
+            }
+    }
+    return block_sum(sum, lds);
 }
 
 struct WalkLds {
@@ -177,9 +209,9 @@ __device__ __forceinline__ int parent_of(const VerifyParams & p, const int s, co
 }
 
 // The walk down the tree, by every wave of a workgroup alike. NORMS: with a
-// draft whose nodes can have several children; norms: of this sequence.
+// draft whose nodes can have several children.
 template <bool NORMS>
-__device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, const int count, const bool report, WalkLds & x, double * norms) {
+__device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, const int count, const bool report, WalkLds & x) {
     const int tid = threadIdx.x, lane = tid & 63;
     const char * target = p.target + (int64_t) s * p.t_nb2;
     const char * draft = p.draft ? p.draft + (int64_t) s * p.d_nb2 : nullptr;
@@ -204,6 +236,7 @@ __device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, cons
     __syncthreads();
     Walked at = {count > 0 ? 0 : -1, 0, count > 0};
     if (tid == 0) x.path[0] = 0;
+    double norm = 1.0;                                                   // of the last row that was left
     while (at.v >= 0) {
         // the children of v in their order
         double mass = 1.0;
@@ -230,19 +263,13 @@ __device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, cons
                     double pc = x.p[c];
                     const double qc = x.q[c];
                     if (NORMS && m > 0) {
-                        // the sum of what the last rejection left
+                        // what the last rejection left, and its sum
                         if (!nothing) {
-                            const char * pr = target + (int64_t) at.v * p.t_nb1;
-                            const char * qr = draft + (int64_t) at.v * p.d_nb1;
-                            double sum = 0.0;
-                            for (int y = tid; y < p.V; y += kThreads)
-                                sum += left_of(weight(*(const float *) (pr + (int64_t) y * 4)), weight(*(const float *) (qr + (int64_t) y * 4)), m, norms);
-                            sum = block_sum(sum, x.red);
-                            nothing = !(sum > 0.0 && sum < __builtin_inf());
-                            if (tid == 0) norms[m - 1] = sum;
-                            __syncthreads();
+                            norm = m == 1 ? reject<1>(p, s, at.v, norm, x.red) : m == 2 ? reject<2>(p, s, at.v, norm, x.red) : reject<3>(p, s, at.v, norm, x.red);
+                            nothing = !(norm > 0.0 && norm < __builtin_inf());
                         }
-                        pc = nothing ? 0.0 : left_of(pc, qc, m, norms) / norms[m - 1];
+                        pc = nothing ? 0.0 : (m == 1 ? left_by_one(pc, qc) : p.rest[(int64_t) s * p.V + tok]) / norm;
+                        __syncthreads();                                 // (all have read it: the next rejection writes there)
                     }
                     pass = pc > 0.0 && (double) x.r[c] * qc < pc;
                 }
@@ -252,6 +279,7 @@ __device__ __forceinline__ Walked walk(const VerifyParams & p, const int s, cons
         }
         if (found < 0) {
             at.m = nothing ? 0 : m;
+            if (NORMS && tid == 0) p.norm[s] = norm;
             break;
         }
         at.v = found;
@@ -274,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(const VerifyParam
     __shared__ WalkLds x;
     const int s = blockIdx.x;
     const int count = nodes_of(p, s, threadIdx.x == 0);
-    const Walked at = walk<true>(p, s, count, true, x, p.norms + (int64_t) s * p.T);
+    const Walked at = walk<true>(p, s, count, true, x);
     write_path(p, s, at, x);
 }
 
@@ -316,9 +344,9 @@ __device__ __forceinline__ Row load_row(const VerifyParams & p, const int s, con
     return x;
 }
 
-// What is left of them, and they themselves. gone: the tokens of the chunk that
-// were rejected, a bit each.
-__device__ __forceinline__ void row_weights(const VerifyParams & p, const Walked & at, const double * norms, const Row & x, const uint32_t * gone,
+// What is left of them, and they themselves. first: the first of them; gone: the
+// tokens of the chunk that were rejected, a bit each.
+__device__ __forceinline__ void row_weights(const VerifyParams & p, const int s, const Walked & at, const Row & x, const int first, const uint32_t * gone,
                                             double (&left)[kEach], double (&own)[kEach]) {
     const bool drafted = p.draft && at.m > 0;
     const int lane = threadIdx.x & 63;
@@ -326,7 +354,15 @@ __device__ __forceinline__ void row_weights(const VerifyParams & p, const Walked
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         own[j] = weight(x.p[j]);
-        left[j] = drafted ? left_of(own[j], weight(x.q[j]), at.m, norms) : out >> j & 1 ? 0.0 : own[j];
+        left[j] = drafted ? left_by_one(own[j], weight(x.q[j])) : out >> j & 1 ? 0.0 : own[j];
+    }
+    if (drafted && at.m > 1) {
+        const double * rest = p.rest + (int64_t) s * p.V, norm = p.norm[s];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const double q = weight(x.q[j]);
+            left[j] = at.m == 2 ? left_by_two(own[j], q, norm) : first + j < p.V ? fmax(rest[first + j] / norm - q, 0.0) : 0.0;
+        }
     }
 }
 
@@ -364,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyParam
         at = {st.x, st.y, 0};
     } else {
         count = nodes_of(p, s, first && threadIdx.x == 0);
-        at = walk<false>(p, s, count, first, x, nullptr);
+        at = walk<false>(p, s, count, first, x);
         if (first) write_path(p, s, at, x);
     }
     if (at.v < 0) return;
@@ -375,7 +411,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyParam
         const Row next = load_row(p, s, at, (chunk + step) * kChunk + lane * kEach);
         if (!p.draft) rejected(x, at, count, chunk, gone[wave]);         // (the walk was this workgroup's own)
         double left[kEach], own[kEach], a = 0.0, b = 0.0;
-        row_weights(p, at, p.norms + (int64_t) s * p.T, row, gone[wave], left, own);
+        row_weights(p, s, at, row, chunk * kChunk + lane * kEach, gone[wave], left, own);
 #pragma unroll
         for (int j = 0; j < kEach; ++j) a += left[j], b += own[j];
         a = wave_sum(a);
@@ -500,7 +536,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyParam
     __syncthreads();
     if (wave) return;
     double left[kEach], weights[kEach], sum = 0.0;
-    row_weights(p, at, p.norms + (int64_t) s * p.T, row, gone, left, weights);
+    row_weights(p, s, at, row, first, gone, left, weights);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         if (own) left[j] = weights[j];
@@ -547,7 +583,7 @@ int64_t entries(const uint64_t bytes) { return (int64_t) (bytes / 4); }
 struct VerifyPlan {
     VerifyParams p;
     int64_t n_seq = 0;
-    size_t norms_at = 0, sums_at = 0, bytes = 0;
+    size_t norm_at = 0, rest_at = 0, sums_at = 0, bytes = 0;
 };
 
 int make_plan(const al_draft_verify_args * a, VerifyPlan * out) {
@@ -591,8 +627,9 @@ int make_plan(const al_draft_verify_args * a, VerifyPlan * out) {
     p.walked = p.draft && p.parents && T > 2;
     pl.n_seq = n;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    pl.norms_at = up((size_t) n * sizeof(int2));
-    pl.sums_at = pl.norms_at + (p.walked ? up((size_t) n * T * sizeof(double)) : 0);
+    pl.norm_at = up((size_t) n * sizeof(int2));
+    pl.rest_at = pl.norm_at + (p.walked ? up((size_t) n * sizeof(double)) : 0);
+    pl.sums_at = pl.rest_at + (p.walked ? up((size_t) n * V * sizeof(double)) : 0);
     pl.bytes = pl.sums_at + (size_t) n * p.chunks * sizeof(pair64);
     *out = pl;
     return AL_OK;
@@ -653,7 +690,8 @@ extern "C" int al_draft_verify_f32(const al_draft_verify_args * a) {
     rc = al_workspace_records("draft_verify", pl.bytes, a->workspace, a->workspace_bytes, a->stream, (void **) &at);
     if (rc != AL_OK) return rc;
     p.state = (int2 *) at;
-    p.norms = (double *) (at + pl.norms_at);
+    p.norm = (double *) (at + pl.norm_at);
+    p.rest = (double *) (at + pl.rest_at);
     p.sums = (pair64 *) (at + pl.sums_at);
     const hipStream_t st = (hipStream_t) a->stream;
     const unsigned n = (unsigned) pl.n_seq;
