@@ -24,8 +24,10 @@
 // What bounds them: chains of loads. The tables of one tree of 26 nodes or of 50
 // of up to 200 take 3.7 us, a launch and two loads in series. Verification is two
 // launches, count and nodes -> their p -> the row -> its sums, and sums -> the
-// chunk: one tree of 26 nodes over 32003 tokens 9.4 us, 30 chains with a draft's
-// rows of 128000 (31 MB) 14.2, 20 trees of 40 nodes over 152000 (12 MB) 13.8.
+// chunk: one tree of 26 nodes over 32003 tokens 9.5 us, 30 chains with a draft's
+// rows of 128000 (31 MB) 13.9, 20 trees of 40 nodes over 152000 (12 MB) 14.0. Trees
+// with a draft's rows are bound by the slowest sequence's rejections one after another,
+// 34 us and more each at 128000 tokens: 8 trees of 40 nodes 105 us, 30 of 26 251.
 
 #include <hip/hip_runtime.h>
 

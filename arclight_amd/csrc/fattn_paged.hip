@@ -57,8 +57,8 @@
 // pages outside of what is seen are not looked up. With little to do every 16 rows
 // are a group of their own (few_row_cells), and many query rows go to the kernel of
 // fattn_paged_rows.hip. Measured, 32 heads over 8: one token over a window of 1024
-// 10.1 us, 30 over windows of 4096 90.3 us (5.6 TB/s), 64 of 1024 55.5, a tree of 26
-// nodes over 2000 cells 16.5.
+// 9.9 us, 30 over windows of 4096 90.1 us (5.6 TB/s), 64 of 1024 55.2, a tree of 26
+// nodes over 2000 cells 16.1.
 
 #include <hip/hip_runtime.h>
 
