@@ -117,7 +117,8 @@ int al_paged_append_f32(const al_paged_append_args * args);
  * or the cell no weight. (al_paged_append_f32 stores what lies beyond f16's
  * range, 65504, as an infinity.)
  * A sequence whose length or count is recorded as an error has NaN rows, and
- * so have all rows that see a cell of a page outside the pool.
+ * so have all rows that see a cell of a page outside the pool (others of that
+ * sequence, which a wave or a workgroup takes with them, may be NaN too).
  * workspace: device scratch (al_paged_fattn_workspace_bytes), NULL: the
  * library's own for (current device, stream), as al_fattn_f16: then one
  * eager call of the same shapes has to come before a capture. Calls and
